@@ -362,10 +362,9 @@ MASK = 0xFFFFFFFF
 def _mix(x):
     """32 bits mixed by two multiplications with odd constants (the fractions of the golden
     ratio and of the square root of 3) between shifted exclusive ors; int64 tensors."""
-    x = (x ^ (x >> 17)) & MASK
-    x = (x * 0x9E3779B9) & MASK
-    x = x ^ (x >> 14)
-    x = (x * 0xBB67AE85) & MASK
+    x = x & MASK
+    x = ((x ^ (x >> 17)) * 0x9E3779B9) & MASK
+    x = ((x ^ (x >> 14)) * 0xBB67AE85) & MASK
     return x ^ (x >> 15)
 
 
