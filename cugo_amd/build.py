@@ -121,8 +121,10 @@ def check_no_packed_fp32(lib: Path) -> None:
 # out of the step loops costs more registers than it saves work: without it
 # play_split_kernel takes no scratch (16 bytes with it) and canonical_kernel 142 VGPRs (179).
 SOURCE_FLAGS = {"kernels.hip": ["-mllvm", "-disable-machine-licm"]}
-SOURCES = ("kernels.hip", "decode.hip", "selfplay.hip", "mlp.hip", "linear.hip")
-HEADERS = (CSRC / "engine.h", REPO / "include" / "cugo_hip.h")
+SOURCES = ("kernels.hip", "decode.hip", "selfplay.hip", "mlp.hip", "linear.hip",
+           "policy_loss.hip", "advantages.hip", "adamw.hip")
+HEADERS = (CSRC / "engine.h", CSRC / "learner.h", REPO / "include" / "cugo_hip.h")
+EXT_SOURCES = ("torch_ext.cpp", "learner_ext.cpp")
 
 
 def build_library(force: bool = True) -> Path:
@@ -163,15 +165,27 @@ def build_extension() -> Path:
     includes = cpp_extension.include_paths(device_type="cuda")
     libdirs = cpp_extension.library_paths(device_type="cuda")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    cmd = [
-        "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+    flags = [
+        "-O2", "-std=c++17", "-fPIC",
         "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
         f"-DTORCH_EXTENSION_NAME={EXT_NAME}", "-DTORCH_API_INCLUDE_EXTENSION_H",
         f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
         *[f"-I{p}" for p in includes],
         f"-I{sysconfig.get_paths()['include']}",
-        str(CSRC / "torch_ext.cpp"),
-        "-o", str(out),
+    ]
+    objdir = PKG / "_build"
+    objdir.mkdir(exist_ok=True)
+    procs, objs = [], []
+    for name in EXT_SOURCES:
+        objs.append(objdir / (name + ".o"))
+        cmd = ["g++", *flags, "-c", str(CSRC / name), "-o", str(objs[-1])]
+        print("+", " ".join(cmd), flush=True)
+        procs.append((name, subprocess.Popen(cmd)))
+    failed = [name for name, p in procs if p.wait() != 0]
+    if failed:
+        raise RuntimeError(f"g++ failed for {failed}")
+    cmd = [
+        "g++", "-shared", *map(str, objs), "-o", str(out),
         f"-L{PKG}", "-lcugo_hip",
         *[f"-L{p}" for p in libdirs],
         "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python",

@@ -1,0 +1,223 @@
+// Generalised advantage estimation over a horizon of two-player games.
+//
+// With s_t = 1 where player 0 moves and -1 where player 1 does, everything is seen from
+// player 0's side:
+//   d_t = reward_t + [not done_t] gamma s_(t+1) V_(t+1) - s_t V_t
+//   a_t = d_t + c_t a_(t+1),  c_t = gamma lam, or 0 at a done step
+// and a mover's advantage is s_t a_t.  a_t is an affine map of a_(t+1), and maps compose:
+// (D, C) after (D', C') is (D + C D', C C').  So the steps are split: a lane takes kSteps
+// consecutive steps of one game in registers and composes their maps, lanes and wavefronts
+// compose theirs (a suffix scan in the wavefront, then over the wavefronts in LDS), and each
+// lane runs its own steps again from the value that follows them.  The data is read once.
+//
+// What bounds it is memory: 10 to 18 bytes a step of a game.  A wavefront's 64 lanes are
+// `columns` games times 64 / columns runs of steps, the fewest columns (a power of two) that
+// hold the games up to 64, so that few games still fill wavefronts; where the workgroups of
+// one run over the steps would leave compute units idle, the steps are also split over
+// workgroups, in two launches: the first composes each chunk's map, the second starts each
+// chunk from the maps of those behind it.
+#include "learner.h"
+
+namespace cugo_amd {
+namespace learner {
+namespace gae {
+
+constexpr int kSteps = 8;   // steps a lane holds
+constexpr int kWaves = 8;   // wavefronts a workgroup
+
+struct GaeArgs {
+  const float* reward;
+  const void* value;
+  const uint8_t* done;
+  const uint8_t* player;
+  const void* bootstrap;
+  const uint8_t* last_player;
+  i64 steps, batch;
+  i64 chunk;    // steps a workgroup takes: a multiple of the steps of one pass over its lanes
+  int chunks;
+  int columns;
+  float gamma, decay;
+  float* advantage;
+  float* returns;
+  float2* maps;  // [chunks, batch]: the chunks' maps (chunks > 1)
+};
+
+// m applied to the value a that follows it, which a done step (m.y = 0) does not read: a NaN
+// of the next game stays there.
+__device__ inline float apply(float2 m, float a) {
+  return m.y == 0.0f ? m.x : __builtin_fmaf(m.y, a, m.x);
+}
+__device__ inline float2 after(float2 m, float2 later) {
+  return make_float2(apply(m, later.x), m.y * later.y);
+}
+
+template <class T, bool kMapsOnly>
+__global__ __launch_bounds__(64 * kWaves) void gae_kernel(const GaeArgs g) {
+  using S = typename T::storage;
+  __shared__ float2 wave_map[kWaves][64];
+  __shared__ float behind[2][64];  // a of the step behind a pass, for each column, in turn
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int column = lane & (g.columns - 1), run = lane / g.columns;
+  const int runs = 64 / g.columns;
+  const i64 game = (i64)blockIdx.x * g.columns + column;
+  const bool ok = game < g.batch;
+  const i64 b = ok ? game : g.batch - 1;
+  const int chunk = blockIdx.y;
+  const i64 first = (i64)chunk * g.chunk;
+  const i64 end = min(first + g.chunk, g.steps);
+  const S* value = static_cast<const S*>(g.value);
+  const i64 pass = (i64)kWaves * runs * kSteps;
+  float carry = 0.0f;
+  if (!kMapsOnly) {
+    for (int k = g.chunks - 1; k > chunk; --k)
+      carry = apply(g.maps[(i64)k * g.batch + b], carry);
+  }
+  float2 total = make_float2(0.0f, 1.0f);  // kMapsOnly: the map of the passes so far
+  int turn = 0;
+  // passes from the chunk's last steps back
+  for (i64 at = first + (end - first - 1) / pass * pass; at >= first; at -= pass, turn ^= 1) {
+    const i64 t0 = at + ((i64)wave * runs + run) * kSteps;
+    float d[kSteps], v[kSteps + 1], sign[kSteps + 1];
+    bool over[kSteps];
+#pragma unroll
+    for (int i = 0; i <= kSteps; ++i) {
+      // steps behind the horizon's end: the bootstrap's place, read by the last step alone
+      const i64 t = min(t0 + i, g.steps);
+      const bool boot = t == g.steps;
+      const i64 at_v = boot ? b : t * g.batch + b;
+      const S* from = boot ? static_cast<const S*>(g.bootstrap) : value;
+      const uint8_t* who = boot ? g.last_player : g.player;
+      v[i] = T::to_float(from[at_v]);
+      sign[i] = who && who[at_v] ? -1.0f : 1.0f;
+      if (i < kSteps) {
+        const i64 at_r = min(t, g.steps - 1) * g.batch + b;
+        d[i] = g.reward[at_r];
+        over[i] = g.done[at_r] != 0;
+      }
+    }
+    float2 map = make_float2(0.0f, 1.0f);
+#pragma unroll
+    for (int i = kSteps - 1; i >= 0; --i) {
+      if (t0 + i < end) {
+        const float next = over[i] ? 0.0f : g.gamma * (sign[i + 1] * v[i + 1]);
+        d[i] = d[i] + next - sign[i] * v[i];
+        map.x = over[i] ? d[i] : __builtin_fmaf(g.decay, map.x, d[i]);
+        map.y = over[i] ? 0.0f : g.decay * map.y;
+      }
+    }
+    // each lane's map and those of the later runs of its column, then of the later runs alone
+    for (int off = g.columns; off < 64; off <<= 1) {
+      const float2 next = make_float2(__shfl_down(map.x, off), __shfl_down(map.y, off));
+      if (lane + off < 64) map = after(map, next);
+    }
+    float2 later = make_float2(__shfl_down(map.x, g.columns), __shfl_down(map.y, g.columns));
+    if (run == runs - 1) later = make_float2(0.0f, 1.0f);
+    if (run == 0) wave_map[wave][column] = map;
+    __syncthreads();
+    if (kMapsOnly) {
+      if (wave == 0 && run == 0) {
+        float2 all = wave_map[0][column];
+        for (int k = 1; k < kWaves; ++k) all = after(all, wave_map[k][column]);
+        total = after(all, total);
+      }
+      __syncthreads();
+      continue;
+    }
+    float a = at + pass >= end ? carry : behind[turn ^ 1][column];
+    for (int k = kWaves - 1; k > wave; --k) a = apply(wave_map[k][column], a);
+    if (wave == 0 && run == 0) behind[turn][column] = apply(map, a);
+    a = apply(later, a);
+#pragma unroll
+    for (int i = kSteps - 1; i >= 0; --i) {
+      if (t0 + i < end) {
+        a = over[i] ? d[i] : __builtin_fmaf(g.decay, a, d[i]);
+        if (ok) {
+          const i64 to = (t0 + i) * g.batch + b;
+          const float mine = sign[i] * a;
+          g.advantage[to] = mine;
+          g.returns[to] = mine + v[i];
+        }
+      }
+    }
+    __syncthreads();  // wave_map and behind[turn ^ 1] are free again
+  }
+  if (kMapsOnly && wave == 0 && run == 0 && ok) g.maps[(i64)chunk * g.batch + b] = total;
+}
+
+// How a call is laid out: the columns of a wavefront, and the chunks the steps are split into
+// so that the launch has about one workgroup a compute unit.
+struct GaeLayout {
+  int columns, chunks;
+  i64 groups, chunk;
+};
+
+inline GaeLayout gae_layout(i64 steps, i64 batch) {
+  GaeLayout l;
+  l.columns = 64;
+  while (l.columns > 1 && l.columns / 2 >= batch) l.columns /= 2;
+  l.groups = (batch + l.columns - 1) / l.columns;
+  const i64 pass = (i64)kWaves * (64 / l.columns) * kSteps;
+  const i64 passes = (steps + pass - 1) / pass;
+  i64 chunks = compute_units() / l.groups;
+  chunks = chunks < 1 ? 1 : chunks < passes ? chunks : passes;
+  const i64 each = (passes + chunks - 1) / chunks;
+  l.chunk = each * pass;
+  l.chunks = (int)((passes + each - 1) / each);
+  return l;
+}
+
+template <class T>
+int launch_gae(const GaeArgs& g, const GaeLayout& l, hipStream_t stream) {
+  const dim3 grid((unsigned)l.groups, (unsigned)l.chunks);
+  if (l.chunks > 1) {
+    gae_kernel<T, true><<<grid, 64 * kWaves, 0, stream>>>(g);
+    const int rc = (int)hipGetLastError();
+    if (rc != 0) return rc;
+  }
+  gae_kernel<T, false><<<grid, 64 * kWaves, 0, stream>>>(g);
+  return (int)hipGetLastError();
+}
+
+}  // namespace gae
+}  // namespace learner
+}  // namespace cugo_amd
+
+using namespace cugo_amd::learner;
+using namespace cugo_amd::learner::gae;
+
+extern "C" {
+
+int64_t cugo_advantages_workspace(int64_t steps, int64_t batch) {
+  if (steps < 1 || batch < 1) return 0;
+  const GaeLayout l = gae_layout(steps, batch);
+  return l.chunks > 1 ? (int64_t)sizeof(float2) * l.chunks * batch : 0;
+}
+
+int cugo_advantages(int value_dtype, const float* reward, const void* value,
+                    const uint8_t* done, const uint8_t* player, const void* bootstrap,
+                    const uint8_t* last_player, int64_t steps, int64_t batch, double gamma,
+                    double lam, float* advantage, float* returns, void* workspace,
+                    int64_t workspace_bytes, hipStream_t stream) {
+  if (steps < 0 || batch < 0 || batch > ((int64_t)1 << 36)) return -1;
+  if (!dtype_known(value_dtype)) return -2;
+  if (steps == 0 || batch == 0) return 0;
+  if (!reward || !value || !done || !bootstrap || !advantage || !returns ||
+      (player != nullptr) != (last_player != nullptr))
+    return -1;
+  const GaeLayout l = gae_layout(steps, batch);
+  if (l.chunks > 1 &&
+      (!workspace || workspace_bytes < (int64_t)sizeof(float2) * l.chunks * batch))
+    return -3;
+  GaeArgs g{};
+  g.reward = reward, g.value = value, g.done = done, g.player = player;
+  g.bootstrap = bootstrap, g.last_player = last_player;
+  g.steps = steps, g.batch = batch, g.chunk = l.chunk, g.chunks = l.chunks;
+  g.columns = l.columns;
+  g.gamma = (float)gamma, g.decay = (float)(gamma * lam);
+  g.advantage = advantage, g.returns = returns, g.maps = static_cast<float2*>(workspace);
+  if (value_dtype == CUGO_DTYPE_F32) return launch_gae<F32>(g, l, stream);
+  if (value_dtype == CUGO_DTYPE_F16) return launch_gae<F16>(g, l, stream);
+  return launch_gae<BF16>(g, l, stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,313 @@
+// The learner's operations of the PyTorch-ROCm extension (policy_loss, scale_gradients,
+// advantages, adamw_step) over the C ABI of libcugo_hip.so.  Like the engine's operations they
+// check their tensors, allocate outputs and scratch with torch, launch on the current stream
+// under the tensors' device and never synchronise.
+#include "ext_common.h"
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+#include <utility>
+
+namespace cugo_ext {
+namespace {
+
+using Optional = c10::optional<torch::Tensor>;
+
+int float_code(const torch::Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kFloat:
+      return CUGO_DTYPE_F32;
+    case at::kHalf:
+      return CUGO_DTYPE_F16;
+    case at::kBFloat16:
+      return CUGO_DTYPE_BF16;
+    default:
+      TORCH_CHECK(false, name, " must be float32, float16 or bfloat16");
+  }
+}
+
+// [n, A] whose rows are runs of memory, like logits' (their distance apart is free).
+void check_rows(const torch::Tensor& t, const torch::Tensor& like, at::ScalarType dtype,
+                const char* name) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK(t.dim() == 2 && t.sizes() == like.sizes() && t.scalar_type() == dtype, name,
+              " must be a ", c10::toString(dtype), " tensor shaped like logits");
+  TORCH_CHECK(t.size(1) == 1 || t.stride(1) == 1, name,
+              " must have its last dimension contiguous");
+  check_same_device(like, t, "logits", name);
+}
+
+void check_entry(const torch::Tensor& t, const torch::Tensor& like, at::ScalarType dtype,
+                 const char* name) {
+  check_1d(t, dtype, name);
+  TORCH_CHECK(t.numel() == like.size(0), name, " must have one entry per row of logits");
+  check_same_device(like, t, "logits", name);
+}
+
+const float* scalar_ptr(const Optional& t, const torch::Tensor& like, const char* name) {
+  if (!t.has_value()) return nullptr;
+  TORCH_CHECK(t->is_cuda() && t->numel() == 1 && t->scalar_type() == at::kFloat, name,
+              " must be a one-element float32 CUDA tensor");
+  check_same_device(like, *t, "input", name);
+  return t->data_ptr<float>();
+}
+
+// -> (out f32 [7]: loss, policy, value, kl, entropy, cut, drift; logp f32 [n]; d_logits or
+// None; d_value or None), cugo_policy_loss.
+std::vector<Optional> policy_loss(torch::Tensor logits, torch::Tensor action,
+                                  torch::Tensor old_logp, torch::Tensor advantage, Optional legal,
+                                  Optional ref_logits, Optional value, Optional returns,
+                                  Optional weight, double clip_low, double clip_high,
+                                  double kl_coef, double entropy_coef, double value_coef,
+                                  Optional scale, bool want_logits, bool want_value) {
+  TORCH_CHECK(logits.is_cuda(), "logits must be a CUDA tensor");
+  TORCH_CHECK(logits.dim() == 2 && logits.size(1) >= 1, "logits must have shape [n, A], A >= 1");
+  TORCH_CHECK(logits.size(1) <= (1 << 30), "at most 2^30 actions");
+  CugoPolicyLoss p{};
+  p.n = logits.size(0);
+  p.actions = logits.size(1);
+  p.logits_dtype = float_code(logits, "logits");
+  check_rows(logits, logits, logits.scalar_type(), "logits");
+  check_entry(action, logits, at::kLong, "action");
+  check_entry(old_logp, logits, at::kFloat, "old_logp");
+  check_entry(advantage, logits, at::kFloat, "advantage");
+  if (legal.has_value()) check_rows(*legal, logits, at::kBool, "legal");
+  if (ref_logits.has_value()) check_rows(*ref_logits, logits, logits.scalar_type(), "ref_logits");
+  TORCH_CHECK(value.has_value() == returns.has_value(), "value and returns go together");
+  if (value.has_value()) {
+    p.value_dtype = float_code(*value, "value");
+    check_entry(*value, logits, value->scalar_type(), "value");
+    check_entry(*returns, logits, at::kFloat, "returns");
+  }
+  if (weight.has_value()) check_entry(*weight, logits, at::kFloat, "weight");
+  TORCH_CHECK(clip_low >= 0 && clip_high >= 0, "the clip's sides must not be negative");
+  TORCH_CHECK(std::isfinite(kl_coef) && std::isfinite(entropy_coef) && std::isfinite(value_coef),
+              "the coefficients must be finite");
+  TORCH_CHECK(!want_value || value.has_value(), "no value to differentiate");
+  const DeviceGuard guard(logits.device());
+  const auto out = torch::empty({7}, on(logits, at::kFloat));
+  const auto logp = torch::empty({p.n}, on(logits, at::kFloat));
+  const auto partials = torch::empty({CUGO_POLICY_LOSS_PARTIALS}, on(logits, at::kDouble));
+  Optional d_logits, d_value;
+  if (want_logits) d_logits = torch::empty({p.n, p.actions}, on(logits, logits.scalar_type()));
+  if (want_value) d_value = torch::empty({p.n}, on(logits, value->scalar_type()));
+  p.logits = logits.data_ptr();
+  p.logits_stride = logits.stride(0);
+  p.action = action.data_ptr<int64_t>();
+  p.old_logp = old_logp.data_ptr<float>();
+  p.advantage = advantage.data_ptr<float>();
+  if (legal.has_value()) p.legal = u8p(*legal), p.legal_stride = legal->stride(0);
+  if (ref_logits.has_value())
+    p.ref_logits = ref_logits->data_ptr(), p.ref_stride = ref_logits->stride(0);
+  if (value.has_value()) p.value = value->data_ptr(), p.returns = returns->data_ptr<float>();
+  if (weight.has_value()) p.weight = weight->data_ptr<float>();
+  p.scale = scalar_ptr(scale, logits, "scale");
+  p.clip_low = clip_low, p.clip_high = clip_high, p.kl_coef = kl_coef;
+  p.entropy_coef = entropy_coef, p.value_coef = value_coef;
+  if (want_logits) p.d_logits = d_logits->data_ptr(), p.d_logits_stride = p.actions;
+  if (want_value) p.d_value = d_value->data_ptr();
+  p.logp = logp.data_ptr<float>();
+  p.out = out.data_ptr<float>();
+  p.partials = partials.data_ptr<double>();
+  check_call(cugo_policy_loss(&p, stream()), "policy_loss");
+  return {out, logp, d_logits, d_value};
+}
+
+// a and b (either may be None) times the one-element float32 factor, in place.
+void scale_gradients(Optional a, Optional b, torch::Tensor factor) {
+  for (const Optional* t : {&a, &b}) {
+    if (!t->has_value()) continue;
+    TORCH_CHECK((*t)->is_cuda() && (*t)->is_contiguous(), "gradients must be contiguous CUDA tensors");
+    check_same_device(factor, **t, "factor", "gradients");
+  }
+  const DeviceGuard guard(factor.device());
+  const float* f = scalar_ptr(factor, factor, "factor");
+  check_call(cugo_scale_gradients(a.has_value() ? float_code(*a, "gradients") : CUGO_DTYPE_F32,
+                                  a.has_value() ? a->data_ptr() : nullptr,
+                                  a.has_value() ? a->numel() : 0,
+                                  b.has_value() ? float_code(*b, "gradients") : CUGO_DTYPE_F32,
+                                  b.has_value() ? b->data_ptr() : nullptr,
+                                  b.has_value() ? b->numel() : 0, f, stream()),
+             "scale_gradients");
+}
+
+// -> (advantage f32 [T, B], returns f32 [T, B]), cugo_advantages.
+std::vector<torch::Tensor> advantages(torch::Tensor reward, torch::Tensor value,
+                                      torch::Tensor done, torch::Tensor bootstrap, double gamma,
+                                      double lam, Optional player, Optional last_player,
+                                      Optional advantage, Optional returns) {
+  TORCH_CHECK(reward.is_cuda() && reward.is_contiguous() && reward.dim() == 2 &&
+                  reward.scalar_type() == at::kFloat,
+              "reward must be a contiguous CUDA float32 [steps, batch] tensor");
+  const int64_t steps = reward.size(0), batch = reward.size(1);
+  const auto check = [&](const torch::Tensor& t, at::IntArrayRef shape, at::ScalarType dtype,
+                         const char* name) {
+    TORCH_CHECK(t.is_contiguous() && t.sizes() == shape && t.scalar_type() == dtype, name,
+                " must be a contiguous ", c10::toString(dtype), " tensor of shape ", shape);
+    check_same_device(reward, t, "reward", name);
+  };
+  const int code = float_code(value, "value");
+  check(value, {steps, batch}, value.scalar_type(), "value");
+  check(done, {steps, batch}, at::kBool, "done");
+  check(bootstrap, {batch}, value.scalar_type(), "bootstrap");
+  TORCH_CHECK(player.has_value() == last_player.has_value(), "player and last_player go together");
+  if (player.has_value()) {
+    check(*player, {steps, batch}, at::kByte, "player");
+    check(*last_player, {batch}, at::kByte, "last_player");
+  }
+  TORCH_CHECK(gamma >= 0 && gamma <= 1 && lam >= 0 && lam <= 1, "gamma and lam must lie in [0, 1]");
+  const DeviceGuard guard(reward.device());
+  auto adv = out_or_new(advantage, {steps, batch}, at::kFloat, reward, "advantage");
+  auto ret = out_or_new(returns, {steps, batch}, at::kFloat, reward, "returns");
+  const int64_t bytes = cugo_advantages_workspace(steps, batch);
+  const auto scratch = torch::empty({bytes}, on(reward, at::kByte));
+  check_call(cugo_advantages(code, reward.data_ptr<float>(), value.data_ptr(), u8p(done),
+                             player.has_value() ? u8p(*player) : nullptr, bootstrap.data_ptr(),
+                             player.has_value() ? u8p(*last_player) : nullptr, steps, batch,
+                             gamma, lam, adv.data_ptr<float>(), ret.data_ptr<float>(),
+                             bytes ? scratch.data_ptr() : nullptr, bytes, stream()),
+             "advantages");
+  return {adv, ret};
+}
+
+// One step of every tensor with a gradient, in place (cugo_adamw); the gradients' norm with
+// max_norm, else None.
+Optional adamw_step(std::vector<torch::Tensor> params, std::vector<Optional> grads,
+                    std::vector<torch::Tensor> exp_avg, std::vector<torch::Tensor> exp_avg_sq,
+                    torch::Tensor steps, std::vector<double> lr, std::vector<double> weight_decay,
+                    double beta1, double beta2, double eps, c10::optional<double> max_norm,
+                    c10::optional<std::vector<Optional>> master,
+                    c10::optional<std::vector<torch::Tensor>> exp_avg_scale,
+                    c10::optional<std::vector<torch::Tensor>> exp_avg_sq_scale,
+                    Optional lr_scale, int64_t seed) {
+  const size_t count = params.size();
+  TORCH_CHECK(count > 0, "no parameters");
+  TORCH_CHECK(grads.size() == count && exp_avg.size() == count && exp_avg_sq.size() == count &&
+                  lr.size() == count && weight_decay.size() == count,
+              "grads, exp_avg, exp_avg_sq, lr and weight_decay must have one entry per parameter");
+  TORCH_CHECK(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1, "betas must lie in [0, 1)");
+  TORCH_CHECK(eps >= 0, "eps must not be negative");
+  TORCH_CHECK(!max_norm.has_value() || *max_norm > 0, "max_norm must be positive");
+  const bool eight = exp_avg_scale.has_value();
+  TORCH_CHECK(exp_avg_sq_scale.has_value() == eight, "both moments have scales, or neither");
+  TORCH_CHECK(!eight || (exp_avg_scale->size() == count && exp_avg_sq_scale->size() == count),
+              "the scales must have one entry per parameter");
+  TORCH_CHECK(!master.has_value() || master->size() == count,
+              "master must have one entry per parameter");
+  const torch::Tensor& first = params[0];
+  TORCH_CHECK(first.is_cuda(), "parameters must be CUDA tensors");
+  check_1d(steps, at::kLong, "steps");
+  TORCH_CHECK((size_t)steps.numel() == count, "steps must have one entry per parameter");
+  check_same_device(first, steps, "parameters", "steps");
+  const auto dense = [&](const torch::Tensor& t, const torch::Tensor& like, at::ScalarType dtype,
+                         const char* name) {
+    TORCH_CHECK(t.is_contiguous() && t.numel() == like.numel() && t.scalar_type() == dtype, name,
+                " must be contiguous ", c10::toString(dtype), " of the parameter's size");
+    check_same_device(first, t, "parameters", name);
+  };
+  std::vector<CugoAdamwTensor> list;
+  std::vector<std::pair<uintptr_t, uintptr_t>> spans;  // what the step writes
+  list.reserve(count);
+  const auto written = [&](const torch::Tensor& t) {
+    const auto at = reinterpret_cast<uintptr_t>(t.data_ptr());
+    if (t.numel() > 0) spans.emplace_back(at, at + t.nbytes());
+  };
+  for (size_t i = 0; i < count; ++i) {
+    const torch::Tensor& w = params[i];
+    CugoAdamwTensor t{};
+    t.param_dtype = (int16_t)float_code(w, "parameters");
+    dense(w, w, w.scalar_type(), "parameters");
+    const Optional m32 = master.has_value() ? (*master)[i] : Optional();
+    const bool wide = w.scalar_type() == at::kFloat;
+    TORCH_CHECK(wide || m32.has_value(), "a 16-bit parameter needs its float32 master");
+    TORCH_CHECK(!wide || !m32.has_value(), "a float32 parameter has no master");
+    if (m32.has_value()) dense(*m32, w, at::kFloat, "master");
+    dense(exp_avg[i], w, eight ? at::kFloat8_e4m3fn : at::kFloat, "exp_avg");
+    dense(exp_avg_sq[i], w, eight ? at::kFloat8_e5m2 : at::kFloat, "exp_avg_sq");
+    if (eight) {
+      const int64_t blocks = (w.numel() + CUGO_ADAMW_BLOCK - 1) / CUGO_ADAMW_BLOCK;
+      for (const auto* s : {&(*exp_avg_scale)[i], &(*exp_avg_sq_scale)[i]}) {
+        check_1d(*s, at::kFloat, "scales");
+        TORCH_CHECK(s->numel() == blocks, "scales must have one entry per block of ",
+                    CUGO_ADAMW_BLOCK, " values");
+        check_same_device(first, *s, "parameters", "scales");
+      }
+    }
+    if (!grads[i].has_value()) continue;  // left as it is
+    const torch::Tensor& g = *grads[i];
+    t.grad_dtype = (int16_t)float_code(g, "gradients");
+    dense(g, w, g.scalar_type(), "gradients");
+    TORCH_CHECK(w.numel() <= (int64_t)1 << 36, "at most 2^36 values a parameter");
+    written(w), written(exp_avg[i]), written(exp_avg_sq[i]);
+    if (m32.has_value()) written(*m32);
+    if (eight) written((*exp_avg_scale)[i]), written((*exp_avg_sq_scale)[i]);
+    t.param = w.data_ptr();
+    t.grad = g.data_ptr();
+    t.master = m32.has_value() ? m32->data_ptr<float>() : nullptr;
+    t.exp_avg = exp_avg[i].data_ptr();
+    t.exp_avg_sq = exp_avg_sq[i].data_ptr();
+    if (eight) {
+      t.exp_avg_scale = (*exp_avg_scale)[i].data_ptr<float>();
+      t.exp_avg_sq_scale = (*exp_avg_sq_scale)[i].data_ptr<float>();
+    }
+    t.step = steps.data_ptr<int64_t>() + i;
+    t.numel = w.numel();
+    t.lr = lr[i], t.weight_decay = weight_decay[i];
+    t.place = (int32_t)i;
+    list.push_back(t);
+  }
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    TORCH_CHECK(spans[i - 1].second <= spans[i].first,
+                "parameters and their states must not overlap in memory");
+  const DeviceGuard guard(first.device());
+  Optional norm;
+  if (max_norm.has_value())
+    norm = list.empty() ? torch::zeros({}, on(first, at::kFloat))
+                        : torch::empty({}, on(first, at::kFloat));
+  const int64_t bytes = cugo_adamw_workspace((int64_t)list.size());
+  const auto scratch = torch::empty({bytes}, on(first, at::kByte));
+  check_call(cugo_adamw(list.data(), (int64_t)list.size(), eight ? 8 : 32, beta1, beta2, eps,
+                        scalar_ptr(lr_scale, first, "lr_scale"), max_norm.value_or(0.0),
+                        (uint64_t)seed, norm.has_value() ? norm->data_ptr<float>() : nullptr,
+                        bytes ? scratch.data_ptr() : nullptr, bytes, stream()),
+             "adamw_step");
+  // what keeps a copy of a parameter by its version (seq_decode's packed weights) sees the change
+  for (size_t i = 0; i < count; ++i)
+    if (grads[i].has_value()) params[i].unsafeGetTensorImpl()->bump_version();
+  return norm;
+}
+
+}  // namespace
+
+void bind_learner(pybind11::module_& m) {
+  namespace py = pybind11;
+  m.attr("ADAMW_BLOCK") = py::int_(CUGO_ADAMW_BLOCK);
+  m.def("policy_loss", &policy_loss,
+        "The clipped policy loss with KL, entropy and value terms, and its gradients",
+        py::arg("logits"), py::arg("action"), py::arg("old_logp"), py::arg("advantage"),
+        py::arg("legal") = py::none(), py::arg("ref_logits") = py::none(),
+        py::arg("value") = py::none(), py::arg("returns") = py::none(),
+        py::arg("weight") = py::none(), py::arg("clip_low") = 0.2, py::arg("clip_high") = 0.2,
+        py::arg("kl_coef") = 0.0, py::arg("entropy_coef") = 0.0, py::arg("value_coef") = 0.5,
+        py::arg("scale") = py::none(), py::arg("want_logits") = false,
+        py::arg("want_value") = false);
+  m.def("scale_gradients", &scale_gradients, "Gradients times a device scalar, in place",
+        py::arg("a"), py::arg("b"), py::arg("factor"));
+  m.def("advantages", &advantages,
+        "Generalised advantage estimation over [steps, batch] of two-player games",
+        py::arg("reward"), py::arg("value"), py::arg("done"), py::arg("bootstrap"),
+        py::arg("gamma"), py::arg("lam"), py::arg("player") = py::none(),
+        py::arg("last_player") = py::none(), py::arg("advantage") = py::none(),
+        py::arg("returns") = py::none());
+  m.def("adamw_step", &adamw_step, "One AdamW step over many tensors, in place",
+        py::arg("params"), py::arg("grads"), py::arg("exp_avg"), py::arg("exp_avg_sq"),
+        py::arg("steps"), py::arg("lr"), py::arg("weight_decay"), py::arg("beta1"),
+        py::arg("beta2"), py::arg("eps"), py::arg("max_norm") = py::none(),
+        py::arg("master") = py::none(), py::arg("exp_avg_scale") = py::none(),
+        py::arg("exp_avg_sq_scale") = py::none(), py::arg("lr_scale") = py::none(),
+        py::arg("seed") = 0);
+}
+
+}  // namespace cugo_ext

@@ -5,27 +5,13 @@
 // messages), allocates the outputs with torch::empty on the states' device, and calls
 // the C ABI on the current HIP stream.  Nothing here synchronises, so the operations
 // can be captured in HIP graphs.
-#include <torch/extension.h>
-
-// PyTorch-ROCm keeps torch's device type "cuda" for HIP devices; these are its native
-// HIP guard and stream accessors for that device type.
-#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include "ext_common.h"
 
 #include <cmath>
-#include <cstdint>
-#include <vector>
-
-#include "../../include/cugo_hip.h"
 
 namespace {
 
-void check_1d(const torch::Tensor& t, at::ScalarType dtype, const char* name) {
-  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
-  TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
-  TORCH_CHECK(t.dim() == 1, name, " must be one-dimensional");
-  TORCH_CHECK(t.scalar_type() == dtype, name, " has the wrong dtype");
-}
+using namespace cugo_ext;
 
 void check_states(const torch::Tensor& s) {
   TORCH_CHECK(s.is_cuda(), "states must be a CUDA tensor");
@@ -37,23 +23,6 @@ void check_states(const torch::Tensor& s) {
               "states must be 8-byte aligned");
 }
 
-void check_same_device(const torch::Tensor& a, const torch::Tensor& b, const char* an,
-                       const char* bn) {
-  TORCH_CHECK(a.device() == b.device(), an, " and ", bn, " must be on the same CUDA device");
-}
-
-void check_call(int rc, const char* op) {
-  TORCH_CHECK(rc == 0, "cugo_hip ", op, " failed with code ", rc);
-}
-
-hipStream_t stream() { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream(); }
-
-using DeviceGuard = c10::hip::HIPGuardMasqueradingAsCUDA;
-
-torch::TensorOptions on(const torch::Tensor& t, at::ScalarType dtype) {
-  return torch::TensorOptions().device(t.device()).dtype(dtype);
-}
-
 std::vector<torch::Tensor> observation_outputs(int64_t n, const torch::Tensor& like) {
   return {torch::empty({n, CUGO_FEATURE_COUNT}, on(like, at::kFloat)),
           torch::empty({n, CUGO_ACTION_COUNT}, on(like, at::kBool)),
@@ -61,25 +30,11 @@ std::vector<torch::Tensor> observation_outputs(int64_t n, const torch::Tensor& l
           torch::empty({n}, on(like, at::kShort))};
 }
 
-// `out` if given (a contiguous tensor of `dtype` and `shape` on like's device: a caller's
-// buffer the kernel writes into), else a new tensor.
-torch::Tensor out_or_new(const c10::optional<torch::Tensor>& out, std::vector<int64_t> shape,
-                         at::ScalarType dtype, const torch::Tensor& like, const char* name) {
-  if (!out.has_value()) return torch::empty(shape, on(like, dtype));
-  TORCH_CHECK(out->is_contiguous() && out->scalar_type() == dtype &&
-                  out->sizes() == at::IntArrayRef(shape),
-              name, " must be a contiguous ", c10::toString(dtype), " tensor of shape ", shape);
-  check_same_device(like, *out, "input", name);
-  return *out;
-}
-
 std::vector<torch::Tensor> step_outputs(int64_t n, const torch::Tensor& like) {
   return {torch::empty({n}, on(like, at::kFloat)), torch::empty({n}, on(like, at::kBool)),
           torch::empty({n}, on(like, at::kBool)), torch::empty({n}, on(like, at::kShort)),
           torch::empty({n}, on(like, at::kBool))};
 }
-
-uint8_t* u8p(const torch::Tensor& t) { return reinterpret_cast<uint8_t*>(t.data_ptr()); }
 
 torch::Tensor create(torch::Tensor seeds, torch::Tensor first) {
   check_1d(seeds, at::kLong, "seeds");
@@ -113,7 +68,8 @@ std::vector<torch::Tensor> observe(torch::Tensor states) {
 // with a sampler, also observe_sample's draw (actions last).
 std::vector<torch::Tensor> observe_bf16(torch::Tensor states, torch::Tensor features,
                                         c10::optional<torch::Tensor> sampler,
-                                        c10::optional<torch::Tensor> legal) {
+                                        c10::optional<torch::Tensor> legal,
+                                        c10::optional<torch::Tensor> player) {
   check_states(states);
   const int64_t n = states.size(0);
   TORCH_CHECK(features.is_contiguous() && features.scalar_type() == at::kBFloat16 &&
@@ -129,7 +85,7 @@ std::vector<torch::Tensor> observe_bf16(torch::Tensor states, torch::Tensor feat
   const DeviceGuard guard(states.device());
   std::vector<torch::Tensor> o{features,
                                out_or_new(legal, {n, CUGO_ACTION_COUNT}, at::kBool, states, "legal"),
-                               torch::empty({n}, on(states, at::kByte)),
+                               out_or_new(player, {n}, at::kByte, states, "player"),
                                torch::empty({n}, on(states, at::kBool)),
                                torch::empty({n}, on(states, at::kShort))};
   if (sampler.has_value()) o.push_back(torch::empty({n}, on(states, at::kLong)));
@@ -538,7 +494,8 @@ std::vector<torch::Tensor> step_observe_spares(torch::Tensor states, torch::Tens
                                                int64_t seed_stride,
                                                c10::optional<torch::Tensor> reward,
                                                c10::optional<torch::Tensor> done,
-                                               c10::optional<torch::Tensor> legal) {
+                                               c10::optional<torch::Tensor> legal,
+                                               c10::optional<torch::Tensor> player) {
   check_states(states);
   check_states(spares);
   const int64_t n = states.size(0);
@@ -566,7 +523,7 @@ std::vector<torch::Tensor> step_observe_spares(torch::Tensor states, torch::Tens
   if (done.has_value()) o[1] = out_or_new(done, {n}, at::kBool, states, "done");
   o.push_back(features);
   o.push_back(out_or_new(legal, {n, CUGO_ACTION_COUNT}, at::kBool, states, "legal"));
-  o.push_back(torch::empty({n}, on(states, at::kByte)));
+  o.push_back(out_or_new(player, {n}, at::kByte, states, "player"));
   o.push_back(torch::empty({n}, on(states, at::kBool)));
   o.push_back(torch::empty({n}, on(states, at::kShort)));
   const bool bf16 = features.scalar_type() == at::kBFloat16;
@@ -1837,7 +1794,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         pybind11::arg("generation"), pybind11::arg("sampler"), pybind11::arg("spares"),
         pybind11::arg("spare_gen"), pybind11::arg("features"), pybind11::arg("seed_stride") = -1,
         pybind11::arg("reward") = pybind11::none(), pybind11::arg("done") = pybind11::none(),
-        pybind11::arg("legal") = pybind11::none());
+        pybind11::arg("legal") = pybind11::none(),
+        pybind11::arg("player") = pybind11::none());
   m.def("gumbel_sample_philox", &gumbel_sample_philox,
         "gumbel_sample with uniforms drawn in the kernel from Philox4x32-10",
         pybind11::arg("logits"), pybind11::arg("legal"), pybind11::arg("seed"),
@@ -1949,7 +1907,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "observe (and observe_sample's draw, given a sampler) with bfloat16 features written "
         "into a given tensor",
         pybind11::arg("states"), pybind11::arg("features"),
-        pybind11::arg("sampler") = pybind11::none(), pybind11::arg("legal") = pybind11::none());
+        pybind11::arg("sampler") = pybind11::none(), pybind11::arg("legal") = pybind11::none(),
+        pybind11::arg("player") = pybind11::none());
   m.def("gumbel_sample", &gumbel_sample, "Masked Gumbel-max action and its log-softmax probability",
         pybind11::arg("logits"), pybind11::arg("legal"), pybind11::arg("uniforms"),
         pybind11::arg("actions") = pybind11::none(), pybind11::arg("logp") = pybind11::none());
@@ -1979,4 +1938,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.attr("START_WORDS") = pybind11::int_(CUGO_START_WORDS);
   m.attr("STATE_BYTES") = pybind11::int_(CUGO_STATE_BYTES);
   m.attr("STATUS_OK") = pybind11::int_(CUGO_STATUS_OK);
+  cugo_ext::bind_learner(m);
 }

@@ -165,9 +165,9 @@ def mlp_forward(ext, packed: PackedActor, x: torch.Tensor,
 
 @dataclass
 class RolloutBuffer:
-    """`horizon` steps of B games: the actor's bf16 input, the legal mask, the sampled
-    action and its log-probability, the value estimate, and the step's reward for seat 0
-    (non-zero only when the game settles) and done flag."""
+    """`horizon` steps of B games: the actor's bf16 input, the legal mask, the player to
+    move, the sampled action and its log-probability, the value estimate, and the step's
+    reward for seat 0 (non-zero only when the game settles) and done flag."""
 
     features: torch.Tensor  # bf16 [H, B, 720]
     legal: torch.Tensor     # bool [H, B, 179]
@@ -176,6 +176,7 @@ class RolloutBuffer:
     value: torch.Tensor     # f32 [H, B]
     reward: torch.Tensor    # f32 [H, B]
     done: torch.Tensor      # bool [H, B]
+    player: torch.Tensor    # uint8 [H, B]
 
     @classmethod
     def empty(cls, horizon: int, batch: int, device) -> "RolloutBuffer":
@@ -183,7 +184,7 @@ class RolloutBuffer:
             return torch.empty((horizon, batch, *shape), dtype=dtype, device=device)
         return cls(e(720, dtype=torch.bfloat16), e(179, dtype=torch.bool), e(dtype=torch.int64),
                    e(dtype=torch.float32), e(dtype=torch.float32), e(dtype=torch.float32),
-                   e(dtype=torch.bool))
+                   e(dtype=torch.bool), e(dtype=torch.uint8))
 
 
 class MlpRollout:
@@ -231,9 +232,11 @@ class MlpRollout:
             self.ext.refill_spares(self.spares, self.spare_gen, self.generation, self.base)
         if self.fused_kernel:  # features and mask straight into the buffer's row t
             self.observation = self.ext.observe_bf16(self.states, self.buffer.features[t],
-                                                     legal=self.buffer.legal[t])
+                                                     legal=self.buffer.legal[t],
+                                                     player=self.buffer.player[t])
         else:
             self.observation = self.ext.observe(self.states)
+            self.buffer.player[t].copy_(self.observation[2])
         return self.observation
 
     def act(self, t: int):
@@ -259,6 +262,7 @@ class MlpRollout:
                                           actions=buf.action[t], logp=buf.logp[t])
         return buf.action[t]
 
+    @torch.no_grad()
     def repack(self) -> None:
         """Re-reads the actor's parameters after they changed (the one-launch forward reads
         a packed copy; a captured graph reads the same tensors, updated in place)."""
@@ -284,14 +288,14 @@ class MlpRollout:
     def step_observe(self, t: int, action: torch.Tensor):
         """step(t, action), then step t + 1's observation of the new states, in one launch
         (`step_observe_spares`): the reward and done flag go into the buffer's row t, the
-        bf16 features and mask into row t + 1."""
+        bf16 features, mask and player into row t + 1."""
         if (t + 1) % REFILL == 0:
             self.ext.refill_spares(self.spares, self.spare_gen, self.generation, self.base)
         buf = self.buffer
         out = self.ext.step_observe_spares(
             self.states, action, self.base, self.generation, self.sampler, self.spares,
             self.spare_gen, buf.features[t + 1], reward=buf.reward[t], done=buf.done[t],
-            legal=buf.legal[t + 1])
+            legal=buf.legal[t + 1], player=buf.player[t + 1])
         self.step_out, self.observation = out[:5], out[5:]
         return self.step_out
 

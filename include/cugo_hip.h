@@ -669,6 +669,119 @@ int cugo_selfplay_advance(const CugoSelfPlayWave* wave, const uint8_t* done,
                           const int64_t* events, const int64_t* actions, const float* logp,
                           hipStream_t stream);
 
+/*
+ * The learner's operators (no counterpart in the reference extension; the reference's PPO
+ * update, python/cugo_ppo50.py:514-739, does their work in torch operations).
+ *
+ * cugo_policy_loss: over n rows of `actions` logits (row stride logits_stride elements, one
+ * after another within a row), with legal bool [n, A] (NULL: every action), the action taken
+ * int64, its log-probability then, the advantage A and the weight w (NULL: 1 / n each), l the
+ * log-softmax over the row's legal actions, r = e^(l_a - old_logp), l' the log-softmax of
+ * ref_logits (NULL: none) over the same actions:
+ *   out[1] = sum w (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A))
+ *   out[2] = sum w (value - returns)^2 / 2             (value NULL: 0)
+ *   out[3] = sum w sum_j p_j (l_j - l'_j)              (ref_logits NULL: 0)
+ *   out[4] = sum w (-sum_j p_j l_j)
+ *   out[5] = sum w [the clip cut the ratio off]
+ *   out[6] = sum w (r - 1 - (l_a - old_logp))
+ *   out[0] = scale (out[1] + value_coef out[2] + kl_coef out[3] - entropy_coef out[4])
+ * and logp[i] = l_a; d_logits [n, A] and d_value [n] (NULL: not wanted) receive the gradients
+ * of out[0], in the logits' and the value's type.  scale: one float of device memory, or NULL
+ * for 1.  A row of weight 0 counts nowhere and has zero gradients, whatever else it holds.  A
+ * row without a legal action (or with none above -inf) has only the value term, and logp 0.
+ * An action that is illegal, outside [0, A) or at -inf has log-probability -inf and ratio 0.
+ * partials: CUGO_POLICY_LOSS_PARTIALS doubles of scratch, in use until the call's launches
+ * end.  The sums' order is fixed.  dtypes: CUGO_DTYPE_F32, _F16 or _BF16. */
+#define CUGO_POLICY_LOSS_PARTIALS 24576
+typedef struct CugoPolicyLoss {
+  int64_t n, actions;
+  int logits_dtype, value_dtype;
+  const void* logits;
+  const void* ref_logits;
+  const uint8_t* legal;
+  int64_t logits_stride, ref_stride, legal_stride;
+  const int64_t* action;
+  const float* old_logp;
+  const float* advantage;
+  const float* weight;
+  const void* value;
+  const float* returns;
+  const float* scale;
+  double clip_low, clip_high, kl_coef, entropy_coef, value_coef;
+  void* d_logits;
+  int64_t d_logits_stride;
+  void* d_value;
+  float* logp;
+  float* out;
+  double* partials;
+} CugoPolicyLoss;
+int cugo_policy_loss(const CugoPolicyLoss* loss, hipStream_t stream);
+
+/* cugo_scale_gradients: a_count values of a and b_count values of b times *factor (device
+ * memory), in place, each rounded to its type; a factor of 1 leaves them unread. */
+int cugo_scale_gradients(int a_dtype, void* a, int64_t a_count, int b_dtype, void* b,
+                         int64_t b_count, const float* factor, hipStream_t stream);
+
+/* cugo_advantages: generalised advantage estimation over [steps, batch] rows (one step's games
+ * one after another) of games between two players.  reward is player 0's, value (value_dtype)
+ * the mover's estimate, player the mover (0 or 1; NULL: always 0), done ends a game with the
+ * step; bootstrap [batch] and last_player [batch] (NULL with player) belong to the state after
+ * the last step.  With s = 1 for player 0 and -1 for player 1,
+ *   d_t = reward_t + [not done_t] gamma s_(t+1) value_(t+1) - s_t value_t
+ *   a_t = d_t + [not done_t] gamma lam a_(t+1)
+ *   advantage_t = s_t a_t, returns_t = advantage_t + value_t           (float32)
+ * What follows a done step is not read into it.  workspace: at least
+ * cugo_advantages_workspace(steps, batch) bytes (may be 0: then it may be NULL), in use until
+ * the call's launches end. */
+int64_t cugo_advantages_workspace(int64_t steps, int64_t batch);
+int cugo_advantages(int value_dtype, const float* reward, const void* value,
+                    const uint8_t* done, const uint8_t* player, const void* bootstrap,
+                    const uint8_t* last_player, int64_t steps, int64_t batch, double gamma,
+                    double lam, float* advantage, float* returns, void* workspace,
+                    int64_t workspace_bytes, hipStream_t stream);
+
+/* One tensor of an AdamW step: numel values of param (param_dtype) with the gradient grad
+ * (grad_dtype), one after another in memory.  master: the float32 values that param is rounded
+ * from, required unless param is float32 (then NULL).  exp_avg and exp_avg_sq: float32, or with
+ * bits = 8 the codes (OCP e4m3 and e5m2) of the value over the scale of its block of
+ * CUGO_ADAMW_BLOCK values, counted from the tensor's start.  step: how many steps were taken,
+ * raised by this one.  place: the tensor's place in the caller's list (the rounding's key). */
+#define CUGO_ADAMW_BLOCK 256
+typedef struct CugoAdamwTensor {
+  void* param;
+  const void* grad;
+  float* master;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* exp_avg_scale;    /* [ceil(numel / CUGO_ADAMW_BLOCK)], bits = 8 only */
+  float* exp_avg_sq_scale; /* [ceil(numel / CUGO_ADAMW_BLOCK)], bits = 8 only */
+  int64_t* step;
+  int64_t numel;
+  double lr, weight_decay;
+  int32_t place;
+  int16_t param_dtype, grad_dtype;
+} CugoAdamwTensor;
+
+/* cugo_adamw: one step of every tensor, with g = grad c, t = ++*step:
+ *   c = 1, or with max_norm > 0: min(1, max_norm / (norm + 1e-6)), norm the 2-norm of all
+ *       gradients of the call (to *norm_out, if not NULL)
+ *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   w = (1 - lr weight_decay) w - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)
+ * in float32 with the factors formed in 64 bits; lr_scale (one float of device memory, or
+ * NULL) multiplies every lr.  With bits = 8 the moments are rounded to their codes
+ * stochastically: the 32-bit word of value i of the tensor at `place` at step t is
+ *   mix(low(i) ^ key), key = mix(mix(mix(k + place) + low(t)) + high(i) K),  (K: kPlaceStep of adamw.hip)
+ *   k = mix(low(seed) ^ mix(high(seed) + 1))
+ * (mix: see mix32 in adamw.hip), whose upper bits round m and whose lower 16 round v; the
+ * scale is the block's largest |value|, at least 2^-100, over 256 for m and 32768 for v; a v
+ * above 0 stays above 0; a block with a NaN or an infinity gets the scale NaN.
+ * No tensor may overlap another.  workspace: at least cugo_adamw_workspace(count) bytes, in
+ * use until the call's launches end. */
+int64_t cugo_adamw_workspace(int64_t count);
+int cugo_adamw(const CugoAdamwTensor* tensors, int64_t count, int bits, double beta1,
+               double beta2, double eps, const float* lr_scale, double max_norm, uint64_t seed,
+               float* norm_out, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

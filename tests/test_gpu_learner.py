@@ -1,0 +1,118 @@
+"""The learner's operators together, as PpoLearner runs them on a rollout."""
+
+from __future__ import annotations
+
+import copy
+
+import pytest
+import torch
+
+from oracle import learner_ref as ref
+from tests.conftest import announce
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+SEED_BASE = 0x243F6A8885A308D3
+
+
+def _rollout(ext, width=512, batch=64, horizon=8):
+    from cugo_amd.rollout import MlpRollout, ResidualMlpActor
+
+    torch.manual_seed(1)
+    actor = ResidualMlpActor(width, 2).to(DEV, torch.bfloat16)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    return MlpRollout(ext, actor, batch, horizon, SEED_BASE, g)
+
+
+@pytest.mark.parametrize("width", [512, 256])
+def test_rollout_records_the_player(ext, width):
+    """The buffer's player column is observe's player of each step's state."""
+    ro = _rollout(ext, width)
+    seen = []
+    act = ro.act
+
+    def watch(t):
+        seen.append(ext.observe(ro.states)[2].clone())
+        return act(t)
+
+    ro.act = watch
+    buf = ro.collect()
+    assert torch.equal(buf.player, torch.stack(seen))
+    assert set(buf.player.unique().tolist()) == {0, 1}
+
+
+@pytest.mark.parametrize("width", [512, 256])
+def test_one_update_step_by_step(ext, width):
+    """update() over one minibatch of everything: the estimate, the loss, its gradients through
+    the actor and the step, each against the oracle on what the one before it gave."""
+    from cugo_amd import learner
+
+    announce(f"one update {width}")
+    ro = _rollout(ext, width)
+    buf = ro.collect()
+    lrn = learner.PpoLearner(ro, lr=1e-3, minibatch=1 << 20, kl_coef=0.2, gamma=0.99)
+    adv, ret = lrn.estimate()
+    features, legal, player, _, _ = ext.observe(ro.states)
+    with torch.no_grad():
+        value = lrn._value(features.bfloat16())
+    want = ref.advantages(buf.reward, buf.value, buf.done, value, 0.99, 0.95, buf.player, player)
+    assert (adv.cpu() - want[0]).abs().max() < 1e-4 * (1 + want[0].abs().max())
+    assert (ret.cpu() - want[1]).abs().max() < 1e-4 * (1 + want[1].abs().max())
+    before = copy.deepcopy(ro.actor)
+    stats = lrn.update(torch.Generator(device=DEV).manual_seed(3))
+    # the same update by hand: torch's backward of the oracle's gradients, the oracle's AdamW
+    n = adv.numel()
+    flat = (adv - adv.mean()) / (adv.std(correction=0) + 1e-8)
+    order = torch.randperm(n, generator=torch.Generator(device=DEV).manual_seed(3), device=DEV)
+    pick = lambda t: t.flatten(0, 1)[order]  # noqa: E731
+    x = pick(buf.features)
+    logits, v = before(x)
+    with torch.no_grad():
+        ref_logits = before(x)[0]
+    got = ref.policy_loss(logits.detach(), pick(buf.action), pick(buf.logp), pick(flat),
+                          pick(buf.legal), ref_logits, v.detach(), pick(ret), None, (0.2, 0.2),
+                          0.2, 0.01, 0.5)
+    assert abs(stats[0].cpu() - got["loss"]) < 1e-4 * (1 + abs(got["loss"]))
+    assert (stats[1:].cpu() - got["stats"]).abs().max() < 1e-4 * (1 + got["stats"].abs().max())
+    torch.autograd.backward([logits, v], [got["d_logits"].to(DEV, torch.bfloat16),
+                                          got["d_value"].to(DEV, torch.bfloat16)])
+    grads = [p.grad for p in before.parameters()]
+    norm = torch.cat([g.double().flatten() for g in grads]).norm().cpu()
+    # the two backward passes differ where a gradient of the logits is a bf16 step away, which
+    # the norm shows at a step's size at most
+    assert abs(lrn.optimizer.grad_norm.cpu() - norm) < 2.0**-7 * norm
+    clip = min(1.0, 1.0 / (float(lrn.optimizer.grad_norm) + 1e-6))
+    for p, q in zip(ro.actor.parameters(), before.parameters()):
+        zero = torch.zeros(p.shape)
+        w, _, _ = ref.adamw(q.detach(), p.grad, zero, zero, 1, 1e-3, (0.9, 0.999), 1e-8, 0.01, clip)
+        master = lrn.optimizer.state[p]["master"]
+        assert (master.cpu() - w).abs().max() < 1e-6
+        assert torch.equal(p, master.bfloat16())
+
+
+def test_the_next_rollout_plays_the_new_weights(ext):
+    """Updates between captured horizons: the packed weights are the actor's, the replay's records
+    come from them, and nothing in the games goes wrong."""
+    from cugo_amd import learner
+    from cugo_amd.rollout import mlp_forward, pack_actor
+
+    announce("updates between replays")
+    ro = _rollout(ext, 512, 256, 16)
+    ro.capture()
+    lrn = learner.PpoLearner(ro, lr=1e-3, minibatch=1000, epochs=2, state_bits=8, gamma=0.99)
+    for k in range(3):
+        buf = ro.replay()
+        fresh = pack_actor(ext, ro.actor)
+        logits, value = mlp_forward(ext, fresh, buf.features[3])
+        assert torch.equal(buf.value[3], value)
+        ell = logits.float().masked_fill(~buf.legal[3], -1e30).log_softmax(1)
+        want = ell.gather(1, buf.action[3][:, None])[:, 0]
+        assert (buf.logp[3] - want).abs().max() < 1e-4
+        was = [p.detach().clone() for p in ro.actor.parameters()]
+        stats = lrn.update()
+        assert torch.isfinite(stats).all()
+        moved = [not torch.equal(p, q) for p, q in zip(ro.actor.parameters(), was)]
+        assert all(moved)
+    steps = {int(lrn.optimizer.state[p]["step"]) for p in ro.actor.parameters()}
+    assert steps == {3 * 2 * -(-256 * 16 // 1000)}
