@@ -1,4 +1,4 @@
-// The learner's operations of the PyTorch-ROCm extension (policy_loss, scale_gradients,
+// The learner's operations of the PyTorch-ROCm extension (policy_loss,
 // advantages, adamw_step) over the C ABI of libcugo_hip.so.  Like the engine's operations they
 // check their tensors, allocate outputs and scratch with torch, launch on the current stream
 // under the tensors' device and never synchronise.
@@ -53,21 +53,103 @@ const float* scalar_ptr(const Optional& t, const torch::Tensor& like, const char
   return t->data_ptr<float>();
 }
 
-// -> (out f32 [7]: loss, policy, value, kl, entropy, cut, drift; logp f32 [n]; d_logits or
-// None; d_value or None), cugo_policy_loss.
-std::vector<Optional> policy_loss(torch::Tensor logits, torch::Tensor action,
-                                  torch::Tensor old_logp, torch::Tensor advantage, Optional legal,
-                                  Optional ref_logits, Optional value, Optional returns,
-                                  Optional weight, double clip_low, double clip_high,
-                                  double kl_coef, double entropy_coef, double value_coef,
-                                  Optional scale, bool want_logits, bool want_value) {
+// The tensors of a loss that are not differentiated, and its numbers.
+struct LossInputs {
+  torch::Tensor action, old_logp, advantage;
+  Optional legal, ref_logits, returns, weight, scale;
+  double clip_low, clip_high, kl_coef, entropy_coef, value_coef;
+  bool want_logits, want_value;
+};
+
+// The loss as an operation of autograd: the forward pass has the gradients already
+// (cugo_policy_loss), the backward pass hands them on, times the loss's own gradient.  They are
+// given away, not kept: a second backward pass would find them scaled or accumulated into.
+struct PolicyLossFn : public torch::autograd::Function<PolicyLossFn> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx,
+                                                torch::Tensor logits, Optional value,
+                                                const LossInputs* in) {
+    CugoPolicyLoss p{};
+    p.n = logits.size(0);
+    p.actions = logits.size(1);
+    p.logits_dtype = float_code(logits, "logits");
+    const auto out = torch::empty({7}, on(logits, at::kFloat));
+    const auto logp = torch::empty({p.n}, on(logits, at::kFloat));
+    const auto partials = torch::empty({CUGO_POLICY_LOSS_PARTIALS}, on(logits, at::kDouble));
+    p.logits = logits.data_ptr();
+    p.logits_stride = logits.stride(0);
+    p.action = in->action.data_ptr<int64_t>();
+    p.old_logp = in->old_logp.data_ptr<float>();
+    p.advantage = in->advantage.data_ptr<float>();
+    if (in->legal.has_value()) p.legal = u8p(*in->legal), p.legal_stride = in->legal->stride(0);
+    if (in->ref_logits.has_value())
+      p.ref_logits = in->ref_logits->data_ptr(), p.ref_stride = in->ref_logits->stride(0);
+    if (value.has_value()) {
+      p.value_dtype = float_code(*value, "value");
+      p.value = value->data_ptr(), p.returns = in->returns->data_ptr<float>();
+    }
+    if (in->weight.has_value()) p.weight = in->weight->data_ptr<float>();
+    p.scale = scalar_ptr(in->scale, logits, "scale");
+    p.clip_low = in->clip_low, p.clip_high = in->clip_high, p.kl_coef = in->kl_coef;
+    p.entropy_coef = in->entropy_coef, p.value_coef = in->value_coef;
+    if (in->want_logits) {
+      const auto d = torch::empty({p.n, p.actions}, on(logits, logits.scalar_type()));
+      p.d_logits = d.data_ptr(), p.d_logits_stride = p.actions;
+      ctx->saved_data["d_logits"] = d;
+    }
+    if (in->want_value) {
+      const auto d = torch::empty({p.n}, on(logits, value->scalar_type()));
+      p.d_value = d.data_ptr();
+      ctx->saved_data["d_value"] = d;
+    }
+    p.logp = logp.data_ptr<float>();
+    p.out = out.data_ptr<float>();
+    p.partials = partials.data_ptr<double>();
+    check_call(cugo_policy_loss(&p, stream()), "policy_loss");
+    auto loss = out.select(0, 0), stats = out.narrow(0, 1, 6);
+    ctx->mark_non_differentiable({stats, logp});
+    ctx->set_materialize_grads(false);
+    return {loss, stats, logp};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "policy_loss can be differentiated once");
+    TORCH_CHECK(!ctx->saved_data.empty(),
+                "policy_loss hands its gradients out once; compute the loss again for a second "
+                "backward pass");
+    const auto take = [&](const char* name) {
+      const auto at = ctx->saved_data.find(name);
+      return at == ctx->saved_data.end() ? torch::Tensor() : at->second.toTensor();
+    };
+    const torch::Tensor d_logits = take("d_logits"), d_value = take("d_value");
+    ctx->saved_data.clear();
+    if (!grads[0].defined()) return {torch::Tensor(), torch::Tensor(), torch::Tensor()};
+    const DeviceGuard guard(grads[0].device());
+    const auto code = [](const torch::Tensor& t) {
+      return t.defined() ? float_code(t, "gradients") : CUGO_DTYPE_F32;
+    };
+    const auto pointer = [](const torch::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    const auto size = [](const torch::Tensor& t) { return t.defined() ? t.numel() : 0; };
+    check_call(cugo_scale_gradients(code(d_logits), pointer(d_logits), size(d_logits),
+                                    code(d_value), pointer(d_value), size(d_value),
+                                    grads[0].data_ptr<float>(), stream()),
+               "scale_gradients");
+    return {d_logits, d_value, torch::Tensor()};
+  }
+};
+
+// -> (loss f32 scalar, differentiable in logits and value; stats f32 [6]: policy, value, kl,
+// entropy, cut, drift; logp f32 [n]), cugo_policy_loss.
+std::vector<torch::Tensor> policy_loss(torch::Tensor logits, torch::Tensor action,
+                                       torch::Tensor old_logp, torch::Tensor advantage,
+                                       Optional legal, Optional ref_logits, Optional value,
+                                       Optional returns, Optional weight, double clip_low,
+                                       double clip_high, double kl_coef, double entropy_coef,
+                                       double value_coef, Optional scale) {
   TORCH_CHECK(logits.is_cuda(), "logits must be a CUDA tensor");
   TORCH_CHECK(logits.dim() == 2 && logits.size(1) >= 1, "logits must have shape [n, A], A >= 1");
   TORCH_CHECK(logits.size(1) <= (1 << 30), "at most 2^30 actions");
-  CugoPolicyLoss p{};
-  p.n = logits.size(0);
-  p.actions = logits.size(1);
-  p.logits_dtype = float_code(logits, "logits");
+  float_code(logits, "logits");
   check_rows(logits, logits, logits.scalar_type(), "logits");
   check_entry(action, logits, at::kLong, "action");
   check_entry(old_logp, logits, at::kFloat, "old_logp");
@@ -76,7 +158,7 @@ std::vector<Optional> policy_loss(torch::Tensor logits, torch::Tensor action,
   if (ref_logits.has_value()) check_rows(*ref_logits, logits, logits.scalar_type(), "ref_logits");
   TORCH_CHECK(value.has_value() == returns.has_value(), "value and returns go together");
   if (value.has_value()) {
-    p.value_dtype = float_code(*value, "value");
+    float_code(*value, "value");
     check_entry(*value, logits, value->scalar_type(), "value");
     check_entry(*returns, logits, at::kFloat, "returns");
   }
@@ -84,52 +166,14 @@ std::vector<Optional> policy_loss(torch::Tensor logits, torch::Tensor action,
   TORCH_CHECK(clip_low >= 0 && clip_high >= 0, "the clip's sides must not be negative");
   TORCH_CHECK(std::isfinite(kl_coef) && std::isfinite(entropy_coef) && std::isfinite(value_coef),
               "the coefficients must be finite");
-  TORCH_CHECK(!want_value || value.has_value(), "no value to differentiate");
+  scalar_ptr(scale, logits, "scale");
   const DeviceGuard guard(logits.device());
-  const auto out = torch::empty({7}, on(logits, at::kFloat));
-  const auto logp = torch::empty({p.n}, on(logits, at::kFloat));
-  const auto partials = torch::empty({CUGO_POLICY_LOSS_PARTIALS}, on(logits, at::kDouble));
-  Optional d_logits, d_value;
-  if (want_logits) d_logits = torch::empty({p.n, p.actions}, on(logits, logits.scalar_type()));
-  if (want_value) d_value = torch::empty({p.n}, on(logits, value->scalar_type()));
-  p.logits = logits.data_ptr();
-  p.logits_stride = logits.stride(0);
-  p.action = action.data_ptr<int64_t>();
-  p.old_logp = old_logp.data_ptr<float>();
-  p.advantage = advantage.data_ptr<float>();
-  if (legal.has_value()) p.legal = u8p(*legal), p.legal_stride = legal->stride(0);
-  if (ref_logits.has_value())
-    p.ref_logits = ref_logits->data_ptr(), p.ref_stride = ref_logits->stride(0);
-  if (value.has_value()) p.value = value->data_ptr(), p.returns = returns->data_ptr<float>();
-  if (weight.has_value()) p.weight = weight->data_ptr<float>();
-  p.scale = scalar_ptr(scale, logits, "scale");
-  p.clip_low = clip_low, p.clip_high = clip_high, p.kl_coef = kl_coef;
-  p.entropy_coef = entropy_coef, p.value_coef = value_coef;
-  if (want_logits) p.d_logits = d_logits->data_ptr(), p.d_logits_stride = p.actions;
-  if (want_value) p.d_value = d_value->data_ptr();
-  p.logp = logp.data_ptr<float>();
-  p.out = out.data_ptr<float>();
-  p.partials = partials.data_ptr<double>();
-  check_call(cugo_policy_loss(&p, stream()), "policy_loss");
-  return {out, logp, d_logits, d_value};
-}
-
-// a and b (either may be None) times the one-element float32 factor, in place.
-void scale_gradients(Optional a, Optional b, torch::Tensor factor) {
-  for (const Optional* t : {&a, &b}) {
-    if (!t->has_value()) continue;
-    TORCH_CHECK((*t)->is_cuda() && (*t)->is_contiguous(), "gradients must be contiguous CUDA tensors");
-    check_same_device(factor, **t, "factor", "gradients");
-  }
-  const DeviceGuard guard(factor.device());
-  const float* f = scalar_ptr(factor, factor, "factor");
-  check_call(cugo_scale_gradients(a.has_value() ? float_code(*a, "gradients") : CUGO_DTYPE_F32,
-                                  a.has_value() ? a->data_ptr() : nullptr,
-                                  a.has_value() ? a->numel() : 0,
-                                  b.has_value() ? float_code(*b, "gradients") : CUGO_DTYPE_F32,
-                                  b.has_value() ? b->data_ptr() : nullptr,
-                                  b.has_value() ? b->numel() : 0, f, stream()),
-             "scale_gradients");
+  const bool grad = at::GradMode::is_enabled();
+  const LossInputs in{action,   old_logp,  advantage, legal,   ref_logits,   returns,    weight,
+                      scale,    clip_low,  clip_high, kl_coef, entropy_coef, value_coef,
+                      grad && logits.requires_grad(),
+                      grad && value.has_value() && value->requires_grad()};
+  return PolicyLossFn::apply(logits, value, &in);
 }
 
 // -> (advantage f32 [T, B], returns f32 [T, B]), cugo_advantages.
@@ -285,16 +329,13 @@ void bind_learner(pybind11::module_& m) {
   namespace py = pybind11;
   m.attr("ADAMW_BLOCK") = py::int_(CUGO_ADAMW_BLOCK);
   m.def("policy_loss", &policy_loss,
-        "The clipped policy loss with KL, entropy and value terms, and its gradients",
+        "The clipped policy loss with KL, entropy and value terms: (loss, stats, logp)",
         py::arg("logits"), py::arg("action"), py::arg("old_logp"), py::arg("advantage"),
         py::arg("legal") = py::none(), py::arg("ref_logits") = py::none(),
         py::arg("value") = py::none(), py::arg("returns") = py::none(),
         py::arg("weight") = py::none(), py::arg("clip_low") = 0.2, py::arg("clip_high") = 0.2,
         py::arg("kl_coef") = 0.0, py::arg("entropy_coef") = 0.0, py::arg("value_coef") = 0.5,
-        py::arg("scale") = py::none(), py::arg("want_logits") = false,
-        py::arg("want_value") = false);
-  m.def("scale_gradients", &scale_gradients, "Gradients times a device scalar, in place",
-        py::arg("a"), py::arg("b"), py::arg("factor"));
+        py::arg("scale") = py::none());
   m.def("advantages", &advantages,
         "Generalised advantage estimation over [steps, batch] of two-player games",
         py::arg("reward"), py::arg("value"), py::arg("done"), py::arg("bootstrap"),

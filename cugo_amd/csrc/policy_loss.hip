@@ -399,23 +399,38 @@ __global__ __launch_bounds__(kThreads) void loss_wide_kernel(const LossArgs g) {
   if (threadIdx.x < kStats) g.partials[(i64)blockIdx.x * kStats + threadIdx.x] = acc;
 }
 
-// The workgroups' sums added up, a wavefront for each, and the loss of them.
-__global__ __launch_bounds__(64 * kStats) void loss_total_kernel(
+// The workgroups' sums added up, and the loss of them.  One workgroup of kTotalThreads (a
+// multiple of kStats, so that a thread's loads are of one sum, and the whole grid's partials are
+// a few loads in flight for each thread): 3 us behind 2,048 workgroups, where a wavefront for each
+// sum took 10.
+constexpr int kTotalThreads = 960;
+static_assert(kTotalThreads % kStats == 0 && kTotalThreads % 64 == 0, "one sum a thread");
+__global__ __launch_bounds__(kTotalThreads) void loss_total_kernel(
     const double* partials, int groups, double kl_coef, double entropy_coef, double value_coef,
     const float* scale, float* out) {
-  __shared__ double sums[kStats];
-  const int k = threadIdx.x / 64, lane = threadIdx.x % 64;
+  constexpr int kEach = kTotalThreads / kStats;  // threads a sum
+  __shared__ double sums[kTotalThreads];
+  __shared__ double totals[kStats];
+  const int count = groups * kStats;
   double total = 0.0;
-  for (int i = lane; i < groups; i += 64) total += partials[(i64)i * kStats + k];
-  for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off);
-  if (lane == 0) {
-    sums[k] = total;
-    out[1 + k] = (float)total;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < count; i += kTotalThreads) total += partials[i];
+  sums[threadIdx.x] = total;
+  __syncthreads();
+  const int k = threadIdx.x / 64, lane = threadIdx.x % 64;
+  if (k < kStats) {
+    total = 0.0;
+    for (int i = lane; i < kEach; i += 64) total += sums[i * kStats + k];
+    for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off);
+    if (lane == 0) {
+      totals[k] = total;
+      out[1 + k] = (float)total;
+    }
   }
   __syncthreads();
   if (threadIdx.x == 0) {
-    const double loss = sums[0] + value_coef * sums[1] + kl_coef * sums[2] -
-                        entropy_coef * sums[3];
+    const double loss = totals[0] + value_coef * totals[1] + kl_coef * totals[2] -
+                        entropy_coef * totals[3];
     out[0] = (float)(loss * (scale ? (double)*scale : 1.0));
   }
 }
@@ -512,7 +527,7 @@ int cugo_policy_loss(const CugoPolicyLoss* p, hipStream_t stream) {
     const int rc = (int)hipGetLastError();
     if (rc != 0) return rc;
   }
-  loss_total_kernel<<<1, 64 * kStats, 0, stream>>>(p->partials, groups, p->kl_coef,
+  loss_total_kernel<<<1, kTotalThreads, 0, stream>>>(p->partials, groups, p->kl_coef,
                                                    p->entropy_coef, p->value_coef, p->scale,
                                                    p->out);
   return (int)hipGetLastError();

@@ -21,7 +21,6 @@ from __future__ import annotations
 from typing import NamedTuple, Sequence
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .rollout import MlpRollout, fused_forward, mlp_forward
 
@@ -40,31 +39,6 @@ class PolicyLoss(NamedTuple):
     loss: torch.Tensor
     stats: torch.Tensor
     logp: torch.Tensor
-
-
-class _PolicyLossFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, ext, logits, value, wants, kwargs):
-        out, logp, d_logits, d_value = ext.policy_loss(
-            logits, value=value, want_logits=wants[0], want_value=wants[1], **kwargs)
-        ctx.ext, ctx.grads, ctx.used = ext, (d_logits, d_value), False
-        loss, stats = out[0], out[1:]
-        ctx.mark_non_differentiable(stats, logp)
-        ctx.set_materialize_grads(False)
-        return loss, stats, logp
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, d_loss, _d_stats, _d_logp):
-        if ctx.used:
-            raise RuntimeError("policy_loss: the gradients are handed out once; compute the "
-                               "loss again for a second backward pass")
-        ctx.used = True
-        (d_logits, d_value), ctx.grads = ctx.grads, None
-        if d_loss is None:
-            return None, None, None, None, None
-        ctx.ext.scale_gradients(d_logits, d_value, d_loss)
-        return None, d_logits, d_value, None, None
 
 
 def policy_loss(ext, logits: torch.Tensor, action: torch.Tensor, old_logp: torch.Tensor,
@@ -94,15 +68,9 @@ def policy_loss(ext, logits: torch.Tensor, action: torch.Tensor, old_logp: torch
     gradients before they are rounded, as float16 gradients need: call `backward()` on the
     scaled loss directly.  The gradients are handed out by one backward pass; a second pass
     through the same loss raises."""
-    grad = torch.is_grad_enabled()
-    wants = (grad and logits.requires_grad,
-             grad and value is not None and value.requires_grad)
-    kwargs = dict(action=action, old_logp=old_logp, advantage=advantage, legal=legal,
-                  ref_logits=None if ref_logits is None else ref_logits.detach(),
-                  returns=returns, weight=weight, clip_low=clip[0], clip_high=clip[1],
-                  kl_coef=kl_coef, entropy_coef=entropy_coef, value_coef=value_coef,
-                  scale=loss_scale)
-    return PolicyLoss(*_PolicyLossFn.apply(ext, logits, value, wants, kwargs))
+    return PolicyLoss(*ext.policy_loss(logits, action, old_logp, advantage, legal, ref_logits,
+                                       value, returns, weight, clip[0], clip[1], kl_coef,
+                                       entropy_coef, value_coef, loss_scale))
 
 
 # ------------------------------------------------------------------------------- advantages

@@ -297,6 +297,9 @@ def test_scaled_losses(ext):
     assert torch.equal(value.grad, plain["d_value"] * 0.5)
     with pytest.raises(RuntimeError, match="once"):
         out.loss.backward()
+    again = learner.policy_loss(ext, logits, on["action"], on["old_logp"], on["advantage"])
+    with pytest.raises(RuntimeError, match="differentiated once"):
+        torch.autograd.grad(again.loss, logits, create_graph=True)
     assert not out.stats.requires_grad and not out.logp.requires_grad
     with torch.no_grad():
         quiet = learner.policy_loss(ext, logits, on["action"], on["old_logp"], on["advantage"])
