@@ -211,32 +211,49 @@ struct UpdateArgs {
   float* norm_out;
 };
 
-// Four values rounded to codes by chance, and the block's scale.  x >= 0 where !kSigned.
+// The largest of 64 lanes' x in every lane: within the rows of 16 lanes, then over the rows by
+// broadcasts of a row's last lane to the next ones (lane 63 then has it).
+__device__ inline uint32_t wavefront_max(uint32_t x) {
+  const auto with = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+  x = with(x, __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, false));
+  x = with(x, __builtin_amdgcn_update_dpp(0, x, 0x124, 0xf, 0xf, false));
+  x = with(x, __builtin_amdgcn_update_dpp(0, x, 0x122, 0xf, 0xf, false));
+  x = with(x, __builtin_amdgcn_update_dpp(0, x, 0x121, 0xf, 0xf, false));
+  x = with(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));  // rows 0, 2 to 1, 3
+  x = with(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));  // rows 1 to 2, 3
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
+// Four values rounded to codes by chance, and the block's scale.  x >= 0 or NaN where !kE4m3.
+// The largest size is found on the bits, where a NaN is above an infinity above all numbers.
 template <bool kE4m3>
 __device__ inline uint32_t to_codes(const float (&x)[kEach], const uint32_t (&word)[kEach],
                                     float& scale) {
   constexpr float kTop = kE4m3 ? 256.0f : 32768.0f;
-  float most = 0.0f, sum = 0.0f;
+  uint32_t most_bits = 0;
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
-    most = fmaxf(most, fabsf(x[e]));
-    sum += x[e] * 0.0f;  // NaN for a NaN or an infinity
+    const uint32_t b = __float_as_uint(x[e]) & 0x7fffffffu;
+    most_bits = b > most_bits ? b : most_bits;
   }
-  most = fmaxf(group_max<64>(most), 0x1p-100f);
+  most_bits = wavefront_max(most_bits);
+  const float most = fmaxf(__uint_as_float(most_bits), 0x1p-100f);
   const float up = kTop / most;
-  scale = __any(sum != 0.0f) ? NAN : most * (1.0f / kTop);
+  scale = most_bits >= 0x7f800000u ? NAN : most * (1.0f / kTop);
   uint32_t codes = 0;
+  if constexpr (kE4m3) {
+    codes = __builtin_amdgcn_cvt_sr_fp8_f32(x[0] * up, word[0], codes, 0);
+    codes = __builtin_amdgcn_cvt_sr_fp8_f32(x[1] * up, word[1], codes, 1);
+    codes = __builtin_amdgcn_cvt_sr_fp8_f32(x[2] * up, word[2], codes, 2);
+    codes = __builtin_amdgcn_cvt_sr_fp8_f32(x[3] * up, word[3], codes, 3);
+  } else {
+    codes = __builtin_amdgcn_cvt_sr_bf8_f32(x[0] * up, word[0] << 16, codes, 0);
+    codes = __builtin_amdgcn_cvt_sr_bf8_f32(x[1] * up, word[1] << 16, codes, 1);
+    codes = __builtin_amdgcn_cvt_sr_bf8_f32(x[2] * up, word[2] << 16, codes, 2);
+    codes = __builtin_amdgcn_cvt_sr_bf8_f32(x[3] * up, word[3] << 16, codes, 3);
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    const float y = x[e] * up;
-    uint32_t c;
-    if constexpr (kE4m3) {
-      c = (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(y, word[e], 0, 0) & 0xffu;
-    } else {
-      c = (uint32_t)__builtin_amdgcn_cvt_sr_bf8_f32(y, word[e] << 16, 0, 0) & 0xffu;
-      c = x[e] > 0.0f && c == 0 ? 1u : c;
-    }
-    codes |= c << (8 * e);
+    for (int e = 0; e < kEach; ++e)
+      if ((codes & (0xffu << (8 * e))) == 0 && x[e] > 0.0f) codes |= 1u << (8 * e);
   }
   return codes;
 }
@@ -269,81 +286,192 @@ __device__ inline void store_codes(void* p, i64 i, i64 n, bool whole, uint32_t c
     if (i + e < n) s[e] = (uint8_t)(codes >> (8 * e));
 }
 
+// sqrt(v) to the hardware's last place or so (v_sqrt_f32; its small arguments scaled up first,
+// which it would flush).
+__device__ inline float root_of(float v) {
+  const bool small = v < 0x1p-96f;
+  const float r = __builtin_amdgcn_sqrtf(small ? v * 0x1p32f : v);
+  return small ? r * 0x1p-16f : r;
+}
+
+struct Numbers {  // of the step, and of the tensor
+  float beta1, beta2, rest1, rest2, eps, clip;
+  float decay, step_size, root;
+};
+
+// The step of one value.  The moments are formed in separately rounded operations, so that their
+// codes follow from IEEE arithmetic; the quotient is the product with the hardware's reciprocal:
+// a last place of the step, not of the weight.
+__device__ inline void advance(const Numbers& c, float grad, float& w, float& m, float& v) {
+  const float x = grad * c.clip;
+  m = m * c.beta1 + x * c.rest1;
+  v = v * c.beta2 + (x * x) * c.rest2;
+  const float by = root_of(v) * c.root + c.eps;
+  w = w * c.decay - c.step_size * (m * __builtin_amdgcn_rcpf(by));
+}
+
+// The moments of four values as a thread holds them between reading and computing.
 template <int kBits>
-__global__ __launch_bounds__(kThreads) void adamw_update_kernel(const UpdateArgs g) {
-  float clip = 1.0f;
-  if (g.max_norm > 0.0) {
-    double sum = 0.0;
-    for (int i = threadIdx.x; i < g.partial_count; i += kThreads) sum += g.partials[i];
-    const float norm = (float)sqrt(workgroup_sum(sum));
-    const float c = (float)g.max_norm / (norm + 1e-6f);
-    clip = c > 1.0f ? 1.0f : c;  // a NaN norm stays one, and so do the weights
-    if (g.norm_out && blockIdx.x == 0 && threadIdx.x == 0) *g.norm_out = norm;
+struct Held;
+template <>
+struct Held<32> {
+  Vec<float, kEach> m, v;
+  __device__ void read(const Tensor& t, i64 i) {
+    m = *reinterpret_cast<const Vec<float, kEach>*>(static_cast<const float*>(t.m) + i);
+    v = *reinterpret_cast<const Vec<float, kEach>*>(static_cast<const float*>(t.v) + i);
   }
-  const uint32_t chunks = g.table.chunk_end[g.table.count - 1];
-  for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
-    const int k = tensor_of(g.table.chunk_end, g.table.count, c);
-    const i64 base = (i64)(c - (k ? g.table.chunk_end[k - 1] : 0)) * kChunk;
-    const Tensor& t = g.table.tensor[k];
-    const Factors f = g.factors[k];
-    const i64 n = t.numel;
-    float* w32 = t.master ? t.master : static_cast<float*>(t.param);
-    const bool fits =
-        aligned(t.grad, kEach * value_bytes(t.grad_dtype)) && aligned(w32, 16) &&
-        aligned(t.param, kEach * value_bytes(t.param_dtype)) &&
-        aligned(t.m, kBits == 8 ? 4 : 16) && aligned(t.v, kBits == 8 ? 4 : 16);
-    const uint32_t key = mix32(f.key + (uint32_t)((uint64_t)base >> 32) * kPlaceStep);
+};
+template <>
+struct Held<8> {
+  uint32_t m, v;
+  float m_scale, v_scale;
+  __device__ void read(const Tensor& t, i64 i) {
+    m = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(t.m) + i);
+    v = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(t.v) + i);
+    const i64 block = i / kBlock;
+    m_scale = t.m_scale[block], v_scale = t.v_scale[block];
+  }
+};
+
+// A whole chunk of an aligned tensor with P parameters and G gradients: kBatch accesses of each
+// stream are in flight before the first is used.
+template <int kBits, class P, class G>
+__device__ inline void whole_chunk(const Tensor& t, const Numbers& c, i64 base, uint32_t key) {
+  using GS = typename G::storage;
+  constexpr bool kMaster = sizeof(typename P::storage) == 2;
+  constexpr int kBatch = kBits == 8 ? 4 : 2;
+  float* w32 = kMaster ? t.master : static_cast<float*>(t.param);
 #pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-      const i64 i = base + (r * kThreads + (int)threadIdx.x) * kEach;
-      const i64 block = i / kBlock;  // the same for the wavefront
-      if (block * kBlock >= n) continue;
-      const bool whole = fits && i + kEach <= n;
-      float gr[kEach], w[kEach], m[kEach], v[kEach];
-      load4(t.grad_dtype, t.grad, i, n, whole, gr);
-      load4_as<F32>(w32, i, n, whole, w);
+  for (int r0 = 0; r0 < kRounds; r0 += kBatch) {
+    Vec<GS, kEach> gv[kBatch];
+    Vec<float, kEach> wv[kBatch];
+    Held<kBits> held[kBatch];
+#pragma unroll
+    for (int r = 0; r < kBatch; ++r) {
+      const i64 i = base + ((r0 + r) * kThreads + (int)threadIdx.x) * kEach;
+      gv[r] = *reinterpret_cast<const Vec<GS, kEach>*>(static_cast<const GS*>(t.grad) + i);
+      wv[r] = *reinterpret_cast<const Vec<float, kEach>*>(w32 + i);
+      held[r].read(t, i);
+    }
+#pragma unroll
+    for (int r = 0; r < kBatch; ++r) {
+      const i64 i = base + ((r0 + r) * kThreads + (int)threadIdx.x) * kEach;
+      float w[kEach], m[kEach], v[kEach];
       if constexpr (kBits == 8) {
-        from_codes<true>(load_codes(t.m, i, n, whole), t.m_scale[block], m);
-        from_codes<false>(load_codes(t.v, i, n, whole), t.v_scale[block], v);
-      } else {
-        load4_as<F32>(t.m, i, n, whole, m);
-        load4_as<F32>(t.v, i, n, whole, v);
+        from_codes<true>(held[r].m, held[r].m_scale, m);
+        from_codes<false>(held[r].v, held[r].v_scale, v);
       }
 #pragma unroll
       for (int e = 0; e < kEach; ++e) {
-        const float x = gr[e] * clip;
-        m[e] = m[e] * g.beta1 + x * g.rest1;
-        v[e] = v[e] * g.beta2 + (x * x) * g.rest2;
-        w[e] = w[e] * f.decay - f.step_size * (m[e] / (sqrtf(v[e]) * f.root + g.eps));
+        w[e] = wv[r].v[e];
+        if constexpr (kBits == 32) m[e] = held[r].m.v[e], v[e] = held[r].v.v[e];
+        advance(c, G::to_float(gv[r].v[e]), w[e], m[e], v[e]);
       }
-      store4_as<F32>(w32, i, n, whole, w);
-      if (t.master) store4(t.param_dtype, t.param, i, n, whole, w);
+      store4_as<F32>(w32, i, 0, true, w);
+      if constexpr (kMaster) store4_as<P>(t.param, i, 0, true, w);
       if constexpr (kBits == 8) {
         uint32_t word[kEach];
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-          word[e] = mix32((uint32_t)(i + e) ^ key);
-          if (i + e >= n) m[e] = v[e] = 0.0f;
-        }
+        for (int e = 0; e < kEach; ++e) word[e] = mix32((uint32_t)(i + e) ^ key);
         float m_scale, v_scale;
-        const uint32_t mc = to_codes<true>(m, word, m_scale);
-        const uint32_t vc = to_codes<false>(v, word, v_scale);
-        store_codes(t.m, i, n, whole, mc);
-        store_codes(t.v, i, n, whole, vc);
+        store_codes(t.m, i, 0, true, to_codes<true>(m, word, m_scale));
+        store_codes(t.v, i, 0, true, to_codes<false>(v, word, v_scale));
         if (threadIdx.x % 64 == 0) {
-          t.m_scale[block] = m_scale;
-          t.v_scale[block] = v_scale;
+          t.m_scale[i / kBlock] = m_scale;
+          t.v_scale[i / kBlock] = v_scale;
         }
       } else {
-        store4_as<F32>(t.m, i, n, whole, m);
-        store4_as<F32>(t.v, i, n, whole, v);
+        store4_as<F32>(t.m, i, 0, true, m);
+        store4_as<F32>(t.v, i, 0, true, v);
       }
     }
   }
 }
 
-inline int groups_for(uint32_t chunks) {
-  const int most = min(compute_units() * 8, kPartials);
+// Any chunk, of any types: a tensor's last one, or one whose addresses fit no wide access.
+template <int kBits>
+__device__ inline void any_chunk(const Tensor& t, const Numbers& c, i64 base, uint32_t key) {
+  const i64 n = t.numel;
+  float* w32 = t.master ? t.master : static_cast<float*>(t.param);
+  for (int r = 0; r < kRounds; ++r) {
+    const i64 i = base + (r * kThreads + (int)threadIdx.x) * kEach;
+    const i64 block = i / kBlock;  // the same for the wavefront
+    if (block * kBlock >= n) continue;
+    float gr[kEach], w[kEach], m[kEach], v[kEach];
+    load4(t.grad_dtype, t.grad, i, n, false, gr);
+    load4_as<F32>(w32, i, n, false, w);
+    if constexpr (kBits == 8) {
+      from_codes<true>(load_codes(t.m, i, n, false), t.m_scale[block], m);
+      from_codes<false>(load_codes(t.v, i, n, false), t.v_scale[block], v);
+    } else {
+      load4_as<F32>(t.m, i, n, false, m);
+      load4_as<F32>(t.v, i, n, false, v);
+    }
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) advance(c, gr[e], w[e], m[e], v[e]);
+    store4_as<F32>(w32, i, n, false, w);
+    if (t.master) store4(t.param_dtype, t.param, i, n, false, w);
+    if constexpr (kBits == 8) {
+      uint32_t word[kEach];
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        word[e] = mix32((uint32_t)(i + e) ^ key);
+        if (i + e >= n) m[e] = v[e] = 0.0f;
+      }
+      float m_scale, v_scale;
+      const uint32_t mc = to_codes<true>(m, word, m_scale);
+      const uint32_t vc = to_codes<false>(v, word, v_scale);
+      store_codes(t.m, i, n, false, mc);
+      store_codes(t.v, i, n, false, vc);
+      if (threadIdx.x % 64 == 0) {
+        t.m_scale[block] = m_scale;
+        t.v_scale[block] = v_scale;
+      }
+    } else {
+      store4_as<F32>(t.m, i, n, false, m);
+      store4_as<F32>(t.v, i, n, false, v);
+    }
+  }
+}
+
+template <int kBits, class P>
+__device__ inline void whole_chunk_of(const Tensor& t, const Numbers& c, i64 base, uint32_t key) {
+  if (t.grad_dtype == CUGO_DTYPE_F32) whole_chunk<kBits, P, F32>(t, c, base, key);
+  else if (t.grad_dtype == CUGO_DTYPE_F16) whole_chunk<kBits, P, F16>(t, c, base, key);
+  else whole_chunk<kBits, P, BF16>(t, c, base, key);
+}
+
+template <int kBits>
+__global__ __launch_bounds__(kThreads) void adamw_update_kernel(const UpdateArgs g) {
+  Numbers c{g.beta1, g.beta2, g.rest1, g.rest2, g.eps, 1.0f, 0.0f, 0.0f, 0.0f};
+  if (g.max_norm > 0.0) {
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < g.partial_count; i += kThreads) sum += g.partials[i];
+    const float norm = (float)sqrt(workgroup_sum(sum));
+    const float clip = (float)g.max_norm / (norm + 1e-6f);
+    c.clip = clip > 1.0f ? 1.0f : clip;  // a NaN norm stays one, and so do the weights
+    if (g.norm_out && blockIdx.x == 0 && threadIdx.x == 0) *g.norm_out = norm;
+  }
+  const uint32_t chunks = g.table.chunk_end[g.table.count - 1];
+  for (uint32_t at = blockIdx.x; at < chunks; at += gridDim.x) {
+    const int k = tensor_of(g.table.chunk_end, g.table.count, at);
+    const i64 base = (i64)(at - (k ? g.table.chunk_end[k - 1] : 0)) * kChunk;
+    const Tensor& t = g.table.tensor[k];
+    const Factors f = g.factors[k];
+    c.decay = f.decay, c.step_size = f.step_size, c.root = f.root;
+    const uint32_t key = mix32(f.key + (uint32_t)((uint64_t)base >> 32) * kPlaceStep);
+    const bool fits =
+        base + kChunk <= t.numel && aligned(t.grad, kEach * value_bytes(t.grad_dtype)) &&
+        aligned(t.param, kEach * value_bytes(t.param_dtype)) && aligned(t.master, 16) &&
+        aligned(t.m, kBits == 8 ? 4 : 16) && aligned(t.v, kBits == 8 ? 4 : 16);
+    if (!fits) any_chunk<kBits>(t, c, base, key);
+    else if (t.param_dtype == CUGO_DTYPE_F32) whole_chunk_of<kBits, F32>(t, c, base, key);
+    else if (t.param_dtype == CUGO_DTYPE_F16) whole_chunk_of<kBits, F16>(t, c, base, key);
+    else whole_chunk_of<kBits, BF16>(t, c, base, key);
+  }
+}
+
+inline int groups_for(uint32_t chunks, int most) {
   return chunks < (uint32_t)most ? (int)chunks : most;
 }
 
@@ -399,7 +527,7 @@ int cugo_adamw(const CugoAdamwTensor* tensors, int64_t count, int bits, double b
     g.norm = max_norm > 0.0;
     g.factors = factors + l * kTable;
     g.partials = partials + partial_count;
-    const int groups = g.norm && end > 0 ? groups_for(end) : 1;
+    const int groups = g.norm && end > 0 ? groups_for(end, kPartials) : 1;
     adamw_count_kernel<<<groups, kThreads, 0, stream>>>(g);
     const int rc = (int)hipGetLastError();
     if (rc != 0) return rc;
@@ -423,7 +551,7 @@ int cugo_adamw(const CugoAdamwTensor* tensors, int64_t count, int bits, double b
     g.partials = partials, g.partial_count = partial_count;
     g.norm_out = l == 0 ? norm_out : nullptr;
     if (end == 0 && !(l == 0 && norm_out && max_norm > 0.0)) continue;
-    const int groups = end > 0 ? groups_for(end) : 1;
+    const int groups = end > 0 ? groups_for(end, compute_units() * 8) : 1;
     if (bits == 8) adamw_update_kernel<8><<<groups, kThreads, 0, stream>>>(g);
     else adamw_update_kernel<32><<<groups, kThreads, 0, stream>>>(g);
     const int rc = (int)hipGetLastError();

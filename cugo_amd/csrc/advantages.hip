@@ -68,9 +68,19 @@ __global__ __launch_bounds__(64 * kWaves) void gae_kernel(const GaeArgs g) {
   const S* value = static_cast<const S*>(g.value);
   const i64 pass = (i64)kWaves * runs * kSteps;
   float carry = 0.0f;
-  if (!kMapsOnly) {
-    for (int k = g.chunks - 1; k > chunk; --k)
-      carry = apply(g.maps[(i64)k * g.batch + b], carry);
+  if (!kMapsOnly && chunk + 1 < g.chunks) {
+    // The maps of the chunks behind this one: each wavefront composes a run of them (its loads
+    // do not wait for one another), and every lane applies the runs.
+    const int behind_it = g.chunks - 1 - chunk;
+    const int each = (behind_it + kWaves - 1) / kWaves;
+    const int from = chunk + 1 + wave * each, to = min(from + each, g.chunks);
+    float2 m = make_float2(0.0f, 1.0f);
+#pragma unroll 4
+    for (int k = from; k < to; ++k) m = after(m, g.maps[(i64)k * g.batch + b]);
+    if (run == 0) wave_map[wave][column] = m;
+    __syncthreads();
+    for (int k = kWaves - 1; k >= 0; --k) carry = apply(wave_map[k][column], carry);
+    __syncthreads();
   }
   float2 total = make_float2(0.0f, 1.0f);  // kMapsOnly: the map of the passes so far
   int turn = 0;
@@ -145,7 +155,7 @@ __global__ __launch_bounds__(64 * kWaves) void gae_kernel(const GaeArgs g) {
 }
 
 // How a call is laid out: the columns of a wavefront, and the chunks the steps are split into
-// so that the launch has about one workgroup a compute unit.
+// so that the launch has about two workgroups a compute unit.
 struct GaeLayout {
   int columns, chunks;
   i64 groups, chunk;
@@ -158,7 +168,7 @@ inline GaeLayout gae_layout(i64 steps, i64 batch) {
   l.groups = (batch + l.columns - 1) / l.columns;
   const i64 pass = (i64)kWaves * (64 / l.columns) * kSteps;
   const i64 passes = (steps + pass - 1) / pass;
-  i64 chunks = compute_units() / l.groups;
+  i64 chunks = 2 * (i64)compute_units() / l.groups;
   chunks = chunks < 1 ? 1 : chunks < passes ? chunks : passes;
   const i64 each = (passes + chunks - 1) / chunks;
   l.chunk = each * pass;

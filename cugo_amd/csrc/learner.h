@@ -16,18 +16,21 @@ typedef int64_t i64;
 
 struct F32 {
   using storage = float;
+  static constexpr uint32_t kNone = 0xff800000u;  // -inf
   __device__ static float to_float(float x) { return x; }
   __device__ static float from_float(float f) { return f; }
 };
 
 struct F16 {
   using storage = _Float16;
+  static constexpr uint32_t kNone = 0xfc00u;  // -inf
   __device__ static float to_float(_Float16 x) { return (float)x; }
   __device__ static _Float16 from_float(float f) { return (_Float16)f; }
 };
 
 struct BF16 {
   using storage = __bf16;
+  static constexpr uint32_t kNone = 0xff80u;  // -inf
   __device__ static float to_float(__bf16 x) { return (float)x; }
   // To nearest even in hardware (v_cvt_pk_bf16_f32), as torch rounds.
   __device__ static __bf16 from_float(float f) { return (__bf16)f; }
@@ -43,6 +46,49 @@ template <class S, int K>
 struct __attribute__((packed, aligned(sizeof(S)))) Any {
   S v[K];
 };
+
+// N bytes as they lie in memory, in registers: `Raw` at their own alignment, `RawAny` at any.
+typedef uint32_t Words2 __attribute__((ext_vector_type(2)));
+typedef uint32_t Words4 __attribute__((ext_vector_type(4)));
+template <int N>
+struct RawOf;
+template <>
+struct RawOf<2> {
+  using Raw = uint16_t;
+};
+template <>
+struct RawOf<4> {
+  using Raw = uint32_t;
+};
+template <>
+struct RawOf<8> {
+  using Raw = Words2;
+};
+template <>
+struct RawOf<16> {
+  using Raw = Words4;
+};
+template <int N>
+using Raw = typename RawOf<N>::Raw;
+template <int N>
+struct __attribute__((packed, aligned(1))) RawAny {
+  Raw<N> v;
+};
+
+// The float32 values of 16 bytes as they are read (8 of 16 bits, or 4 of 32).
+template <class T>
+__device__ inline void unpack(const Words4& w, float (&f)[16 / sizeof(typename T::storage)]) {
+  if constexpr (sizeof(typename T::storage) == 4) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f[k] = __uint_as_float(w[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      f[2 * k] = T::to_float(__builtin_bit_cast(typename T::storage, (uint16_t)w[k]));
+      f[2 * k + 1] = T::to_float(__builtin_bit_cast(typename T::storage, (uint16_t)(w[k] >> 16)));
+    }
+  }
+}
 
 // x from the lane that kCtrl, a rotation within the 16 lanes of a DPP row, names.
 template <int kCtrl>

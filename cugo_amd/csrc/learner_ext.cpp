@@ -168,6 +168,13 @@ std::vector<torch::Tensor> policy_loss(torch::Tensor logits, torch::Tensor actio
               "the coefficients must be finite");
   scalar_ptr(scale, logits, "scale");
   const DeviceGuard guard(logits.device());
+  // rows too far apart for 32-bit offsets are copied together
+  const auto near = [](const torch::Tensor& t) {
+    return t.size(1) > 1024 || t.stride(0) < (1 << 24) ? t : t.contiguous();
+  };
+  logits = near(logits);
+  if (legal.has_value()) legal = near(*legal);
+  if (ref_logits.has_value()) ref_logits = near(*ref_logits);
   const bool grad = at::GradMode::is_enabled();
   const LossInputs in{action,   old_logp,  advantage, legal,   ref_logits,   returns,    weight,
                       scale,    clip_low,  clip_high, kl_coef, entropy_coef, value_coef,

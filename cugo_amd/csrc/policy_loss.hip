@@ -22,6 +22,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 namespace cugo_amd {
 namespace learner {
 namespace loss {
@@ -55,70 +57,106 @@ struct LossArgs {
   double* partials;
 };
 
-__device__ inline float load_value(const void* p, int dtype, i64 i) {
+// The address of value r.
+__device__ inline const void* at_row(const void* p, int dtype, i64 r) {
+  return static_cast<const char*>(p) + r * (dtype == CUGO_DTYPE_F32 ? 4 : 2);
+}
+
+__device__ inline float load_value(const void* p, int dtype, uint32_t i) {
   if (dtype == CUGO_DTYPE_F32) return static_cast<const float*>(p)[i];
   if (dtype == CUGO_DTYPE_F16) return (float)static_cast<const _Float16*>(p)[i];
   return (float)static_cast<const __bf16*>(p)[i];
 }
 
-__device__ inline void store_value(void* p, int dtype, i64 i, float x) {
+__device__ inline void store_value(void* p, int dtype, uint32_t i, float x) {
   if (dtype == CUGO_DTYPE_F32) static_cast<float*>(p)[i] = x;
   else if (dtype == CUGO_DTYPE_F16) static_cast<_Float16*>(p)[i] = (_Float16)x;
   else static_cast<__bf16*>(p)[i] = (__bf16)x;
 }
 
+// What a row's terms need beside its logits, read ahead of them.
+struct RowInputs {
+  float w, old, adv, value, returns;
+};
+
+// Row r + i; r is the same for the workgroup, so that a lane's addresses are scalars and 32 bits.
+__device__ inline RowInputs row_inputs(const LossArgs& g, i64 r, uint32_t i) {
+  RowInputs in;
+  in.w = g.weight ? (g.weight + r)[i] : g.even;
+  in.old = (g.old_logp + r)[i];
+  in.adv = (g.advantage + r)[i];
+  in.value = in.returns = 0.0f;
+  if (g.value) {
+    in.value = load_value(at_row(g.value, g.value_dtype, r), g.value_dtype, i);
+    in.returns = (g.returns + r)[i];
+  }
+  return in;
+}
+
+// Exponents are in base 2: x = z k - top k with k = log2 e, one multiply-add, so that
+// e^(z - top) = 2^x up to a factor that all of a row's exponentials share (the rounding of top k),
+// which their sum's logarithm takes out again.
+// Where the largest logit is so large that top k may not fit, logits that are not equal to it
+// are 1e30 away and more, so that any k tells them apart: a small one is taken.
+struct Scale {
+  float k, shift;
+  __device__ float operator()(float z) const { return __builtin_fmaf(z, k, shift); }
+};
+__device__ inline Scale scale_for(float top) {
+  const float k = fabsf(top) > 1e37f && fabsf(top) < INFINITY ? 0x1p-10f : kLog2e;
+  return Scale{k, top == -INFINITY ? 0.0f : -top * k};
+}
+__device__ inline float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
 // A row's terms from the sums over its actions.  Every lane that serves the row computes them.
 struct RowTerms {
-  float a, b, c;   // d loss / d z_j = e_j (a + b d_j + c t_j) - [j = action] pull, with
-  float pull;      // t_j = z_j - top, e_j = e^{t_j}, d_j = t_j - t'_j
+  float a, b, c;   // d loss / d z_j = 2^x_j (a + b d_j + c x_j) - [j = action] pull, with
+  float pull;      // d_j = x_j - x'_j
   float stat[kStats];
   float logp, d_value;
   bool live;       // the row has policy terms and a weight
 };
 
-// top: the row's largest legal logit; s = sum e; u = sum e t; ref_log = log s'; ds = sum e d;
-// at: the action's t, or -inf.
+// s = sum 2^x; u = sum 2^x x; ds = sum 2^x d; sr = sum 2^x'; at: the action's x, or -inf.
 template <bool kRef>
-__device__ inline RowTerms row_terms(const LossArgs& g, i64 r, bool some, float s, float u,
-                                     float ds, float ref_log, float at) {
+__device__ inline RowTerms row_terms(const LossArgs& g, const RowInputs& in, bool some, float s,
+                                     float u, float ds, float sr, float at) {
   RowTerms x;
-  const float w = g.weight ? g.weight[r] : g.even;
-  const float old = g.old_logp[r], adv = g.advantage[r];
-  const float inv = some ? 1.0f / s : 0.0f;
-  const float ls = some ? __builtin_amdgcn_logf(s) * kLn2 : 0.0f;  // v_log_f32: base 2
-  const float entropy = ls - u * inv;
-  const float shift = ls - ref_log;  // l_j - l'_j = d_j - shift
-  const float kl = kRef ? ds * inv - shift : 0.0f;
-  x.logp = some ? at - ls : 0.0f;
-  const float drift = x.logp - old;
-  const float ratio = x.logp == -INFINITY ? 0.0f : expf(drift);
+  const float inv = some ? __builtin_amdgcn_rcpf(s) : 0.0f;
+  const float ls = some ? __builtin_amdgcn_logf(s) : 0.0f;  // v_log_f32: base 2
+  const float mean = u * inv;
+  const float entropy = (ls - mean) * kLn2;
+  const float shift = kRef ? ls - __builtin_amdgcn_logf(sr) : 0.0f;  // l_j - l'_j = (d_j - shift) ln 2
+  const float kl2 = ds * inv;
+  const float kl = kRef ? (kl2 - shift) * kLn2 : 0.0f;
+  x.logp = some ? (at - ls) * kLn2 : 0.0f;
+  const float drift = x.logp - in.old;
+  const float ratio = x.logp == -INFINITY ? 0.0f : exp2_of(drift * kLog2e);
   const float bound = fminf(fmaxf(ratio, g.least), g.most);
-  const bool cut = ratio * adv > bound * adv;
-  const float gain = cut ? bound * adv : ratio * adv;
-  x.live = some && w != 0.0f;
-  const float wp = x.live ? w : 0.0f;
-  x.stat[0] = x.live ? -gain * wp : 0.0f;
-  x.stat[2] = x.live ? kl * wp : 0.0f;
-  x.stat[3] = x.live ? entropy * wp : 0.0f;
-  x.stat[4] = cut ? wp : 0.0f;
-  x.stat[5] = x.live ? (ratio - 1.0f - drift) * wp : 0.0f;
-  const float unit = g.scale ? *g.scale : 1.0f;
-  const float pull = cut ? 0.0f : ratio * adv;
-  const float per = wp * unit * inv;
-  x.a = per * (pull + g.entropy_coef * (entropy - ls) - (kRef ? g.kl_coef * (shift + kl) : 0.0f));
-  x.b = kRef ? per * g.kl_coef : 0.0f;
-  x.c = per * g.entropy_coef;
-  x.pull = wp * unit * pull;
+  const bool cut = ratio * in.adv > bound * in.adv;
+  const float gain = (cut ? bound : ratio) * in.adv;
+  x.live = some && in.w != 0.0f;
+  x.stat[0] = x.live ? -gain * in.w : 0.0f;
+  x.stat[2] = x.live ? kl * in.w : 0.0f;
+  x.stat[3] = x.live ? entropy * in.w : 0.0f;
+  x.stat[4] = x.live && cut ? in.w : 0.0f;
+  x.stat[5] = x.live ? (ratio - 1.0f - drift) * in.w : 0.0f;
+  const float wu = in.w * (g.scale ? *g.scale : 1.0f);
+  const float pull = cut ? 0.0f : ratio * in.adv;
+  const float per = wu * inv;
+  // c_e p (l + H) = c_e p ln 2 (x - mean);  c_k p (l - l' - K) = c_k p ln 2 (d - kl2)
+  x.c = per * (g.entropy_coef * kLn2);
+  x.b = kRef ? per * (g.kl_coef * kLn2) : 0.0f;
+  x.a = per * pull - x.c * mean - (kRef ? x.b * kl2 : 0.0f);
+  x.pull = wu * pull;
   x.stat[1] = x.d_value = 0.0f;
-  if (g.value && w != 0.0f) {
-    const float err = load_value(g.value, g.value_dtype, r) - g.returns[r];
-    x.stat[1] = w * 0.5f * err * err;
-    x.d_value = w * unit * g.value_coef * err;
+  if (g.value && in.w != 0.0f) {
+    const float err = in.value - in.returns;
+    x.stat[1] = in.w * 0.5f * err * err;
+    x.d_value = wu * g.value_coef * err;
   }
   return x;
 }
-
-__device__ inline float exp_of(float t) { return __builtin_amdgcn_exp2f(t * kLog2e); }
 
 // A workgroup's sums (kStats of each of its 256 / G groups of lanes, in acc of the group's lane
 // j = the sum's place) to its partials: in a fixed order, so a call's results are the same
@@ -135,267 +173,654 @@ __device__ inline void write_partials(double acc, int j, double* partials) {
   }
 }
 
-// Rows of up to 4 V G actions (V in 1..4): G lanes a row, vector i of E elements of lane j at
-// action (i G + j) E, so that the row's lanes read one run of memory an instruction; the row
-// stays in registers.  The last vector of a row that ends inside it is moved back to end with
-// the row, where it repeats elements of other lanes: those (`mine` false) are left out of the
-// sums, and their gradients stored twice, the same value.
+// Element i from a base that is the same for the wavefront: a scalar address and 32 bits of
+// offset, where 64-bit addresses of every access would hold twice the registers.
+template <class S>
+__device__ inline S* element(S* base, uint32_t i) {
+  return reinterpret_cast<S*>(reinterpret_cast<uintptr_t>(base) + i * (uint32_t)sizeof(S));
+}
+
+// What one lane wrote to LDS before is what another lane of the wavefront reads after.
+__device__ inline void wavefront_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Rows of up to E V G actions (V in 1..4): G lanes a row, vector i of E elements of lane j at
+// action (i G + j) E, so that the row's lanes read one run of memory an instruction.  The last
+// vector of a row that ends inside it is read moved back, to end with the row; the elements that
+// it repeats of other lanes (`mine` false) count as illegal and are not stored.
+// The row goes through LDS as it was read, in slots: an action's slot is its number, but in the
+// moved vector.  From there it is gone through for its largest logit, for its sums and for its
+// gradient, a vector of each lane at a time: kept in registers for that, a row of 179 actions
+// took 96 to 112 of them and left four wavefronts a SIMD.
+// A game's row has about ten legal actions of 179, and an exponential or a product for each action
+// takes longer than memory does: where each row of a wavefront has at most two legal actions a
+// lane, a list of their slots is made, a lane computes two of them, and the gradient is put
+// together in LDS.
+// XX
 template <class T, int G, int V, int E, bool kRef>
 __global__ __launch_bounds__(kThreads) void loss_rows_kernel(const LossArgs g) {
   using S = typename T::storage;
-  const int j = threadIdx.x & (G - 1);
+  constexpr int kBytes = E * sizeof(S);
+  using Slots = Vec<S, E>;
+  constexpr int kRows = kThreads / G;
+  constexpr int kSlots = V * G * E;
+  constexpr bool kList = kSlots <= 256;  // a slot fits a byte
+  __shared__ __align__(16) S z_slots[kRows][kSlots];
+  __shared__ __align__(16) S q_slots[kRef ? kRows : 1][kRef ? kSlots : E];
+  __shared__ uint8_t lists[kList ? kRows : 1][2 * G];
+  const int j = threadIdx.x & (G - 1), row = threadIdx.x / G;
   const int at = ((V - 1) * G + j) * E;  // the last vector's first action, where it fits
   const int last = min(at, g.actions - E);
-  bool mine[E];
+  // the bits of the lane's elements (element e of vector i at bit E i + e) that are its own
+  uint32_t own = (1u << (E * (V - 1))) - 1u;
 #pragma unroll
-  for (int e = 0; e < E; ++e) mine[e] = last + e >= at;
-  const bool any_mine = at < g.actions;
-  constexpr int kRows = kThreads / G;
+  for (int e = 0; e < E; ++e) own |= (last + e >= at ? 1u : 0u) << (E * (V - 1) + e);
+  S* zl = z_slots[row];
+  S* ql = q_slots[kRef ? row : 0];
   const i64 tiles = (g.n + kRows - 1) / kRows;
   double acc = 0.0;
   for (i64 tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const i64 row = tile * kRows + threadIdx.x / G;
-    const bool ok = row < g.n;
-    const i64 r = ok ? row : g.n - 1;  // loads are unconditional; the sums leave it out
-    const S* zs = static_cast<const S*>(g.logits) + r * g.logits_stride;
-    const S* qs = static_cast<const S*>(g.ref) + (kRef ? r * g.ref_stride : 0);
-    const uint8_t* ls = g.legal ? g.legal + r * g.legal_stride : nullptr;
-    Any<S, E> zv[V], qv[V];
-    Any<uint8_t, E> lv[V];
+    const i64 r0 = tile * kRows;
+    const bool ok = r0 + row < g.n;
+    // loads are unconditional, of a row that exists; the sums leave it out
+    const uint32_t i0 = (uint32_t)(ok ? row : (int)(g.n - 1 - r0));
+    const i64 act = (g.action + r0)[i0];
+    const RowInputs in = row_inputs(g, r0, i0);
+    uint32_t bits = own;
+    {
+      const S* zb = static_cast<const S*>(g.logits) + r0 * g.logits_stride;
+      const S* qb = static_cast<const S*>(g.ref) + (kRef ? r0 * g.ref_stride : 0);
+      const uint32_t z_at = i0 * (uint32_t)g.logits_stride;
+      const uint32_t q_at = kRef ? i0 * (uint32_t)g.ref_stride : 0u;
+      Raw<kBytes> z[V], q[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int k = i + 1 < V ? (i * G + j) * E : last;
-      zv[i] = *reinterpret_cast<const Any<S, E>*>(zs + k);
-      if constexpr (kRef) qv[i] = *reinterpret_cast<const Any<S, E>*>(qs + k);
-      if (ls) lv[i] = *reinterpret_cast<const Any<uint8_t, E>*>(ls + k);
-      else
+      for (int i = 0; i < V; ++i) {
+        const uint32_t k = (uint32_t)(i + 1 < V ? (i * G + j) * E : last);
+        z[i] = reinterpret_cast<const RawAny<kBytes>*>(element(zb, z_at + k))->v;
+        if constexpr (kRef)
+          q[i] = reinterpret_cast<const RawAny<kBytes>*>(element(qb, q_at + k))->v;
+      }
+      if (g.legal) {
+        const uint8_t* lb = g.legal + r0 * g.legal_stride;
+        const uint32_t l_at = i0 * (uint32_t)g.legal_stride;
+        uint32_t legal = 0;
+        if constexpr (E == 4) {
+          uint32_t w[V];
 #pragma unroll
-        for (int e = 0; e < E; ++e) lv[i].v[e] = 1;
-    }
-    const i64 act = g.action[r];
-    const bool inside = act >= 0 && act < g.actions;
-    const i64 ac = inside ? act : 0;
-    const bool taken = inside && (!ls || ls[ac]);
-    const float za = T::to_float(zs[ac]);
-    float t[V * E], d[kRef ? V * E : 1];
-    float top = -INFINITY, top_ref = -INFINITY;
+          for (int i = 0; i < V; ++i)
+            w[i] = reinterpret_cast<const RawAny<4>*>(
+                       lb + (l_at + (uint32_t)(i + 1 < V ? (i * G + j) * E : last)))->v;
+          // a byte that is not 0 sets its upper bit, and a product of bytes gathers those
+          uint32_t low = 0, high = 0;
 #pragma unroll
-    for (int i = 0; i < V * E; ++i) {
-      const bool on = lv[i / E].v[i % E] != 0;
-      t[i] = on ? T::to_float(zv[i / E].v[i % E]) : -INFINITY;
-      top = fmaxf(top, t[i]);
-      if constexpr (kRef) {
-        d[i] = on ? T::to_float(qv[i / E].v[i % E]) : -INFINITY;
-        top_ref = fmaxf(top_ref, d[i]);
+          for (int i = 0; i < V; ++i) {
+            const uint32_t set = (((w[i] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | w[i]) & 0x80808080u;
+            uint32_t& sum = i < 2 ? low : high;
+            sum = __builtin_amdgcn_udot4(set, i % 2 ? 0x80402010u : 0x08040201u, sum, false);
+          }
+          legal = (low >> 7) | (high << 1);
+        } else {
+          legal = lb[l_at + (uint32_t)last] != 0;
+        }
+        bits &= legal;
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int k = (i * G + j) * E;
+        *reinterpret_cast<Raw<kBytes>*>(zl + k) = z[i];
+        if constexpr (kRef) *reinterpret_cast<Raw<kBytes>*>(ql + k) = q[i];
       }
     }
-    top = group_max<G>(top);
-    const bool some = top > -INFINITY;
-    top = some ? top : 0.0f;
-    if constexpr (kRef) {
-      top_ref = group_max<G>(top_ref);
-      top_ref = top_ref > -INFINITY ? top_ref : 0.0f;
+    // the action's slot, where the row has it: its lane, and the bit of it there
+    const int moved_from = g.actions & ~(E - 1);
+    const int slot_of_act = act < 0 || act >= g.actions ? -1
+                            : (int)act >= moved_from   ? (int)act + E - (g.actions & (E - 1))
+                                                       : (int)act;
+    int count = 0, upto = 0, total = 2 * G + 1;
+    if constexpr (kList) {
+      count = upto = __popc(bits);  // summed up over the lanes of the row up to this one
+      upto += __builtin_amdgcn_update_dpp(0, upto, 0x111, 0xf, 0xf, false);
+      upto += __builtin_amdgcn_update_dpp(0, upto, 0x112, 0xf, 0xf, false);
+      upto += __builtin_amdgcn_update_dpp(0, upto, 0x114, 0xf, 0xf, false);
+      upto += __builtin_amdgcn_update_dpp(0, upto, 0x118, 0xf, 0xf, false);
+      total = __builtin_amdgcn_update_dpp(0, upto, 0x15f, 0xf, 0xf, false);  // lane 15's
     }
-    float s = 0.0f, u = 0.0f, sr = 0.0f, ds = 0.0f, p[V * E];
-#pragma unroll
-    for (int i = 0; i < V * E; ++i) {
-      const bool here = i / E + 1 < V || mine[i % E];
-      t[i] -= top;
-      p[i] = exp_of(t[i]);
-      const bool has = !(p[i] == 0.0f);
-      const float ps = here ? p[i] : 0.0f;
-      if constexpr (kRef) {
-        const float q = d[i] - top_ref;
-        sr += here ? exp_of(q) : 0.0f;
-        d[i] = has ? t[i] - q : 0.0f;
-        ds = __builtin_fmaf(ps, d[i], ds);
+    const bool listed = kList && __all(total <= 2 * G);
+    float top = -INFINITY, top_ref = -INFINITY, s = 0.0f, u = 0.0f, sr = 0.0f, ds = 0.0f;
+    float xa = -INFINITY;
+    RowTerms x;
+    if (listed) {
+      uint8_t* list = lists[kList ? row : 0];
+      for (int to = upto - count; bits; ++to) {
+        const int k = __builtin_ctz(bits);
+        bits &= bits - 1;
+        list[to] = (uint8_t)(k / E * (G * E) + j * E + k % E);
       }
-      t[i] = has ? t[i] : 0.0f;
-      s += ps;
-      u = __builtin_fmaf(ps, t[i], u);
+      wavefront_sync();
+      int slot[2];
+      float t[2], d[2], p[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const bool there = j + G * h < total;
+        slot[h] = there ? list[j + G * h] : -2;
+        t[h] = there ? T::to_float(zl[slot[h]]) : -INFINITY;
+        top = fmaxf(top, t[h]);
+        if constexpr (kRef) {
+          d[h] = there ? T::to_float(ql[slot[h]]) : -INFINITY;
+          top_ref = fmaxf(top_ref, d[h]);
+        }
+      }
+      top = group_max<G>(top);
+      const Scale scale = scale_for(top);
+      Scale scale_ref{};
+      if constexpr (kRef) scale_ref = scale_for(group_max<G>(top_ref));
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        t[h] = scale(t[h]);
+        xa = slot[h] == slot_of_act ? t[h] : xa;
+        p[h] = exp2_of(t[h]);
+        const bool has = !(p[h] == 0.0f);
+        if constexpr (kRef) {
+          const float tr = scale_ref(d[h]);
+          sr += exp2_of(tr);
+          d[h] = has ? t[h] - tr : 0.0f;
+          ds = __builtin_fmaf(p[h], d[h], ds);
+        }
+        t[h] = has ? t[h] : 0.0f;
+        s += p[h];
+        u = __builtin_fmaf(p[h], t[h], u);
+      }
+      s = group_sum<G>(s);
+      u = group_sum<G>(u);
+      xa = group_max<G>(xa);
+      if constexpr (kRef) {
+        ds = group_sum<G>(ds);
+        sr = group_sum<G>(sr);
+      }
+      x = row_terms<kRef>(g, in, top > -INFINITY, s, u, ds, sr, xa);
+      if (g.d_logits) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          *reinterpret_cast<Raw<kBytes>*>(zl + (i * G + j) * E) = Raw<kBytes>{};
+        __builtin_amdgcn_wave_barrier();  // LDS takes a wavefront's accesses in order
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float f = __builtin_fmaf(x.c, t[h], x.a);
+          if constexpr (kRef) f = __builtin_fmaf(x.b, d[h], f);
+          f = __builtin_fmaf(p[h], f, -(slot[h] == slot_of_act ? x.pull : 0.0f));
+          if (slot[h] >= 0 && x.live) zl[slot[h]] = T::from_float(f);
+        }
+        wavefront_sync();
+      }
+    } else {
+      wavefront_sync();
+      // vector i of the lane, illegal elements at -inf
+      const auto logits = [&](int i, float (&z)[E], float (&q)[E]) {
+        const Slots zv = *reinterpret_cast<const Slots*>(zl + (i * G + j) * E);
+        Slots qv;
+        if constexpr (kRef) qv = *reinterpret_cast<const Slots*>(ql + (i * G + j) * E);
+        const uint32_t on = bits >> (E * i);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          z[e] = on >> e & 1 ? T::to_float(zv.v[e]) : -INFINITY;
+          q[e] = kRef && on >> e & 1 ? T::to_float(qv.v[e]) : -INFINITY;
+        }
+      };
+      float z[E], q[E];
+#pragma unroll 1
+      for (int i = 0; i < V; ++i) {
+        logits(i, z, q);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          top = fmaxf(top, z[e]);
+          if constexpr (kRef) top_ref = fmaxf(top_ref, q[e]);
+        }
+      }
+      top = group_max<G>(top);
+      const Scale scale = scale_for(top);
+      Scale scale_ref{};
+      if constexpr (kRef) scale_ref = scale_for(group_max<G>(top_ref));
+#pragma unroll 1
+      for (int i = 0; i < V; ++i) {
+        logits(i, z, q);
+        const int k = (i * G + j) * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float t = scale(z[e]);
+          xa = k + e == slot_of_act ? t : xa;
+          const float p = exp2_of(t);
+          const bool has = !(p == 0.0f);
+          if constexpr (kRef) {
+            const float tr = scale_ref(q[e]);
+            sr += exp2_of(tr);
+            ds = __builtin_fmaf(p, has ? t - tr : 0.0f, ds);
+          }
+          s += p;
+          u = __builtin_fmaf(p, has ? t : 0.0f, u);
+        }
+      }
+      s = group_sum<G>(s);
+      u = group_sum<G>(u);
+      xa = group_max<G>(xa);
+      if constexpr (kRef) {
+        ds = group_sum<G>(ds);
+        sr = group_sum<G>(sr);
+      }
+      x = row_terms<kRef>(g, in, top > -INFINITY, s, u, ds, sr, xa);
+      if (g.d_logits) {
+#pragma unroll 1
+        for (int i = 0; i < V; ++i) {
+          logits(i, z, q);
+          const int k = (i * G + j) * E;
+          Slots o;
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const float t = scale(z[e]);
+            const float p = exp2_of(t);
+            const bool has = !(p == 0.0f);
+            float h = __builtin_fmaf(x.c, has ? t : 0.0f, x.a);
+            if constexpr (kRef) h = __builtin_fmaf(x.b, has ? t - scale_ref(q[e]) : 0.0f, h);
+            const float f = __builtin_fmaf(p, h, -(k + e == slot_of_act && has ? x.pull : 0.0f));
+            o.v[e] = T::from_float(x.live ? f : 0.0f);
+          }
+          *reinterpret_cast<Slots*>(zl + k) = o;  // where this lane alone reads it
+        }
+      }
     }
-    s = group_sum<G>(s);
-    u = group_sum<G>(u);
-    float ref_log = 0.0f;
-    if constexpr (kRef) {
-      ds = group_sum<G>(ds);
-      ref_log = __builtin_amdgcn_logf(group_sum<G>(sr)) * kLn2;
+    if (g.d_logits && ok) {
+      S* ob = static_cast<S*>(g.d_logits) + r0 * g.d_stride;
+      const uint32_t o_at = i0 * (uint32_t)g.d_stride;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int k = (i * G + j) * E;
+        if (k + E <= g.actions) {
+          reinterpret_cast<RawAny<kBytes>*>(element(ob, o_at + (uint32_t)k))->v =
+              *reinterpret_cast<const Raw<kBytes>*>(zl + k);
+        } else if (i + 1 == V && k < g.actions) {  // the moved vector: its own elements
+#pragma unroll
+          for (int e = 1; e < E; ++e)
+            if (last + e >= at) *element(ob, o_at + (uint32_t)(last + e)) = zl[k + e];
+        }
+      }
     }
-    const RowTerms x = row_terms<kRef>(g, r, some, s, u, ds, ref_log,
-                                       taken ? za - top : -INFINITY);
+    wavefront_sync();  // the next rows' logits come after these reads
     float stat = x.stat[5];
 #pragma unroll
     for (int k = 0; k < kStats - 1; ++k) stat = j == k ? x.stat[k] : stat;
     acc += ok ? (double)stat : 0.0;
-    if (!ok) continue;
-    if (j == 0) {
-      g.logp[r] = x.logp;
-      if (g.d_value) store_value(g.d_value, g.value_dtype, r, x.d_value);
-    }
-    if (g.d_logits) {
-      S* out = static_cast<S*>(g.d_logits) + r * g.d_stride;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int k = i + 1 < V ? (i * G + j) * E : last;
-        Any<S, E> o;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const int m = i * E + e;
-          float h = __builtin_fmaf(x.c, t[m], x.a);
-          if constexpr (kRef) h = __builtin_fmaf(x.b, d[m], h);
-          const float hit = act == k + e ? x.pull : 0.0f;
-          const float f = __builtin_fmaf(p[m], h, -hit);
-          o.v[e] = T::from_float(x.live ? f : 0.0f);
-        }
-        if (i + 1 < V || any_mine) *reinterpret_cast<Any<S, E>*>(out + k) = o;
-      }
+    if (ok && j == 0) {
+      (g.logp + r0)[i0] = x.logp;
+      if (g.d_value)
+        store_value(const_cast<void*>(at_row(g.d_value, g.value_dtype, r0)), g.value_dtype, i0,
+                    x.d_value);
     }
   }
   write_partials<G>(acc, j, g.partials);
 }
 
-// Longer rows: a workgroup a row, in two passes over it.  The first keeps each thread's
-// running maximum and the sums under it, moved along with the maximum; the second reads the
-// row again, from the caches, for the gradient.
+// Longer rows: a workgroup a row.
 
-// The factor that a move of the maximum by `move` (<= 0) puts on sums of e^t, and a sum of
-// e^t t moved so; s is the sum of e^t.  What underflows is dropped, whatever it was: logits of
-// the type's lowest value make infinities of such a sum until an ordinary one comes.
-__device__ inline float moved(float f, float u, float s, float move) {
-  return f == 0.0f ? 0.0f : f * __builtin_fmaf(s, move, u);
+// E actions from action c on as a thread holds them, as they were read: from c, or where the row
+// ends before c + E its last E, of which those before c are another thread's.  Those and the
+// illegal ones are put to -inf.
+template <class T, bool kRef>
+struct Piece {
+  using S = typename T::storage;
+  static constexpr int E = 16 / sizeof(S);
+  static constexpr int kPer = E / 4;  // elements a word
+  Words4 z, q;
+
+  // Element e of w at -inf.
+  __device__ static void drop(Words4& w, int e) {
+    constexpr uint32_t kOnes = sizeof(S) == 4 ? 0xffffffffu : 0xffffu;
+    const int at = sizeof(S) == 4 ? 0 : 16 * (e % kPer);
+    w[e / kPer] = (w[e / kPer] & ~(kOnes << at)) | (T::kNone << at);
+  }
+  // first: where the E elements start, min(c, actions - E).
+  __device__ void read(const S* zs, const S* qs, const uint8_t* ls, int c, int first) {
+    z = reinterpret_cast<const RawAny<16>*>(element(zs, (uint32_t)first))->v;
+    if constexpr (kRef) q = reinterpret_cast<const RawAny<16>*>(element(qs, (uint32_t)first))->v;
+    uint32_t gone = (1u << (c - first)) - 1u;  // elements to drop
+    if (ls) {
+      const Raw<E> on = reinterpret_cast<const RawAny<E>*>(ls + (uint32_t)first)->v;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        uint32_t word;
+        if constexpr (E == 4) word = on;
+        else word = on[e / 4];
+        gone |= (word & (0xffu << (8 * (e % 4))) ? 0u : 1u) << e;
+      }
+    }
+    if (gone == 0) return;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (!(gone >> e & 1)) continue;
+      drop(z, e);
+      if constexpr (kRef) drop(q, e);
+    }
+  }
+  __device__ void values(float (&zf)[E], float (&qf)[E]) const {
+    unpack<T>(z, zf);
+    if constexpr (kRef) unpack<T>(q, qf);
+  }
+  // The values are unpacked again where they are used next, and not kept instead.
+  __device__ void forget() {
+    asm volatile("" : "+v"(z));
+    if constexpr (kRef) asm volatile("" : "+v"(q));
+  }
+};
+
+// The largest of each of kN numbers over the workgroup, in every thread.
+template <int kWide, int kN>
+__device__ inline void workgroup_max(float (&x)[kN], float (*shared)[kN]) {
+#pragma unroll
+  for (int i = 0; i < kN; ++i) x[i] = group_max<64>(x[i]);
+  if (threadIdx.x % 64 == 0) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) shared[threadIdx.x / 64][i] = x[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kWide / 64; ++k) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) x[i] = fmaxf(x[i], shared[k][i]);
+  }
 }
 
+template <int kWide>
+__device__ inline void workgroup_sums(float (&x)[4], float (*shared)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = group_sum<64>(x[i]);
+  if (threadIdx.x % 64 == 0)
+    *reinterpret_cast<float4*>(shared[threadIdx.x / 64]) = make_float4(x[0], x[1], x[2], x[3]);
+  __syncthreads();
+  x[0] = x[1] = x[2] = x[3] = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kWide / 64; ++k) {
+    const float4 w = *reinterpret_cast<const float4*>(shared[k]);
+    x[0] += w.x, x[1] += w.y, x[2] += w.z, x[3] += w.w;
+  }
+}
+
+// A row's terms and its outputs other than the gradient of the logits.  sums: of 2^x, 2^x x,
+// 2^x d and 2^x'.
 template <class T, bool kRef>
-__global__ __launch_bounds__(kThreads) void loss_wide_kernel(const LossArgs g) {
+__device__ inline RowTerms finish_row(const LossArgs& g, i64 r, i64 act, const RowInputs& in,
+                                      bool some, const Scale& scale, const float (&sums)[4],
+                                      double& acc) {
   using S = typename T::storage;
-  constexpr int E = 16 / sizeof(S);
-  constexpr int kWaves = kThreads / 64;
-  __shared__ float shared[kWaves][6];
+  const S* zs = static_cast<const S*>(g.logits) + r * g.logits_stride;
+  const bool inside = act >= 0 && act < g.actions;
+  const bool taken = inside && (!g.legal || g.legal[r * g.legal_stride + act]);
+  const float za = T::to_float(zs[inside ? act : 0]);
+  const RowTerms x = row_terms<kRef>(g, in, some, sums[0], sums[1], sums[2], sums[3],
+                                     taken ? scale(za) : -INFINITY);
+  float stat = x.stat[5];
+#pragma unroll
+  for (int k = 0; k < kStats - 1; ++k) stat = (int)threadIdx.x == k ? x.stat[k] : stat;
+  acc += (double)stat;
+  if (threadIdx.x == 0) {
+    g.logp[r] = x.logp;
+    if (g.d_value)
+      store_value(const_cast<void*>(at_row(g.d_value, g.value_dtype, r)), g.value_dtype, 0,
+                  x.d_value);
+  }
+  return x;
+}
+
+// The sums over a piece: of 2^x, 2^x x, 2^x d and 2^x'.  kFinite: no x or x' is -inf or so far
+// from the others that its difference is (see loss_held_kernel).
+template <bool kRef, bool kFinite, int E>
+__device__ inline void add_sums(const float (&z)[E], const float (&q)[E], const Scale& scale,
+                                const Scale& scale_ref, float (&sums)[4]) {
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float t = scale(z[e]);
+    const float p = exp2_of(t);
+    const bool has = kFinite || !(p == 0.0f);
+    sums[0] += p;
+    sums[1] = __builtin_fmaf(p, has ? t : 0.0f, sums[1]);
+    if constexpr (kRef) {
+      const float tr = scale_ref(q[e]);
+      sums[2] = __builtin_fmaf(p, has ? t - tr : 0.0f, sums[2]);
+      sums[3] += exp2_of(tr);
+    }
+  }
+}
+
+// The gradients of a piece's actions.
+template <class T, bool kRef, bool kFinite, int E>
+__device__ inline void store_gradients(const LossArgs& g, typename T::storage* out, int c, i64 act,
+                                       const RowTerms& x, const float (&z)[E],
+                                       const float (&q)[E], const Scale& scale,
+                                       const Scale& scale_ref, int first) {
+  using S = typename T::storage;
+  float f[E];
+  const float bc = x.b + x.c;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float t = scale(z[e]);
+    const float p = exp2_of(t);
+    float h;
+    if constexpr (kFinite) {
+      h = __builtin_fmaf(bc, t, x.a);  // a + b (t - t') + c t
+      if constexpr (kRef) h = __builtin_fmaf(-x.b, scale_ref(q[e]), h);
+    } else {
+      const bool has = !(p == 0.0f);
+      h = __builtin_fmaf(x.c, has ? t : 0.0f, x.a);
+      if constexpr (kRef) h = __builtin_fmaf(x.b, has ? t - scale_ref(q[e]) : 0.0f, h);
+    }
+    f[e] = p * h;
+  }
+  const i64 at = act - first;
+  if (at >= 0 && at < E) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] -= at == e ? x.pull : 0.0f;
+  }
+  if (!x.live) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] = 0.0f;
+  }
+  Vec<S, E> o;
+#pragma unroll
+  for (int e = 0; e < E; ++e) o.v[e] = T::from_float(f[e]);
+  if (c == first) {
+    reinterpret_cast<RawAny<16>*>(element(out, (uint32_t)c))->v = __builtin_bit_cast(Words4, o);
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (first + e >= c) out[first + e] = o.v[e];
+  }
+}
+
+// Rows of up to kWide P E actions: the row stays in registers, as it was read, through a pass
+// for the largest logit, one for the sums and one for the gradient; so memory sees it once.
+// Arithmetic comes next to memory in what bounds it (16 instructions an action and pass with a
+// KL term, of which the exponentials take four cycles' worth each), so a row whose logits are all
+// within 2^100 of its largest, as a row without masked entries is, leaves out the tests for 0 times
+// infinity.  XX
+template <class T, int kWide, int P, bool kRef>
+__global__ __launch_bounds__(kWide) __attribute__((amdgpu_waves_per_eu(4))) void loss_held_kernel(
+    const LossArgs g) {
+  using S = typename T::storage;
+  constexpr int E = Piece<T, kRef>::E;
+  __shared__ float tops[kWide / 64][4];
+  __shared__ __align__(16) float totals[kWide / 64][4];
   double acc = 0.0;
   for (i64 r = blockIdx.x; r < g.n; r += gridDim.x) {
     const S* zs = static_cast<const S*>(g.logits) + r * g.logits_stride;
     const S* qs = static_cast<const S*>(g.ref) + (kRef ? r * g.ref_stride : 0);
     const uint8_t* ls = g.legal ? g.legal + r * g.legal_stride : nullptr;
-    float top = -INFINITY, s = 0.0f, u = 0.0f, top_ref = -INFINITY, sr = 0.0f, ds = 0.0f;
-    // E elements from action c on, or the row's last E where it ends before c + E
-    auto read = [&](int c, int& k, float (&z)[E], float (&q)[E]) {
-      k = min(c, g.actions - E);
-      const Any<S, E> zv = *reinterpret_cast<const Any<S, E>*>(zs + k);
-      Any<S, E> qv;
-      if constexpr (kRef) qv = *reinterpret_cast<const Any<S, E>*>(qs + k);
-      Any<uint8_t, E> lv;
-      if (ls) lv = *reinterpret_cast<const Any<uint8_t, E>*>(ls + k);
+    // strips of kWide E actions: whole ones, and a last one that may end inside
+    constexpr int kStrip = kWide * E;
+    const int whole = min(g.actions / kStrip, P - 1);
+    const int mine = (int)threadIdx.x * E;
+    const int tail_at = whole * kStrip + mine, tail_first = min(tail_at, g.actions - E);
+    const bool in_tail = tail_at < g.actions;
+    Piece<T, kRef> piece[P - 1], tail;
+#pragma unroll
+    for (int i = 0; i < P - 1; ++i)
+      if (i < whole)
+        piece[i].read(zs + i * kStrip, qs + (kRef ? i * kStrip : 0), ls ? ls + i * kStrip : ls, mine,
+                      mine);
+    if (in_tail) tail.read(zs, qs, ls, tail_at, tail_first);
+    const i64 act = g.action[r];
+    const RowInputs in = row_inputs(g, r, 0);
+    float z[E], q[E];
+    // the largest logits, and the smallest with their signs turned
+    float ends[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    const auto find_ends = [&](Piece<T, kRef>& held) {
+      held.values(z, q);
+      float low = INFINITY, low_ref = INFINITY;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const bool on = !ls || lv.v[e] != 0;
-        z[e] = on ? T::to_float(zv.v[e]) : -INFINITY;
-        if constexpr (kRef) q[e] = on ? T::to_float(qv.v[e]) : -INFINITY;
+        ends[0] = fmaxf(ends[0], z[e]);
+        low = fminf(low, z[e]);
+        if constexpr (kRef) {
+          ends[1] = fmaxf(ends[1], q[e]);
+          low_ref = fminf(low_ref, q[e]);
+        }
+      }
+      ends[2] = fmaxf(ends[2], -low);
+      if constexpr (kRef) ends[3] = fmaxf(ends[3], -low_ref);
+      held.forget();
+    };
+#pragma unroll
+    for (int i = 0; i < P - 1; ++i)
+      if (i < whole) find_ends(piece[i]);
+    if (in_tail) find_ends(tail);
+    workgroup_max<kWide, 4>(ends, tops);
+    const bool some = ends[0] > -INFINITY;
+    const bool finite = ends[0] + ends[2] < 0x1p100f && (!kRef || ends[1] + ends[3] < 0x1p100f);
+    const Scale scale = scale_for(ends[0]), scale_ref = scale_for(ends[1]);
+    float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const auto add = [&](auto is_finite) {
+      const auto of = [&](Piece<T, kRef>& held) {
+        held.values(z, q);
+        add_sums<kRef, decltype(is_finite)::value, E>(z, q, scale, scale_ref, sums);
+        held.forget();
+      };
+#pragma unroll
+      for (int i = 0; i < P - 1; ++i)
+        if (i < whole) of(piece[i]);
+      if (in_tail) of(tail);
+    };
+    if (finite) add(std::true_type{});
+    else add(std::false_type{});
+    workgroup_sums<kWide>(sums, totals);
+    const RowTerms x = finish_row<T, kRef>(g, r, act, in, some, scale, sums, acc);
+    if (!g.d_logits) continue;
+    S* out = static_cast<S*>(g.d_logits) + r * g.d_stride;
+    const auto store = [&](auto is_finite) {
+      constexpr bool kFinite = decltype(is_finite)::value;
+#pragma unroll
+      for (int i = 0; i < P - 1; ++i) {
+        if (i >= whole) continue;
+        piece[i].values(z, q);
+        store_gradients<T, kRef, kFinite, E>(g, out + i * kStrip, mine, act - i * kStrip, x, z, q,
+                                             scale, scale_ref, mine);
+      }
+      if (in_tail) {
+        tail.values(z, q);
+        store_gradients<T, kRef, kFinite, E>(g, out, tail_at, act, x, z, q, scale, scale_ref,
+                                             tail_first);
       }
     };
-    for (int c = threadIdx.x * E; c < g.actions; c += kThreads * E) {
-      int k;
-      float z[E], q[E];
-      read(c, k, z, q);
+    if (finite) store(std::true_type{});
+    else store(std::false_type{});
+  }
+  // lanes 0 .. kStats - 1 of the workgroup hold its sums
+  if (threadIdx.x < kStats) g.partials[(i64)blockIdx.x * kStats + threadIdx.x] = acc;
+}
+
+// Rows of any length, in two passes over memory.  The first keeps each thread's running maximum
+// and the sums under it, moved along with the maximum; the second reads the row again for the
+// gradient.
+
+// A sum of 2^x y moved by a change of maximum that puts the factor f on 2^x and adds `by` to y;
+// s is the sum of 2^x.  What underflows is dropped, whatever it was: logits of the type's lowest
+// value make infinities of such a sum until an ordinary one comes.
+__device__ inline float moved(float f, float sum, float s, float by) {
+  return f == 0.0f ? 0.0f : f * __builtin_fmaf(s, by, sum);
+}
+
+template <class T, int kWide, bool kRef>
+__global__ __launch_bounds__(kWide) void loss_long_kernel(const LossArgs g) {
+  using S = typename T::storage;
+  constexpr int E = Piece<T, kRef>::E;
+  __shared__ float tops[kWide / 64][2];
+  __shared__ __align__(16) float totals[kWide / 64][4];
+  double acc = 0.0;
+  for (i64 r = blockIdx.x; r < g.n; r += gridDim.x) {
+    const S* zs = static_cast<const S*>(g.logits) + r * g.logits_stride;
+    const S* qs = static_cast<const S*>(g.ref) + (kRef ? r * g.ref_stride : 0);
+    const uint8_t* ls = g.legal ? g.legal + r * g.legal_stride : nullptr;
+    const i64 act = g.action[r];
+    const RowInputs in = row_inputs(g, r, 0);
+    float top = -INFINITY, s = 0.0f, u = 0.0f, top_ref = -INFINITY, sr = 0.0f, ds = 0.0f;
+    Piece<T, kRef> piece;
+    float z[E], q[E];
+    for (int c = threadIdx.x * E; c < g.actions; c += kWide * E) {
+      const int first = min(c, g.actions - E);
+      piece.read(zs, qs, ls, c, first);
+      piece.values(z, q);
       float most = top, most_ref = top_ref;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         most = fmaxf(most, z[e]);
         if constexpr (kRef) most_ref = fmaxf(most_ref, q[e]);
       }
-      const float base = most > -INFINITY ? most : 0.0f;
-      const float f = exp_of(top - base);
-      float base_ref = 0.0f;
+      const Scale now = scale_for(most), now_ref = scale_for(most_ref);
+      const float by = now(top), f = exp2_of(by);
       if constexpr (kRef) {
-        base_ref = most_ref > -INFINITY ? most_ref : 0.0f;
-        ds = moved(f, ds, s, (top - base) - (top_ref - base_ref));
-        sr *= exp_of(top_ref - base_ref);
+        const float by_ref = now_ref(top_ref);
+        ds = moved(f, ds, s, by - by_ref);
+        sr *= exp2_of(by_ref);
         top_ref = most_ref;
       }
-      u = moved(f, u, s, top - base);
+      u = moved(f, u, s, by);
       s *= f;
       top = most;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const bool here = k + e >= c;
-        const float t = z[e] - base;
-        const float p = here ? exp_of(t) : 0.0f;
+        const float t = now(z[e]);
+        const float p = exp2_of(t);
         const bool has = !(p == 0.0f);
         s += p;
         u = __builtin_fmaf(p, has ? t : 0.0f, u);
         if constexpr (kRef) {
-          const float tr = q[e] - base_ref;
-          sr += here ? exp_of(tr) : 0.0f;
+          const float tr = now_ref(q[e]);
+          sr += exp2_of(tr);
           ds = __builtin_fmaf(p, has ? t - tr : 0.0f, ds);
         }
       }
     }
     // the threads' sums under the row's maximum
-    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-    __syncthreads();  // the last row's values have been read
-    float all = group_max<64>(top), all_ref = kRef ? group_max<64>(top_ref) : 0.0f;
-    if (lane == 0) shared[wave][0] = all, shared[wave][1] = all_ref;
-    __syncthreads();
-    for (int k = 0; k < kWaves; ++k) {
-      all = fmaxf(all, shared[k][0]);
-      all_ref = fmaxf(all_ref, shared[k][1]);
-    }
-    const bool some = all > -INFINITY;
-    all = some ? all : 0.0f;
-    const float f = exp_of(top - all);
-    u = group_sum<64>(moved(f, u, s, top - all));
+    float all[2] = {top, top_ref};
+    workgroup_max<kWide, 2>(all, tops);
+    const bool some = all[0] > -INFINITY;
+    const Scale scale = scale_for(all[0]), scale_ref = scale_for(all[1]);
+    const float by = scale(top), f = exp2_of(by);
+    float sums[4] = {s * f, moved(f, u, s, by), 0.0f, 0.0f};
     if constexpr (kRef) {
-      all_ref = all_ref > -INFINITY ? all_ref : 0.0f;
-      ds = group_sum<64>(moved(f, ds, s, (top - all) - (top_ref - all_ref)));
-      sr = group_sum<64>(sr * exp_of(top_ref - all_ref));
+      const float by_ref = scale_ref(top_ref);
+      sums[2] = moved(f, ds, s, by - by_ref);
+      sums[3] = sr * exp2_of(by_ref);
     }
-    s = group_sum<64>(s * f);
-    if (lane == 0) shared[wave][2] = s, shared[wave][3] = u, shared[wave][4] = ds, shared[wave][5] = sr;
-    __syncthreads();
-    s = u = ds = sr = 0.0f;
-    for (int k = 0; k < kWaves; ++k) {
-      s += shared[k][2];
-      u += shared[k][3];
-      ds += shared[k][4];
-      sr += shared[k][5];
-    }
-    const float ref_log = kRef ? __builtin_amdgcn_logf(sr) * kLn2 : 0.0f;
-    const i64 act = g.action[r];
-    const bool inside = act >= 0 && act < g.actions;
-    const bool taken = inside && (!ls || ls[act]);
-    const float za = T::to_float(zs[inside ? act : 0]);
-    const RowTerms x = row_terms<kRef>(g, r, some, s, u, ds, ref_log,
-                                       taken ? za - all : -INFINITY);
-    float stat = x.stat[5];
-#pragma unroll
-    for (int k = 0; k < kStats - 1; ++k) stat = (int)threadIdx.x == k ? x.stat[k] : stat;
-    acc += (double)stat;
-    if (threadIdx.x == 0) {
-      g.logp[r] = x.logp;
-      if (g.d_value) store_value(g.d_value, g.value_dtype, r, x.d_value);
-    }
-    if (g.d_logits) {
-      S* out = static_cast<S*>(g.d_logits) + r * g.d_stride;
-      for (int c = threadIdx.x * E; c < g.actions; c += kThreads * E) {
-        int k;
-        float z[E], q[E];
-        read(c, k, z, q);
-        Any<S, E> o;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float t = z[e] - all;
-          const float p = exp_of(t);
-          const bool has = !(p == 0.0f);
-          float h = __builtin_fmaf(x.c, has ? t : 0.0f, x.a);
-          if constexpr (kRef) h = __builtin_fmaf(x.b, has ? t - (q[e] - all_ref) : 0.0f, h);
-          const float hit = act == k + e ? x.pull : 0.0f;
-          const float v = __builtin_fmaf(p, h, -hit);
-          o.v[e] = T::from_float(x.live ? v : 0.0f);
-        }
-        *reinterpret_cast<Any<S, E>*>(out + k) = o;
-      }
+    workgroup_sums<kWide>(sums, totals);
+    const RowTerms x = finish_row<T, kRef>(g, r, act, in, some, scale, sums, acc);
+    if (!g.d_logits) continue;
+    S* out = static_cast<S*>(g.d_logits) + r * g.d_stride;
+    for (int c = threadIdx.x * E; c < g.actions; c += kWide * E) {
+      const int first = min(c, g.actions - E);
+      piece.read(zs, qs, ls, c, first);
+      piece.values(z, q);
+      store_gradients<T, kRef, false, E>(g, out, c, act, x, z, q, scale, scale_ref, first);
     }
   }
-  // lanes 0 .. kStats - 1 of the workgroup hold its sums
   if (threadIdx.x < kStats) g.partials[(i64)blockIdx.x * kStats + threadIdx.x] = acc;
 }
 
@@ -467,12 +892,24 @@ inline int groups_for(i64 tiles) {
   return (int)(tiles < cap ? tiles : cap);
 }
 
+// Rows of up to kRowsMost actions are addressed by 32 bits within a workgroup's 4 or 16 rows.
+constexpr int kRowsMost = 1024;
+constexpr i64 kStrideMost = (i64)1 << 24;
+
 template <class T, bool kRef>
 int launch_loss(const LossArgs& g, hipStream_t stream) {
   const auto rows = [&](auto kernel, int lanes) {
     const int per = kThreads / lanes;
     const int groups = groups_for((g.n + per - 1) / per);
     kernel<<<groups, kThreads, 0, stream>>>(g);
+    return groups;
+  };
+  // a workgroup a row: as many as are resident at once
+  const auto wide = [&](auto kernel, int threads) {
+    const i64 most = (i64)compute_units() * (2048 / threads);
+    const i64 cap = most < kMaxGroups ? most : kMaxGroups;
+    const int groups = (int)(g.n < cap ? g.n : cap);
+    kernel<<<groups, threads, 0, stream>>>(g);
     return groups;
   };
   const int a = g.actions;
@@ -483,8 +920,11 @@ int launch_loss(const LossArgs& g, hipStream_t stream) {
   if (a <= 256) return rows(loss_rows_kernel<T, 16, 4, 4, kRef>, 16);
   if (a <= 512) return rows(loss_rows_kernel<T, 64, 2, 4, kRef>, 64);
   if (a <= 768) return rows(loss_rows_kernel<T, 64, 3, 4, kRef>, 64);
-  if (a <= 1024) return rows(loss_rows_kernel<T, 64, 4, 4, kRef>, 64);
-  return rows(loss_wide_kernel<T, kRef>, kThreads);
+  if (a <= kRowsMost) return rows(loss_rows_kernel<T, 64, 4, 4, kRef>, 64);
+  constexpr int E = 16 / sizeof(typename T::storage);
+  if (a <= 256 * 4 * E) return wide(loss_held_kernel<T, 256, 4, kRef>, 256);
+  if (a <= 512 * 8 * E) return wide(loss_held_kernel<T, 512, 8, kRef>, 512);
+  return wide(loss_long_kernel<T, 1024, kRef>, 1024);
 }
 
 }  // namespace loss
@@ -503,6 +943,9 @@ int cugo_policy_loss(const CugoPolicyLoss* p, hipStream_t stream) {
   if (p->n > 0 && (!p->logits || !p->action || !p->old_logp || !p->advantage || !p->logp))
     return -1;
   if ((p->value != nullptr) != (p->returns != nullptr) || (p->d_value && !p->value)) return -1;
+  if (p->actions <= kRowsMost && (p->logits_stride >= kStrideMost || p->ref_stride >= kStrideMost ||
+                                  p->legal_stride >= kStrideMost || p->d_logits_stride >= kStrideMost))
+    return -4;
   LossArgs g{};
   g.logits = p->logits, g.ref = p->ref_logits, g.legal = p->legal;
   g.logits_stride = p->logits_stride, g.ref_stride = p->ref_stride;

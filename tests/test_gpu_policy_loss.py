@@ -7,7 +7,13 @@ most 16), and 16 for the exponential's and the logarithm's own last places (v_ex
 are good to one) and the differences around them.  A probability and a ratio then carry E
 relative to themselves; a gradient w p (pull + c_k (d - K) + c_e (l + H)) carries 4 E of w p times
 the sum of its parts' sizes, the taken action's w pull once more; stored, half a step of its type
-(or half of float16's smallest value)."""
+(or half of float16's smallest value).
+
+Exponents are formed as z k - round(top k): the rounding, u |top| k at most, is the same for all
+of a row.  It leaves l and K as it leaves the sums (both sides of a difference have it), but the
+parts of a gradient, which are differences x - mean and d - mean, keep the roundings of the mean:
+2 u of that shift, so 4 u (u |top| + u |top'|) of w p (c_k + c_e) at most, where a row of one action
+has nothing else."""
 
 from __future__ import annotations
 
@@ -78,11 +84,13 @@ def check(x, got, scale=1.0):
     z = x["logits"].double().masked_fill(~on, -math.inf)
     ell = ref.log_softmax(z).nan_to_num(nan=0, neginf=0, posinf=0)
     p = torch.where(on, ell.exp(), 0.0)
+    tops = [z.max(1).values.nan_to_num(nan=0, neginf=0)]
     size = torch.where(p > 1e-46, ell.abs(), 0.0)
     d = torch.zeros_like(ell)
     if x["ref"] is not None:
         q = x["ref"].double().masked_fill(~on, -math.inf)
         lq = ref.log_softmax(q).nan_to_num(nan=0, neginf=0, posinf=0)
+        tops.append(q.max(1).values.nan_to_num(nan=0, neginf=0))
         d = torch.where(p > 1e-46, (ell - lq).abs(), 0.0)
         size = torch.maximum(size, torch.where(p > 1e-46, lq.abs(), 0.0))
     err = U * (4 * size + adds + 16)          # E of each entry
@@ -122,6 +130,8 @@ def check(x, got, scale=1.0):
             parts = pull[:, None] + 0.3 * (d + (p * d).sum(1, keepdim=True)) + \
                 0.05 * (size + (p * size).sum(1, keepdim=True))
             t = 4 * p * parts * (err + row[:, None] + e_act[:, None])
+            shift = sum(torch.where(y.abs() < 1e30, y.abs(), 0.0) for y in tops)
+            t = t + p * 0.35 * 4 * U * U * shift[:, None]
             t.scatter_add_(1, x["action"].clamp(0, a - 1)[:, None],
                            (4 * pull * (e_act + 4 * U))[:, None])
             t = t * w[:, None] * abs(scale)
@@ -138,7 +148,8 @@ def check(x, got, scale=1.0):
 SIZES = [(5, 1), (9, 2), (6, 3), (7, 4), (3, 5), (17, 16), (5, 17), (4, 63), (4, 64), (4, 65),
          (3, 128), (3, 129), (40, 179), (3, 191), (3, 192), (3, 193), (3, 255), (3, 256), (3, 257),
          (2, 512), (5, 513), (2, 767), (2, 769), (3, 1024), (3, 1025), (2, 2047), (3, 2049),
-         (2, 4099), (1, 179), (1, 33001), (2, 8192)]
+         (2, 4099), (1, 179), (1, 33001), (2, 8192), (2, 8193), (1, 16384), (2, 16385), (1, 32768),
+         (1, 32769)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
@@ -153,7 +164,7 @@ def test_against_the_oracle(ext, n, a, dtype):
         check(x, call(ext, x, grad=False))
 
 
-@pytest.mark.parametrize("a", [2, 40, 179, 300, 1500])
+@pytest.mark.parametrize("a", [2, 40, 179, 300, 1500, 9000, 40000])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_special_entries(ext, a, dtype):
     """-inf, the type's lowest value, NaN and infinities in illegal places, rows whose legal
@@ -195,7 +206,7 @@ def test_special_entries(ext, a, dtype):
 
 
 def test_nan_in_a_legal_logit_shows(ext):
-    for a in (3, 179, 600, 2000):
+    for a in (3, 179, 600, 2000, 33000):
         for bad in (math.nan, math.inf):
             x = make(3, a, torch.float32, a, share=0.9, weight=False)
             x["legal"][0, 0] = True
