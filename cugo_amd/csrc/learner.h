@@ -96,7 +96,7 @@ __device__ inline float rotated(float x) {
   return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), kCtrl, 0xf, 0xf, false));
 }
 
-// The sum and the largest over groups of G lanes (16 or 64), the same value in every lane.
+// The sum and the largest over groups of G lanes (16, 32 or 64), the same value in every lane.
 // v_max_f32 takes the other operand for a NaN: a NaN shows in the sums of exponentials.
 template <int G>
 __device__ inline float group_sum(float x) {
@@ -104,10 +104,8 @@ __device__ inline float group_sum(float x) {
   x += rotated<0x124>(x);
   x += rotated<0x122>(x);
   x += rotated<0x121>(x);
-  if constexpr (G == 64) {
-    x += __shfl_xor(x, 16);
-    x += __shfl_xor(x, 32);
-  }
+  if constexpr (G >= 32) x += __shfl_xor(x, 16);
+  if constexpr (G == 64) x += __shfl_xor(x, 32);
   return x;
 }
 template <int G>
@@ -116,10 +114,8 @@ __device__ inline float group_max(float x) {
   x = fmaxf(x, rotated<0x124>(x));
   x = fmaxf(x, rotated<0x122>(x));
   x = fmaxf(x, rotated<0x121>(x));
-  if constexpr (G == 64) {
-    x = fmaxf(x, __shfl_xor(x, 16));
-    x = fmaxf(x, __shfl_xor(x, 32));
-  }
+  if constexpr (G >= 32) x = fmaxf(x, __shfl_xor(x, 16));
+  if constexpr (G == 64) x = fmaxf(x, __shfl_xor(x, 32));
   return x;
 }
 

@@ -187,10 +187,51 @@ __device__ inline void wavefront_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// What a row has besides its logits, for the rows of 16 lanes: lane 0 of the 16 reads the old
+// log-probability, lane 1 the advantage and so on, one access instead of six (the addresser, not
+// memory, is what short rows keep busy), and all take the values from those lanes.
+struct RowReader {
+  const char* base;
+  int shift;  // of the row's number
+
+  __device__ explicit RowReader(const LossArgs& g) {
+    const int k = threadIdx.x & 15;
+    const void* p = k == 1 ? g.advantage : g.old_logp;
+    p = k == 2 && g.returns ? static_cast<const void*>(g.returns) : p;
+    p = k == 3 && g.weight ? static_cast<const void*>(g.weight) : p;
+    p = k == 4 && g.value && g.value_dtype == CUGO_DTYPE_F32 ? g.value : p;
+    p = k == 5 ? static_cast<const void*>(g.action) : p;
+    p = k == 6 ? static_cast<const void*>(reinterpret_cast<const int32_t*>(g.action) + 1) : p;
+    base = static_cast<const char*>(p);
+    shift = k == 5 || k == 6 ? 3 : 2;
+  }
+  template <int kLane>
+  __device__ static int from(int x) {
+    return __builtin_amdgcn_update_dpp(0, x, 0x150 + kLane, 0xf, 0xf, false);
+  }
+  // Row r; lane's part of it, to be passed to inputs() once the row's logits are asked for too.
+  __device__ int read(i64 r) const { return *reinterpret_cast<const int*>(base + (r << shift)); }
+  __device__ RowInputs inputs(const LossArgs& g, int x, i64 r0, uint32_t i0, i64& act) const {
+    RowInputs in;
+    in.old = __int_as_float(from<0>(x));
+    in.adv = __int_as_float(from<1>(x));
+    in.w = g.weight ? __int_as_float(from<3>(x)) : g.even;
+    in.value = in.returns = 0.0f;
+    if (g.value) {
+      in.returns = __int_as_float(from<2>(x));
+      in.value = g.value_dtype == CUGO_DTYPE_F32
+                     ? __int_as_float(from<4>(x))
+                     : load_value(at_row(g.value, g.value_dtype, r0), g.value_dtype, i0);
+    }
+    act = (i64)(((uint64_t)(uint32_t)from<6>(x) << 32) | (uint32_t)from<5>(x));
+    return in;
+  }
+};
+
 // Rows of up to E V G actions (V in 1..4): G lanes a row, vector i of E elements of lane j at
 // action (i G + j) E, so that the row's lanes read one run of memory an instruction.  The last
 // vector of a row that ends inside it is read moved back, to end with the row; the elements that
-// it repeats of other lanes (`mine` false) count as illegal and are not stored.
+// it repeats of other lanes count as illegal here, and their gradients are stored twice, the same.
 // The row goes through LDS as it was read, in slots: an action's slot is its number, but in the
 // moved vector.  From there it is gone through for its largest logit, for its sums and for its
 // gradient, a vector of each lane at a time: kept in registers for that, a row of 179 actions
@@ -220,6 +261,7 @@ __global__ __launch_bounds__(kThreads) void loss_rows_kernel(const LossArgs g) {
   for (int e = 0; e < E; ++e) own |= (last + e >= at ? 1u : 0u) << (E * (V - 1) + e);
   S* zl = z_slots[row];
   S* ql = q_slots[kRef ? row : 0];
+  const RowReader reader(g);
   const i64 tiles = (g.n + kRows - 1) / kRows;
   double acc = 0.0;
   for (i64 tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
@@ -227,8 +269,7 @@ __global__ __launch_bounds__(kThreads) void loss_rows_kernel(const LossArgs g) {
     const bool ok = r0 + row < g.n;
     // loads are unconditional, of a row that exists; the sums leave it out
     const uint32_t i0 = (uint32_t)(ok ? row : (int)(g.n - 1 - r0));
-    const i64 act = (g.action + r0)[i0];
-    const RowInputs in = row_inputs(g, r0, i0);
+    const int part = reader.read(r0 + i0);
     uint32_t bits = own;
     {
       const S* zb = static_cast<const S*>(g.logits) + r0 * g.logits_stride;
@@ -274,7 +315,9 @@ __global__ __launch_bounds__(kThreads) void loss_rows_kernel(const LossArgs g) {
         if constexpr (kRef) *reinterpret_cast<Raw<kBytes>*>(ql + k) = q[i];
       }
     }
-    // the action's slot, where the row has it: its lane, and the bit of it there
+    i64 act;
+    const RowInputs in = reader.inputs(g, part, r0, i0, act);
+    // the action's slot, where the row has it
     const int moved_from = g.actions & ~(E - 1);
     const int slot_of_act = act < 0 || act >= g.actions ? -1
                             : (int)act >= moved_from   ? (int)act + E - (g.actions & (E - 1))
@@ -426,8 +469,9 @@ __global__ __launch_bounds__(kThreads) void loss_rows_kernel(const LossArgs g) {
             const float f = __builtin_fmaf(p, h, -(k + e == slot_of_act && has ? x.pull : 0.0f));
             o.v[e] = T::from_float(x.live ? f : 0.0f);
           }
-          *reinterpret_cast<Slots*>(zl + k) = o;  // where this lane alone reads it
+          *reinterpret_cast<Slots*>(zl + k) = o;  // where this lane alone has read
         }
+        wavefront_sync();
       }
     }
     if (g.d_logits && ok) {
@@ -436,14 +480,16 @@ __global__ __launch_bounds__(kThreads) void loss_rows_kernel(const LossArgs g) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const int k = (i * G + j) * E;
-        if (k + E <= g.actions) {
-          reinterpret_cast<RawAny<kBytes>*>(element(ob, o_at + (uint32_t)k))->v =
-              *reinterpret_cast<const Raw<kBytes>*>(zl + k);
-        } else if (i + 1 == V && k < g.actions) {  // the moved vector: its own elements
+        Raw<kBytes> o = *reinterpret_cast<const Raw<kBytes>*>(zl + k);
+        if (i + 1 == V && k < g.actions && k > last) {
+          // the moved vector again: what it repeats lies in those elements' own slots
+          Slots m;
 #pragma unroll
-          for (int e = 1; e < E; ++e)
-            if (last + e >= at) *element(ob, o_at + (uint32_t)(last + e)) = zl[k + e];
+          for (int e = 0; e < E; ++e) m.v[e] = zl[last + e < at ? last + e : k + e];
+          o = __builtin_bit_cast(Raw<kBytes>, m);
         }
+        if (k < g.actions)
+          reinterpret_cast<RawAny<kBytes>*>(element(ob, o_at + (uint32_t)(i + 1 < V ? k : last)))->v = o;
       }
     }
     wavefront_sync();  // the next rows' logits come after these reads
@@ -896,11 +942,15 @@ __global__ __launch_bounds__(kThreads) void scale_kernel(int a_dtype, void* a, i
   scale_any(b_dtype, b, b_count, f);
 }
 
-// The workgroups of a launch over `tiles` pieces of work: as many as are resident at once.
-inline int groups_for(i64 tiles) {
-  const i64 most = (i64)compute_units() * 8;
+// A workgroup for each of `pieces` of work, or as many as can be resident at once, which then go
+// round.
+template <auto kKernel>
+int launch_rows(const LossArgs& g, i64 pieces, int threads, hipStream_t stream) {
+  const i64 most = (i64)compute_units() * (2048 / threads);
   const i64 cap = most < kMaxGroups ? most : kMaxGroups;
-  return (int)(tiles < cap ? tiles : cap);
+  const int groups = (int)(pieces < cap ? pieces : cap);
+  kKernel<<<groups, threads, 0, stream>>>(g);
+  return groups;
 }
 
 // Rows of up to kRowsMost actions are addressed by 32 bits within a workgroup's 4 or 16 rows.
@@ -909,33 +959,30 @@ constexpr i64 kStrideMost = (i64)1 << 24;
 
 template <class T, bool kRef>
 int launch_loss(const LossArgs& g, hipStream_t stream) {
-  const auto rows = [&](auto kernel, int lanes) {
-    const int per = kThreads / lanes;
-    const int groups = groups_for((g.n + per - 1) / per);
-    kernel<<<groups, kThreads, 0, stream>>>(g);
-    return groups;
-  };
-  // a workgroup a row: as many as are resident at once
-  const auto wide = [&](auto kernel, int threads) {
-    const i64 most = (i64)compute_units() * (2048 / threads);
-    const i64 cap = most < kMaxGroups ? most : kMaxGroups;
-    const int groups = (int)(g.n < cap ? g.n : cap);
-    kernel<<<groups, threads, 0, stream>>>(g);
-    return groups;
-  };
-  const int a = g.actions;
-  if (a < 4) return rows(loss_rows_kernel<T, 16, 1, 1, kRef>, 16);
-  if (a <= 64) return rows(loss_rows_kernel<T, 16, 1, 4, kRef>, 16);
-  if (a <= 128) return rows(loss_rows_kernel<T, 16, 2, 4, kRef>, 16);
-  if (a <= 192) return rows(loss_rows_kernel<T, 16, 3, 4, kRef>, 16);
-  if (a <= 256) return rows(loss_rows_kernel<T, 16, 4, 4, kRef>, 16);
-  if (a <= 512) return rows(loss_rows_kernel<T, 64, 2, 4, kRef>, 64);
-  if (a <= 768) return rows(loss_rows_kernel<T, 64, 3, 4, kRef>, 64);
-  if (a <= kRowsMost) return rows(loss_rows_kernel<T, 64, 4, 4, kRef>, 64);
   constexpr int E = 16 / sizeof(typename T::storage);
-  if (a <= 256 * 4 * E) return wide(loss_held_kernel<T, 256, 4, kRef>, 256);
-  if (a <= 512 * 8 * E) return wide(loss_held_kernel<T, 512, 8, kRef>, 512);
-  return wide(loss_long_kernel<T, 1024, kRef>, 1024);
+  const int a = g.actions;
+#define CUGO_LOSS_ROWS(G, V, E)                                             \
+  launch_rows<loss_rows_kernel<T, G, V, E, kRef>>(                          \
+      g, (g.n + kThreads / G - 1) / (kThreads / G), kThreads, stream)
+#define CUGO_LOSS_HELD(THREADS, P) \
+  launch_rows<loss_held_kernel<T, THREADS, P, kRef>>(g, g.n, THREADS, stream)
+  if (a < 4) return CUGO_LOSS_ROWS(16, 1, 1);
+  if (a <= 64) return CUGO_LOSS_ROWS(16, 1, 4);
+  if (a <= 128) return CUGO_LOSS_ROWS(16, 2, 4);
+  if (a <= 192) return CUGO_LOSS_ROWS(16, 3, 4);
+  if (a <= 256) return CUGO_LOSS_ROWS(16, 4, 4);
+  if (a <= 384) return CUGO_LOSS_ROWS(32, 3, 4);
+  if (a <= 512) return CUGO_LOSS_ROWS(32, 4, 4);
+  if (a <= 768) return CUGO_LOSS_ROWS(64, 3, 4);
+  if (a <= kRowsMost) return CUGO_LOSS_ROWS(64, 4, 4);
+  if (a <= 64 * 4 * E) return CUGO_LOSS_HELD(64, 4);
+  if (a <= 128 * 4 * E) return CUGO_LOSS_HELD(128, 4);
+  if (a <= 256 * 4 * E) return CUGO_LOSS_HELD(256, 4);
+  if (a <= 512 * 4 * E) return CUGO_LOSS_HELD(512, 4);
+  if (a <= 512 * 8 * E) return CUGO_LOSS_HELD(512, 8);
+#undef CUGO_LOSS_ROWS
+#undef CUGO_LOSS_HELD
+  return launch_rows<loss_long_kernel<T, 1024, kRef>>(g, g.n, 1024, stream);
 }
 
 }  // namespace loss

@@ -147,7 +147,7 @@ def check(x, got, scale=1.0):
 
 SIZES = [(5, 1), (9, 2), (6, 3), (7, 4), (3, 5), (17, 16), (5, 17), (4, 63), (4, 64), (4, 65),
          (3, 128), (3, 129), (40, 179), (3, 191), (3, 192), (3, 193), (3, 255), (3, 256), (3, 257),
-         (2, 512), (5, 513), (2, 767), (2, 769), (3, 1024), (3, 1025), (2, 2047), (3, 2049),
+         (3, 383), (3, 385), (2, 512), (5, 513), (2, 767), (2, 769), (3, 1024), (3, 1025), (2, 2047), (2, 2048), (3, 2049), (2, 4096), (2, 4097),
          (2, 4099), (1, 179), (1, 33001), (2, 8192), (2, 8193), (1, 16384), (2, 16385), (1, 32768),
          (1, 32769)]
 
