@@ -222,16 +222,51 @@ std::vector<torch::Tensor> advantages(torch::Tensor reward, torch::Tensor value,
   return {adv, ret};
 }
 
+// A Python list of tensors (None where `optional`), read in place: converting one into a vector of
+// tensors takes as long as launching a kernel for a model's parameters and their states.
+class TensorList {
+ public:
+  TensorList(const pybind11::handle& list, const char* name, bool optional) {
+    TORCH_CHECK(PyList_Check(list.ptr()), name, " must be a list of tensors");
+    const Py_ssize_t n = PyList_GET_SIZE(list.ptr());
+    items_.reserve((size_t)n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      PyObject* item = PyList_GET_ITEM(list.ptr(), i);
+      if (optional && item == Py_None) {
+        items_.push_back(nullptr);
+        continue;
+      }
+      TORCH_CHECK(THPVariable_Check(item), name, " must be a list of tensors");
+      items_.push_back(&THPVariable_Unpack(item));
+    }
+  }
+  size_t size() const { return items_.size(); }
+  bool has(size_t i) const { return items_[i] != nullptr; }
+  const torch::Tensor& operator[](size_t i) const { return *items_[i]; }
+
+ private:
+  std::vector<const torch::Tensor*> items_;
+};
+
 // One step of every tensor with a gradient, in place (cugo_adamw); the gradients' norm with
 // max_norm, else None.
-Optional adamw_step(std::vector<torch::Tensor> params, std::vector<Optional> grads,
-                    std::vector<torch::Tensor> exp_avg, std::vector<torch::Tensor> exp_avg_sq,
-                    torch::Tensor steps, std::vector<double> lr, std::vector<double> weight_decay,
-                    double beta1, double beta2, double eps, c10::optional<double> max_norm,
-                    c10::optional<std::vector<Optional>> master,
-                    c10::optional<std::vector<torch::Tensor>> exp_avg_scale,
-                    c10::optional<std::vector<torch::Tensor>> exp_avg_sq_scale,
-                    Optional lr_scale, int64_t seed) {
+Optional adamw_step(const pybind11::list& params_list, const pybind11::list& grads_list,
+                    const pybind11::list& exp_avg_list, const pybind11::list& exp_avg_sq_list,
+                    torch::Tensor steps, const std::vector<double>& lr,
+                    const std::vector<double>& weight_decay, double beta1, double beta2, double eps,
+                    c10::optional<double> max_norm, const pybind11::object& master_list,
+                    const pybind11::object& exp_avg_scale_list,
+                    const pybind11::object& exp_avg_sq_scale_list, Optional lr_scale,
+                    int64_t seed) {
+  const TensorList params(params_list, "params", false), grads(grads_list, "grads", true);
+  const TensorList exp_avg(exp_avg_list, "exp_avg", false);
+  const TensorList exp_avg_sq(exp_avg_sq_list, "exp_avg_sq", false);
+  const pybind11::list none;
+  const bool masters = !master_list.is_none(), eight = !exp_avg_scale_list.is_none();
+  TORCH_CHECK(exp_avg_sq_scale_list.is_none() != eight, "both moments have scales, or neither");
+  const TensorList master(masters ? master_list : none, "master", true);
+  const TensorList exp_avg_scale(eight ? exp_avg_scale_list : none, "exp_avg_scale", false);
+  const TensorList exp_avg_sq_scale(eight ? exp_avg_sq_scale_list : none, "exp_avg_sq_scale", false);
   const size_t count = params.size();
   TORCH_CHECK(count > 0, "no parameters");
   TORCH_CHECK(grads.size() == count && exp_avg.size() == count && exp_avg_sq.size() == count &&
@@ -240,12 +275,9 @@ Optional adamw_step(std::vector<torch::Tensor> params, std::vector<Optional> gra
   TORCH_CHECK(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1, "betas must lie in [0, 1)");
   TORCH_CHECK(eps >= 0, "eps must not be negative");
   TORCH_CHECK(!max_norm.has_value() || *max_norm > 0, "max_norm must be positive");
-  const bool eight = exp_avg_scale.has_value();
-  TORCH_CHECK(exp_avg_sq_scale.has_value() == eight, "both moments have scales, or neither");
-  TORCH_CHECK(!eight || (exp_avg_scale->size() == count && exp_avg_sq_scale->size() == count),
+  TORCH_CHECK(!eight || (exp_avg_scale.size() == count && exp_avg_sq_scale.size() == count),
               "the scales must have one entry per parameter");
-  TORCH_CHECK(!master.has_value() || master->size() == count,
-              "master must have one entry per parameter");
+  TORCH_CHECK(!masters || master.size() == count, "master must have one entry per parameter");
   const torch::Tensor& first = params[0];
   TORCH_CHECK(first.is_cuda(), "parameters must be CUDA tensors");
   check_1d(steps, at::kLong, "steps");
@@ -269,38 +301,38 @@ Optional adamw_step(std::vector<torch::Tensor> params, std::vector<Optional> gra
     CugoAdamwTensor t{};
     t.param_dtype = (int16_t)float_code(w, "parameters");
     dense(w, w, w.scalar_type(), "parameters");
-    const Optional m32 = master.has_value() ? (*master)[i] : Optional();
+    const torch::Tensor* m32 = masters && master.has(i) ? &master[i] : nullptr;
     const bool wide = w.scalar_type() == at::kFloat;
-    TORCH_CHECK(wide || m32.has_value(), "a 16-bit parameter needs its float32 master");
-    TORCH_CHECK(!wide || !m32.has_value(), "a float32 parameter has no master");
-    if (m32.has_value()) dense(*m32, w, at::kFloat, "master");
+    TORCH_CHECK(wide || m32, "a 16-bit parameter needs its float32 master");
+    TORCH_CHECK(!wide || !m32, "a float32 parameter has no master");
+    if (m32) dense(*m32, w, at::kFloat, "master");
     dense(exp_avg[i], w, eight ? at::kFloat8_e4m3fn : at::kFloat, "exp_avg");
     dense(exp_avg_sq[i], w, eight ? at::kFloat8_e5m2 : at::kFloat, "exp_avg_sq");
     if (eight) {
       const int64_t blocks = (w.numel() + CUGO_ADAMW_BLOCK - 1) / CUGO_ADAMW_BLOCK;
-      for (const auto* s : {&(*exp_avg_scale)[i], &(*exp_avg_sq_scale)[i]}) {
+      for (const auto* s : {&exp_avg_scale[i], &exp_avg_sq_scale[i]}) {
         check_1d(*s, at::kFloat, "scales");
         TORCH_CHECK(s->numel() == blocks, "scales must have one entry per block of ",
                     CUGO_ADAMW_BLOCK, " values");
         check_same_device(first, *s, "parameters", "scales");
       }
     }
-    if (!grads[i].has_value()) continue;  // left as it is
-    const torch::Tensor& g = *grads[i];
+    if (!grads.has(i)) continue;  // left as it is
+    const torch::Tensor& g = grads[i];
     t.grad_dtype = (int16_t)float_code(g, "gradients");
     dense(g, w, g.scalar_type(), "gradients");
     TORCH_CHECK(w.numel() <= (int64_t)1 << 36, "at most 2^36 values a parameter");
     written(w), written(exp_avg[i]), written(exp_avg_sq[i]);
-    if (m32.has_value()) written(*m32);
-    if (eight) written((*exp_avg_scale)[i]), written((*exp_avg_sq_scale)[i]);
+    if (m32) written(*m32);
+    if (eight) written(exp_avg_scale[i]), written(exp_avg_sq_scale[i]);
     t.param = w.data_ptr();
     t.grad = g.data_ptr();
-    t.master = m32.has_value() ? m32->data_ptr<float>() : nullptr;
+    t.master = m32 ? m32->data_ptr<float>() : nullptr;
     t.exp_avg = exp_avg[i].data_ptr();
     t.exp_avg_sq = exp_avg_sq[i].data_ptr();
     if (eight) {
-      t.exp_avg_scale = (*exp_avg_scale)[i].data_ptr<float>();
-      t.exp_avg_sq_scale = (*exp_avg_sq_scale)[i].data_ptr<float>();
+      t.exp_avg_scale = exp_avg_scale[i].data_ptr<float>();
+      t.exp_avg_sq_scale = exp_avg_sq_scale[i].data_ptr<float>();
     }
     t.step = steps.data_ptr<int64_t>() + i;
     t.numel = w.numel();
@@ -326,7 +358,7 @@ Optional adamw_step(std::vector<torch::Tensor> params, std::vector<Optional> gra
              "adamw_step");
   // what keeps a copy of a parameter by its version (seq_decode's packed weights) sees the change
   for (size_t i = 0; i < count; ++i)
-    if (grads[i].has_value()) params[i].unsafeGetTensorImpl()->bump_version();
+    if (grads.has(i)) params[i].unsafeGetTensorImpl()->bump_version();
   return norm;
 }
 
