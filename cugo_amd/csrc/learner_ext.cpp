@@ -7,7 +7,6 @@
 #include <algorithm>
 #include <cmath>
 #include <string>
-#include <utility>
 
 namespace cugo_ext {
 namespace {
@@ -72,7 +71,9 @@ struct PolicyLossFn : public torch::autograd::Function<PolicyLossFn> {
     p.n = logits.size(0);
     p.actions = logits.size(1);
     p.logits_dtype = float_code(logits, "logits");
-    const auto out = torch::empty({7}, on(logits, at::kFloat));
+    // tensors of their own, not parts of one, so that a loss may be divided in place
+    const auto loss = torch::empty({}, on(logits, at::kFloat));
+    const auto stats = torch::empty({6}, on(logits, at::kFloat));
     const auto logp = torch::empty({p.n}, on(logits, at::kFloat));
     const auto partials = torch::empty({CUGO_POLICY_LOSS_PARTIALS}, on(logits, at::kDouble));
     p.logits = logits.data_ptr();
@@ -102,10 +103,10 @@ struct PolicyLossFn : public torch::autograd::Function<PolicyLossFn> {
       ctx->saved_data["d_value"] = d;
     }
     p.logp = logp.data_ptr<float>();
-    p.out = out.data_ptr<float>();
+    p.loss = loss.data_ptr<float>();
+    p.stats = stats.data_ptr<float>();
     p.partials = partials.data_ptr<double>();
     check_call(cugo_policy_loss(&p, stream()), "policy_loss");
-    auto loss = out.select(0, 0), stats = out.narrow(0, 1, 6);
     ctx->mark_non_differentiable({stats, logp});
     ctx->set_materialize_grads(false);
     return {loss, stats, logp};
@@ -183,6 +184,33 @@ std::vector<torch::Tensor> policy_loss(torch::Tensor logits, torch::Tensor actio
   return PolicyLossFn::apply(logits, value, &in);
 }
 
+// The memory that calls write and read, and whether what one writes overlaps any other part.
+class Spans {
+ public:
+  explicit Spans(size_t expected = 8) { spans_.reserve(expected); }
+  void add(const torch::Tensor& t, bool written) {
+    const auto at = reinterpret_cast<uintptr_t>(t.data_ptr());
+    if (t.numel() > 0) spans_.push_back({at, at + t.nbytes(), written});
+  }
+  bool overlap() {
+    std::sort(spans_.begin(), spans_.end(), [](const Span& a, const Span& b) { return a.from < b.from; });
+    uintptr_t any = 0, written = 0;  // the furthest ends so far
+    for (const Span& s : spans_) {
+      if (s.from < (s.written ? any : written)) return true;
+      any = std::max(any, s.to);
+      if (s.written) written = std::max(written, s.to);
+    }
+    return false;
+  }
+
+ private:
+  struct Span {
+    uintptr_t from, to;
+    bool written;
+  };
+  std::vector<Span> spans_;
+};
+
 // -> (advantage f32 [T, B], returns f32 [T, B]), cugo_advantages.
 std::vector<torch::Tensor> advantages(torch::Tensor reward, torch::Tensor value,
                                       torch::Tensor done, torch::Tensor bootstrap, double gamma,
@@ -211,6 +239,11 @@ std::vector<torch::Tensor> advantages(torch::Tensor reward, torch::Tensor value,
   const DeviceGuard guard(reward.device());
   auto adv = out_or_new(advantage, {steps, batch}, at::kFloat, reward, "advantage");
   auto ret = out_or_new(returns, {steps, batch}, at::kFloat, reward, "returns");
+  Spans spans;
+  for (const auto* t : {&reward, &value, &done, &bootstrap}) spans.add(*t, false);
+  if (player.has_value()) spans.add(*player, false), spans.add(*last_player, false);
+  spans.add(adv, true), spans.add(ret, true);
+  TORCH_CHECK(!spans.overlap(), "advantage and returns must not overlap the inputs or each other");
   const int64_t bytes = cugo_advantages_workspace(steps, batch);
   const auto scratch = torch::empty({bytes}, on(reward, at::kByte));
   check_call(cugo_advantages(code, reward.data_ptr<float>(), value.data_ptr(), u8p(done),
@@ -290,12 +323,9 @@ Optional adamw_step(const pybind11::list& params_list, const pybind11::list& gra
     check_same_device(first, t, "parameters", name);
   };
   std::vector<CugoAdamwTensor> list;
-  std::vector<std::pair<uintptr_t, uintptr_t>> spans;  // what the step writes
+  Spans spans(7 * count);
   list.reserve(count);
-  const auto written = [&](const torch::Tensor& t) {
-    const auto at = reinterpret_cast<uintptr_t>(t.data_ptr());
-    if (t.numel() > 0) spans.emplace_back(at, at + t.nbytes());
-  };
+  const auto written = [&](const torch::Tensor& t) { spans.add(t, true); };
   for (size_t i = 0; i < count; ++i) {
     const torch::Tensor& w = params[i];
     CugoAdamwTensor t{};
@@ -322,6 +352,7 @@ Optional adamw_step(const pybind11::list& params_list, const pybind11::list& gra
     t.grad_dtype = (int16_t)float_code(g, "gradients");
     dense(g, w, g.scalar_type(), "gradients");
     TORCH_CHECK(w.numel() <= (int64_t)1 << 36, "at most 2^36 values a parameter");
+    spans.add(g, false);
     written(w), written(exp_avg[i]), written(exp_avg_sq[i]);
     if (m32) written(*m32);
     if (eight) written(exp_avg_scale[i]), written(exp_avg_sq_scale[i]);
@@ -340,10 +371,8 @@ Optional adamw_step(const pybind11::list& params_list, const pybind11::list& gra
     t.place = (int32_t)i;
     list.push_back(t);
   }
-  std::sort(spans.begin(), spans.end());
-  for (size_t i = 1; i < spans.size(); ++i)
-    TORCH_CHECK(spans[i - 1].second <= spans[i].first,
-                "parameters and their states must not overlap in memory");
+  spans.add(steps, true);
+  TORCH_CHECK(!spans.overlap(), "parameters, gradients and states must not overlap in memory");
   const DeviceGuard guard(first.device());
   Optional norm;
   if (max_norm.has_value())

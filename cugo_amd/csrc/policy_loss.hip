@@ -118,10 +118,13 @@ struct RowTerms {
 };
 
 // s = sum 2^x; u = sum 2^x x; ds = sum 2^x d; sr = sum 2^x'; at: the action's x, or -inf.
+// A row with an action above -inf has a sum of 1 and more, or NaN for a NaN among its logits,
+// which the largest logit does not show.
 template <bool kRef>
-__device__ inline RowTerms row_terms(const LossArgs& g, const RowInputs& in, bool some, float s,
-                                     float u, float ds, float sr, float at) {
+__device__ inline RowTerms row_terms(const LossArgs& g, const RowInputs& in, float s, float u,
+                                     float ds, float sr, float at) {
   RowTerms x;
+  const bool some = !(s == 0.0f);
   const float inv = some ? __builtin_amdgcn_rcpf(s) : 0.0f;
   const float ls = some ? __builtin_amdgcn_logf(s) : 0.0f;  // v_log_f32: base 2
   const float mean = u * inv;
@@ -383,7 +386,7 @@ __global__ __launch_bounds__(kThreads) void loss_rows_kernel(const LossArgs g) {
         ds = group_sum<G>(ds);
         sr = group_sum<G>(sr);
       }
-      x = row_terms<kRef>(g, in, top > -INFINITY, s, u, ds, sr, xa);
+      x = row_terms<kRef>(g, in, s, u, ds, sr, xa);
       if (g.d_logits) {
 #pragma unroll
         for (int i = 0; i < V; ++i)
@@ -452,7 +455,7 @@ __global__ __launch_bounds__(kThreads) void loss_rows_kernel(const LossArgs g) {
         ds = group_sum<G>(ds);
         sr = group_sum<G>(sr);
       }
-      x = row_terms<kRef>(g, in, top > -INFINITY, s, u, ds, sr, xa);
+      x = row_terms<kRef>(g, in, s, u, ds, sr, xa);
       if (g.d_logits) {
 #pragma unroll 1
         for (int i = 0; i < V; ++i) {
@@ -595,14 +598,13 @@ __device__ inline void workgroup_sums(float (&x)[4], float (*shared)[4]) {
 // 2^x d and 2^x'.
 template <class T, bool kRef>
 __device__ inline RowTerms finish_row(const LossArgs& g, i64 r, i64 act, const RowInputs& in,
-                                      bool some, const Scale& scale, const float (&sums)[4],
-                                      double& acc) {
+                                      const Scale& scale, const float (&sums)[4], double& acc) {
   using S = typename T::storage;
   const S* zs = static_cast<const S*>(g.logits) + r * g.logits_stride;
   const bool inside = act >= 0 && act < g.actions;
   const bool taken = inside && (!g.legal || g.legal[r * g.legal_stride + act]);
   const float za = T::to_float(zs[inside ? act : 0]);
-  const RowTerms x = row_terms<kRef>(g, in, some, sums[0], sums[1], sums[2], sums[3],
+  const RowTerms x = row_terms<kRef>(g, in, sums[0], sums[1], sums[2], sums[3],
                                      taken ? scale(za) : -INFINITY);
   float stat = x.stat[5];
 #pragma unroll
@@ -739,7 +741,6 @@ __global__ __launch_bounds__(kWide) __attribute__((amdgpu_waves_per_eu(4))) void
       if (i < whole) find_ends(piece[i]);
     if (in_tail) find_ends(tail);
     workgroup_max<kWide, 4>(ends, tops);
-    const bool some = ends[0] > -INFINITY;
     const bool finite = ends[0] + ends[2] < 0x1p100f && (!kRef || ends[1] + ends[3] < 0x1p100f);
     const Scale scale = scale_for(ends[0]), scale_ref = scale_for(ends[1]);
     float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -757,7 +758,7 @@ __global__ __launch_bounds__(kWide) __attribute__((amdgpu_waves_per_eu(4))) void
     if (finite) add(std::true_type{});
     else add(std::false_type{});
     workgroup_sums<kWide>(sums, totals);
-    const RowTerms x = finish_row<T, kRef>(g, r, act, in, some, scale, sums, acc);
+    const RowTerms x = finish_row<T, kRef>(g, r, act, in, scale, sums, acc);
     if (!g.d_logits) continue;
     S* out = static_cast<S*>(g.d_logits) + r * g.d_stride;
     const auto store = [&](auto is_finite) {
@@ -847,7 +848,6 @@ __global__ __launch_bounds__(kWide) void loss_long_kernel(const LossArgs g) {
     // the threads' sums under the row's maximum
     float all[2] = {top, top_ref};
     workgroup_max<kWide, 2>(all, tops);
-    const bool some = all[0] > -INFINITY;
     const Scale scale = scale_for(all[0]), scale_ref = scale_for(all[1]);
     const float by = scale(top), f = exp2_of(by);
     float sums[4] = {s * f, moved(f, u, s, by), 0.0f, 0.0f};
@@ -857,7 +857,7 @@ __global__ __launch_bounds__(kWide) void loss_long_kernel(const LossArgs g) {
       sums[3] = sr * exp2_of(by_ref);
     }
     workgroup_sums<kWide>(sums, totals);
-    const RowTerms x = finish_row<T, kRef>(g, r, act, in, some, scale, sums, acc);
+    const RowTerms x = finish_row<T, kRef>(g, r, act, in, scale, sums, acc);
     if (!g.d_logits) continue;
     S* out = static_cast<S*>(g.d_logits) + r * g.d_stride;
     for (int c = threadIdx.x * E; c < g.actions; c += kWide * E) {
@@ -878,7 +878,7 @@ constexpr int kTotalThreads = 960;
 static_assert(kTotalThreads % kStats == 0 && kTotalThreads % 64 == 0, "one sum a thread");
 __global__ __launch_bounds__(kTotalThreads) void loss_total_kernel(
     const double* partials, int groups, double kl_coef, double entropy_coef, double value_coef,
-    const float* scale, float* out) {
+    const float* scale, float* loss_out, float* stats_out) {
   constexpr int kEach = kTotalThreads / kStats;  // threads a sum
   __shared__ double sums[kTotalThreads];
   __shared__ double totals[kStats];
@@ -895,14 +895,14 @@ __global__ __launch_bounds__(kTotalThreads) void loss_total_kernel(
     for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off);
     if (lane == 0) {
       totals[k] = total;
-      out[1 + k] = (float)total;
+      stats_out[k] = (float)total;
     }
   }
   __syncthreads();
   if (threadIdx.x == 0) {
     const double loss = totals[0] + value_coef * totals[1] + kl_coef * totals[2] -
                         entropy_coef * totals[3];
-    out[0] = (float)(loss * (scale ? (double)*scale : 1.0));
+    *loss_out = (float)(loss * (scale ? (double)*scale : 1.0));
   }
 }
 
@@ -995,7 +995,7 @@ using namespace cugo_amd::learner::loss;
 extern "C" {
 
 int cugo_policy_loss(const CugoPolicyLoss* p, hipStream_t stream) {
-  if (!p || p->n < 0 || p->actions < 1 || p->actions > (1 << 30) || !p->out || !p->partials)
+  if (!p || p->n < 0 || p->actions < 1 || p->actions > (1 << 30) || !p->loss || !p->stats || !p->partials)
     return -1;
   if (!dtype_known(p->logits_dtype) || (p->value && !dtype_known(p->value_dtype))) return -2;
   if (p->n > 0 && (!p->logits || !p->action || !p->old_logp || !p->advantage || !p->logp))
@@ -1030,7 +1030,7 @@ int cugo_policy_loss(const CugoPolicyLoss* p, hipStream_t stream) {
   }
   loss_total_kernel<<<1, kTotalThreads, 0, stream>>>(p->partials, groups, p->kl_coef,
                                                    p->entropy_coef, p->value_coef, p->scale,
-                                                   p->out);
+                                                   p->loss, p->stats);
   return (int)hipGetLastError();
 }
 

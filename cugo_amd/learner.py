@@ -89,7 +89,7 @@ def advantages(ext, reward: torch.Tensor, value: torch.Tensor, done: torch.Tenso
     player); done bool ends a game with the step, and nothing after it is read into it.
     bootstrap [batch] (value's type) and last_player [batch] belong to the state behind the last
     step.  Advantages and returns are the mover's.  `advantage` and `returns`, if given,
-    receive the results."""
+    receive the results; they must not overlap the inputs."""
     return tuple(ext.advantages(reward, value.detach(), done, bootstrap.detach(), gamma, lam,
                                 player, last_player, advantage, returns))
 
@@ -177,12 +177,13 @@ class AdamW(torch.optim.Optimizer):
         """Creates the state of parameters that have none (the first `step` does; call it before
         capturing one)."""
         params = self._all()
-        if self._steps is not None and self._steps.numel() == len(params):
+        if (self._steps is not None and self._steps.numel() == len(params)
+                and all(p in self.state for p in params)):
             return
         steps = torch.zeros(len(params), dtype=torch.int64, device=params[0].device)
         for i, p in enumerate(params):
             s = self.state[p]
-            if "exp_avg" not in s:
+            if not s:
                 s.update(self._new_state(p))
             if "step" in s:
                 steps[i] = s["step"]

@@ -678,15 +678,15 @@ int cugo_selfplay_advance(const CugoSelfPlayWave* wave, const uint8_t* done,
  * int64, its log-probability then, the advantage A and the weight w (NULL: 1 / n each), l the
  * log-softmax over the row's legal actions, r = e^(l_a - old_logp), l' the log-softmax of
  * ref_logits (NULL: none) over the same actions:
- *   out[1] = sum w (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A))
- *   out[2] = sum w (value - returns)^2 / 2             (value NULL: 0)
- *   out[3] = sum w sum_j p_j (l_j - l'_j)              (ref_logits NULL: 0)
- *   out[4] = sum w (-sum_j p_j l_j)
- *   out[5] = sum w [the clip cut the ratio off]
- *   out[6] = sum w (r - 1 - (l_a - old_logp))
- *   out[0] = scale (out[1] + value_coef out[2] + kl_coef out[3] - entropy_coef out[4])
+ *   stats[0] = sum w (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A))
+ *   stats[1] = sum w (value - returns)^2 / 2             (value NULL: 0)
+ *   stats[2] = sum w sum_j p_j (l_j - l'_j)              (ref_logits NULL: 0)
+ *   stats[3] = sum w (-sum_j p_j l_j)
+ *   stats[4] = sum w [the clip cut the ratio off]
+ *   stats[5] = sum w (r - 1 - (l_a - old_logp))
+ *   *loss = scale (stats[0] + value_coef stats[1] + kl_coef stats[2] - entropy_coef stats[3])
  * and logp[i] = l_a; d_logits [n, A] and d_value [n] (NULL: not wanted) receive the gradients
- * of out[0], in the logits' and the value's type.  scale: one float of device memory, or NULL
+ * of *loss, in the logits' and the value's type.  scale: one float of device memory, or NULL
  * for 1.  A row of weight 0 counts nowhere and has zero gradients, whatever else it holds.  A
  * row without a legal action (or with none above -inf) has only the value term, and logp 0.
  * An action that is illegal, outside [0, A) or at -inf has log-probability -inf and ratio 0.
@@ -713,7 +713,8 @@ typedef struct CugoPolicyLoss {
   int64_t d_logits_stride;
   void* d_value;
   float* logp;
-  float* out;
+  float* loss;
+  float* stats;
   double* partials;
 } CugoPolicyLoss;
 int cugo_policy_loss(const CugoPolicyLoss* loss, hipStream_t stream);

@@ -318,6 +318,8 @@ def test_refusals(ext):
         exp_avg_scale=[y["exp_avg_scale"][0]] * 2, exp_avg_sq_scale=[y["exp_avg_sq_scale"][0]] * 2)
     bad(wide, exp_avg_sq=wide["exp_avg"])
     bad(wide, params=[wide["params"][0], wide["params"][0][10:30]])
+    bad(wide, grads=[wide["params"][0], wide["grads"][1]])
+    bad(wide, grads=[wide["exp_avg"][0], wide["grads"][1]])
     bad(y, grads=y["grads"][:1])
     bad(y, grads=[y["grads"][0], y["grads"][1].long()])
     bad(y, grads=[y["grads"][0], y["grads"][0]])
@@ -396,6 +398,16 @@ def test_optimizer_state_is_saved_and_loaded(ext, bits):
     wrong = learner.AdamW(ext, b.parameters(), state_bits=40 - bits)
     with pytest.raises(ValueError, match="fit"):
         wrong.load_state_dict(saved)
+
+
+def test_one_gradient_for_two_parameters(ext):
+    """Gradients are read only: two parameters may share one."""
+    x = make([700, 700], torch.float32, torch.float32, 11)
+    x["grads"][1] = x["grads"][0]
+    y = to_device(x)
+    y["grads"][1] = y["grads"][0]
+    norm = step(ext, y, max_norm=1.0)
+    check(x, y, norm, 1.0)
 
 
 def test_optimizer_groups_rates_and_gradients_of_none(ext):

@@ -146,6 +146,7 @@ def test_refusals(ext):
                  dict(done=x["done"].t().contiguous().t()), dict(bootstrap=x["bootstrap"].half()),
                  dict(bootstrap=x["bootstrap"][:3]), dict(player=None), dict(last_player=None),
                  dict(player=x["player"].long()), dict(gamma=1.5), dict(lam=-0.1),
+                 dict(advantage=x["reward"]), dict(advantage=x["value"]),
                  dict(advantage=torch.empty(4, 6, device=DEV)),
                  dict(advantage=torch.empty(6, 4, device=DEV, dtype=torch.float64))):
         with pytest.raises(RuntimeError):

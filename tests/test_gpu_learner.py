@@ -116,3 +116,55 @@ def test_the_next_rollout_plays_the_new_weights(ext):
         assert all(moved)
     steps = {int(lrn.optimizer.state[p]["step"]) for p in ro.actor.parameters()}
     assert steps == {3 * 2 * -(-256 * 16 // 1000)}
+
+
+def test_loss_and_step_captured_together(ext):
+    """Logits that are parameters themselves, learnt by replays of one captured loss, backward pass
+    and AdamW step, with eager work in between: bit for bit the eager steps on copies."""
+    from cugo_amd import learner
+
+    announce("loss and step captured")
+    n, a = 300, 179
+    g = torch.Generator(device=DEV).manual_seed(4)
+    legal = torch.rand(n, a, generator=g, device=DEV) < 0.2
+    legal[:, 3] = True
+    action = (torch.rand(n, a, generator=g, device=DEV) * legal).argmax(1)
+    old = torch.full((n,), -3.0, device=DEV)
+    advantage = torch.randn(n, generator=g, device=DEV)
+    start = torch.randn(n, a, generator=g, device=DEV)
+
+    def fresh():
+        return dict(w=start.bfloat16().requires_grad_(), master=start.clone(),
+                    m=torch.zeros(n, a, dtype=torch.float8_e4m3fn, device=DEV),
+                    v=torch.zeros(n, a, dtype=torch.float8_e5m2, device=DEV),
+                    ms=torch.zeros(-(-n * a // 256), device=DEV),
+                    vs=torch.zeros(-(-n * a // 256), device=DEV),
+                    steps=torch.zeros(1, dtype=torch.int64, device=DEV))
+
+    def once(s):
+        out = learner.policy_loss(ext, s["w"], action, old, advantage, legal=legal,
+                                  entropy_coef=0.01)
+        grad, = torch.autograd.grad(out.loss, [s["w"]])
+        norm = learner.adamw_step(ext, [s["w"]], [grad], [s["m"]], [s["v"]], s["steps"], lr=0.01,
+                                  max_norm=0.1, master=[s["master"]], exp_avg_scale=[s["ms"]],
+                                  exp_avg_sq_scale=[s["vs"]], seed=3)
+        return out.loss.detach(), norm
+
+    eager, played = fresh(), fresh()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        once(played)
+    torch.cuda.current_stream().wait_stream(side)
+    once(eager)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, norm = once(played)
+    for _ in range(6):
+        graph.replay()
+        want_loss, want_norm = once(eager)
+        assert torch.equal(loss, want_loss) and torch.equal(norm, want_norm)
+    torch.cuda.synchronize()
+    for k in eager:
+        assert torch.equal(eager[k].detach().float(), played[k].detach().float()), k
+    assert int(played["steps"]) == 7

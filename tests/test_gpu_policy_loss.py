@@ -216,6 +216,53 @@ def test_nan_in_a_legal_logit_shows(ext):
             assert not torch.isnan(got["d_logits"][2]).any()
 
 
+def test_nan_in_the_only_legal_logit_shows(ext):
+    """No other logit is there to be the largest: the row must not pass for one without any."""
+    for a in (1, 3, 40, 179, 300, 1024, 2000, 9000, 40000):
+        for only_it in (True, False):
+            x = make(3, a, torch.bfloat16, a, weight=False)
+            x["legal"][0] = False
+            x["legal"][0, a // 2] = only_it
+            x["logits"][0] = math.nan if not only_it else x["logits"][0]
+            x["logits"][0, a // 2] = math.nan
+            x["action"][0] = a // 2
+            got = call(ext, x)
+            if only_it:
+                assert torch.isnan(got["loss"]) and torch.isnan(got["logp"][0]), a
+                assert torch.isnan(got["d_logits"][0, a // 2]), a
+            else:  # all of the row illegal
+                assert not torch.isnan(got["loss"]) and (got["d_logits"][0] == 0).all(), a
+
+
+def test_loss_divided_in_place(ext):
+    from cugo_amd import learner
+
+    x = make(5, 30, torch.float32, 3, weight=False)
+    on = {k: v.to(DEV) for k, v in x.items() if isinstance(v, torch.Tensor)}
+    want = call(ext, x)
+    logits = on["logits"].requires_grad_()
+    out = learner.policy_loss(ext, logits, on["action"], on["old_logp"], on["advantage"],
+                              legal=on["legal"], ref_logits=on["ref"], value=on["value"],
+                              returns=on["returns"], **ARGS)
+    loss = out.loss
+    loss /= 4
+    out.stats.mul_(2)
+    loss.backward()
+    assert torch.equal(logits.grad, want["d_logits"] * 0.25)
+    assert torch.equal(loss.detach(), want["loss"] / 4)
+
+
+def test_rows_far_apart(ext):
+    """Rows more than 2^24 elements apart, of few and of many actions: the contiguous results."""
+    for a in (2, 179, 2000):
+        x = make(3, a, torch.bfloat16, a, weight=False)
+        room = torch.zeros(3, (1 << 24) + 3, dtype=torch.bfloat16, device=DEV)
+        room[:, 1:1 + a] = x["logits"].to(DEV)
+        p, q = call(ext, dict(x, logits=room[:, 1:1 + a])), call(ext, x)
+        for k in p:
+            assert torch.equal(p[k], q[k]), k
+
+
 def test_strides_and_offsets(ext):
     """Logits that are the columns of a wider head, from an odd column on; reference logits of
     one row for all; a mask cut out of a wider one: the results of contiguous copies, bit by bit."""
