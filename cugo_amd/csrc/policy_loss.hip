@@ -93,19 +93,14 @@ __device__ inline RowInputs row_inputs(const LossArgs& g, i64 r, uint32_t i) {
   return in;
 }
 
-// Exponents are in base 2: x = z k - top k with k = log2 e, one multiply-add, so that
-// e^(z - top) = 2^x up to a factor that all of a row's exponentials share (the rounding of top k),
-// which their sum's logarithm takes out again.
-// Where the largest logit is so large that top k may not fit, logits that are not equal to it
-// are 1e30 away and more, so that any k tells them apart: a small one is taken.
+// Exponents are in base 2: x = (z - top) log2 e, so that e^(z - top) = 2^x.  The difference comes
+// first: the largest logit has x = 0 exactly, and a row's only action the log-probability 0 (as one
+// multiply-add, z k - top k, x would keep the rounding of top k).
 struct Scale {
-  float k, shift;
-  __device__ float operator()(float z) const { return __builtin_fmaf(z, k, shift); }
+  float top;
+  __device__ float operator()(float z) const { return (z - top) * kLog2e; }
 };
-__device__ inline Scale scale_for(float top) {
-  const float k = fabsf(top) > 1e37f && fabsf(top) < INFINITY ? 0x1p-10f : kLog2e;
-  return Scale{k, top == -INFINITY ? 0.0f : -top * k};
-}
+__device__ inline Scale scale_for(float top) { return Scale{top == -INFINITY ? 0.0f : top}; }
 __device__ inline float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // A row's terms from the sums over its actions.  Every lane that serves the row computes them.

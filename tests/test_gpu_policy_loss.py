@@ -7,13 +7,7 @@ most 16), and 16 for the exponential's and the logarithm's own last places (v_ex
 are good to one) and the differences around them.  A probability and a ratio then carry E
 relative to themselves; a gradient w p (pull + c_k (d - K) + c_e (l + H)) carries 4 E of w p times
 the sum of its parts' sizes, the taken action's w pull once more; stored, half a step of its type
-(or half of float16's smallest value).
-
-Exponents are formed as z k - round(top k): the rounding, u |top| k at most, is the same for all
-of a row.  It leaves l and K as it leaves the sums (both sides of a difference have it), but the
-parts of a gradient, which are differences x - mean and d - mean, keep the roundings of the mean:
-2 u of that shift, so 4 u (u |top| + u |top'|) of w p (c_k + c_e) at most, where a row of one action
-has nothing else."""
+(or half of float16's smallest value)."""
 
 from __future__ import annotations
 
@@ -84,13 +78,11 @@ def check(x, got, scale=1.0):
     z = x["logits"].double().masked_fill(~on, -math.inf)
     ell = ref.log_softmax(z).nan_to_num(nan=0, neginf=0, posinf=0)
     p = torch.where(on, ell.exp(), 0.0)
-    tops = [z.max(1).values.nan_to_num(nan=0, neginf=0)]
     size = torch.where(p > 1e-46, ell.abs(), 0.0)
     d = torch.zeros_like(ell)
     if x["ref"] is not None:
         q = x["ref"].double().masked_fill(~on, -math.inf)
         lq = ref.log_softmax(q).nan_to_num(nan=0, neginf=0, posinf=0)
-        tops.append(q.max(1).values.nan_to_num(nan=0, neginf=0))
         d = torch.where(p > 1e-46, (ell - lq).abs(), 0.0)
         size = torch.maximum(size, torch.where(p > 1e-46, lq.abs(), 0.0))
     err = U * (4 * size + adds + 16)          # E of each entry
@@ -130,8 +122,6 @@ def check(x, got, scale=1.0):
             parts = pull[:, None] + 0.3 * (d + (p * d).sum(1, keepdim=True)) + \
                 0.05 * (size + (p * size).sum(1, keepdim=True))
             t = 4 * p * parts * (err + row[:, None] + e_act[:, None])
-            shift = sum(torch.where(y.abs() < 1e30, y.abs(), 0.0) for y in tops)
-            t = t + p * 0.35 * 4 * U * U * shift[:, None]
             t.scatter_add_(1, x["action"].clamp(0, a - 1)[:, None],
                            (4 * pull * (e_act + 4 * U))[:, None])
             t = t * w[:, None] * abs(scale)
@@ -214,6 +204,21 @@ def test_nan_in_a_legal_logit_shows(ext):
             got = call(ext, x)
             assert torch.isnan(got["loss"]) and torch.isnan(got["logp"][0])
             assert not torch.isnan(got["d_logits"][2]).any()
+
+
+def test_the_only_legal_action_is_certain(ext):
+    """Log-probability, entropy and KL term 0 exactly, whatever the logit; and no gradient but the
+    pull's rounding."""
+    for dtype in (torch.float32, torch.bfloat16):
+        for a in (1, 2, 64, 179, 300, 1024, 2000, 40000):
+            x = make(4, a, dtype, a, weight=False)
+            x["logits"] = (x["logits"].float() * 7.3).to(dtype)
+            x["legal"][:] = False
+            x["action"] = torch.tensor([0, a // 3, a // 2, a - 1])
+            x["legal"][torch.arange(4), x["action"]] = True
+            got = call(ext, x)
+            assert (got["logp"] == 0).all() and (got["stats"][2:4] == 0).all(), (a, dtype)
+            assert (got["d_logits"][~x["legal"].to(DEV)] == 0).all()
 
 
 def test_nan_in_the_only_legal_logit_shows(ext):
