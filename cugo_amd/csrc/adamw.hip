@@ -6,8 +6,12 @@
 //
 // The tensors' addresses travel in the kernel's arguments (nothing to copy to the device, and a
 // captured launch keeps them); a workgroup takes chunks of kChunk values and finds each chunk's
-// tensor by bisection.  Memory bounds it: 28 bytes a value with float32 moments, a bf16 weight
-// and its float32 master, 16 with 8-bit moments.
+// tensor by bisection.  Memory bounds it: 28 bytes a value with float32 moments and parameters or
+// with a bf16 weight, its master and a bf16 gradient, 16 of the latter with 8-bit moments.  35.4M
+// values: 174 us (5.7 TB/s, the gradients partly from the last-level cache, which the 48 us of the
+// norm's launch filled), with 8-bit moments 118 us (4.8 TB/s).  A whole chunk's loads are all in
+// flight before the first is used (187 and 158 us when each access waited for its own).  2M values
+// take 14 us, most of it the latencies of a launch in which a wavefront has one chunk.
 //
 // 8-bit moments: a block of 256 values shares a float32 scale, its largest value; m is kept as
 // e4m3 and v, whose values span the squares of the gradients' range, as e5m2.  b2 = 0.999 moves
@@ -28,7 +32,7 @@ constexpr int kThreads = 256;
 constexpr int kEach = 4;                        // values of a thread's access
 constexpr int kRounds = 4;                      // accesses of a thread in a chunk
 constexpr int kChunk = kThreads * kEach * kRounds;
-constexpr int kTable = 32;                      // tensors of a launch: 3.4 KB of arguments
+constexpr int kTable = 32;                      // tensors of a launch: 2.5 KB of arguments
 constexpr int kPartials = 1024;                 // most workgroups of a launch
 constexpr int kBlock = CUGO_ADAMW_BLOCK;
 static_assert(kBlock == 64 * kEach, "a block is one access of a wavefront");

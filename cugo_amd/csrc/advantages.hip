@@ -10,7 +10,9 @@
 // compose theirs (a suffix scan in the wavefront, then over the wavefronts in LDS), and each
 // lane runs its own steps again from the value that follows them.  The data is read once.
 //
-// What bounds it is memory: 10 to 18 bytes a step of a game.  A wavefront's 64 lanes are
+// What bounds it is memory, 16 to 18 bytes a step of a game (128 steps of 65,536 games in 31 us,
+// 4.8 TB/s), and below about a million steps the two or three rounds of latency of a launch (5 us
+// for 64 x 300).  A wavefront's 64 lanes are
 // `columns` games times 64 / columns runs of steps, the fewest columns (a power of two) that
 // hold the games up to 64, so that few games still fill wavefronts; where the workgroups of
 // one run over the steps would leave compute units idle, the steps are also split over
@@ -154,8 +156,12 @@ __global__ __launch_bounds__(64 * kWaves) void gae_kernel(const GaeArgs g) {
   if (kMapsOnly && wave == 0 && run == 0 && ok) g.maps[(i64)chunk * g.batch + b] = total;
 }
 
-// How a call is laid out: the columns of a wavefront, and the chunks the steps are split into
-// so that the launch has about two workgroups a compute unit.
+// How a call is laid out: the columns of a wavefront, and the chunks the steps are split into, as
+// many as give the launch two workgroups a compute unit.  Two passes are not split: the second
+// costs less than the second launch and the second reading.  us unsplit / with one / two / four
+// workgroups a compute unit: 128 x 8,192 (two passes) 9.7 / 11.3 / 11.4 / 11.3, 128 x 16,384 13.1 /
+// 13.1 / 16.0 / 16.0, 256 x 1,024 (four) 15.0 / 10.1 / 10.1 / 10.1, 1,024 x 4,096 80 / 43.5 / 30.3 /
+// 31.2, 20,001 x 45 1,468 / 18.4 / 15.2 / 15.2.
 struct GaeLayout {
   int columns, chunks;
   i64 groups, chunk;
@@ -169,7 +175,7 @@ inline GaeLayout gae_layout(i64 steps, i64 batch) {
   const i64 pass = (i64)kWaves * (64 / l.columns) * kSteps;
   const i64 passes = (steps + pass - 1) / pass;
   i64 chunks = 2 * (i64)compute_units() / l.groups;
-  chunks = chunks < 1 ? 1 : chunks < passes ? chunks : passes;
+  chunks = chunks < 1 || passes <= 2 ? 1 : chunks < passes ? chunks : passes;
   const i64 each = (passes + chunks - 1) / chunks;
   l.chunk = each * pass;
   l.chunks = (int)((passes + each - 1) / each);

@@ -237,8 +237,9 @@ struct RowReader {
 // A game's row has about ten legal actions of 179, and an exponential or a product for each action
 // takes longer than memory does: where each row of a wavefront has at most two legal actions a
 // lane, a list of their slots is made, a lane computes two of them, and the gradient is put
-// together in LDS.
-// XX
+// together in LDS.  1,048,576 x 179 bf16 with a KL term, 10 legal actions a row: 298 us (4.5 TB/s;
+// the arithmetic is half of that), with 60, where the list does not hold them, 373, and 379 for
+// the earlier form that computed all of the actions always.
 template <class T, int G, int V, int E, bool kRef>
 __global__ __launch_bounds__(kThreads) void loss_rows_kernel(const LossArgs g) {
   using S = typename T::storage;
@@ -681,10 +682,12 @@ __device__ inline void store_gradients(const LossArgs& g, typename T::storage* o
 
 // Rows of up to kWide P E actions: the row stays in registers, as it was read, through a pass
 // for the largest logit, one for the sums and one for the gradient; so memory sees it once.
-// Arithmetic comes next to memory in what bounds it (16 instructions an action and pass with a
-// KL term, of which the exponentials take four cycles' worth each), so a row whose logits are all
-// within 2^100 of its largest, as a row without masked entries is, leaves out the tests for 0 times
-// infinity.  XX
+// 4,096 x 32,000 bf16 with a KL term: 186 us, 4.2 TB/s, where two passes over memory
+// (loss_long_kernel) took 244.  Arithmetic comes next to memory in what bounds it (about 27
+// instructions an action with a KL term, three of them exponentials at a quarter of the rate), so a
+// row whose logits are all within 2^100 of its largest, as a row without masked entries is, leaves
+// out the tests for 0 times infinity (270 us with them, and with registers spilled).  Registers for
+// two workgroups of 512 threads a compute unit, so that one reads while the other computes.
 template <class T, int kWide, int P, bool kRef>
 __global__ __launch_bounds__(kWide) __attribute__((amdgpu_waves_per_eu(4))) void loss_held_kernel(
     const LossArgs g) {
@@ -778,7 +781,8 @@ __global__ __launch_bounds__(kWide) __attribute__((amdgpu_waves_per_eu(4))) void
   if (threadIdx.x < kStats) g.partials[(i64)blockIdx.x * kStats + threadIdx.x] = acc;
 }
 
-// Rows of any length, in two passes over memory.  The first keeps each thread's running maximum
+// Rows of any length, in two passes over memory (2,048 x 65,536 bf16 with a KL term: 235 us, 3.4 TB/s
+// counted once).  The first keeps each thread's running maximum
 // and the sums under it, moved along with the maximum; the second reads the row again for the
 // gradient.
 
@@ -937,8 +941,8 @@ __global__ __launch_bounds__(kThreads) void scale_kernel(int a_dtype, void* a, i
   scale_any(b_dtype, b, b_count, f);
 }
 
-// A workgroup for each of `pieces` of work, or as many as can be resident at once, which then go
-// round.
+// A workgroup for each of `pieces` of work, or as many as a device holds of that many threads, which
+// then go round (fewer, only as many as their registers leave resident, took the same time).
 template <auto kKernel>
 int launch_rows(const LossArgs& g, i64 pieces, int threads, hipStream_t stream) {
   const i64 most = (i64)compute_units() * (2048 / threads);
@@ -961,6 +965,11 @@ int launch_loss(const LossArgs& g, hipStream_t stream) {
       g, (g.n + kThreads / G - 1) / (kThreads / G), kThreads, stream)
 #define CUGO_LOSS_HELD(THREADS, P) \
   launch_rows<loss_held_kernel<T, THREADS, P, kRef>>(g, g.n, THREADS, stream)
+  // Lanes, vectors and threads by what a row needs; us of 2^27 bf16 logits with a KL term on both
+  // sides of the lines: 256 actions 230, 257 348 (16 lanes against 32; 541 on 64 lanes), 512 225, 513
+  // 356, 1,024 230 and 1,025 316 (a workgroup of 64 threads: 199 and 562 of 256), 2,048 170, 4,096
+  // 178, 8,192 167 and 8,193 276, 32,768 184 and 32,769 265.  Rows of 768 take 245 on 64 lanes and 253
+  // as a workgroup of 64 threads, with a mask 249 and 353.
   if (a < 4) return CUGO_LOSS_ROWS(16, 1, 1);
   if (a <= 64) return CUGO_LOSS_ROWS(16, 1, 4);
   if (a <= 128) return CUGO_LOSS_ROWS(16, 2, 4);
