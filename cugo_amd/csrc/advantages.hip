@@ -5,7 +5,7 @@
 //   d_t = reward_t + [not done_t] gamma s_(t+1) V_(t+1) - s_t V_t
 //   a_t = d_t + c_t a_(t+1),  c_t = gamma lam, or 0 at a done step
 // and a mover's advantage is s_t a_t.  a_t is an affine map of a_(t+1), and maps compose:
-// (D, C) after (D', C') is (D + C D', C C').  So the steps are split: a lane takes kSteps
+// (D, C) after (D', C') is (D + C D', C C').  So the steps are split: a lane takes 4 or 8
 // consecutive steps of one game in registers and composes their maps, lanes and wavefronts
 // compose theirs (a suffix scan in the wavefront, then over the wavefronts in LDS), and each
 // lane runs its own steps again from the value that follows them.  The data is read once.
@@ -24,8 +24,7 @@ namespace cugo_amd {
 namespace learner {
 namespace gae {
 
-constexpr int kSteps = 8;   // steps a lane holds
-constexpr int kWaves = 8;   // wavefronts a workgroup
+constexpr int kMostWaves = 16; // wavefronts a workgroup, at most
 
 struct GaeArgs {
   const float* reward;
@@ -53,14 +52,15 @@ __device__ inline float2 after(float2 m, float2 later) {
   return make_float2(apply(m, later.x), m.y * later.y);
 }
 
-template <class T, bool kMapsOnly>
-__global__ __launch_bounds__(64 * kWaves) void gae_kernel(const GaeArgs g) {
+// kSteps: the steps a lane holds.
+template <class T, int kSteps, bool kMapsOnly>
+__global__ __launch_bounds__(64 * kMostWaves) void gae_kernel(const GaeArgs g) {
   using S = typename T::storage;
-  __shared__ float2 wave_map[kWaves][64];
+  __shared__ float2 wave_map[kMostWaves][64];
   __shared__ float behind[2][64];  // a of the step behind a pass, for each column, in turn
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int column = lane & (g.columns - 1), run = lane / g.columns;
-  const int runs = 64 / g.columns;
+  const int runs = 64 / g.columns, waves = (int)blockDim.x >> 6;
   const i64 game = (i64)blockIdx.x * g.columns + column;
   const bool ok = game < g.batch;
   const i64 b = ok ? game : g.batch - 1;
@@ -68,20 +68,20 @@ __global__ __launch_bounds__(64 * kWaves) void gae_kernel(const GaeArgs g) {
   const i64 first = (i64)chunk * g.chunk;
   const i64 end = min(first + g.chunk, g.steps);
   const S* value = static_cast<const S*>(g.value);
-  const i64 pass = (i64)kWaves * runs * kSteps;
+  const i64 pass = (i64)waves * runs * kSteps;
   float carry = 0.0f;
   if (!kMapsOnly && chunk + 1 < g.chunks) {
     // The maps of the chunks behind this one: each wavefront composes a run of them (its loads
     // do not wait for one another), and every lane applies the runs.
     const int behind_it = g.chunks - 1 - chunk;
-    const int each = (behind_it + kWaves - 1) / kWaves;
+    const int each = (behind_it + waves - 1) / waves;
     const int from = chunk + 1 + wave * each, to = min(from + each, g.chunks);
     float2 m = make_float2(0.0f, 1.0f);
 #pragma unroll 4
     for (int k = from; k < to; ++k) m = after(m, g.maps[(i64)k * g.batch + b]);
     if (run == 0) wave_map[wave][column] = m;
     __syncthreads();
-    for (int k = kWaves - 1; k >= 0; --k) carry = apply(wave_map[k][column], carry);
+    for (int k = waves - 1; k >= 0; --k) carry = apply(wave_map[k][column], carry);
     __syncthreads();
   }
   float2 total = make_float2(0.0f, 1.0f);  // kMapsOnly: the map of the passes so far
@@ -129,14 +129,14 @@ __global__ __launch_bounds__(64 * kWaves) void gae_kernel(const GaeArgs g) {
     if (kMapsOnly) {
       if (wave == 0 && run == 0) {
         float2 all = wave_map[0][column];
-        for (int k = 1; k < kWaves; ++k) all = after(all, wave_map[k][column]);
+        for (int k = 1; k < waves; ++k) all = after(all, wave_map[k][column]);
         total = after(all, total);
       }
       __syncthreads();
       continue;
     }
     float a = at + pass >= end ? carry : behind[turn ^ 1][column];
-    for (int k = kWaves - 1; k > wave; --k) a = apply(wave_map[k][column], a);
+    for (int k = waves - 1; k > wave; --k) a = apply(wave_map[k][column], a);
     if (wave == 0 && run == 0) behind[turn][column] = apply(map, a);
     a = apply(later, a);
 #pragma unroll
@@ -156,14 +156,19 @@ __global__ __launch_bounds__(64 * kWaves) void gae_kernel(const GaeArgs g) {
   if (kMapsOnly && wave == 0 && run == 0 && ok) g.maps[(i64)chunk * g.batch + b] = total;
 }
 
-// How a call is laid out: the columns of a wavefront, and the chunks the steps are split into, as
-// many as give the launch two workgroups a compute unit.  Two passes are not split: the second
-// costs less than the second launch and the second reading.  us unsplit / with one / two / four
-// workgroups a compute unit: 128 x 8,192 (two passes) 9.7 / 11.3 / 11.4 / 11.3, 128 x 16,384 13.1 /
-// 13.1 / 16.0 / 16.0, 256 x 1,024 (four) 15.0 / 10.1 / 10.1 / 10.1, 1,024 x 4,096 80 / 43.5 / 30.3 /
-// 31.2, 20,001 x 45 1,468 / 18.4 / 15.2 / 15.2.
+// How a call is laid out: the columns of a wavefront, the steps a lane holds and the wavefronts of
+// a workgroup, and the chunks that the steps are split into.
+// One or two passes are not split: the second pass costs less than a second launch and a second
+// reading.  Their lanes hold 4 steps, in as many wavefronts as the steps need (16 at most).  More
+// passes are split into as many chunks as give the launch two workgroups of 8 wavefronts a compute
+// unit; lanes then hold 8 steps, or 4 where games do not fill a wavefront's lanes.  us, 4 steps and up
+// to 16 wavefronts / 8 steps and 8 wavefronts: unsplit 128 x 32,768 16.3 / 18.0, 128 x 512 7.7 / 8.4,
+// 16 x 65,536 5.9 / 10.7; split 20,001 x 45 17.9 / 15.2, 1,024 x 4,096 28.5 / 29.7; 4 steps and 8
+// wavefronts / 8 and 8: 70,000 x 1 11.1 / 19.2, 1,000 x 10 8.7 / 10.0, 20,001 x 45 17.0 / 15.2.
+// Unsplit / one / two / four workgroups a compute unit: 128 x 8,192 (two passes) 9.7 / 11.3 / 11.4 /
+// 11.3, 256 x 1,024 (four) 15.0 / 10.1 / 10.1 / 10.1, 1,024 x 4,096 80 / 43.5 / 30.3 / 31.2.
 struct GaeLayout {
-  int columns, chunks;
+  int columns, steps, waves, chunks;
   i64 groups, chunk;
 };
 
@@ -172,26 +177,42 @@ inline GaeLayout gae_layout(i64 steps, i64 batch) {
   l.columns = 64;
   while (l.columns > 1 && l.columns / 2 >= batch) l.columns /= 2;
   l.groups = (batch + l.columns - 1) / l.columns;
-  const i64 pass = (i64)kWaves * (64 / l.columns) * kSteps;
-  const i64 passes = (steps + pass - 1) / pass;
+  const int runs = 64 / l.columns;
+  const i64 lanes = (steps + runs * 4 - 1) / (runs * 4);  // wavefronts that hold all of the steps
   i64 chunks = 2 * (i64)compute_units() / l.groups;
-  chunks = chunks < 1 || passes <= 2 ? 1 : chunks < passes ? chunks : passes;
+  if (lanes <= 2 * kMostWaves || chunks < 2) {
+    l.steps = 4;
+    l.waves = (int)(lanes < kMostWaves ? lanes : kMostWaves);
+    l.chunks = 1;
+    l.chunk = steps;
+    return l;
+  }
+  l.steps = l.columns == 64 ? 8 : 4;
+  l.waves = 8;
+  const i64 pass = (i64)l.waves * runs * l.steps;
+  const i64 passes = (steps + pass - 1) / pass;
+  if (chunks > passes) chunks = passes;
   const i64 each = (passes + chunks - 1) / chunks;
   l.chunk = each * pass;
   l.chunks = (int)((passes + each - 1) / each);
   return l;
 }
 
-template <class T>
+template <class T, int kSteps>
 int launch_gae(const GaeArgs& g, const GaeLayout& l, hipStream_t stream) {
   const dim3 grid((unsigned)l.groups, (unsigned)l.chunks);
   if (l.chunks > 1) {
-    gae_kernel<T, true><<<grid, 64 * kWaves, 0, stream>>>(g);
+    gae_kernel<T, kSteps, true><<<grid, 64 * l.waves, 0, stream>>>(g);
     const int rc = (int)hipGetLastError();
     if (rc != 0) return rc;
   }
-  gae_kernel<T, false><<<grid, 64 * kWaves, 0, stream>>>(g);
+  gae_kernel<T, kSteps, false><<<grid, 64 * l.waves, 0, stream>>>(g);
   return (int)hipGetLastError();
+}
+
+template <class T>
+int launch_gae(const GaeArgs& g, const GaeLayout& l, hipStream_t stream) {
+  return l.steps == 4 ? launch_gae<T, 4>(g, l, stream) : launch_gae<T, 8>(g, l, stream);
 }
 
 }  // namespace gae

@@ -1,8 +1,8 @@
 """advantages against the oracle in 64 bits.
 
 Tolerance, counted before any run: an advantage is a sum of terms d_k (gamma lam)^(k - t), each a
-few roundings of its parts; a term passes one multiply-add for each step inside a lane (8), each
-doubling of the scan (6), each wavefront (8), each pass and each chunk behind it, so u (32 + T / 64)
+few roundings of its parts; a term passes one multiply-add for each step inside a lane (4 or 8),
+each doubling of the scan (6), each wavefront (8 or 16), each pass and each chunk behind it, so u (32 + T / 64)
 of the sum of the parts' sizes bounds it, u = 2^-24; returns add one rounding."""
 
 from __future__ import annotations
@@ -59,7 +59,8 @@ def check(x, gamma, lam, got):
 @pytest.mark.parametrize("t,b", [(1, 1), (1, 70), (2, 5), (7, 3), (8, 64), (9, 65), (63, 33),
                                  (64, 1), (65, 2), (128, 300), (513, 1), (512, 17), (4097, 2),
                                  (1000, 33), (4096, 64), (5000, 3), (20001, 45), (70001, 1),
-                                 (129, 40000), (3, 70001)])
+                                 (129, 40000), (3, 70001), (5, 9), (16, 130), (17, 64), (61, 100),
+                                 (65, 700), (127, 65), (130, 64), (200, 31), (600, 500), (257, 9000)])
 def test_against_the_oracle(ext, t, b, dtype):
     announce(f"advantages {t}x{b} {dtype}")
     for k, (gamma, lam, share, players) in enumerate([(0.997, 0.95, 0.05, True),
