@@ -36,18 +36,14 @@ struct BF16 {
   __device__ static __bf16 from_float(float f) { return (__bf16)f; }
 };
 
-// K consecutive elements, read or written in one access; `Any` at an address that is only an
-// element's (global loads and stores take any alignment on gfx950).
+// K consecutive elements, read or written in one access.
 template <class S, int K>
 struct alignas(sizeof(S) * K) Vec {
   S v[K];
 };
-template <class S, int K>
-struct __attribute__((packed, aligned(sizeof(S)))) Any {
-  S v[K];
-};
 
-// N bytes as they lie in memory, in registers: `Raw` at their own alignment, `RawAny` at any.
+// N bytes as they lie in memory, in registers: `Raw` at their own alignment, `RawAny` at any
+// (global loads and stores of gfx950 take any alignment).
 typedef uint32_t Words2 __attribute__((ext_vector_type(2)));
 typedef uint32_t Words4 __attribute__((ext_vector_type(4)));
 template <int N>

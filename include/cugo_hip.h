@@ -733,8 +733,8 @@ int cugo_scale_gradients(int a_dtype, void* a, int64_t a_count, int b_dtype, voi
  *   a_t = d_t + [not done_t] gamma lam a_(t+1)
  *   advantage_t = s_t a_t, returns_t = advantage_t + value_t           (float32)
  * What follows a done step is not read into it.  workspace: at least
- * cugo_advantages_workspace(steps, batch) bytes (may be 0: then it may be NULL), in use until
- * the call's launches end. */
+ * cugo_advantages_workspace(steps, batch) bytes (asked on the device of the call; may be 0: then
+ * it may be NULL), in use until the call's launches end. */
 int64_t cugo_advantages_workspace(int64_t steps, int64_t batch);
 int cugo_advantages(int value_dtype, const float* reward, const void* value,
                     const uint8_t* done, const uint8_t* player, const void* bootstrap,

@@ -400,6 +400,49 @@ def test_optimizer_state_is_saved_and_loaded(ext, bits):
         wrong.load_state_dict(saved)
 
 
+def test_offsets_past_32_bits(ext):
+    """A tensor of more than 2^32 values with 8-bit moments: its last blocks' values, scales and
+    codes, whose rounding words take the index's upper bits."""
+    from cugo_amd import learner
+
+    n = (1 << 32) + 3 * ref.BLOCK + 77
+    tail = 2 * ref.BLOCK + 77
+    announce(f"adamw {n}")
+    blocks = -(-n // ref.BLOCK)
+    w = torch.zeros(n, dtype=torch.bfloat16, device=DEV)
+    grad = torch.zeros(n, dtype=torch.bfloat16, device=DEV)
+    master = torch.zeros(n, device=DEV)
+    g = torch.randn(tail, generator=torch.Generator().manual_seed(1)).bfloat16()
+    grad[-tail:] = g.to(DEV)
+    m = torch.zeros(n, dtype=torch.float8_e4m3fn, device=DEV)
+    v = torch.zeros(n, dtype=torch.float8_e5m2, device=DEV)
+    ms, vs = torch.zeros(blocks, device=DEV), torch.zeros(blocks, device=DEV)
+    steps = torch.zeros(1, dtype=torch.int64, device=DEV)
+    norm = learner.adamw_step(ext, [w], [grad], [m], [v], steps, lr=0.1, weight_decay=0.0,
+                              max_norm=1e9, master=[master], exp_avg_scale=[ms],
+                              exp_avg_sq_scale=[vs], seed=77)
+    assert abs(float(norm) - float(g.double().norm())) < 1e-5 * float(norm)
+    assert (master[:-tail][::9973] == 0).all()
+    # from moments of zero the first step is lr g / (|g| + eps), within 16 u and the moments' 14
+    goal = -0.1 * g.double() / (g.double().abs() + EPS)
+    off = float((master[-tail:].cpu().double() - goal).abs().max())
+    assert off <= 0.1 * 30 * U
+    g32 = g.float()
+    for got, scale, z, top, mant, least in (
+            (m, ms, g32 * (1 - 0.9), 256.0, 3, -6),
+            (v, vs, (g32 * g32) * (1 - 0.999), 32768.0, 2, -14)):
+        most = torch.stack([x.abs().max() for x in z.split(ref.BLOCK)])
+        assert torch.equal(scale[-3:].cpu(), most * (1 / top))
+        up = (z.abs() * (top / most).repeat_interleave(ref.BLOCK)[:tail]).tolist()
+        for i in range(0, tail, 7):
+            word = ref.word(77, 0, 1, n - tail + i)
+            bits = word if mant == 3 else (word << 16) & ref.MASK
+            want = ref.code(up[i], bits, mant, least)
+            if mant == 2 and z[i] > 0:
+                want = max(want, 1)
+            assert int(got[n - tail + i].view(torch.uint8)) & 127 == want, i
+
+
 def test_one_gradient_for_two_parameters(ext):
     """Gradients are read only: two parameters may share one."""
     x = make([700, 700], torch.float32, torch.float32, 11)

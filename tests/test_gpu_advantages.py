@@ -122,6 +122,24 @@ def test_outputs_streams_graphs(ext):
         assert torch.equal(again[0], want[k][0])
 
 
+def test_offsets_past_32_bits(ext):
+    """More than 2^31 steps: the last games are those of a call on them alone."""
+    t, b = 70, 31_000_001
+    announce(f"advantages {t}x{b}")
+    g = torch.Generator(device=DEV).manual_seed(3)
+    reward = torch.empty(t, b, device=DEV).normal_(generator=g)
+    value = torch.empty(t, b, dtype=torch.bfloat16, device=DEV).normal_(generator=g)
+    done = torch.zeros(t, b, dtype=torch.bool, device=DEV)
+    done[30] = True
+    bootstrap = torch.ones(b, dtype=torch.bfloat16, device=DEV)
+    adv, ret = ext.advantages(reward, value, done, bootstrap, 0.99, 0.95)
+    for cols in (slice(0, 100), slice(b // 2, b // 2 + 100), slice(b - 100, b)):
+        part = [x[..., cols].contiguous() for x in (reward, value, done, bootstrap)]
+        a, r = ext.advantages(*part, 0.99, 0.95)
+        diff = torch.maximum((adv[:, cols] - a).abs().max(), (ret[:, cols] - r).abs().max())
+        assert diff < 1e-4, diff  # another split of the steps: other roundings of sums below 100
+
+
 def test_empty(ext):
     for t, b in ((0, 5), (5, 0), (0, 0)):
         x = make(t, b, torch.float32, 1)

@@ -463,3 +463,58 @@ def test_refusals(ext):
                  dict(loss_scale=torch.ones(1))):
         with pytest.raises(RuntimeError):
             go(**over)
+
+
+def _bits_of(t):
+    return t.view(torch.int16) if t.element_size() == 2 else t.view(torch.int32)
+
+
+@pytest.mark.parametrize("n,a", [(12_100_000, 179), (66_000, 33_000)])
+def test_offsets_past_32_bits(ext, n, a):
+    """More than 2^31 logits: the first, a middle and the last rows are those of calls on them alone,
+    with the weights of the whole."""
+    announce(f"policy_loss {n}x{a}")
+    g = torch.Generator(device=DEV).manual_seed(8)
+    logits = torch.empty(n, a, dtype=torch.bfloat16, device=DEV).normal_(generator=g).requires_grad_()
+    action = torch.randint(0, a, (n,), generator=g, device=DEV)
+    old = torch.full((n,), -math.log(a), device=DEV)
+    adv = torch.randn(n, generator=g, device=DEV)
+    weight = torch.full((n,), 0.01, device=DEV)
+    loss, stats, logp = ext.policy_loss(logits, action, old, adv, weight=weight, entropy_coef=0.1)
+    grad, = torch.autograd.grad(loss, [logits])
+    for first in (0, n // 2 + 1, n - 40):
+        rows = slice(first, first + 40)
+        part = logits.detach()[rows].clone().requires_grad_()
+        p_loss, _, p_logp = ext.policy_loss(part, action[rows].clone(), old[rows].clone(),
+                                            adv[rows].clone(), weight=weight[rows].clone(),
+                                            entropy_coef=0.1)
+        p_grad, = torch.autograd.grad(p_loss, [part])
+        assert torch.equal(logp[rows], p_logp)
+        assert torch.equal(_bits_of(grad[rows].contiguous()), _bits_of(p_grad))
+    assert torch.isfinite(loss)
+
+
+def test_two_streams_at_once(ext):
+    """Calls of two streams side by side keep to their own scratch memory."""
+    xs = [make(3000, 179, torch.bfloat16, 70 + k, weight=False) for k in range(2)]
+    want = [call(ext, x) for x in xs]
+    on = [{k: v.to(DEV) for k, v in x.items() if isinstance(v, torch.Tensor)} for x in xs]
+    from cugo_amd import learner
+
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                out = learner.policy_loss(
+                    ext, on[k]["logits"].requires_grad_(), on[k]["action"], on[k]["old_logp"],
+                    on[k]["advantage"], legal=on[k]["legal"], ref_logits=on[k]["ref"],
+                    value=on[k]["value"], returns=on[k]["returns"], **ARGS)
+                got[k].append((out.loss.detach(), out.stats,
+                               *torch.autograd.grad(out.loss, [on[k]["logits"]])))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for loss, stats, grad in got[k]:
+            assert torch.equal(loss, want[k]["loss"]) and torch.equal(stats, want[k]["stats"])
+            assert torch.equal(grad, want[k]["d_logits"])
