@@ -10,8 +10,8 @@
 // compose theirs (a suffix scan in the wavefront, then over the wavefronts in LDS), and each
 // lane runs its own steps again from the value that follows them.  The data is read once.
 //
-// What bounds it is memory, 16 to 18 bytes a step of a game (128 steps of 65,536 games in 31 us,
-// 4.8 TB/s), and below about a million steps the two or three rounds of latency of a launch (5 us
+// What bounds it is memory, 16 to 18 bytes a step of a game (128 steps of 65,536 games in 29 us,
+// 5.2 TB/s), and below about a million steps the two or three rounds of latency of a launch (5 us
 // for 64 x 300).  A wavefront's 64 lanes are
 // `columns` games times 64 / columns runs of steps, the fewest columns (a power of two) that
 // hold the games up to 64, so that few games still fill wavefronts; where the workgroups of
@@ -43,8 +43,8 @@ struct GaeArgs {
   float2* maps;  // [chunks, batch]: the chunks' maps (chunks > 1)
 };
 
-// m applied to the value a that follows it, which a done step (m.y = 0) does not read: a NaN
-// of the next game stays there.
+// m applied to the value a that follows it, which a factor of 0 (a done step, or lam = 0) does not
+// read: a NaN of the next game stays there.
 __device__ inline float apply(float2 m, float a) {
   return m.y == 0.0f ? m.x : __builtin_fmaf(m.y, a, m.x);
 }
@@ -113,6 +113,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void gae_kernel(const GaeArgs g) {
       if (t0 + i < end) {
         const float next = over[i] ? 0.0f : g.gamma * (sign[i + 1] * v[i + 1]);
         d[i] = d[i] + next - sign[i] * v[i];
+        over[i] = over[i] || g.decay == 0.0f;  // from here on: nothing is read from behind
         map.x = over[i] ? d[i] : __builtin_fmaf(g.decay, map.x, d[i]);
         map.y = over[i] ? 0.0f : g.decay * map.y;
       }

@@ -92,6 +92,20 @@ def test_nothing_passes_a_done_step(ext):
         assert torch.isfinite(got[0]).all() and torch.isfinite(got[1]).all()
 
 
+def test_nothing_passes_a_factor_of_zero(ext):
+    """With lam = 0 a step reads the next one's value alone, not what becomes of it."""
+    for t, b in ((40, 70), (700, 3), (3000, 100)):
+        x = make(t, b, torch.float32, t, share=0.0)
+        x["reward"][5::9] = float("nan")
+        adv, _ = call(ext, x, 0.99, 0.0)
+        bad = torch.isnan(x["reward"])
+        assert torch.equal(torch.isnan(adv).cpu(), bad)
+        y = dict(x, reward=x["reward"].nan_to_num(nan=0.0))
+        check({k: v[:5] if v.dim() == 2 else v for k, v in y.items()} | {
+            "bootstrap": y["value"][5], "last_player": y["player"][5]}, 0.99, 0.0,
+            [z[:5] for z in call(ext, x, 0.99, 0.0)])
+
+
 def test_outputs_streams_graphs(ext):
     """Results in given tensors; a side stream; captured and replayed on new inputs."""
     xs = [make(700, 5, torch.float32, 20 + k) for k in range(3)]

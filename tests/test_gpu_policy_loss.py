@@ -221,6 +221,21 @@ def test_the_only_legal_action_is_certain(ext):
             assert (got["d_logits"][~x["legal"].to(DEV)] == 0).all()
 
 
+def test_a_reference_without_the_action_is_infinitely_far(ext):
+    """A legal action that the other policy never takes: the KL term is infinite, the rest is not."""
+    for a in (2, 40, 179, 300, 1000, 2000, 9000, 40000):
+        for dtype in (torch.float32, torch.bfloat16):
+            x = make(3, a, dtype, a, weight=False, share=0.9)
+            x["legal"][0, :2] = True
+            x["ref"][0, 0] = -math.inf
+            got = call(ext, x)
+            assert got["stats"][2] == math.inf and got["loss"] == math.inf, a
+            assert torch.isfinite(got["stats"][[0, 1, 3, 4, 5]]).all()
+            x["legal"][0, 0] = False  # illegal: of no account
+            x["action"][0] = 1
+            assert torch.isfinite(call(ext, x)["loss"]), a
+
+
 def test_nan_in_the_only_legal_logit_shows(ext):
     """No other logit is there to be the largest: the row must not pass for one without any."""
     for a in (1, 3, 40, 179, 300, 1024, 2000, 9000, 40000):
