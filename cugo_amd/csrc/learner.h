@@ -86,33 +86,38 @@ __device__ inline void unpack(const Words4& w, float (&f)[16 / sizeof(typename T
   }
 }
 
-// x from the lane that kCtrl, a rotation within the 16 lanes of a DPP row, names.
+// x from the lane that the DPP control kCtrl names: within four lanes, or the 16 of a row.
 template <int kCtrl>
-__device__ inline float rotated(float x) {
+__device__ inline float exchanged(float x) {
   return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), kCtrl, 0xf, 0xf, false));
 }
 
-// The sum and the largest over groups of G lanes (16, 32 or 64), the same value in every lane.
+// The sum and the largest over groups of G lanes (4 to 64), the same value in every lane: by
+// exchanges within four lanes, within eight (the half row mirrored) or 16 (rotations), and beyond.
 // v_max_f32 takes the other operand for a NaN: a NaN shows in the sums of exponentials.
-template <int G>
-__device__ inline float group_sum(float x) {
-  x += rotated<0x128>(x);
-  x += rotated<0x124>(x);
-  x += rotated<0x122>(x);
-  x += rotated<0x121>(x);
-  if constexpr (G >= 32) x += __shfl_xor(x, 16);
-  if constexpr (G == 64) x += __shfl_xor(x, 32);
+template <int G, class With>
+__device__ inline float group_reduce(float x, With with) {
+  if constexpr (G <= 8) {
+    x = with(x, exchanged<0xb1>(x));
+    x = with(x, exchanged<0x4e>(x));
+    if constexpr (G == 8) x = with(x, exchanged<0x141>(x));
+  } else {
+    x = with(x, exchanged<0x128>(x));
+    x = with(x, exchanged<0x124>(x));
+    x = with(x, exchanged<0x122>(x));
+    x = with(x, exchanged<0x121>(x));
+  }
+  if constexpr (G >= 32) x = with(x, __shfl_xor(x, 16));
+  if constexpr (G == 64) x = with(x, __shfl_xor(x, 32));
   return x;
 }
 template <int G>
+__device__ inline float group_sum(float x) {
+  return group_reduce<G>(x, [](float a, float b) { return a + b; });
+}
+template <int G>
 __device__ inline float group_max(float x) {
-  x = fmaxf(x, rotated<0x128>(x));
-  x = fmaxf(x, rotated<0x124>(x));
-  x = fmaxf(x, rotated<0x122>(x));
-  x = fmaxf(x, rotated<0x121>(x));
-  if constexpr (G >= 32) x = fmaxf(x, __shfl_xor(x, 16));
-  if constexpr (G == 64) x = fmaxf(x, __shfl_xor(x, 32));
-  return x;
+  return group_reduce<G>(x, [](float a, float b) { return fmaxf(a, b); });
 }
 
 inline bool dtype_known(int d) {

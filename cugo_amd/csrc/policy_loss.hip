@@ -156,13 +156,17 @@ __device__ inline RowTerms row_terms(const LossArgs& g, const RowInputs& in, flo
   return x;
 }
 
-// A workgroup's sums (kStats of each of its 256 / G groups of lanes, in acc of the group's lane
-// j = the sum's place) to its partials: in a fixed order, so a call's results are the same
+// A workgroup's sums to its partials: lane j of each of its 256 / G groups of lanes holds sum j in
+// acc[0] (and sum j + G in acc[1], for G = 4).  In a fixed order, so a call's results are the same
 // every time.
 template <int G>
-__device__ inline void write_partials(double acc, int j, double* partials) {
+constexpr int kHeld = (kStats + G - 1) / G;  // sums a lane holds
+template <int G>
+__device__ inline void write_partials(const double (&acc)[kHeld<G>], int j, double* partials) {
   __shared__ double sums[kThreads / G][kStats];
-  if (j < kStats) sums[threadIdx.x / G][j] = acc;
+#pragma unroll
+  for (int h = 0; h < kHeld<G>; ++h)
+    if (j + h * G < kStats) sums[threadIdx.x / G][j + h * G] = acc[h];
   __syncthreads();
   if (threadIdx.x < kStats) {
     double total = 0.0;
@@ -185,7 +189,7 @@ __device__ inline void wavefront_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// What a row has besides its logits, for the rows of 16 lanes: lane 0 of the 16 reads the old
+// What a row has besides its logits, for the rows of 16 lanes and more: lane 0 of 16 reads the old
 // log-probability, lane 1 the advantage and so on, one access instead of six (the addresser, not
 // memory, is what short rows keep busy), and all take the values from those lanes.
 struct RowReader {
@@ -235,8 +239,8 @@ struct RowReader {
 // gradient, a vector of each lane at a time: kept in registers for that, a row of 179 actions
 // took 96 to 112 of them and left four wavefronts a SIMD.
 // A game's row has about ten legal actions of 179, and an exponential or a product for each action
-// takes longer than memory does: where each row of a wavefront has at most two legal actions a
-// lane, a list of their slots is made, a lane computes two of them, and the gradient is put
+// takes longer than memory does: where each row of a wavefront of 16-lane rows has at most two legal
+// actions a lane, a list of their slots is made, a lane computes two of them, and the gradient is put
 // together in LDS.  1,048,576 x 179 bf16 with a KL term, 10 legal actions a row: 298 us (4.5 TB/s;
 // the arithmetic is half of that), with 60, where the list does not hold them, 373, and 379 for
 // the earlier form that computed all of the actions always.
@@ -247,7 +251,9 @@ __global__ __launch_bounds__(kThreads) void loss_rows_kernel(const LossArgs g) {
   using Slots = Vec<S, E>;
   constexpr int kRows = kThreads / G;
   constexpr int kSlots = V * G * E;
-  constexpr bool kList = kSlots <= 256;  // a slot fits a byte
+  // A slot of 16 lanes fits a byte, and their counts one DPP row; on fewer lanes rows are too short
+  // for a list to pay.
+  constexpr bool kList = G == 16;
   __shared__ __align__(16) S z_slots[kRows][kSlots];
   __shared__ __align__(16) S q_slots[kRef ? kRows : 1][kRef ? kSlots : E];
   __shared__ uint8_t lists[kList ? kRows : 1][2 * G];
@@ -262,13 +268,14 @@ __global__ __launch_bounds__(kThreads) void loss_rows_kernel(const LossArgs g) {
   S* ql = q_slots[kRef ? row : 0];
   const RowReader reader(g);
   const i64 tiles = (g.n + kRows - 1) / kRows;
-  double acc = 0.0;
+  double acc[kHeld<G>] = {};
   for (i64 tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const i64 r0 = tile * kRows;
     const bool ok = r0 + row < g.n;
     // loads are unconditional, of a row that exists; the sums leave it out
     const uint32_t i0 = (uint32_t)(ok ? row : (int)(g.n - 1 - r0));
-    const int part = reader.read(r0 + i0);
+    int part = 0;
+    if constexpr (G >= 16) part = reader.read(r0 + i0);
     uint32_t bits = own;
     {
       const S* zb = static_cast<const S*>(g.logits) + r0 * g.logits_stride;
@@ -315,7 +322,13 @@ __global__ __launch_bounds__(kThreads) void loss_rows_kernel(const LossArgs g) {
       }
     }
     i64 act;
-    const RowInputs in = reader.inputs(g, part, r0, i0, act);
+    RowInputs in;
+    if constexpr (G >= 16) {
+      in = reader.inputs(g, part, r0, i0, act);
+    } else {
+      in = row_inputs(g, r0, i0);
+      act = (g.action + r0)[i0];
+    }
     // the action's slot, where the row has it
     const int moved_from = g.actions & ~(E - 1);
     const int slot_of_act = act < 0 || act >= g.actions ? -1
@@ -492,10 +505,13 @@ __global__ __launch_bounds__(kThreads) void loss_rows_kernel(const LossArgs g) {
       }
     }
     wavefront_sync();  // the next rows' logits come after these reads
-    float stat = x.stat[5];
 #pragma unroll
-    for (int k = 0; k < kStats - 1; ++k) stat = j == k ? x.stat[k] : stat;
-    acc += ok ? (double)stat : 0.0;
+    for (int h = 0; h < kHeld<G>; ++h) {
+      float stat = x.stat[kStats - 1];
+#pragma unroll
+      for (int k = 0; k < kStats - 1; ++k) stat = j + h * G == k ? x.stat[k] : stat;
+      acc[h] += ok ? (double)stat : 0.0;
+    }
     if (ok && j == 0) {
       (g.logp + r0)[i0] = x.logp;
       if (g.d_value)
@@ -952,7 +968,8 @@ int launch_rows(const LossArgs& g, i64 pieces, int threads, hipStream_t stream) 
   return groups;
 }
 
-// Rows of up to kRowsMost actions are addressed by 32 bits within a workgroup's 4 or 16 rows.
+// Rows of up to kRowsMost actions are addressed by 32 bits within a workgroup's rows: 64 at most, so
+// that the last of kStrideMost float32 elements apart begins below 2^32 bytes.
 constexpr int kRowsMost = 1024;
 constexpr i64 kStrideMost = (i64)1 << 24;
 
@@ -970,8 +987,15 @@ int launch_loss(const LossArgs& g, hipStream_t stream) {
   // 356, 1,024 230 and 1,025 316 (a workgroup of 64 threads: 199 and 562 of 256), 2,048 170, 4,096
   // 178, 8,192 167 and 8,193 276, 32,768 184 and 32,769 265.  Rows of 768 take 245 on 64 lanes and 253
   // as a workgroup of 64 threads, with a mask 249 and 353.
-  if (a < 4) return CUGO_LOSS_ROWS(16, 1, 1);
-  if (a <= 64) return CUGO_LOSS_ROWS(16, 1, 4);
+  // Few actions, us of 2^21 rows (2^26 logits, where those are fewer) against 16 lanes: 4 actions 89
+  // and 261, 16 89 and 251, 32 143 and 272, 48 125 and 228; 64 on 8 lanes 142 and 174 (133 on 4,
+  // which float32 rows take 224 for, and 172 on 8, 182 on 16), with 10 of them legal 147 and 141.
+  // Rows of 96 take 372 a 2^27 logits on 16 lanes and 247 on 8, but with 10 legal 227 and 255.
+  if (a < 4) return CUGO_LOSS_ROWS(4, 1, 1);
+  if (a <= 16) return CUGO_LOSS_ROWS(4, 1, 4);
+  if (a <= 32) return CUGO_LOSS_ROWS(4, 2, 4);
+  if (a <= 48) return CUGO_LOSS_ROWS(4, 3, 4);
+  if (a <= 64) return CUGO_LOSS_ROWS(8, 2, 4);
   if (a <= 128) return CUGO_LOSS_ROWS(16, 2, 4);
   if (a <= 192) return CUGO_LOSS_ROWS(16, 3, 4);
   if (a <= 256) return CUGO_LOSS_ROWS(16, 4, 4);

@@ -154,7 +154,7 @@ def test_against_the_oracle(ext, n, a, dtype):
         check(x, call(ext, x, grad=False))
 
 
-@pytest.mark.parametrize("a", [2, 40, 179, 300, 1500, 9000, 40000])
+@pytest.mark.parametrize("a", [2, 7, 20, 40, 60, 179, 300, 1500, 9000, 40000])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_special_entries(ext, a, dtype):
     """-inf, the type's lowest value, NaN and infinities in illegal places, rows whose legal
@@ -281,6 +281,38 @@ def test_rows_far_apart(ext):
         p, q = call(ext, dict(x, logits=room[:, 1:1 + a])), call(ext, x)
         for k in p:
             assert torch.equal(p[k], q[k]), k
+
+
+FEW = [(1, 1), (65, 1), (63, 3), (64, 4), (130, 7), (66, 15), (67, 18), (65, 31), (64, 32), (3, 33),
+       (65, 47), (129, 48), (33, 49), (31, 50), (70, 61), (300, 5)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,a", FEW)
+def test_few_actions(ext, n, a, dtype):
+    """Rows of 4 and of 8 lanes, on both sides of each line, and workgroups that end inside."""
+    for k, (legal, with_ref, weight, value) in enumerate([
+            (True, True, True, torch.float32), (False, True, False, None),
+            (True, False, False, torch.bfloat16), (False, False, True, torch.float16)]):
+        announce(f"policy_loss {n}x{a} {dtype} variant {k}")
+        x = make(n, a, dtype, 100 * a + k, legal, with_ref, value, weight)
+        check(x, call(ext, x))
+        check(x, call(ext, x, grad=False))
+
+
+@pytest.mark.parametrize("a", [1, 3, 4, 30, 48, 64])
+def test_few_actions_as_far_apart_as_rows_are_addressed(ext, a):
+    """float32 rows 2^24 - 1 elements apart: the last of a workgroup's 64 begins 4,227,858,180 bytes
+    behind the first."""
+    n, stride = 65, (1 << 24) - 1
+    announce(f"far apart {n}x{a}")
+    x = make(n, a, torch.float32, a, weight=False)
+    room = torch.empty((n - 1) * stride + a, dtype=torch.float32, device=DEV)
+    logits = room.as_strided((n, a), (stride, 1))
+    logits.copy_(x["logits"])
+    p, q = call(ext, dict(x, logits=logits)), call(ext, x)
+    for k in p:
+        assert torch.equal(p[k], q[k]), k
 
 
 def test_strides_and_offsets(ext):
