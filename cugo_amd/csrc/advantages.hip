@@ -48,8 +48,13 @@ struct GaeArgs {
 __device__ inline float apply(float2 m, float a) {
   return m.y == 0.0f ? m.x : __builtin_fmaf(m.y, a, m.x);
 }
+// The product of two factors in [0, 1]: 0 only where one of them is, and not where it underflows,
+// so that a NaN or an infinity far behind in the same game shows in every step before it.
+__device__ inline float product(float a, float b) {
+  return a == 0.0f || b == 0.0f ? 0.0f : fmaxf(a * b, 0x1p-149f);
+}
 __device__ inline float2 after(float2 m, float2 later) {
-  return make_float2(apply(m, later.x), m.y * later.y);
+  return make_float2(apply(m, later.x), product(m.y, later.y));
 }
 
 // kSteps: the steps a lane holds.
@@ -115,7 +120,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void gae_kernel(const GaeArgs g) {
         d[i] = d[i] + next - sign[i] * v[i];
         over[i] = over[i] || g.decay == 0.0f;  // from here on: nothing is read from behind
         map.x = over[i] ? d[i] : __builtin_fmaf(g.decay, map.x, d[i]);
-        map.y = over[i] ? 0.0f : g.decay * map.y;
+        map.y = over[i] ? 0.0f : product(g.decay, map.y);
       }
     }
     // each lane's map and those of the later runs of its column, then of the later runs alone

@@ -106,6 +106,23 @@ def test_nothing_passes_a_factor_of_zero(ext):
             [z[:5] for z in call(ext, x, 0.99, 0.0)])
 
 
+def test_what_is_not_finite_shows_however_far_ahead(ext):
+    """gamma lam to the power of the steps between is far below the least float32: a NaN or an
+    infinity is still in every step before it, as in the recurrence, up to the game's beginning."""
+    for t, b, decay in ((400, 70, 0.5), (3000, 1, 0.9), (2000, 3, 1e-3), (5000, 45, 0.25),
+                        (1200, 2, 1e-30)):
+        x = make(t, b, torch.float32, t, share=0.0)
+        x["done"][t // 3] = True
+        x["reward"][t - 7, 0] = float("nan")
+        if b > 1:
+            x["reward"][t - 3, 1] = float("inf")
+            x["value"][t - 9, b - 1] = float("nan")
+        adv, _ = call(ext, x, 1.0, decay)
+        want, _ = ref.advantages(**x, gamma=1.0, lam=decay)
+        assert torch.equal(torch.isfinite(adv).cpu(), torch.isfinite(want)), (t, b, decay)
+        assert torch.equal(torch.isnan(adv).cpu(), torch.isnan(want)), (t, b, decay)
+
+
 def test_outputs_streams_graphs(ext):
     """Results in given tensors; a side stream; captured and replayed on new inputs."""
     xs = [make(700, 5, torch.float32, 20 + k) for k in range(3)]
