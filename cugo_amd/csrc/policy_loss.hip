@@ -1032,6 +1032,9 @@ int cugo_policy_loss(const CugoPolicyLoss* p, hipStream_t stream) {
   if (p->actions <= kRowsMost && (p->logits_stride >= kStrideMost || p->ref_stride >= kStrideMost ||
                                   p->legal_stride >= kStrideMost || p->d_logits_stride >= kStrideMost))
     return -4;
+  if (p->logits_stride < 0 || p->ref_stride < 0 || p->legal_stride < 0 ||
+      (p->d_logits && p->n > 1 && p->d_logits_stride < p->actions))
+    return -4;
   LossArgs g{};
   g.logits = p->logits, g.ref = p->ref_logits, g.legal = p->legal;
   g.logits_stride = p->logits_stride, g.ref_stride = p->ref_stride;

@@ -68,6 +68,15 @@ def test_policy_loss(lib):
         assert lib.cugo_policy_loss(ctypes.byref(x), None) == code, over
 
 
+def test_policy_loss_strides(lib):
+    """Rows that run backwards, and gradients whose rows overlap."""
+    for over in (dict(logits_stride=-179), dict(legal_stride=-1), dict(ref_stride=-179),
+                 dict(actions=2000, logits_stride=-2000), dict(d_logits=AT, d_logits_stride=178),
+                 dict(d_logits=AT, d_logits_stride=0)):
+        x = _loss(**over)
+        assert lib.cugo_policy_loss(ctypes.byref(x), None) == -4, over
+
+
 def test_scale_gradients(lib):
     assert lib.cugo_scale_gradients(F32, AT, -1, F32, None, 0, AT, None) == -1
     assert lib.cugo_scale_gradients(F32, None, 4, F32, None, 0, AT, None) == -1
