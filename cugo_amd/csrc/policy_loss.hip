@@ -478,7 +478,8 @@ __global__ __launch_bounds__(kThreads) void loss_rows_kernel(const LossArgs g) {
             const bool has = !(p == 0.0f);
             float h = __builtin_fmaf(x.c, has ? t : 0.0f, x.a);
             if constexpr (kRef) h = __builtin_fmaf(x.b, has ? t - scale_ref(q[e]) : 0.0f, h);
-            const float f = __builtin_fmaf(p, h, -(k + e == slot_of_act && has ? x.pull : 0.0f));
+            // the pull, whatever p is: an action so far below the others that p is 0 has a ratio
+            const float f = __builtin_fmaf(p, h, -(k + e == slot_of_act ? x.pull : 0.0f));
             o.v[e] = T::from_float(x.live ? f : 0.0f);
           }
           *reinterpret_cast<Slots*>(zl + k) = o;  // where this lane alone has read

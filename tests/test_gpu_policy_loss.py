@@ -565,3 +565,49 @@ def test_two_streams_at_once(ext):
         for loss, stats, grad in got[k]:
             assert torch.equal(loss, want[k]["loss"]) and torch.equal(stats, want[k]["stats"])
             assert torch.equal(grad, want[k]["d_logits"])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("a,few", [(7, False), (20, False), (40, False), (64, False), (100, False),
+                                   (179, False), (179, True), (300, False), (600, False),
+                                   (1000, False), (1000, True), (2000, False), (2000, True),
+                                   (9000, False), (40000, False), (40000, True)])
+def test_a_taken_action_far_below_the_others(ext, a, few, dtype):
+    """100 below the row's largest logit a probability is 0 in float32; the log-probability and the
+    ratio are not, and the gradient has the action's pull."""
+    for with_ref in (True, False):
+        announce(f"far action {a} {few} {dtype} {with_ref}")
+        x = make(6, a, dtype, a, legal=few, with_ref=with_ref, weight=False, value=None,
+                 share=8 / a)
+        on = x["legal"] if few else torch.ones(6, a, dtype=torch.bool)
+        on[:, :2] = True
+        x["action"] = torch.tensor([a - 1, 0, a // 2, 1, a - 1, 0])
+        on[torch.arange(6), x["action"]] = True
+        for i in (0, 2, 4, 5):
+            others = on[i].clone()
+            others[x["action"][i]] = False
+            x["logits"][i, x["action"][i]] = x["logits"][i][others].float().max() - 100
+        z = x["logits"].double().masked_fill(~on, -math.inf)
+        logp = ref.log_softmax(z).gather(1, x["action"][:, None])[:, 0]
+        assert (logp[[0, 2, 4, 5]] < -99).all()
+        x["old_logp"] = (logp + 0.1).float()  # inside the clip
+        x["advantage"] = torch.tensor([1.0, -1.0, -2.0, 0.5, 0.7, 3.0])
+        got = call(ext, x)
+        check(x, got)
+        taken = got["d_logits"].cpu().gather(1, x["action"][:, None])[:, 0].float()
+        assert (taken[[0, 2, 4, 5]].abs() > 0.05).all(), taken
+
+
+def test_a_rows_gradient_is_its_own(ext):
+    """Whatever the masks of the rows beside it: few legal actions are listed, many are not."""
+    a = 179
+    x = make(4, a, torch.float32, 1, weight=False, value=None, share=0.05)
+    x["legal"][:, :2] = True
+    x["action"][:] = 1
+    x["logits"][0, 1] = -100.0
+    x["old_logp"][0] = -100.0
+    few = call(ext, x)
+    many = call(ext, dict(x, legal=x["legal"] | (torch.arange(4) > 0)[:, None]))
+    assert few["d_logits"][0].abs().max() > 0.01
+    # both carry the errors counted above, below 64 u (4 |l| = 400 in the exponent) of the pull
+    assert (few["d_logits"][0] - many["d_logits"][0]).abs().max() <= 2 * (400 + 64) * U
