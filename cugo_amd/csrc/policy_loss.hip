@@ -17,7 +17,8 @@
 // term alone.  An action that is illegal, outside the row or at a logit of -inf has
 // probability 0: log-probability -inf, ratio 0, no gradient through the ratio.
 // A logit whose exponential is 0 beside the row's largest (-inf, the type's lowest value) has
-// p l = 0, as the limit is.
+// p l = 0, as the limit is, and p times the row's terms 0 where those are infinite or NaN: what is
+// illegal has no gradient whatever the rest of the row holds.
 #include "learner.h"
 
 #include <math.h>
@@ -140,7 +141,7 @@ __device__ inline RowTerms row_terms(const LossArgs& g, const RowInputs& in, flo
   x.stat[4] = x.live && cut ? in.w : 0.0f;
   x.stat[5] = x.live ? (ratio - 1.0f - drift) * in.w : 0.0f;
   const float wu = in.w * (g.scale ? *g.scale : 1.0f);
-  const float pull = cut ? 0.0f : ratio * in.adv;
+  const float pull = cut || x.logp == -INFINITY ? 0.0f : ratio * in.adv;
   const float per = wu * inv;
   // c_e p (l + H) = c_e p ln 2 (x - mean);  c_k p (l - l' - K) = c_k p ln 2 (d - kl2)
   x.c = per * (g.entropy_coef * kLn2);
@@ -405,6 +406,7 @@ __global__ __launch_bounds__(kThreads) void loss_rows_kernel(const LossArgs g) {
         for (int h = 0; h < 2; ++h) {
           float f = __builtin_fmaf(x.c, t[h], x.a);
           if constexpr (kRef) f = __builtin_fmaf(x.b, d[h], f);
+          f = p[h] == 0.0f ? 0.0f : f;
           f = __builtin_fmaf(p[h], f, -(slot[h] == slot_of_act ? x.pull : 0.0f));
           if (slot[h] >= 0 && x.live) zl[slot[h]] = T::from_float(f);
         }
@@ -476,8 +478,9 @@ __global__ __launch_bounds__(kThreads) void loss_rows_kernel(const LossArgs g) {
             const float t = scale(z[e]);
             const float p = exp2_of(t);
             const bool has = !(p == 0.0f);
-            float h = __builtin_fmaf(x.c, has ? t : 0.0f, x.a);
-            if constexpr (kRef) h = __builtin_fmaf(x.b, has ? t - scale_ref(q[e]) : 0.0f, h);
+            float h = __builtin_fmaf(x.c, t, x.a);
+            if constexpr (kRef) h = __builtin_fmaf(x.b, t - scale_ref(q[e]), h);
+            h = has ? h : 0.0f;
             // the pull, whatever p is: an action so far below the others that p is 0 has a ratio
             const float f = __builtin_fmaf(p, h, -(k + e == slot_of_act ? x.pull : 0.0f));
             o.v[e] = T::from_float(x.live ? f : 0.0f);
@@ -670,9 +673,9 @@ __device__ inline void store_gradients(const LossArgs& g, typename T::storage* o
       h = __builtin_fmaf(bc, t, x.a);  // a + b (t - t') + c t
       if constexpr (kRef) h = __builtin_fmaf(-x.b, scale_ref(q[e]), h);
     } else {
-      const bool has = !(p == 0.0f);
-      h = __builtin_fmaf(x.c, has ? t : 0.0f, x.a);
-      if constexpr (kRef) h = __builtin_fmaf(x.b, has ? t - scale_ref(q[e]) : 0.0f, h);
+      h = __builtin_fmaf(x.c, t, x.a);
+      if constexpr (kRef) h = __builtin_fmaf(x.b, t - scale_ref(q[e]), h);
+      h = p == 0.0f ? 0.0f : h;
     }
     f[e] = p * h;
   }

@@ -611,3 +611,34 @@ def test_a_rows_gradient_is_its_own(ext):
     assert few["d_logits"][0].abs().max() > 0.01
     # both carry the errors counted above, below 64 u (4 |l| = 400 in the exponent) of the pull
     assert (few["d_logits"][0] - many["d_logits"][0]).abs().max() <= 2 * (400 + 64) * U
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("a", [3, 20, 40, 64, 100, 179, 300, 600, 1000, 2000, 9000, 40000])
+def test_illegal_actions_have_no_gradient_in_rows_that_are_not_finite(ext, a, dtype):
+    """NaN or infinite advantages, logits and KL terms, and an illegal action with an infinite
+    advantage: the loss shows them, the illegal entries' gradients are 0 all the same, whether few
+    of the actions are legal or most."""
+    for share in (0.04, 0.9):
+        announce(f"not finite {a} {dtype} {share}")
+        x = make(5, a, dtype, a, weight=False, share=share)
+        x["legal"][:, 0] = True
+        x["legal"][:, a // 2] = False
+        x["action"][:] = 0
+        x["old_logp"][:] = -1.0
+        x["advantage"][0] = math.nan
+        x["ref"][1, 0] = -math.inf
+        x["logits"][2, 0] = math.nan
+        x["logits"][3, 0] = math.inf
+        x["advantage"][4], x["action"][4] = math.inf, a // 2
+        for rows in (range(5), *([i] for i in range(5))):
+            keep = list(rows)
+            y = {k: v[keep] if isinstance(v, torch.Tensor) else v for k, v in x.items()}
+            got = call(ext, y)
+            assert not torch.isfinite(got["loss"]), keep
+            assert (got["d_logits"].cpu()[~y["legal"]] == 0).all(), keep
+            if keep == [0]:
+                # so has a legal one without probability, listed or not
+                y["logits"], y["legal"] = y["logits"].clone(), y["legal"].clone()
+                y["legal"][0, a - 1], y["logits"][0, a - 1] = True, -math.inf
+                assert call(ext, y)["d_logits"][0, a - 1] == 0
