@@ -1033,8 +1033,10 @@ int cugo_policy_loss(const CugoPolicyLoss* p, hipStream_t stream) {
   if (p->n > 0 && (!p->logits || !p->action || !p->old_logp || !p->advantage || !p->logp))
     return -1;
   if ((p->value != nullptr) != (p->returns != nullptr) || (p->d_value && !p->value)) return -1;
-  if (p->actions <= kRowsMost && (p->logits_stride >= kStrideMost || p->ref_stride >= kStrideMost ||
-                                  p->legal_stride >= kStrideMost || p->d_logits_stride >= kStrideMost))
+  // (one row has no next one: its stride multiplies 0)
+  if (p->actions <= kRowsMost && p->n > 1 &&
+      (p->logits_stride >= kStrideMost || p->ref_stride >= kStrideMost ||
+       p->legal_stride >= kStrideMost || p->d_logits_stride >= kStrideMost))
     return -4;
   if (p->logits_stride < 0 || p->ref_stride < 0 || p->legal_stride < 0 ||
       (p->d_logits && p->n > 1 && p->d_logits_stride < p->actions))

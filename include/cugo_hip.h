@@ -692,7 +692,8 @@ int cugo_selfplay_advance(const CugoSelfPlayWave* wave, const uint8_t* done,
  * An action that is illegal, outside [0, A) or at -inf has log-probability -inf and ratio 0.
  * partials: CUGO_POLICY_LOSS_PARTIALS doubles of scratch, in use until the call's launches
  * end.  The sums' order is fixed.  Rows' strides must not be negative, with at most 1,024
- * actions be below 2^24 elements, and rows of d_logits must not overlap (-4 otherwise).
+ * actions and more than one row be below 2^24 elements, and rows of d_logits must not overlap
+ * (-4 otherwise).
  * dtypes: CUGO_DTYPE_F32, _F16 or _BF16. */
 #define CUGO_POLICY_LOSS_PARTIALS 24576
 typedef struct CugoPolicyLoss {

@@ -642,3 +642,22 @@ def test_illegal_actions_have_no_gradient_in_rows_that_are_not_finite(ext, a, dt
                 y["logits"], y["legal"] = y["logits"].clone(), y["legal"].clone()
                 y["legal"][0, a - 1], y["logits"][0, a - 1] = True, -math.inf
                 assert call(ext, y)["d_logits"][0, a - 1] == 0
+
+
+@pytest.mark.parametrize("a", [1, 3, 40, 64, 179, 300, 1024, 2000])
+@pytest.mark.parametrize("n", [0, 1])
+def test_one_row_of_a_far_stride(ext, n, a):
+    """A single row, or none, has no next one: its stride is of no account, 2^24 elements and more
+    included."""
+    stride = (1 << 24) + 3
+    x = make(1, a, torch.bfloat16, a, weight=False, share=0.9)
+    x = {k: v[:n] if isinstance(v, torch.Tensor) else v for k, v in x.items()}
+    room = {k: torch.zeros(a, dtype=x[k].dtype, device=DEV) for k in ("logits", "legal", "ref")}
+    apart = {}
+    for k, t in room.items():
+        apart[k] = t.as_strided((n, a), (stride, 1))
+        apart[k].copy_(x[k])
+    assert n == 0 or apart["logits"].stride(0) == stride
+    p, q = call(ext, {**x, **apart}), call(ext, x)
+    for k in p:
+        assert torch.equal(p[k], q[k]), k
