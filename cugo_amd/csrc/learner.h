@@ -43,18 +43,21 @@ struct alignas(sizeof(S) * K) Vec {
 };
 
 // N bytes as they lie in memory, in registers: `Raw` at their own alignment, `RawAny` at any
-// (global loads and stores of gfx950 take any alignment).
-typedef uint32_t Words2 __attribute__((ext_vector_type(2)));
-typedef uint32_t Words4 __attribute__((ext_vector_type(4)));
+// (global loads and stores of gfx950 take any alignment).  What is read or written as one of them
+// is the elements' memory, so they may alias any type.
+typedef uint16_t HalfWord __attribute__((may_alias));
+typedef uint32_t Words1 __attribute__((may_alias));
+typedef uint32_t Words2 __attribute__((ext_vector_type(2), may_alias));
+typedef uint32_t Words4 __attribute__((ext_vector_type(4), may_alias));
 template <int N>
 struct RawOf;
 template <>
 struct RawOf<2> {
-  using Raw = uint16_t;
+  using Raw = HalfWord;
 };
 template <>
 struct RawOf<4> {
-  using Raw = uint32_t;
+  using Raw = Words1;
 };
 template <>
 struct RawOf<8> {
@@ -67,7 +70,7 @@ struct RawOf<16> {
 template <int N>
 using Raw = typename RawOf<N>::Raw;
 template <int N>
-struct __attribute__((packed, aligned(1))) RawAny {
+struct __attribute__((packed, aligned(1), may_alias)) RawAny {
   Raw<N> v;
 };
 

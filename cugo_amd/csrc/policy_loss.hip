@@ -398,10 +398,11 @@ __global__ __launch_bounds__(kThreads) void loss_rows_kernel(const LossArgs g) {
       }
       x = row_terms<kRef>(g, in, s, u, ds, sr, xa);
       if (g.d_logits) {
+        wavefront_sync();
 #pragma unroll
         for (int i = 0; i < V; ++i)
           *reinterpret_cast<Raw<kBytes>*>(zl + (i * G + j) * E) = Raw<kBytes>{};
-        __builtin_amdgcn_wave_barrier();  // LDS takes a wavefront's accesses in order
+        wavefront_sync();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float f = __builtin_fmaf(x.c, t[h], x.a);
