@@ -474,3 +474,39 @@ def test_optimizer_groups_rates_and_gradients_of_none(ext):
         opt.step()
     with pytest.raises(ValueError):
         learner.AdamW(ext, net.parameters(), state_bits=16)
+
+
+def _moved(t, by):
+    """t's values `by` elements behind an aligned address."""
+    bits = (lambda x: x.view(torch.uint8) if x.element_size() == 1 else x)
+    room = torch.zeros(t.numel() + 8, dtype=bits(t).dtype, device=DEV)
+    room[by:by + t.numel()].copy_(bits(t))
+    return room[by:by + t.numel()].view(t.dtype)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("param,grad", [(torch.float32, torch.float32),
+                                        (torch.bfloat16, torch.bfloat16),
+                                        (torch.float16, torch.float32)])
+def test_whole_chunks_at_any_address(ext, bits, param, grad):
+    """Tensors of several whole chunks of 4,096 values, one stream at a time (and all of them) away
+    from a wide access's alignment: the bits of aligned tensors."""
+    sizes = [4096, 8192 + 5, 12288]
+    x = make(sizes, param, grad, 12, bits)
+    y = to_device(x)
+    norm = step(ext, y, max_norm=1.0)
+    check(x, y, norm, 1.0)
+    streams = ["params", "grads", "exp_avg", "exp_avg_sq"]
+    streams += ["master"] if param != torch.float32 else []
+    for which in [[s] for s in streams] + [streams]:
+        for by in (1, 2, 3):
+            announce(f"adamw {bits} {param} {grad} {which} {by}")
+            z = to_device(x)
+            for s in which:
+                z[s] = [_moved(t, by) for t in z[s]]
+            assert torch.equal(step(ext, z, max_norm=1.0), norm)
+            for k in ("params", "master", "exp_avg", "exp_avg_sq", "exp_avg_scale",
+                      "exp_avg_sq_scale"):
+                for p, q in zip(y[k] or [], z[k] or []):
+                    same = (lambda t: t.view(torch.uint8) if t.element_size() == 1 else t)
+                    assert torch.equal(same(p), same(q)), (which, by, k)
