@@ -17,9 +17,7 @@ _MODULE = "cugo_amd._cugo_torch50_hip"
 def load_extension(*, verbose: bool = False) -> Any:
     import torch
 
-    # same condition and message as the reference; a process that uses the GPU already has one
-    # (asking the driver each time took 4 us of a loop's step)
-    if not torch.cuda.is_initialized() and not torch.cuda.is_available():
+    if not torch.cuda.is_available():  # same condition and message as the reference
         raise RuntimeError("PyTorch CUDA is not available")
     try:
         module = importlib.import_module(_MODULE)

@@ -88,6 +88,20 @@ def test_load_extension_fails_loudly_without_gpu(monkeypatch):
         raise AssertionError("load_extension must raise without a GPU")
 
 
+def test_load_extension_asks_each_time(monkeypatch):
+    """Whether or not something in the process used a GPU before."""
+    import pytest
+    import torch
+
+    import cugo_amd
+
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: False)
+    for used in (True, False):
+        monkeypatch.setattr(torch.cuda, "is_initialized", lambda used=used: used)
+        with pytest.raises(RuntimeError, match="not available"):
+            cugo_amd.load_extension()
+
+
 def test_drop_in_modules_import_under_reference_names():
     """With cugo_amd/ first on sys.path, the reference's import lines resolve to this
     package's modules (python/cugo_torch50_ext.py, python/cugo_seq_attention50.py)."""
