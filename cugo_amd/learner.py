@@ -18,6 +18,8 @@ current stream without synchronising and can be captured in a HIP graph.
 
 from __future__ import annotations
 
+import copy
+import importlib
 from typing import NamedTuple, Sequence
 
 import torch
@@ -154,6 +156,20 @@ class AdamW(torch.optim.Optimizer):
         self._steps: torch.Tensor | None = None
         super().__init__(params, dict(lr=lr, weight_decay=weight_decay))
 
+    def __getstate__(self) -> dict:
+        return {**super().__getstate__(), "betas": self.betas, "eps": self.eps,
+                "max_norm": self.max_norm, "state_bits": self.state_bits, "seed": self.seed,
+                "grad_norm": self.grad_norm, "extension": self.ext.__name__}
+
+    def __setstate__(self, state: dict) -> None:
+        """Of a copy (the extension is found again by its name), or of the base class's
+        load_state_dict, which passes state and groups alone."""
+        state = dict(state)
+        if "extension" in state:
+            self.ext = importlib.import_module(state.pop("extension"))
+        super().__setstate__(state)
+        self._steps = None  # gathered again from the parameters' own counts
+
     def _all(self) -> list[torch.Tensor]:
         return [p for g in self.param_groups for p in g["params"]]
 
@@ -279,8 +295,6 @@ class PpoLearner:
 
     def set_reference(self) -> None:
         """Keeps a copy of the actor as it is now for the KL term."""
-        import copy
-
         self.reference = copy.deepcopy(self.ro.actor).requires_grad_(False)
 
     @torch.no_grad()
