@@ -135,12 +135,31 @@ def adamw_step(ext, params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor
                           lr_scale, seed)
 
 
+def _of_all_groups(name: str) -> property:
+    """An option that one step has once: a group's entry, the same in every group."""
+
+    def get(self):
+        first, *others = (g[name] for g in self.param_groups)
+        plain = tuple(first) if isinstance(first, (list, tuple)) else first
+        for x in others:
+            if x is not first and (tuple(x) if isinstance(x, (list, tuple)) else x) != plain:
+                raise ValueError(f"{name} must be the same for every group")
+        return plain
+
+    def put(self, value) -> None:
+        for g in self.param_groups:
+            g[name] = value
+
+    return property(get, put)
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW over `adamw_step`: one call for all parameters of all groups.
 
-    Groups may set lr and weight_decay; betas and eps are the optimizer's.  lr may be a
-    one-element float32 tensor on the device, the same for every group.  state_bits 32 keeps
-    the moments in float32, 8 in 8 bits (about 2 bytes a value instead of 8).  16-bit
+    Groups may set lr and weight_decay.  betas, eps, max_norm and seed are in the groups too
+    (for schedulers and checkpoints), the same in every one, as an lr that is a one-element
+    float32 tensor on the device is.  state_bits 32 keeps the moments in float32, 8 in 8 bits
+    (about 2 bytes a value instead of 8).  16-bit
     parameters get a float32 master in the state.  `grad_norm` is the last step's norm when
     max_norm is set."""
 
@@ -150,15 +169,17 @@ class AdamW(torch.optim.Optimizer):
                  state_bits: int = 32, seed: int = 0) -> None:
         if state_bits not in (8, 32):
             raise ValueError("state_bits must be 8 or 32")
-        self.ext, self.betas, self.eps = ext, betas, eps
-        self.max_norm, self.state_bits, self.seed = max_norm, state_bits, seed
+        self.ext, self.state_bits = ext, state_bits
         self.grad_norm: torch.Tensor | None = None
         self._steps: torch.Tensor | None = None
-        super().__init__(params, dict(lr=lr, weight_decay=weight_decay))
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
+                                      max_norm=max_norm, seed=seed))
+
+    betas, eps = _of_all_groups("betas"), _of_all_groups("eps")
+    max_norm, seed = _of_all_groups("max_norm"), _of_all_groups("seed")
 
     def __getstate__(self) -> dict:
-        return {**super().__getstate__(), "betas": self.betas, "eps": self.eps,
-                "max_norm": self.max_norm, "state_bits": self.state_bits, "seed": self.seed,
+        return {**super().__getstate__(), "state_bits": self.state_bits,
                 "grad_norm": self.grad_norm, "extension": self.ext.__name__}
 
     def __setstate__(self, state: dict) -> None:
@@ -243,7 +264,10 @@ class AdamW(torch.optim.Optimizer):
         """The base class would convert the state to the parameters' types; here every entry
         keeps its own."""
         saved = state_dict["state"]
-        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
+        # an option that the saved groups do not have stays as it is
+        mine = {k: getattr(self, k) for k in ("betas", "eps", "max_norm", "seed")}
+        groups = [{**mine, **g} for g in state_dict["param_groups"]]
+        super().load_state_dict({"state": {}, "param_groups": groups})
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         self.state.clear()
         self._steps = None

@@ -5,6 +5,7 @@ from __future__ import annotations
 import copy
 import io
 import pickle
+import warnings
 
 import pytest
 import torch
@@ -67,3 +68,46 @@ def test_copied_and_pickled(ext, bits):
         other._steps += 1
         assert [int(other.state[p]["step"]) for p in other._all()] == [6, 7, 8, 9]
     assert opt._steps.tolist() == [5, 6, 7, 8]
+
+
+def test_a_checkpoint_carries_the_options(ext):
+    """Into an optimizer made with others; one written before the options were in the groups leaves
+    them as they are."""
+    _, opt = _optimizer(ext)
+    _, other = _optimizer(ext, betas=(0.7, 0.9), eps=1e-3, max_norm=None, seed=1, lr=1.0)
+    saved = opt.state_dict()
+    other.load_state_dict(saved)
+    assert (other.betas, other.eps, other.max_norm, other.seed) == ((0.8, 0.95), 1e-6, 0.5, 9)
+    assert [g["lr"] for g in other.param_groups] == [1e-3, 1e-2]
+    for g in saved["param_groups"]:
+        for k in ("betas", "eps", "max_norm", "seed"):
+            del g[k]
+    _, old = _optimizer(ext, betas=(0.7, 0.9), eps=1e-3, max_norm=None, seed=1)
+    old.load_state_dict(saved)
+    assert (old.betas, old.eps, old.max_norm, old.seed) == ((0.7, 0.9), 1e-3, None, 1)
+
+
+def test_options_of_the_whole_step(ext):
+    """Schedulers may move the betas, together; groups that differ in them are refused."""
+    from cugo_amd import learner
+
+    _, opt = _optimizer(ext)
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")  # no step before the scheduler's
+        schedule = torch.optim.lr_scheduler.OneCycleLR(opt, max_lr=0.1, total_steps=10)
+        assert opt.betas[0] == 0.95 and opt.betas[1] == 0.95
+        for _ in range(3):
+            schedule.step()
+    assert 0.85 <= opt.betas[0] < 0.95
+    opt.betas, opt.seed = (0.5, 0.6), 3
+    assert all(g["betas"] == (0.5, 0.6) and g["seed"] == 3 for g in opt.param_groups)
+    opt.param_groups[1]["betas"] = [0.5, 0.6]
+    assert opt.betas == (0.5, 0.6)
+    for name, value in (("betas", (0.5, 0.7)), ("eps", 0.1), ("max_norm", 7.0), ("seed", 4)):
+        _, opt = _optimizer(ext)
+        opt.param_groups[1][name] = value
+        with pytest.raises(ValueError, match=name):
+            opt.step()
+    with pytest.raises(ValueError, match="betas"):
+        learner.AdamW(ext, [dict(params=[torch.nn.Parameter(torch.zeros(2))], betas=(0.1, 0.1)),
+                            dict(params=[torch.nn.Parameter(torch.zeros(2))])]).step()
