@@ -178,6 +178,17 @@ class AdamW(torch.optim.Optimizer):
     betas, eps = _of_all_groups("betas"), _of_all_groups("eps")
     max_norm, seed = _of_all_groups("max_norm"), _of_all_groups("seed")
 
+    def add_param_group(self, param_group: dict) -> None:
+        o = {**self.defaults, **param_group}
+        for name in ("lr", "weight_decay", "eps"):
+            if not isinstance(o[name], torch.Tensor) and not o[name] >= 0:
+                raise ValueError(f"{name} must not be negative: {o[name]}")
+        if not all(0 <= b < 1 for b in o["betas"]):
+            raise ValueError(f"betas must lie in [0, 1): {o['betas']}")
+        if o["max_norm"] is not None and not o["max_norm"] > 0:
+            raise ValueError(f"max_norm must be positive: {o['max_norm']}")
+        super().add_param_group(param_group)
+
     def __getstate__(self) -> dict:
         return {**super().__getstate__(), "state_bits": self.state_bits,
                 "grad_norm": self.grad_norm, "extension": self.ext.__name__}

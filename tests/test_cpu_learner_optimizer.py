@@ -111,3 +111,22 @@ def test_options_of_the_whole_step(ext):
     with pytest.raises(ValueError, match="betas"):
         learner.AdamW(ext, [dict(params=[torch.nn.Parameter(torch.zeros(2))], betas=(0.1, 0.1)),
                             dict(params=[torch.nn.Parameter(torch.zeros(2))])]).step()
+
+
+def test_options_that_make_no_sense_are_refused(ext):
+    """As torch's own optimizer does, for the defaults and for a group's."""
+    from cugo_amd import learner
+
+    p = lambda: torch.nn.Parameter(torch.zeros(2))  # noqa: E731
+    nan = float("nan")
+    for bad in (dict(lr=-1e-3), dict(lr=nan), dict(weight_decay=-0.1), dict(weight_decay=nan),
+                dict(betas=(1.0, 0.9)), dict(betas=(0.9, -0.1)), dict(eps=-1e-8),
+                dict(max_norm=0.0), dict(max_norm=-1.0)):
+        with pytest.raises(ValueError, match=next(iter(bad))):
+            learner.AdamW(ext, [p()], **bad)
+        opt = learner.AdamW(ext, [p()])
+        with pytest.raises(ValueError, match=next(iter(bad))):
+            opt.add_param_group(dict(params=[p()], **bad))
+        assert len(opt.param_groups) == 1
+    learner.AdamW(ext, [p()], lr=torch.tensor([0.1]), weight_decay=0.0, max_norm=None)
+    learner.AdamW(ext, [p()], lr=0.0, eps=0.0, betas=(0.0, 0.0))
