@@ -159,9 +159,8 @@ class AdamW(torch.optim.Optimizer):
     Groups may set lr and weight_decay.  betas, eps, max_norm and seed are in the groups too
     (for schedulers and checkpoints), the same in every one, as an lr that is a one-element
     float32 tensor on the device is.  state_bits 32 keeps the moments in float32, 8 in 8 bits
-    (about 2 bytes a value instead of 8).  16-bit
-    parameters get a float32 master in the state.  `grad_norm` is the last step's norm when
-    max_norm is set."""
+    (about 2 bytes a value instead of 8).  16-bit parameters get a float32 master in the state.
+    `grad_norm` is the last step's norm when max_norm is set."""
 
     def __init__(self, ext, params, lr: float | torch.Tensor = 3e-4,
                  betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
@@ -273,15 +272,10 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict: dict) -> None:
         """The base class would convert the state to the parameters' types; here every entry
-        keeps its own."""
+        keeps its own.  A state that does not fit is refused before anything is changed."""
         saved = state_dict["state"]
-        # an option that the saved groups do not have stays as it is
-        mine = {k: getattr(self, k) for k in ("betas", "eps", "max_norm", "seed")}
-        groups = [{**mine, **g} for g in state_dict["param_groups"]]
-        super().load_state_dict({"state": {}, "param_groups": groups})
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        self.state.clear()
-        self._steps = None
+        states = []
         for i, p in zip(ids, self._all()):
             if i not in saved:
                 continue
@@ -291,7 +285,16 @@ class AdamW(torch.optim.Optimizer):
                 if got is None or got.shape != t.shape or got.dtype != t.dtype:
                     raise ValueError(f"the saved state's {name} does not fit the parameter")
                 t.copy_(got)
-            fresh["step"] = saved[i]["step"].clone()
+            if "step" not in saved[i]:
+                raise ValueError("the saved state has no step")
+            fresh["step"] = torch.as_tensor(saved[i]["step"], dtype=torch.int64).clone()
+            states.append((p, fresh))
+        # an option that the saved groups do not have stays as it is
+        mine = {k: getattr(self, k) for k in ("betas", "eps", "max_norm", "seed")}
+        groups = [{**mine, **g} for g in state_dict["param_groups"]]
+        super().load_state_dict({"state": {}, "param_groups": groups})
+        self.state.clear()
+        for p, fresh in states:
             self.state[p].update(fresh)
 
 

@@ -130,3 +130,49 @@ def test_options_that_make_no_sense_are_refused(ext):
         assert len(opt.param_groups) == 1
     learner.AdamW(ext, [p()], lr=torch.tensor([0.1]), weight_decay=0.0, max_norm=None)
     learner.AdamW(ext, [p()], lr=0.0, eps=0.0, betas=(0.0, 0.0))
+
+
+def test_a_checkpoint_that_does_not_fit_changes_nothing(ext):
+    _, opt = _optimizer(ext)
+    keep = copy.deepcopy(opt)
+    saved = copy.deepcopy(opt.state_dict())
+    saved["param_groups"][0]["lr"] = 7.0
+    del saved["state"][0]
+    short = copy.deepcopy(saved)
+    short["state"][3]["exp_avg"] = short["state"][3]["exp_avg"][:1]
+    other = copy.deepcopy(saved)
+    other["state"][3]["exp_avg_sq"] = other["state"][3]["exp_avg_sq"].float()
+    lacking = copy.deepcopy(saved)
+    del lacking["state"][3]["step"]
+    fewer = copy.deepcopy(saved)
+    fewer["param_groups"].pop()
+    fewer["param_groups"][0]["params"] = [0, 1, 2, 3]
+    for bad in (short, other, lacking, fewer):
+        with pytest.raises(ValueError):
+            opt.load_state_dict(bad)
+        _same(opt, keep)
+
+
+def test_a_checkpoint_of_torchs_own(ext):
+    """Float32 parameters: the same moments, and steps, which torch counts in float32 on the host."""
+    from cugo_amd import learner
+
+    net, _ = _optimizer(ext, torch.float32)
+    theirs = torch.optim.AdamW(net.parameters(), lr=3e-3, betas=(0.8, 0.9))
+    for p in net.parameters():
+        p.grad = torch.randn_like(p)
+    theirs.step()
+    saved = theirs.state_dict()
+    ours = learner.AdamW(ext, net.parameters(), max_norm=2.0)
+    ours.load_state_dict(saved)
+    assert ours.betas == (0.8, 0.9) and ours.max_norm == 2.0
+    ours.prepare()
+    assert ours._steps.tolist() == [1, 1, 1, 1]
+    for p in net.parameters():
+        for k in ("exp_avg", "exp_avg_sq"):
+            assert torch.equal(ours.state[p][k], theirs.state[p][k])
+    for s in saved["state"].values():
+        s["step"] = 3  # as older ones counted
+    ours.load_state_dict(saved)
+    ours.prepare()
+    assert ours._steps.tolist() == [3, 3, 3, 3]
