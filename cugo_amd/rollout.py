@@ -176,7 +176,7 @@ class RolloutBuffer:
     value: torch.Tensor     # f32 [H, B]
     reward: torch.Tensor    # f32 [H, B]
     done: torch.Tensor      # bool [H, B]
-    player: torch.Tensor    # uint8 [H, B]
+    player: torch.Tensor | None = None  # uint8 [H, B]; not recorded where there is none
 
     @classmethod
     def empty(cls, horizon: int, batch: int, device) -> "RolloutBuffer":
@@ -185,6 +185,9 @@ class RolloutBuffer:
         return cls(e(720, dtype=torch.bfloat16), e(179, dtype=torch.bool), e(dtype=torch.int64),
                    e(dtype=torch.float32), e(dtype=torch.float32), e(dtype=torch.float32),
                    e(dtype=torch.bool), e(dtype=torch.uint8))
+
+    def player_row(self, t: int) -> torch.Tensor | None:
+        return None if self.player is None else self.player[t]
 
 
 class MlpRollout:
@@ -233,10 +236,11 @@ class MlpRollout:
         if self.fused_kernel:  # features and mask straight into the buffer's row t
             self.observation = self.ext.observe_bf16(self.states, self.buffer.features[t],
                                                      legal=self.buffer.legal[t],
-                                                     player=self.buffer.player[t])
+                                                     player=self.buffer.player_row(t))
         else:
             self.observation = self.ext.observe(self.states)
-            self.buffer.player[t].copy_(self.observation[2])
+            if self.buffer.player is not None:
+                self.buffer.player[t].copy_(self.observation[2])
         return self.observation
 
     def act(self, t: int):
@@ -295,7 +299,7 @@ class MlpRollout:
         out = self.ext.step_observe_spares(
             self.states, action, self.base, self.generation, self.sampler, self.spares,
             self.spare_gen, buf.features[t + 1], reward=buf.reward[t], done=buf.done[t],
-            legal=buf.legal[t + 1], player=buf.player[t + 1])
+            legal=buf.legal[t + 1], player=buf.player_row(t + 1))
         self.step_out, self.observation = out[:5], out[5:]
         return self.step_out
 

@@ -168,3 +168,22 @@ def test_loss_and_step_captured_together(ext):
     for k in eager:
         assert torch.equal(eager[k].detach().float(), played[k].detach().float()), k
     assert int(played["steps"]) == 7
+
+
+@pytest.mark.parametrize("width", [512, 256])
+def test_a_buffer_without_the_player(ext, width):
+    """A RolloutBuffer of the seven columns that it had before `player` still takes a rollout, the
+    same one; an update from it is refused, as it cannot tell whose the values are."""
+    from cugo_amd import learner
+    from cugo_amd.rollout import RolloutBuffer
+
+    announce(f"seven columns {width}")
+    one, two = _rollout(ext, width), _rollout(ext, width)
+    names = ("features", "legal", "action", "logp", "value", "reward", "done")
+    two.buffer = RolloutBuffer(*(torch.empty_like(getattr(one.buffer, k)) for k in names))
+    a, b = one.collect(), two.collect()
+    for k in names:
+        assert torch.equal(getattr(a, k), getattr(b, k)), k
+    assert b.player is None
+    with pytest.raises(RuntimeError, match="player"):
+        learner.PpoLearner(two).update()
