@@ -510,3 +510,41 @@ def test_whole_chunks_at_any_address(ext, bits, param, grad):
                 for p, q in zip(y[k] or [], z[k] or []):
                     same = (lambda t: t.view(torch.uint8) if t.element_size() == 1 else t)
                     assert torch.equal(same(p), same(q)), (which, by, k)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_copied_optimizers_step_alike(ext, bits):
+    """A deep copy, and one loaded from a checkpoint into other options, take the same steps, moved
+    betas among them."""
+    import copy
+
+    from cugo_amd import learner
+
+    net = _net(torch.bfloat16)
+    opt = learner.AdamW(ext, net.parameters(), lr=1e-3, betas=(0.8, 0.95), max_norm=0.3,
+                        state_bits=bits, seed=4)
+
+    def steps(nets, opts, count, seed):
+        for k in range(count):
+            g = torch.Generator(device=DEV).manual_seed(seed + k)
+            grads = [torch.randn(p.shape, generator=g, device=DEV).bfloat16()
+                     for p in nets[0].parameters()]
+            for n, o in zip(nets, opts):
+                for p, x in zip(n.parameters(), grads):
+                    p.grad = x.clone()
+                o.betas = (0.8 + 0.01 * k, 0.95)
+                o.step()
+
+    steps([net], [opt], 3, 1)
+    net2, two = copy.deepcopy((net, opt))
+    net3 = copy.deepcopy(net)
+    three = learner.AdamW(ext, net3.parameters(), lr=1.0, state_bits=bits)
+    three.load_state_dict(opt.state_dict())
+    assert three.seed == 4 and three.max_norm == 0.3
+    steps([net, net2, net3], [opt, two, three], 3, 10)
+    for other, o in ((net2, two), (net3, three)):
+        assert torch.equal(o.grad_norm, opt.grad_norm)
+        for p, q in zip(net.parameters(), other.parameters()):
+            assert torch.equal(p, q) and int(o.state[q]["step"]) == 6
+            for k in ("master", "exp_avg", "exp_avg_sq"):
+                assert torch.equal(opt.state[p][k].float(), o.state[q][k].float()), k
