@@ -8,16 +8,18 @@
 // (D, C) after (D', C') is (D + C D', C C').  So the steps are split: a lane takes 4 or 8
 // consecutive steps of one game in registers and composes their maps, lanes and wavefronts
 // compose theirs (a suffix scan in the wavefront, then over the wavefronts in LDS), and each
-// lane runs its own steps again from the value that follows them.  The data is read once.
+// lane runs its own steps again from the value that follows them.  The data is read once, or twice
+// where the steps are split over workgroups.
 //
-// What bounds it is memory, 16 to 18 bytes a step of a game (128 steps of 65,536 games in 29 us,
-// 5.2 TB/s), and below about a million steps the two or three rounds of latency of a launch (5 us
-// for 64 x 300).  A wavefront's 64 lanes are
+// What bounds it is memory, 16 to 18 bytes a step of a game and 8 to 10 more where it is read twice
+// (128 steps of 65,536 games in 29 us, 5.2 TB/s), and below about a million steps the two or three
+// rounds of latency of a launch (5 us for 64 x 300).  A wavefront's 64 lanes are
 // `columns` games times 64 / columns runs of steps, the fewest columns (a power of two) that
 // hold the games up to 64, so that few games still fill wavefronts; where the workgroups of
 // one run over the steps would leave compute units idle, the steps are also split over
-// workgroups, in two launches: the first composes each chunk's map, the second starts each
-// chunk from the maps of those behind it.
+// workgroups, in two launches: the first composes each chunk's map (the first chunk's with the
+// others', though no chunk lies before it), the second starts each chunk from the maps of those
+// behind it.
 #include "learner.h"
 
 namespace cugo_amd {

@@ -9,8 +9,8 @@
 // H = -sum_j p_j l_j, K = sum_j p_j (l_j - l'_j), and G = r A, or 0 where the clip cut it off:
 //   d loss / d z_j = w [ G (p_j - [j = a]) + c_k p_j (l_j - l'_j - K) + c_e p_j (l_j + H) ]
 //   d loss / d V = w c_v (V - R)
-// The loss and both gradients come from one reading of the logits: the gradient for a factor
-// of one on the loss needs nothing that the loss does not.
+// The loss and both gradients come from one reading of the logits (two, where a row is too long to
+// be held): the gradient for a factor of one on the loss needs nothing that the loss does not.
 //
 // Rows the sums leave out: w = 0 leaves out everything (whatever the row holds, its gradients
 // are zeros); a row without a legal action, or whose legal logits are all -inf, has the value
@@ -243,8 +243,7 @@ struct RowReader {
 // takes longer than memory does: where each row of a wavefront of 16-lane rows has at most two legal
 // actions a lane, a list of their slots is made, a lane computes two of them, and the gradient is put
 // together in LDS.  1,048,576 x 179 bf16 with a KL term, 10 legal actions a row: 298 us (4.5 TB/s;
-// the arithmetic is half of that), with 60, where the list does not hold them, 373, and 379 for
-// the earlier form that computed all of the actions always.
+// the arithmetic is half of that), with 63, where the list does not hold them, 416.
 template <class T, int G, int V, int E, bool kRef>
 __global__ __launch_bounds__(kThreads) void loss_rows_kernel(const LossArgs g) {
   using S = typename T::storage;
@@ -707,8 +706,10 @@ __device__ inline void store_gradients(const LossArgs& g, typename T::storage* o
 // (loss_long_kernel) took 244.  Arithmetic comes next to memory in what bounds it (about 27
 // instructions an action with a KL term, three of them exponentials at a quarter of the rate), so a
 // row whose logits are all within 2^100 of its largest, as a row without masked entries is, leaves
-// out the tests for 0 times infinity (270 us with them, and with registers spilled).  Registers for
-// two workgroups of 512 threads a compute unit, so that one reads while the other computes.
+// out the tests for 0 times infinity: with a mask 248 us.  A last piece that is read moved back (a
+// row whose length is no multiple of 16 bytes) counts as masked: 32,001 actions take 226.
+// Registers for two workgroups of 512 threads a compute unit, so that one reads while the other
+// computes; with 8 pieces and a reference the 128 of them are four too few (20 bytes of scratch).
 template <class T, int kWide, int P, bool kRef>
 __global__ __launch_bounds__(kWide) __attribute__((amdgpu_waves_per_eu(4))) void loss_held_kernel(
     const LossArgs g) {
@@ -802,7 +803,7 @@ __global__ __launch_bounds__(kWide) __attribute__((amdgpu_waves_per_eu(4))) void
   if (threadIdx.x < kStats) g.partials[(i64)blockIdx.x * kStats + threadIdx.x] = acc;
 }
 
-// Rows of any length, in two passes over memory (2,048 x 65,536 bf16 with a KL term: 235 us, 3.4 TB/s
+// Rows of any length, in two passes over memory (2,048 x 65,536 bf16 with a KL term: 239 us, 3.4 TB/s
 // counted once).  The first keeps each thread's running maximum
 // and the sums under it, moved along with the maximum; the second reads the row again for the
 // gradient.
@@ -992,6 +993,10 @@ int launch_loss(const LossArgs& g, hipStream_t stream) {
   // 356, 1,024 230 and 1,025 316 (a workgroup of 64 threads: 199 and 562 of 256), 2,048 170, 4,096
   // 178, 8,192 167 and 8,193 276, 32,768 184 and 32,769 265.  Rows of 768 take 245 on 64 lanes and 253
   // as a workgroup of 64 threads, with a mask 249 and 353.
+  // Just above a line much of what a row's lanes hold is empty, and is gone through all the same:
+  // 257 to 264 actions 354 to 346, 320 287, 384 240; 1,032 255, 1,536 182, 2,048 170; 8,200 221,
+  // 12,288 190.  An odd length costs nothing in itself, but rows of over 1,024 actions pay for the
+  // last piece moved back (see loss_held_kernel): 1,025 323, 8,193 285.
   // Few actions, us of 2^21 rows (2^26 logits, where those are fewer) against 16 lanes: 4 actions 89
   // and 261, 16 89 and 251, 32 143 and 272, 48 125 and 228; 64 on 8 lanes 142 and 174 (133 on 4,
   // which float32 rows take 224 for, and 172 on 8, 182 on 16), with 10 of them legal 147 and 141.

@@ -4,11 +4,13 @@ The reference's PPO update (python/cugo_ppo50.py:514-739) runs these in torch op
 each is HIP kernels behind one call:
 
   * `advantages`: generalised advantage estimation over a horizon of two-player games, each
-    decision seen from its mover's side; one pass over the rollout buffer's columns;
+    decision seen from its mover's side; the rollout buffer's columns are read once, or twice
+    where few games over many steps are split over the device;
   * `policy_loss`: the clipped policy loss over each row's legal actions with a KL term to
     another policy, an entropy bonus and the value loss.  The loss and the gradients of the
-    logits and the value come from one reading of the logits; `backward()` hands the gradients
-    on (multiplied by the loss's own gradient where that is not 1);
+    logits and the value come from one reading of the logits (two of rows of over 32,768
+    actions, 16,384 in float32); `backward()` hands the gradients on (multiplied by the loss's
+    own gradient where that is not 1);
   * `adamw_step`: one AdamW step over many tensors at once, the gradients' norm clipped, the
     moments in float32 or in 8 bits; `AdamW` is the torch optimizer over it.
 
@@ -59,7 +61,7 @@ def policy_loss(ext, logits: torch.Tensor, action: torch.Tensor, old_logp: torch
     old_logp and advantage float32 [n]; legal bool [n, A] (None: every action is); ref_logits
     like logits (None: no KL term); value [n] (any of the three types) with returns float32
     [n]; weight float32 [n] (None: 1 / n each).  Gradients reach logits and value, rounded once
-    to their types.
+    to their types (and once more where the loss's own gradient is not 1).
 
     A row of weight 0 counts nowhere and gets zero gradients, whatever it holds.  A row
     without a legal action has only the value term (its logp is 0).  An illegal action has
