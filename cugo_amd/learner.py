@@ -172,14 +172,19 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("state_bits must be 8 or 32")
         self.ext, self.state_bits = ext, state_bits
         self.grad_norm: torch.Tensor | None = None
-        self._steps: torch.Tensor | None = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
                                       max_norm=max_norm, seed=seed))
+        self._steps: torch.Tensor | None = None
 
     betas, eps = _of_all_groups("betas"), _of_all_groups("eps")
     max_norm, seed = _of_all_groups("max_norm"), _of_all_groups("seed")
 
+    def _options(self) -> dict:
+        return {k: getattr(self, k) for k in ("betas", "eps", "max_norm", "seed")}
+
     def add_param_group(self, param_group: dict) -> None:
+        if hasattr(self, "_steps"):  # made already: the options as they are now
+            param_group = {**self._options(), **param_group}
         o = {**self.defaults, **param_group}
         for name in ("lr", "weight_decay", "eps"):
             if not isinstance(o[name], torch.Tensor) and not o[name] >= 0:
@@ -292,8 +297,7 @@ class AdamW(torch.optim.Optimizer):
             fresh["step"] = torch.as_tensor(saved[i]["step"], dtype=torch.int64).clone()
             states.append((p, fresh))
         # an option that the saved groups do not have stays as it is
-        mine = {k: getattr(self, k) for k in ("betas", "eps", "max_norm", "seed")}
-        groups = [{**mine, **g} for g in state_dict["param_groups"]]
+        groups = [{**self._options(), **g} for g in state_dict["param_groups"]]
         super().load_state_dict({"state": {}, "param_groups": groups})
         self.state.clear()
         for p, fresh in states:

@@ -176,3 +176,21 @@ def test_a_checkpoint_of_torchs_own(ext):
     ours.load_state_dict(saved)
     ours.prepare()
     assert ours._steps.tolist() == [3, 3, 3, 3]
+
+
+def test_a_later_group_takes_the_options_as_they_are_now(ext):
+    """Set, moved by a scheduler or loaded since the optimizer was made."""
+    _, opt = _optimizer(ext)
+    opt.betas, opt.max_norm, opt.seed = (0.5, 0.6), None, 3
+    for g in opt.param_groups:
+        g["eps"] = 0.25
+    two = copy.deepcopy(opt)
+    _, three = _optimizer(ext, betas=(0.7, 0.9))
+    three.load_state_dict(opt.state_dict())
+    for o in (opt, two, three):
+        o.add_param_group(dict(params=[torch.nn.Parameter(torch.zeros(2).bfloat16())]))
+        assert (o.betas, o.max_norm, o.seed, o.eps) == ((0.5, 0.6), None, 3, 0.25)
+        assert o.param_groups[2]["lr"] == 1e-3  # a group's own, as the optimizer was made with
+    opt.add_param_group(dict(params=[torch.nn.Parameter(torch.zeros(2).bfloat16())], seed=4))
+    with pytest.raises(ValueError, match="seed"):
+        opt.seed
