@@ -122,9 +122,11 @@ def check_no_packed_fp32(lib: Path) -> None:
 # play_split_kernel takes no scratch (16 bytes with it) and canonical_kernel 142 VGPRs (179).
 SOURCE_FLAGS = {"kernels.hip": ["-mllvm", "-disable-machine-licm"]}
 SOURCES = ("kernels.hip", "decode.hip", "selfplay.hip", "mlp.hip", "linear.hip",
-           "policy_loss.hip", "advantages.hip", "adamw.hip")
-HEADERS = (CSRC / "engine.h", CSRC / "learner.h", REPO / "include" / "cugo_hip.h")
-EXT_SOURCES = ("torch_ext.cpp", "learner_ext.cpp")
+           "policy_loss.hip", "advantages.hip", "adamw.hip", "paged_cache.hip",
+           "tree_attention.hip")
+HEADERS = (CSRC / "engine.h", CSRC / "learner.h", CSRC / "paged.h",
+           REPO / "include" / "cugo_hip.h")
+EXT_SOURCES = ("torch_ext.cpp", "learner_ext.cpp", "paged_ext.cpp")
 
 
 def build_library(force: bool = True) -> Path:

@@ -1,4 +1,4 @@
-// What the binding's source files (torch_ext.cpp, learner_ext.cpp) share: checks of tensors with
+// What the binding's source files (torch_ext.cpp, learner_ext.cpp, paged_ext.cpp) share: checks of tensors with
 // the reference's messages (torch50_ext.cu:26-51), the current stream, outputs.
 #ifndef CUGO_EXT_COMMON_H_
 #define CUGO_EXT_COMMON_H_
@@ -57,6 +57,9 @@ inline uint8_t* u8p(const torch::Tensor& t) { return reinterpret_cast<uint8_t*>(
 
 // learner_ext.cpp: the learner's operations, added to the module.
 void bind_learner(pybind11::module_& m);
+
+// paged_ext.cpp: the paged cache's operations, added to the module.
+void bind_paged(pybind11::module_& m);
 
 }  // namespace cugo_ext
 

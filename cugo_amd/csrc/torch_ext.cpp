@@ -1939,4 +1939,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.attr("STATE_BYTES") = pybind11::int_(CUGO_STATE_BYTES);
   m.attr("STATUS_OK") = pybind11::int_(CUGO_STATUS_OK);
   cugo_ext::bind_learner(m);
+  cugo_ext::bind_paged(m);
 }

@@ -786,6 +786,102 @@ int cugo_adamw(const CugoAdamwTensor* tensors, int64_t count, int bits, double b
                double beta2, double eps, const float* lr_scale, double max_norm, uint64_t seed,
                float* norm_out, void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
+/*
+ * The paged key/value cache (no counterpart in the reference, whose cache has a run of slots for
+ * every row, python/cugo_seq50.py:325-339): rows hold their tokens in pages of a common pool, and
+ * rows that began alike share their pages.
+ *
+ * k and v: [layers, pages, kv_heads, page, dh] of `dtype`; table: int32 [rows, width], the pages of
+ * each row in order (entries past a row's pages mean nothing and are left as they were); length:
+ * int64 [rows], the tokens a row has pages for (taken as 0 below 0, as width * page above that);
+ * refs: int32 [pages], how many rows hold a page; free: uint64 [ceil(pages / 64)], bit p % 64 of
+ * word p / 64 set where refs[p] is 0.  dh 32, 64, 128 or 256; page 16, 32, 64, 128 or 256;
+ * width * page below 2^31 - 2^16; k and v 16-byte aligned.  A table entry outside the pool is never
+ * followed.  A cache is changed by one call at a time.
+ *
+ * All of its calls return -1 for sizes or pointers that cannot be, -2 for an unsupported dtype, -3
+ * for an unsupported dh or page, -4 for a misaligned pointer or stride, -5 for a workspace that is
+ * too small.  Workspaces are in use until the call's launches end. */
+typedef struct CugoPagedCache {
+  void* k;
+  void* v;
+  int32_t* table;
+  int64_t* length;
+  int32_t* refs;
+  uint64_t* free;
+  int64_t layers, pages, kv_heads, page, dh, rows, width;
+  int dtype;
+} CugoPagedCache;
+
+/* cugo_paged_append: new token i's key and value (k_new and v_new [n, kv_heads, dh] of the cache's
+ * type, tokens k_stride and v_stride elements apart) to position pos[i] of row rows[i] (NULL: i)
+ * in one layer.  Nothing is written where the row or the position (outside [0, length)) is none,
+ * nor into a page that several rows hold.  Two tokens must not have the same place. */
+int cugo_paged_append(const CugoPagedCache* cache, int64_t layer, const void* k_new,
+                      int64_t k_stride, const void* v_new, int64_t v_stride, const int64_t* pos,
+                      const int64_t* rows, int64_t n, hipStream_t stream);
+
+/* cugo_paged_branch: row dst[i] becomes the first min(length of src[i], length[i]) tokens of row
+ * src[i] with pages for length[i], for n entries at once, as the rows are before the call.  In
+ * order:
+ *   refused (ok[i] = 0, nothing changed): an entry whose rows are none, whose length is not in [0,
+ *     width * page], or whose dst is also another entry's dst or src
+ *   dst's pages are given back (dst = src: those behind length[i]); a page that no row holds any
+ *     more is free
+ *   pages that are kept whole, or in which nothing will be written, are shared with src; the page
+ *     in which the kept tokens end, where length[i] goes beyond them, is copied in every layer
+ *     (dst = src: only if another row holds it too), and the rest are new
+ *   new pages are the lowest free ones, entry after entry; an entry that, with the entries
+ *     before it, needs more than there are gets none: ok[i] = 0, and dst is empty (dst = src: as it
+ *     was)
+ * A page that dst = src gives up for a copy is free for later calls only.  ok: bool [n]. */
+int64_t cugo_paged_branch_workspace(const CugoPagedCache* cache, int64_t n);
+int cugo_paged_branch(const CugoPagedCache* cache, const int64_t* dst, const int64_t* src,
+                      const int64_t* length, int64_t n, uint8_t* ok, void* workspace,
+                      int64_t workspace_bytes, hipStream_t stream);
+
+/* cugo_paged_accept: of the tokens of row rows[i] from position start[i] on, those at start[i] +
+ * keep[i][j], j below the first negative entry (keep int64 [n, most], rows keep_stride elements
+ * apart), move to start[i] + j in every layer; the row's length becomes start[i] plus their count, and
+ * the pages behind are given back.  Refused (ok[i] = 0, nothing changed): an entry whose row is
+ * none or another entry's too, whose start is not in [0, length], whose kept ones do not rise or lie
+ * behind the length, or that would write into a page that several rows hold.  ok: bool [n]. */
+int64_t cugo_paged_accept_workspace(const CugoPagedCache* cache, int64_t n);
+int cugo_paged_accept(const CugoPagedCache* cache, const int64_t* rows, const int64_t* start,
+                      const int64_t* keep, int64_t keep_stride, int64_t most, int64_t n,
+                      uint8_t* ok, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/* cugo_tree_attention: n sequences' queries over the rows they belong to, in one layer.  q [tokens,
+ * heads, dh] (tokens q_stride elements apart), heads a multiple of kv_heads; sequence i has the
+ * queries offsets[i] ... offsets[i + 1] - 1 (NULL: tokens / n each; tokens outside every sequence
+ * are left as they were) and row rows[i] (NULL: i).  With prefix[i] in [0, length] (taken into it),
+ * query number j of sequence i attends the row's positions t < length with
+ *   t < prefix[i], or bit (t - prefix[i]) of its mask set              (mask given)
+ *   t <= prefix[i] + j                                                 (mask NULL)
+ *   out = sum_t softmax_t(q . k_t scale) v_t                           (out [tokens, heads, dh])
+ * mask: uint64 [tokens, words], or [tokens / n, words] with mask_rows = tokens / n and offsets
+ * NULL, the same for every sequence; bit b is bit b % 64 of word b / 64.  A query that attends
+ * nothing gets zeros; one whose row is none, or that attends a position whose page is none, NaN.
+ * What masked places hold is never used.  Sums and softmax in float32; with 16-bit types the weights
+ * are rounded to the type before they meet v.  workspace: at least
+ * cugo_tree_attention_workspace(...) bytes (asked on the device of the call; may be 0). */
+typedef struct CugoTreeAttention {
+  const CugoPagedCache* cache;
+  int64_t layer;
+  const void* q;
+  int64_t q_stride, tokens, heads, n;
+  const int64_t* prefix;
+  const int64_t* rows;
+  const int64_t* offsets;
+  const uint64_t* mask;
+  int64_t mask_rows, words;
+  float scale;
+  void* out;
+} CugoTreeAttention;
+int64_t cugo_tree_attention_workspace(const CugoTreeAttention* call);
+int cugo_tree_attention(const CugoTreeAttention* call, void* workspace, int64_t workspace_bytes,
+                        hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
