@@ -67,7 +67,7 @@ def test_caches(lib, over, code):
     assert lib.cugo_paged_append(c, 0, AT, 64, AT, 64, AT, None, 1, None) == code
     assert lib.cugo_paged_branch(c, AT, AT, AT, 1, AT, AT, 1 << 30, None) == code
     assert lib.cugo_paged_accept(c, AT, AT, AT, 1, 1, 1, AT, AT, 1 << 30, None) == code
-    a = Attention(cache=ctypes.addressof(c._obj), q=AT, q_stride=64, tokens=1, heads=2, n=1,
+    a = Attention(cache=ctypes.addressof(c._obj), q=AT, q_stride=64, tokens=1, heads=2, n=1, scale=1.0,
                   prefix=AT, out=AT)
     assert lib.cugo_tree_attention(ctypes.byref(a), AT, 1 << 30, None) == code
     assert lib.cugo_paged_branch_workspace(c, 4) == lib.cugo_paged_accept_workspace(c, 4) == 0
@@ -131,13 +131,14 @@ def test_accept(lib):
 def test_tree_attention(lib):
     cache = _cache()
 
-    def go(scratch=True, **over):
+    def go(**over):
         x = dict(cache=ctypes.addressof(cache), layer=1, q=AT, q_stride=128, tokens=6, heads=4, n=2,
-                 prefix=AT, mask_rows=6, words=1, out=AT)
+                 prefix=AT, mask_rows=6, words=1, scale=1.0, out=AT)
         a = Attention(**{**x, **over})
         return lib.cugo_tree_attention(ctypes.byref(a), AT, 1 << 30, None)
 
     assert go(tokens=0) == go(tokens=0, n=0) == 0
+    assert go(scale=0.0) == go(scale=float("nan")) == go(scale=float("inf")) == -1
     for over in (dict(layer=2), dict(layer=-1), dict(tokens=-1), dict(n=-1), dict(n=0),
                  dict(heads=0), dict(heads=3), dict(heads=1 << 17), dict(q_stride=127),
                  dict(tokens=1 << 24, offsets=AT), dict(n=1 << 24, offsets=AT), dict(tokens=7),
