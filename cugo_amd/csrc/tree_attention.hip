@@ -11,12 +11,12 @@
 // it.
 //
 // Scores are formed as S^T = K Q^T (16 x 16 matrix instructions, K the A operand), so that a lane
-// has one query's scores (lane & 15) of a few tokens; those are the weights' places in the B operand
-// of O^T += V^T P^T too, if a tile's tokens are dealt to the rows of the two K operands as
-// 8 (r / 4) + r % 4 (+ 4): weights never move between lanes.  V^T's A operand takes, for one
-// element of the head, 8 tokens a lane: a lane loads W consecutive elements of each of its tokens (16
-// lanes cover a token's row) and turns the 8 x W block by v_perm_b32, so keys and values both come
-// straight from memory into registers in whole rows.
+// has one query's scores (lane & 15) of tokens 4 g ... 4 g + 3 of each 16 (g = lane >> 4).  A lane's
+// weights are the B operand of O^T += V^T P^T as they are, with those tokens in the product's inner
+// places 8 g ... 8 g + 7, which V^T's A operand only has to follow: weights never move between lanes.
+// That operand takes, for one element of the head, a lane's 8 tokens: a lane loads W consecutive
+// elements of each (16 lanes cover a token's row) and turns the 8 x W block by v_perm_b32, so keys
+// and values both come from memory into registers in whole rows.
 //
 // The running maximum moves only when a score exceeds it by more than 2^8 in the weight (kSlack):
 // until then weights are at most 2^8, which neither type nor the sums mind, and a tile needs no
@@ -68,13 +68,12 @@ struct Call {
   const i64* offsets;
   const u64* mask;
   char* out;
-  float* part_o;     // of split rows: [splits, tokens * heads, dh]
-  float* part_ml;    // [splits, tokens * heads, 2]: maximum (base 2) and sum
+  float* part_o;   // shared-out items' parts: [workgroups, 2, rows, dh]
+  float* part_ml;  // [workgroups, 2, rows, 2]: maximum (base 2) and sum
+  int* notes;      // [workgroups, kNote]
   int tokens, n, each;  // each: queries a sequence without offsets
   int heads, group, words;
-  int tiles;         // of 16 MT rows, over all sequences
-  int items;         // (tile, key head, split) in all
-  int parts, splits;
+  int items;       // (tile of rows, key head), at most so many
   float scale_log2;  // > 0: a negative scale turns q's signs
   uint32_t flip;
 };
@@ -122,10 +121,39 @@ struct Shape {
   static constexpr int H = DH / (16 * W);          // runs a value
   static constexpr int RW = W * E / 4;             // words a run
   static constexpr int NJ = DH / 16;               // 16 x 16 tiles of O^T
+  // The place of a lane's token e in the tile, after 4 g.
+  __device__ static constexpr int place(int e) { return e + (e >= 4 ? 12 : 0); }
   // The element that row 4 g + i of tile j of O^T is.
   __device__ static int element(int j, int row) { return j / W * 16 * W + W * row + j % W; }
 };
 
+// The parts of a tile's keys and values that a lane holds; at0 and at1: its first and second 16 tokens.
+template <class T, int DH>
+__device__ inline void load_keys(const char* at0, const char* at1,
+                                 u32x4 (&k)[Shape<T, DH>::KL][Shape<T, DH>::KC]) {
+  using Sh = Shape<T, DH>;
+  const unsigned lane = threadIdx.x & 63, mine = (lane & 15) * (DH * Sh::E) + (lane >> 4) * 16;
+#pragma unroll
+  for (int a = 0; a < Sh::KL; ++a)
+#pragma unroll
+    for (int p = 0; p < Sh::KC; ++p)
+      k[a][p] = *reinterpret_cast<const u32x4*>((a ? at1 : at0) + mine + p * 64);
+}
+template <class T, int DH>
+__device__ inline void load_values(const char* at0, const char* at1,
+                                   uint32_t (&v)[Shape<T, DH>::N][Shape<T, DH>::H][Shape<T, DH>::RW]) {
+  using Sh = Shape<T, DH>;
+  const unsigned lane = threadIdx.x & 63;
+  const unsigned mine = (lane >> 4) * (4 * DH * Sh::E) + (lane & 15) * (Sh::W * Sh::E);
+#pragma unroll
+  for (int t = 0; t < Sh::N; ++t)
+#pragma unroll
+    for (int h = 0; h < Sh::H; ++h)
+      load_words<Sh::RW>((t < 4 ? at0 : at1) + mine + (t & 3) * DH * Sh::E + h * 16 * Sh::W * Sh::E,
+                         v[t][h]);
+}
+
+// What a wavefront holds of 16 MT queries, and its work on a tile of tokens.
 template <class T, int DH, int MT>
 struct Wave {
   using Sh = Shape<T, DH>;
@@ -135,36 +163,29 @@ struct Wave {
   f32x4 sum[MT];
   float top[MT];
 
-  struct Tile {
+  struct Keys {
     u32x4 k[KL][KC];
+  };
+  struct Values {
     uint32_t v[N][Sh::H][Sh::RW];
   };
+  // A product operand of N numbers, rounded to the type.
+  struct Weights {
+    uint32_t w[4];
+  };
 
-  // Reads tile `tile` whose halves lie in pages id0 and id1 (of the pool).
-  __device__ static void load(const Cache& c, const char* k_head, const char* v_head, int tile,
-                              int id0, int id1, Tile& x) {
-    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    const int in_page = (1 << c.page_shift) - 1;
-    const int from = tile * KT & in_page;
-    const int k_token = Sh::kWide ? r : 8 * (r >> 2) + (r & 3);
-    const char* kb = k_head + (i64)(!Sh::kWide && k_token >= 16 ? id1 : id0) * c.page_bytes +
-                     ((from + k_token) & in_page) * (DH * Sh::E) + g * 16;
-    const char* vb = v_head + (i64)(!Sh::kWide && g >= 2 ? id1 : id0) * c.page_bytes +
-                     ((from + N * g) & in_page) * (DH * Sh::E) + r * (Sh::W * Sh::E);
+  __device__ void clear() {
 #pragma unroll
-    for (int a = 0; a < KL; ++a)
+    for (int m = 0; m < MT; ++m) {
+      top[m] = kNegInf;
+      sum[m] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int p = 0; p < KC; ++p)
-        x.k[a][p] = *reinterpret_cast<const u32x4*>(kb + a * 4 * DH * Sh::E + p * 64);
-#pragma unroll
-    for (int t = 0; t < N; ++t)
-#pragma unroll
-      for (int h = 0; h < Sh::H; ++h)
-        load_words<Sh::RW>(vb + t * DH * Sh::E + h * 16 * Sh::W * Sh::E, x.v[t][h]);
+      for (int j = 0; j < NJ; ++j) acc[m][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
   }
 
   // d[e]: the product of query lane & 15 with the lane's token e.
-  __device__ static void scores(const Tile& x, const u32x4 (&qm)[KC], float (&d)[N]) {
+  __device__ static void scores(const Keys& x, const u32x4 (&qm)[KC], float (&d)[N]) {
 #pragma unroll
     for (int a = 0; a < KL; ++a) {
       f32x4 s = {0.f, 0.f, 0.f, 0.f};
@@ -184,10 +205,6 @@ struct Wave {
     }
   }
 
-  // A product operand of N numbers, rounded to the type.
-  struct Weights {
-    uint32_t w[4];
-  };
   __device__ static Weights pack(const float (&p)[N]) {
     Weights x;
     if constexpr (Sh::kWide) {
@@ -216,7 +233,7 @@ struct Wave {
     }
   }
   // Element j of the lane's N tokens.
-  __device__ static Weights column(const Tile& x, int j) {
+  __device__ static Weights column(const Values& x, int j) {
     Weights y;
     const int h = j / Sh::W, e = j % Sh::W;
     if constexpr (Sh::kWide) {
@@ -231,25 +248,44 @@ struct Wave {
     return y;
   }
 
-  // The tile's share of every query.  `seen[m]`: bits of the lane's tokens that query m may
-  // attend; all: every query attends every token.
-  __device__ void fold(Tile& x, float scale, bool all, const uint32_t (&seen)[MT], int inside,
-                       bool bad) {
-    float d[MT][N];
-    float most[MT];
+  // SUB tiles' share of every query.  keys(s) and values(s): the lane's parts of tile s.  all: every
+  // query attends every token; otherwise seen(s, m) has the bits of the lane's tokens that query m
+  // attends, and positions from inside(s) on after the tile's 4 g are past the row's end.  bad(s, half):
+  // the tokens of that half have no page.
+  template <int SUB, class KeysOf, class ValuesOf, class Seen, class Inside, class Bad>
+  __device__ void fold(float scale, bool all, KeysOf keys, ValuesOf values, Seen seen,
+                       Inside inside, Bad bad) {
+    float d[SUB][MT][N], most[MT];
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) {
+      const Keys& x = keys(s);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        scores(x, q[m], d[s][m]);
+#pragma unroll
+        for (int a = 0; a < KL; ++a)
+          if (bad(s, a))
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[s][m][4 * a + e] = __builtin_nanf("");
+      }
+    }
+    if (!all)
+#pragma unroll
+      for (int s = 0; s < SUB; ++s)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const uint32_t bits = seen(s, m);
+#pragma unroll
+          for (int e = 0; e < N; ++e) d[s][m][e] = bits >> e & 1 ? d[s][m][e] : kNegInf;
+        }
     bool more = false;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      scores(x, q[m], d[m]);
-      if (bad)
+      most[m] = kNegInf;
 #pragma unroll
-        for (int e = 0; e < N; ++e) d[m][e] = __builtin_nanf("");
-      if (!all)
+      for (int s = 0; s < SUB; ++s)
 #pragma unroll
-        for (int e = 0; e < N; ++e) d[m][e] = seen[m] >> e & 1 ? d[m][e] : kNegInf;
-      most[m] = d[m][0];
-#pragma unroll
-      for (int e = 1; e < N; ++e) most[m] = fmaxf(most[m], d[m][e]);
+        for (int e = 0; e < N; ++e) most[m] = fmaxf(most[m], d[s][m][e]);
       most[m] *= scale;
       more = more || most[m] - kSlack > top[m];
     }
@@ -264,68 +300,69 @@ struct Wave {
         for (int j = 0; j < NJ; ++j) acc[m][j] *= less;
       }
     }
-    Weights w[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const float base = top[m] == kNegInf ? 0.f : top[m];
-#pragma unroll
-      for (int e = 0; e < N; ++e) d[m][e] = exp2_fast(__builtin_fmaf(d[m][e], scale, -base));
-      w[m] = pack(d[m]);
-    }
     float one[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) one[e] = 1.f;
     const Weights ones = pack(one);
+    Weights w[SUB][MT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) sum[m] = product(ones, w[m], sum[m]);
-    if (!all) {
-      // tokens past the row's end hold anything; among the others infinities and NaN are rare
-      bool odd = false;
+    for (int m = 0; m < MT; ++m) {
+      const float base = top[m] == kNegInf ? 0.f : top[m];
 #pragma unroll
-      for (int t = 0; t < N; ++t)
+      for (int s = 0; s < SUB; ++s) {
 #pragma unroll
-        for (int h = 0; h < Sh::H; ++h)
-#pragma unroll
-          for (int e = 0; e < Sh::RW; ++e) {
-            const uint32_t y = t < inside ? x.v[t][h][e] : 0u;
-            x.v[t][h][e] = y;
-            if constexpr (Sh::kWide) odd = odd || (y & 0x7f800000u) == 0x7f800000u;
-            else odd = odd || (y & T_inf()) == T_inf() || (y >> 16 & T_inf()) == T_inf();
-          }
-      if (__ballot(odd)) {
-        fold_odd(x, seen);
-        return fold_values<true>(x, w);
+        for (int e = 0; e < N; ++e) d[s][m][e] = exp2_fast(__builtin_fmaf(d[s][m][e], scale, -base));
+        w[s][m] = pack(d[s][m]);
+        sum[m] = product(ones, w[s][m], sum[m]);
       }
     }
-    fold_values<false>(x, w);
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) {
+      Values x = values(s);
+      if (!all) {
+        // tokens past the row's end hold anything; among the others infinities and NaN are rare
+        const int until = inside(s);
+        bool odd = false;
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+          for (int h = 0; h < Sh::H; ++h)
+#pragma unroll
+            for (int e = 0; e < Sh::RW; ++e) {
+              const uint32_t y = Sh::place(t) < until ? x.v[t][h][e] : 0u;
+              x.v[t][h][e] = y;
+              if constexpr (Sh::kWide) odd = odd || (y & inf_bits()) == inf_bits();
+              else odd = odd || (y & inf_bits()) == inf_bits() || (y >> 16 & inf_bits()) == inf_bits();
+            }
+        if (__ballot(odd)) {
+          fold_odd(x, [&](int m) { return seen(s, m); });
+#pragma unroll
+          for (int t = 0; t < N; ++t)
+#pragma unroll
+            for (int h = 0; h < Sh::H; ++h)
+#pragma unroll
+              for (int e = 0; e < Sh::RW; ++e) x.v[t][h][e] = only_finite(x.v[t][h][e]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const Weights a = column(x, j);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[m][j] = product(a, w[s][m], acc[m][j]);
+      }
+    }
   }
 
-  __device__ static constexpr uint32_t T_inf() {
+  __device__ static constexpr uint32_t inf_bits() {
     if constexpr (Sh::kWide) return 0x7f800000u;
     else return T::kInf;
   }
-
-  template <bool kFinite>
-  __device__ void fold_values(const Tile& x, const Weights (&w)[MT]) {
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      Weights a = column(x, j);
-      if constexpr (kFinite) a = only_finite(a);
-#pragma unroll
-      for (int m = 0; m < MT; ++m) acc[m][j] = product(a, w[m], acc[m][j]);
-    }
-  }
-  __device__ static Weights only_finite(Weights a) {
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      if constexpr (Sh::kWide) {
-        a.w[t] = (a.w[t] & T_inf()) == T_inf() ? 0u : a.w[t];
-      } else {
-        if ((a.w[t] & T_inf()) == T_inf()) a.w[t] &= 0xffff0000u;
-        if ((a.w[t] >> 16 & T_inf()) == T_inf()) a.w[t] &= 0x0000ffffu;
-      }
-    }
-    return a;
+  // The word with its infinite numbers and NaN as zeros.
+  __device__ static uint32_t only_finite(uint32_t w) {
+    if constexpr (Sh::kWide) return (w & inf_bits()) == inf_bits() ? 0u : w;
+    if ((w & inf_bits()) == inf_bits()) w &= 0xffff0000u;
+    if ((w >> 16 & inf_bits()) == inf_bits()) w &= 0x0000ffffu;
+    return w;
   }
   // 1 where a value is an infinity of the sign `negative`, or NaN (which is both), else 0.
   __device__ static Weights infinite(const Weights& a, bool negative) {
@@ -339,40 +376,39 @@ struct Wave {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           const uint32_t v = a.w[t] >> 16 * b & 0xffffu;
-          const bool nan = (v & 0x7fffu) > T_inf();
-          y[2 * t + b] = nan || v == (T_inf() | (negative ? 0x8000u : 0u)) ? 1.f : 0.f;
+          const bool nan = (v & 0x7fffu) > inf_bits();
+          y[2 * t + b] = nan || v == (inf_bits() | (negative ? 0x8000u : 0u)) ? 1.f : 0.f;
         }
       }
     }
     return pack(y);
   }
   // What infinite values and NaN bring to the queries that attend them.
-  __device__ void fold_odd(const Tile& x, const uint32_t (&seen)[MT]) {
-#pragma unroll 1
+  template <class Seen>
+  __device__ void fold_odd(const Values& x, Seen seen) {
+    Weights who[MT];
+#pragma unroll
     for (int m = 0; m < MT; ++m) {
+      const uint32_t bits = seen(m);
       float yes[N];
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        uint32_t s = seen[0];
+      for (int e = 0; e < N; ++e) yes[e] = bits >> e & 1 ? 1.f : 0.f;
+      who[m] = pack(yes);
+    }
 #pragma unroll
-        for (int i = 1; i < MT; ++i) s = m == i ? seen[i] : s;
-        yes[e] = s >> e & 1 ? 1.f : 0.f;
-      }
-      const Weights who = pack(yes);
+    for (int j = 0; j < NJ; ++j) {
+      // one after another: interleaved, this rare path would decide the kernel's registers
+      __builtin_amdgcn_sched_barrier(0);
+      const Weights a = column(x, j), positive = infinite(a, false), negative = infinite(a, true);
+      const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const Weights a = column(x, j);
-        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-        const f32x4 up = product(infinite(a, false), who, zero);
-        const f32x4 down = product(infinite(a, true), who, zero);
+      for (int m = 0; m < MT; ++m) {
+        const f32x4 up = product(positive, who[m], zero), down = product(negative, who[m], zero);
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
-          if (m == i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if (up[e] > 0.f) acc[i][j][e] += -kNegInf;
-              if (down[e] > 0.f) acc[i][j][e] += kNegInf;
-            }
+        for (int e = 0; e < 4; ++e) {
+          if (up[e] > 0.f) acc[m][j][e] += -kNegInf;
+          if (down[e] > 0.f) acc[m][j][e] += kNegInf;
+        }
       }
     }
   }
@@ -397,20 +433,41 @@ __device__ inline uint32_t seen_bits(int at, int limit, int prefix, const u64* m
   return left >= N ? bits : left <= 0 ? 0u : bits & ((1u << left) - 1);
 }
 
+// A sequence as its wavefronts see it.
+struct Sequence {
+  int first, queries;  // its queries
+  i64 row;
+  bool exists;  // the row
+  int length, prefix;
+  int end;  // positions that some query may attend lie before it
+};
+__device__ inline Sequence sequence_at(const Call& a, int i) {
+  Sequence s;
+  s.first = i * a.each;
+  s.queries = a.each;
+  if (a.offsets != nullptr) {
+    const i64 first = a.offsets[i], end = a.offsets[i + 1];
+    const bool fine = first >= 0 && end <= a.tokens && first < end;
+    s.first = fine ? (int)first : 0;
+    s.queries = fine ? (int)(end - first) : 0;
+  }
+  s.row = a.rows ? a.rows[i] : i;
+  s.exists = s.row >= 0 && s.row < a.c.rows;
+  s.length = s.exists ? row_length(a.c, a.c.length[s.row]) : 0;
+  const i64 given = a.prefix[i];
+  s.prefix = (int)(given < 0 ? 0 : given > s.length ? s.length : given);
+  s.end = (int)min((i64)s.length, (i64)s.prefix + (a.mask ? (i64)64 * a.words : (i64)s.queries));
+  return s;
+}
+
 // The sequence of tile x and the tile's place in it.  With offsets, sequence i's tiles begin at
 // floor((offsets[i] - offsets[0]) group / rows a tile) + i, which leaves room for what each needs.
-struct Place {
-  int sequence, tile, first, queries;
-};
-__device__ inline Place place_of(const Call& a, int x, int rows) {
-  Place p;
+__device__ inline int find_tile(const Call& a, int x, int rows, int& tile) {
   if (a.offsets == nullptr) {
     const int each = (int)(((i64)a.each * a.group + rows - 1) / rows);
-    p.sequence = (unsigned)x / (unsigned)each;
-    p.tile = x - p.sequence * each;
-    p.first = p.sequence * a.each;
-    p.queries = a.each;
-    return p;
+    const int i = (unsigned)x / (unsigned)each;
+    tile = x - i * each;
+    return i;
   }
   const int lane = threadIdx.x & 63;
   const i64 origin = a.offsets[0];
@@ -423,19 +480,131 @@ __device__ inline Place place_of(const Call& a, int x, int rows) {
   int low = 0, span = a.n;
   while (span > 1) {
     const int step = (span + 63) >> 6;
-    const int at = low + lane * step;
-    const bool before = lane * step < span && start(at) <= x;
+    const bool before = lane * step < span && start(low + lane * step) <= x;
     const int last = 63 - __clzll((long long)(__ballot(before) | 1));
-    span = min(step, low + span - (low + last * step));
+    span = min(step, span - last * step);
     low += last * step;
   }
-  p.sequence = __builtin_amdgcn_readfirstlane(low);
-  p.tile = x - start(p.sequence);
-  const i64 first = a.offsets[p.sequence], end = a.offsets[p.sequence + 1];
-  const bool fine = first >= 0 && end <= a.tokens && first < end;
-  p.first = fine ? (int)first : 0;
-  p.queries = fine ? (int)(end - first) : 0;
-  return p;
+  low = __builtin_amdgcn_readfirstlane(low);
+  tile = x - start(low);
+  return low;
+}
+
+// Sharing out: the work of all items (a tile of rows over one key head) in a row, an item's being its
+// sequence's tiles of tokens; workgroup b of B does what lies between W b / B and W (b + 1) / B.
+// An item that a border cuts has parts, joined by a second launch.  Every workgroup sums up the
+// sequences' work for itself (kMostShared of them at most).
+constexpr int kMostShared = 1024;
+constexpr int kNote = 8;
+
+// before[i]: the work of the sequences before i; before[n]: all of it.  `scratch`: kWaves numbers.
+__device__ inline void sum_work(const Call& a, int rows, int tokens, u64* before, u64* scratch) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  u64 carry = 0;
+  for (int base = 0; base < a.n; base += 64 * kWaves) {
+    const int i = base + threadIdx.x;
+    u64 x = 0;
+    if (i < a.n) {
+      const Sequence s = sequence_at(a, i);
+      const int tiles = (int)(((i64)s.queries * a.group + rows - 1) / rows);
+      x = (u64)tiles * a.c.kv_heads * max(1, (s.end + tokens - 1) / tokens);
+    }
+    const u64 mine = x;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const u64 y = __shfl_up(x, off);
+      if (lane >= off) x += y;
+    }
+    if (lane == 63) scratch[wave] = x;
+    __syncthreads();
+    u64 total = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      if (w < wave) x += scratch[w];
+      total += scratch[w];
+    }
+    if (i < a.n) before[i] = carry + x - mine;
+    carry += total;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) before[a.n] = carry;
+  __syncthreads();
+}
+
+// One workgroup's (or wavefront's) work on an item.
+struct Job {
+  Sequence s;
+  int head, tile;  // the key head; the tile of rows
+  int from, to;    // tiles of tokens
+  int slot;        // -1: the whole item; 0: its end or middle, 1: its beginning
+  bool ends;       // to is the item's end
+};
+
+// The jobs of a workgroup in order.
+struct Share {
+  const u64* before;
+  u64 at, end;
+  int n;
+  __device__ bool next(const Call& a, int rows, int tokens, Job& job) {
+    if (at >= end) return false;
+    int low = 0, high = n;  // before[low] <= at < before[high]
+    while (high - low > 1) {
+      const int mid = (low + high) >> 1;
+      if (before[mid] <= at) low = mid;
+      else high = mid;
+    }
+    low = __builtin_amdgcn_readfirstlane(low);
+    job.s = sequence_at(a, low);
+    const int tiles = (int)(((i64)job.s.queries * a.group + rows - 1) / rows);
+    const int each = max(1, (job.s.end + tokens - 1) / tokens);
+    const u64 offset = at - before[low];
+    const u64 item = offset / (unsigned)each;
+    job.from = (int)(offset - item * each);
+    job.to = (int)min((u64)each, job.from + (end - at));
+    job.head = (int)(item / (unsigned)tiles);
+    job.tile = (int)(item - (u64)job.head * tiles);
+    job.ends = job.to == each;
+    job.slot = job.from > 0 ? 0 : job.ends ? -1 : 1;
+    at += job.to - job.from;
+    return true;
+  }
+};
+
+// Workgroups in an order that gives consecutive ones to one XCD (they go round the 8 of them): tiles
+// of one sequence read the same keys.
+__device__ inline unsigned in_order() {
+  const unsigned groups = gridDim.x, whole = groups & ~7u;
+  return blockIdx.x < whole ? (blockIdx.x & 7) * (whole >> 3) + (blockIdx.x >> 3) : blockIdx.x;
+}
+
+__device__ inline Share share_of(const Call& a, unsigned group, int rows, int tokens, int least,
+                                 u64* before, u64* scratch) {
+  sum_work(a, rows, tokens, before, scratch);
+  const u64 all = before[a.n];
+  // no less than `least` tiles of tokens each, unless there are more items; one at least
+  u64 groups = max(all / (unsigned)least, (u64)a.items);
+  groups = max(min(min(groups, (u64)gridDim.x), all), (u64)1);
+  Share s;
+  s.before = before;
+  s.n = a.n;
+  s.at = s.end = 0;
+  if (group < groups) s.at = all * group / groups, s.end = all * (group + 1) / groups;
+  return s;
+}
+
+// What a workgroup tells the launch that joins: [0] it began an item that others went on with, of
+// which [1] first query, [2] first row, [3] rows, [4] key head; [5] it ended an item that others
+// began.
+__device__ inline void note(const Call& a, unsigned group, const Job& job, int row0, int M) {
+  int* at = a.notes + group * kNote;
+  if (job.slot == 1) {
+    at[0] = 1, at[1] = job.s.first, at[2] = row0, at[3] = M, at[4] = job.head;
+  } else if (job.slot == 0) {
+    at[5] = job.ends;
+  }
+}
+__device__ inline void nothing_noted(const Call& a, unsigned group) {
+  a.notes[group * kNote] = a.notes[group * kNote + 5] = 0;
 }
 
 // Stores W consecutive elements.
@@ -457,326 +626,543 @@ __device__ inline void store_floats(float* p, const float (&x)[W]) {
   }
 }
 
-// One item: a tile of 16 MT rows of a sequence over one key head, or a split of its tokens.  parts =
-// 1: an item a wavefront.  parts = 4: an item a workgroup, whose wavefronts take every fourth tile
-// of tokens and merge what they have through LDS.
-template <class T, int DH, int MT>
-__global__ __launch_bounds__(64 * kWaves) void tree_kernel(Call a) {
-  using Sh = Shape<T, DH>;
-  using S = typename T::storage;
-  using Wv = Wave<T, DH, MT>;
-  constexpr int KT = Sh::KT, N = Sh::N, NJ = Sh::NJ, KC = Sh::KC;
-  constexpr int kRows = 16 * MT;
-  extern __shared__ float merged[];
-  const Cache& c = a.c;
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // consecutive items to one XCD (workgroups go round the 8 of them): tiles of one sequence read
-  // the same keys
-  const unsigned groups = gridDim.x, whole = groups & ~7u;
-  const unsigned group = blockIdx.x < whole ? (blockIdx.x & 7) * (whole >> 3) + (blockIdx.x >> 3)
-                                            : blockIdx.x;
-  const bool together = a.parts > 1;
-  const unsigned item = together ? group : group * kWaves + wave;
-  if (item >= (unsigned)a.items) return;
-  int x, head, split = 0;
-  if (together) {
-    x = item % (unsigned)a.tiles;
-    const unsigned rest = item / (unsigned)a.tiles;
-    head = rest % (unsigned)c.kv_heads;
-    split = rest / (unsigned)c.kv_heads;
-  } else {
-    head = item % (unsigned)c.kv_heads;
-    x = item / (unsigned)c.kv_heads;
-  }
-  const Place p = place_of(a, x, kRows);
-  const int M = p.queries * a.group;
-  const int row0 = p.tile * kRows;
-  if (row0 >= M) return;
-  // this lane's queries
+// The 16 MT queries of a wavefront: query lane & 15 of each 16 is the lane's.
+template <int MT>
+struct Queries {
   bool real[MT];
-  int query[MT], token[MT], q_head[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int row = row0 + 16 * m + r;
-    real[m] = row < M;
-    query[m] = (unsigned)min(row, M - 1) / (unsigned)a.group;
-    token[m] = p.first + query[m];
-    q_head[m] = head * a.group + (min(row, M - 1) - query[m] * a.group);
-  }
-  const i64 cache_row = a.rows ? a.rows[p.sequence] : p.sequence;
-  const bool exists = cache_row >= 0 && cache_row < c.rows;
-  Wv w;
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    w.top[m] = kNegInf;
-    w.sum[m] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) w.acc[m][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  if (exists) {
-    const int length = row_length(c, c.length[cache_row]);
-    const i64 given = a.prefix[p.sequence];
-    const int prefix = (int)(given < 0 ? 0 : given > length ? length : given);
-    // positions that some query of the tile attends end at `end`, those that all do at `full`
-    const int q_first = (unsigned)row0 / (unsigned)a.group;
-    const int q_last = (unsigned)min(row0 + kRows - 1, M - 1) / (unsigned)a.group;
-    const int end = (int)min((i64)length, (i64)prefix + (a.mask ? (i64)64 * a.words : (i64)q_last + 1));
-    const int full = min(end, a.mask ? prefix : prefix + q_first + 1);
-    const int count = (end + KT - 1) / KT, full_tiles = full / KT;
-    const int each = (count + a.splits - 1) / a.splits;
-    const int from = split * each, to = min(count, from + each);
-    const int step = a.parts;
-    const int begin = from + (together ? wave : 0);
+  int index[MT];  // in the sequence
+  int token[MT], head[MT];
+  __device__ void find(const Call& a, const Sequence& s, int key_head, int row0, int M) {
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      const char* at = a.q + token[m] * a.q_stride + (q_head[m] * DH * Sh::E + g * 16);
+      const int row = row0 + 16 * m + (threadIdx.x & 15), held = min(row, M - 1);
+      real[m] = row < M;
+      index[m] = (unsigned)held / (unsigned)a.group;
+      token[m] = s.first + index[m];
+      head[m] = key_head * a.group + (held - index[m] * a.group);
+    }
+  }
+  template <class Wv>
+  __device__ void load(const Call& a, Wv& w) const {
+    using Sh = typename Wv::Sh;
 #pragma unroll
-      for (int k = 0; k < KC; ++k) {
+    for (int m = 0; m < MT; ++m) {
+      const char* at = a.q + token[m] * a.q_stride + head[m] * (Sh::KC * 64) + (threadIdx.x >> 4 & 3) * 16;
+#pragma unroll
+      for (int k = 0; k < Sh::KC; ++k) {
         u32x4 y = *reinterpret_cast<const u32x4*>(at + k * 64);
         y ^= a.flip;
         w.q[m][k] = real[m] ? y : u32x4{0, 0, 0, 0};
       }
     }
-    const i64 head_offset = a.layer_offset + slot_offset(c, 0, head, 0);
-    const char* k_head = c.k + head_offset;
-    const char* v_head = c.v + head_offset;
-    const int32_t* table = c.table + cache_row * c.width;
-    // the pages of the next 64 tiles, one a lane; -1 for none
-    int ids0 = -1, ids1 = -1;
-    const auto pages_from = [&](int tile) {
-      const int mine = tile + lane * step;
-      ids0 = ids1 = -1;
-      if (mine < to) {
-        const int first = mine * KT, last = min(first + KT, end) - 1;
-        ids0 = page_of(c, table[first >> c.page_shift]);
-        ids1 = page_of(c, table[last >> c.page_shift]);
-      }
-    };
-    typename Wv::Tile now, next;
-    int at = 0;  // the current tile among the 64
-    int id0 = 0, id1 = 0, next0 = 0, next1 = 0;
-    pages_from(begin);
-    if (begin < to) {
-      id0 = __builtin_amdgcn_readlane(ids0, 0), id1 = __builtin_amdgcn_readlane(ids1, 0);
-      Wv::load(c, k_head, v_head, begin, max(id0, 0), max(id1, 0), now);
-    }
-    for (int tile = begin; tile < to; tile += step) {
-      if (++at == 64) {
-        at = 0;
-        pages_from(tile + step);
-      }
-      if (tile + step < to) {
-        next0 = __builtin_amdgcn_readlane(ids0, at), next1 = __builtin_amdgcn_readlane(ids1, at);
-        Wv::load(c, k_head, v_head, tile + step, max(next0, 0), max(next1, 0), next);
-      }
-      const bool all = tile < full_tiles;
-      uint32_t seen[MT];
-      const int mine = tile * KT + N * g;
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        seen[m] = (1u << N) - 1;
-        if (!all) {
-          const u64* mask = a.mask ? a.mask + (a.mask_rows == a.tokens ? token[m] : query[m]) * (i64)a.words : nullptr;
-          seen[m] = seen_bits<N>(mine, a.mask ? end : min(end, prefix + query[m] + 1), prefix, mask, a.words);
-        }
-      }
-      const bool bad = (!Sh::kWide && g >= 2 ? id1 : id0) < 0;
-      w.fold(now, a.scale_log2, all, seen, end - mine, bad);
-      now = next;
-      id0 = next0, id1 = next1;
-    }
   }
-  // the lane's rows of O^T: element(j, 4 g + i) of query r
-  const auto finish = [&](int m, int i, const f32x4 (&o)[NJ], float total, float top) {
-    (void)top;
-    if (!real[m]) return;
-    const i64 out_row = (i64)token[m] * a.heads + q_head[m];
-    if (a.splits > 1) {
-      float* po = a.part_o + ((i64)split * a.tokens * a.heads + out_row) * DH;
-#pragma unroll
-      for (int h = 0; h < Sh::H; ++h) {
-        float y[Sh::W];
-#pragma unroll
-        for (int e = 0; e < Sh::W; ++e) y[e] = o[h * Sh::W + e][i];
-        store_floats<Sh::W>(po + Sh::element(h * Sh::W, 4 * g + i), y);
-      }
-      if (i == 0 && g == 0) {
-        float* ml = a.part_ml + ((i64)split * a.tokens * a.heads + out_row) * 2;
-        *reinterpret_cast<float2*>(ml) = make_float2(top, total);
-      }
-      return;
-    }
-    const float scale = !exists ? __builtin_nanf("") : total == 0.f ? 0.f : 1.f / total;
-    S* out = reinterpret_cast<S*>(a.out) + out_row * DH;
+  // Bits of a lane's N tokens that its query m attends, `at` being the first one's position.
+  template <int N>
+  __device__ uint32_t seen(const Call& a, const Sequence& s, int m, int at) const {
+    const u64* mask = a.mask ? a.mask + (a.mask_rows == a.tokens ? token[m] : index[m]) * (i64)a.words : nullptr;
+    const int limit = a.mask ? s.end : min(s.end, s.prefix + index[m] + 1);
+    uint32_t bits = seen_bits<4>(at, limit, s.prefix, mask, a.words);
+    if constexpr (N == 8) bits |= seen_bits<4>(at + 16, limit, s.prefix, mask, a.words) << 4;
+    return bits;
+  }
+};
+
+// The lane's row 4 g + i of O^T (element(j, 4 g + i) of query m) to its place: out, or a part.
+// `part_row`: the query's row in the part's slot, or -1.
+template <class T, int DH, int MT>
+__device__ inline void finish(const Call& a, const Queries<MT>& q, int m, int i, i64 part_row,
+                              bool exists, const f32x4 (&o)[DH / 16], int from, float total, float top) {
+  using Sh = Shape<T, DH>;
+  using S = typename T::storage;
+  if (!q.real[m]) return;
+  const int g = threadIdx.x >> 4 & 3;
+  if (part_row >= 0) {
 #pragma unroll
     for (int h = 0; h < Sh::H; ++h) {
       float y[Sh::W];
 #pragma unroll
-      for (int e = 0; e < Sh::W; ++e) y[e] = o[h * Sh::W + e][i] * scale;
-      store_run<S, Sh::W>(out + Sh::element(h * Sh::W, 4 * g + i), y);
+      for (int e = 0; e < Sh::W; ++e) y[e] = o[h * Sh::W + e][from];
+      store_floats<Sh::W>(a.part_o + part_row * DH + Sh::element(h * Sh::W, 4 * g + i), y);
     }
-  };
-  if (!together) {
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) finish(m, i, w.acc[m], w.sum[m][0], w.top[m]);
+    if (i == 0 && g == 0) *reinterpret_cast<float2*>(a.part_ml + part_row * 2) = make_float2(top, total);
     return;
   }
-  // merge: [wave][m][j][i][lane] sums, then [wave][m][2][lane] maxima and totals
-  constexpr int kEach = MT * NJ * 4 * 64;
-  float* tops = merged + kWaves * kEach;
+  const float scale = !exists ? __builtin_nanf("") : total == 0.f ? 0.f : 1.f / total;
+  S* out = reinterpret_cast<S*>(a.out) + ((i64)q.token[m] * a.heads + q.head[m]) * DH;
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
+  for (int h = 0; h < Sh::H; ++h) {
+    float y[Sh::W];
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) merged[wave * kEach + ((m * NJ + j) * 4 + i) * 64 + lane] = w.acc[m][j][i];
-    tops[((wave * MT + m) * 2 + 0) * 64 + lane] = w.top[m];
-    tops[((wave * MT + m) * 2 + 1) * 64 + lane] = w.sum[m][0];
-  }
-  __syncthreads();
-  const int i = wave;  // each wavefront finishes every fourth row
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    float top = kNegInf, total = 0.f, less[kWaves];
-#pragma unroll
-    for (int v = 0; v < kWaves; ++v) top = fmaxf(top, tops[((v * MT + m) * 2) * 64 + lane]);
-#pragma unroll
-    for (int v = 0; v < kWaves; ++v) {
-      const float t = tops[((v * MT + m) * 2) * 64 + lane];
-      less[v] = t == kNegInf ? 0.f : exp2_fast(t - top);
-      total += tops[((v * MT + m) * 2 + 1) * 64 + lane] * less[v];
-    }
-    f32x4 o[NJ];
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      float y = 0.f;
-#pragma unroll
-      for (int v = 0; v < kWaves; ++v)
-        y += merged[v * kEach + ((m * NJ + j) * 4 + i) * 64 + lane] * less[v];
-      o[j] = f32x4{y, y, y, y};
-    }
-    finish(m, i, o, total, top);
+    for (int e = 0; e < Sh::W; ++e) y[e] = o[h * Sh::W + e][from] * scale;
+    store_run<S, Sh::W>(out + Sh::element(h * Sh::W, 4 * g + i), y);
   }
 }
 
-// out of split rows: a wavefront's 64 / (DH / 4) rows, four elements a lane.
+// Who does an item.
+enum Mode {
+  kEach,    // a wavefront
+  kGroup,   // a workgroup, whose wavefronts take every fourth tile of tokens and merge through LDS
+  kShared,  // workgroups that share out all items' tokens
+};
+
+template <class T, int DH, int MT>
+constexpr size_t merge_bytes() {
+  return (size_t)kWaves * MT * 64 * (DH / 4 + 2) * sizeof(float);
+}
+constexpr size_t kShareBytes = (kMostShared + 1 + kWaves) * sizeof(u64);
+
+template <class T, int DH, int MT, int MODE>
+__global__ __launch_bounds__(64 * kWaves) void tree_kernel(Call a) {
+  using Sh = Shape<T, DH>;
+  using Wv = Wave<T, DH, MT>;
+  constexpr int KT = Sh::KT, N = Sh::N, NJ = Sh::NJ;
+  constexpr int kRows = 16 * MT;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const Cache& c = a.c;
+  const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned group = in_order();
+  Job job;
+  Share share;
+  if constexpr (MODE == kShared) {
+    u64* before = reinterpret_cast<u64*>(lds + merge_bytes<T, DH, MT>());
+    if (threadIdx.x == 0) nothing_noted(a, group);
+    // a tile of tokens each wavefront
+    share = share_of(a, group, kRows, KT, kWaves, before, before + kMostShared + 1);
+    if (!share.next(a, kRows, KT, job)) return;
+  } else {
+    const unsigned item = MODE == kEach ? group * kWaves + wave : group;
+    if (item >= (unsigned)a.items) return;
+    const int x = item / (unsigned)c.kv_heads;
+    job.head = item - x * (unsigned)c.kv_heads;
+    job.s = sequence_at(a, find_tile(a, x, kRows, job.tile));
+    job.from = 0, job.to = 1 << 30, job.slot = -1;
+    if ((i64)job.tile * kRows >= (i64)job.s.queries * a.group) return;
+  }
+  while (true) {
+    const Sequence& s = job.s;
+    const int M = s.queries * a.group, row0 = job.tile * kRows;
+    Queries<MT> q;
+    q.find(a, s, job.head, row0, M);
+    Wv w;
+    w.clear();
+    if (s.exists) {
+      // positions that some query of the tile attends end at `end`, those that all do at `full`
+      const int q_first = (unsigned)row0 / (unsigned)a.group;
+      const int q_last = (unsigned)min(row0 + kRows - 1, M - 1) / (unsigned)a.group;
+      const int end = a.mask ? s.end : min(s.end, s.prefix + q_last + 1);
+      const int full_tiles = min(end, a.mask ? s.prefix : s.prefix + q_first + 1) / KT;
+      const int to = min(job.to, (end + KT - 1) / KT);
+      const int step = MODE == kEach ? 1 : kWaves;
+      const int begin = job.from + (MODE == kEach ? 0 : wave);
+      q.load(a, w);
+      const i64 head_offset = a.layer_offset + slot_offset(c, 0, job.head, 0);
+      const char* k_head = c.k + head_offset;
+      const char* v_head = c.v + head_offset;
+      const int32_t* table = c.table + s.row * c.width;
+      // the pages of the next 64 tiles, one a lane; -1 for none
+      int ids0 = -1, ids1 = -1;
+      const auto pages_from = [&](int tile) {
+        const int mine = tile + lane * step;
+        ids0 = ids1 = -1;
+        if (mine < to) {
+          const int first = mine * KT, last = min(first + KT, end) - 1;
+          ids0 = page_of(c, table[first >> c.page_shift]);
+          ids1 = page_of(c, table[last >> c.page_shift]);
+        }
+      };
+      typename Wv::Keys now, next;
+      typename Wv::Values values;
+      int at = 0;  // the current tile among the 64
+      int id0 = 0, id1 = 0, next0 = 0, next1 = 0;
+      pages_from(begin);
+      const int in_page = (1 << c.page_shift) - 1;
+      const auto offset = [&](int id, int position) {  // of 16 tokens from a position on
+        return (i64)max(id, 0) * c.page_bytes + (position & in_page) * (DH * Sh::E);
+      };
+      if (begin < to) {
+        id0 = __builtin_amdgcn_readlane(ids0, 0), id1 = __builtin_amdgcn_readlane(ids1, 0);
+        load_keys<T, DH>(k_head + offset(id0, begin * KT), k_head + offset(id1, begin * KT + 16), now.k);
+      }
+      for (int tile = begin; tile < to; tile += step) {
+        load_values<T, DH>(v_head + offset(id0, tile * KT), v_head + offset(id1, tile * KT + 16), values.v);
+        if (++at == 64) {
+          at = 0;
+          pages_from(tile + step);
+        }
+        if (tile + step < to) {
+          next0 = __builtin_amdgcn_readlane(ids0, at), next1 = __builtin_amdgcn_readlane(ids1, at);
+          load_keys<T, DH>(k_head + offset(next0, (tile + step) * KT),
+                           k_head + offset(next1, (tile + step) * KT + 16), next.k);
+        }
+        const int mine = tile * KT + 4 * g;
+        w.template fold<1>(
+            a.scale_log2, tile < full_tiles, [&](int) -> const typename Wv::Keys& { return now; },
+            [&](int) -> const typename Wv::Values& { return values; },
+            [&](int, int m) { return q.template seen<N>(a, s, m, mine); },
+            [&](int) { return end - mine; },
+            [&](int, int half) { return (half ? id1 : id0) < 0; });
+        now = next;
+        id0 = next0, id1 = next1;
+      }
+    }
+    const i64 slot = MODE == kShared && job.slot >= 0 ? ((i64)group * 2 + job.slot) * kRows : -1;
+    if constexpr (MODE == kEach) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          finish<T, DH, MT>(a, q, m, i, -1, s.exists, w.acc[m], i, w.sum[m][0], w.top[m]);
+      return;
+    } else {
+      // merge: [wave][m][j][i][lane] sums, then [wave][m][2][lane] maxima and totals
+      float* merged = reinterpret_cast<float*>(lds);
+      constexpr int kPart = MT * NJ * 4 * 64;
+      float* tops = merged + kWaves * kPart;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            merged[wave * kPart + ((m * NJ + j) * 4 + i) * 64 + lane] = w.acc[m][j][i];
+        tops[((wave * MT + m) * 2 + 0) * 64 + lane] = w.top[m];
+        tops[((wave * MT + m) * 2 + 1) * 64 + lane] = w.sum[m][0];
+      }
+      __syncthreads();
+      const int i = wave;  // each wavefront finishes every fourth row
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        float top = kNegInf, total = 0.f, less[kWaves];
+#pragma unroll
+        for (int v = 0; v < kWaves; ++v) top = fmaxf(top, tops[((v * MT + m) * 2) * 64 + lane]);
+#pragma unroll
+        for (int v = 0; v < kWaves; ++v) {
+          const float t = tops[((v * MT + m) * 2) * 64 + lane];
+          less[v] = t == kNegInf ? 0.f : exp2_fast(t - top);
+          total += tops[((v * MT + m) * 2 + 1) * 64 + lane] * less[v];
+        }
+        f32x4 o[NJ];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          o[j][0] = 0.f;
+#pragma unroll
+          for (int v = 0; v < kWaves; ++v)
+            o[j][0] += merged[v * kPart + ((m * NJ + j) * 4 + i) * 64 + lane] * less[v];
+        }
+        finish<T, DH, MT>(a, q, m, i, slot < 0 ? -1 : slot + 16 * m + r, s.exists, o, 0, total, top);
+      }
+    }
+    if constexpr (MODE != kShared) return;
+    if (threadIdx.x == 0) note(a, group, job, row0, M);
+    if (!share.next(a, kRows, KT, job)) return;
+    __syncthreads();  // the merge's last readers
+  }
+}
+
+// Many rows: a workgroup's 4 wavefronts have 32 rows each and share tiles of 64 tokens, which go
+// through LDS (two buffers; a thread holds the next tile's 16-byte parts in registers meanwhile).
+// A key's row there is 16 bytes longer than it has to be, so that the 16 rows of an operand come from
+// different banks.
 template <class T, int DH>
-__global__ __launch_bounds__(256) void join_kernel(Call a) {
+struct Chunk {
+  static constexpr int kTokens = 64, kRows = 128, MT = 2;
+  static constexpr int kParts = DH / 8;                 // 16-byte parts a token
+  static constexpr int kMine = kTokens * kParts / 256;  // of them a thread moves
+  static constexpr int kStep = 256 / kParts;            // tokens between them
+  static constexpr int kKey = DH * 2 + 16, kValue = DH * 2;  // bytes from token to token
+  static constexpr int kValues = kTokens * kKey;        // where a buffer's values begin
+  static constexpr int kBytes = kValues + kTokens * kValue;
+};
+
+template <class T, int DH, int MODE>
+__global__ __launch_bounds__(64 * kWaves, 2) void chunk_kernel(Call a) {
+  using Ch = Chunk<T, DH>;
+  constexpr int MT = Ch::MT;
+  using Sh = Shape<T, DH>;
+  using Wv = Wave<T, DH, MT>;
+  constexpr int N = Sh::N, NJ = Sh::NJ;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const Cache& c = a.c;
+  const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned group = in_order();
+  Job job;
+  Share share;
+  if constexpr (MODE == kShared) {
+    u64* before = reinterpret_cast<u64*>(lds + 2 * Ch::kBytes);
+    if (threadIdx.x == 0) nothing_noted(a, group);
+    share = share_of(a, group, Ch::kRows, Ch::kTokens, 4, before, before + kMostShared + 1);
+    if (!share.next(a, Ch::kRows, Ch::kTokens, job)) return;
+  } else {
+    if (group >= (unsigned)a.items) return;
+    const int x = group / (unsigned)c.kv_heads;
+    job.head = group - x * (unsigned)c.kv_heads;
+    job.s = sequence_at(a, find_tile(a, x, Ch::kRows, job.tile));
+    job.from = 0, job.to = 1 << 30, job.slot = -1;
+    if ((i64)job.tile * Ch::kRows >= (i64)job.s.queries * a.group) return;
+  }
+  const int token_of = threadIdx.x / Ch::kParts, part_of = threadIdx.x % Ch::kParts;
+  while (true) {
+    const Sequence& s = job.s;
+    const int M = s.queries * a.group, row0 = job.tile * Ch::kRows, mine0 = row0 + wave * 32;
+    Queries<MT> q;
+    q.find(a, s, job.head, mine0, M);
+    Wv w;
+    w.clear();
+    if (s.exists) {
+      // positions that some query of the workgroup attends end at `end`, those that all of the
+      // wavefront's do at `full`
+      const int q_first = (unsigned)min(mine0, M - 1) / (unsigned)a.group;
+      const int q_last = (unsigned)min(row0 + Ch::kRows - 1, M - 1) / (unsigned)a.group;
+      const int end = a.mask ? s.end : min(s.end, s.prefix + q_last + 1);
+      const int full = min(end, a.mask ? s.prefix : s.prefix + q_first + 1);
+      const int to = min(job.to, (end + Ch::kTokens - 1) / Ch::kTokens);
+      q.load(a, w);
+      const i64 head_offset = a.layer_offset + slot_offset(c, 0, job.head, 0);
+      const char* k_head = c.k + head_offset;
+      const char* v_head = c.v + head_offset;
+      const int32_t* table = c.table + s.row * c.width;
+      // the pages of the next 64 blocks of 16 tokens, one a lane; -1 for none (past the end: the last)
+      int ids = -1;
+      const auto pages_from = [&](int tile) {
+        const int first = min(tile * Ch::kTokens + lane * 16, end - 1);
+        ids = page_of(c, table[first >> c.page_shift]);
+      };
+      u32x4 kept_k[Ch::kMine], kept_v[Ch::kMine];
+      int id[4];
+      const auto fetch = [&](int tile, int block) {  // block: the tile's first among the lanes' 64
+#pragma unroll
+        for (int b = 0; b < 4; ++b) id[b] = __builtin_amdgcn_readlane(ids, block + b);
+        const int in_page = (1 << c.page_shift) - 1;
+#pragma unroll
+        for (int i = 0; i < Ch::kMine; ++i) {
+          const int token = token_of + i * Ch::kStep;
+          const int b = (wave * 64 / Ch::kParts + i * Ch::kStep) >> 4;  // the same for the wavefront
+          const int page = max(__builtin_amdgcn_readlane(ids, block + b), 0);
+          const i64 at = (i64)page * c.page_bytes +
+                         ((tile * Ch::kTokens + token) & in_page) * (DH * 2) + part_of * 16;
+          kept_k[i] = *reinterpret_cast<const u32x4*>(k_head + at);
+          kept_v[i] = *reinterpret_cast<const u32x4*>(v_head + at);
+        }
+      };
+      const auto put = [&](int buffer) {
+        char* at = lds + buffer * Ch::kBytes + part_of * 16;
+#pragma unroll
+        for (int i = 0; i < Ch::kMine; ++i) {
+          const int token = token_of + i * Ch::kStep;
+          *reinterpret_cast<u32x4*>(at + token * Ch::kKey) = kept_k[i];
+          *reinterpret_cast<u32x4*>(at + Ch::kValues + token * Ch::kValue) = kept_v[i];
+        }
+      };
+      int block = 0;
+      if (job.from < to) {
+        pages_from(job.from);
+        fetch(job.from, 0);
+        put(0);
+        __syncthreads();
+      }
+      int buffer = 0;
+      for (int tile = job.from; tile < to; ++tile) {
+        int now[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) now[b] = id[b];
+        if (tile + 1 < to) {
+          block += 4;
+          if (block == 64) {
+            block = 0;
+            pages_from(tile + 1);
+          }
+          fetch(tile + 1, block);
+        }
+        const char* keys = lds + buffer * Ch::kBytes + r * Ch::kKey + g * 16;
+        const char* values = lds + buffer * Ch::kBytes + Ch::kValues + 4 * g * Ch::kValue + r * (Sh::W * 2);
+        const int first = tile * Ch::kTokens + 4 * g;
+        if (mine0 < M)
+          w.template fold<2>(
+              a.scale_log2, (tile + 1) * Ch::kTokens <= full,
+              [&](int t) {
+                typename Wv::Keys x;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                  for (int p = 0; p < Sh::KC; ++p)
+                    x.k[h][p] = *reinterpret_cast<const u32x4*>(keys + (32 * t + 16 * h) * Ch::kKey + p * 64);
+                return x;
+              },
+              [&](int t) {
+                typename Wv::Values x;
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                  load_words<Sh::RW>(values + (32 * t + Sh::place(e)) * Ch::kValue, x.v[e][0]);
+                return x;
+              },
+              [&](int t, int m) { return q.template seen<N>(a, s, m, first + 32 * t); },
+              [&](int t) { return end - first - 32 * t; },
+              [&](int t, int half) { return now[2 * t + half] < 0; });
+        buffer ^= 1;
+        if (tile + 1 < to) put(buffer);
+        __syncthreads();
+      }
+    }
+    const i64 slot = MODE == kShared && job.slot >= 0 ? ((i64)group * 2 + job.slot) * Ch::kRows : -1;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        finish<T, DH, MT>(a, q, m, i, slot < 0 ? -1 : slot + wave * 32 + 16 * m + r, s.exists, w.acc[m],
+                          i, w.sum[m][0], w.top[m]);
+    if constexpr (MODE != kShared) return;
+    if (threadIdx.x == 0) note(a, group, job, row0, M);
+    if (!share.next(a, Ch::kRows, Ch::kTokens, job)) return;
+  }
+}
+
+// Joins the parts of the item that a workgroup began: four elements a lane, DH / 4 lanes a row.
+template <class T, int DH>
+__global__ __launch_bounds__(256) void join_kernel(Call a, int rows) {
   using S = typename T::storage;
   constexpr int kLanes = DH / 4;
-  const i64 rows = (i64)a.tokens * a.heads;
-  const i64 row = (i64)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
-  if (row >= rows) return;
-  if (a.offsets) {
-    const i64 token = row / a.heads;
-    if (token < a.offsets[0] || token >= a.offsets[a.n]) return;
+  const unsigned group = blockIdx.x;
+  const int* said = a.notes + group * kNote;
+  if (!said[0]) return;
+  const int lane = threadIdx.x & 63;
+  int parts = 2;  // with the one that ends it
+  for (unsigned base = group + 1; base < gridDim.x; base += 64) {
+    const bool ends = base + lane < gridDim.x && a.notes[(base + lane) * kNote + 5];
+    const unsigned long long ballot = __ballot(ends);
+    if (ballot) {
+      parts += (int)(base - group - 1) + __builtin_ctzll(ballot);
+      break;
+    }
   }
+  const int first = said[1], row0 = said[2], M = said[3], key_head = said[4];
   const int at = threadIdx.x % kLanes * 4;
-  float top = kNegInf;
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[(s * rows + row) * 2]);
-  float total = 0.f;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < a.splits; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (s * rows + row) * 2);
-    const f32x4 y = *reinterpret_cast<const f32x4*>(a.part_o + (s * rows + row) * DH + at);
-    const float less = ml.x == kNegInf ? 0.f : exp2_fast(ml.x - top);
-    total += ml.y * less;
-    o += y * less;
-  }
-  const float scale = total == 0.f ? 0.f : 1.f / total;
-  float y[4];
+  for (int row = blockIdx.y * (256 / kLanes) + threadIdx.x / kLanes; row < rows && row0 + row < M;
+       row += gridDim.y * (256 / kLanes)) {
+    const auto slot = [&](int k) { return ((i64)(group + k) * 2 + (k == 0)) * rows + row; };
+    float top = kNegInf;
+    for (int k = 0; k < parts; ++k) top = fmaxf(top, a.part_ml[slot(k) * 2]);
+    float total = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < parts; ++k) {
+      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + slot(k) * 2);
+      const f32x4 y = *reinterpret_cast<const f32x4*>(a.part_o + slot(k) * DH + at);
+      const float less = ml.x == kNegInf ? 0.f : exp2_fast(ml.x - top);
+      total += ml.y * less;
+      o += y * less;
+    }
+    const float scale = total == 0.f ? 0.f : 1.f / total;
+    float y[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) y[e] = o[e] * scale;
-  store_run<S, 4>(reinterpret_cast<S*>(a.out) + row * DH + at, y);
+    for (int e = 0; e < 4; ++e) y[e] = o[e] * scale;
+    const int query = (unsigned)(row0 + row) / (unsigned)a.group;
+    const int head = key_head * a.group + (row0 + row - query * a.group);
+    store_run<S, 4>(reinterpret_cast<S*>(a.out) + ((i64)(first + query) * a.heads + head) * DH + at, y);
+  }
 }
 
 // ------------------------------------------------------------------------------ the host's part
 
-// What a call's launch is: rows a wavefront, wavefronts an item, splits.
-struct Plan {
-  int mt;
-  i64 groups;
-};
-
 inline int current_units() {
-  int device = 0, count = 0;
-  if (hipGetDevice(&device) != hipSuccess ||
-      hipDeviceGetAttribute(&count, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess)
-    return 256;
-  return count > 0 ? count : 256;
+  thread_local int device = -1, count = 256;
+  int now = 0;
+  if (hipGetDevice(&now) != hipSuccess) return 256;
+  if (now != device) {
+    int units = 0;
+    count = hipDeviceGetAttribute(&units, hipDeviceAttributeMultiprocessorCount, now) == hipSuccess &&
+                    units > 0 ? units : 256;
+    device = now;
+  }
+  return count;
 }
 
-// Rows a sequence has on the mean decide MT (more rows than it has would be empty); an item a
-// wavefront where there are enough of them, else four wavefronts an item, and splits of long
-// rows (by the table's width: lengths are on the device) until a compute unit has four workgroups.
-inline int plan(Call* a, int dh, Plan* p) {
+// What a call's launch is.
+struct Plan {
+  int rows;    // a tile's: 16 MT of tree_kernel, 128 of chunk_kernel
+  Mode mode;
+  i64 groups;  // workgroups
+};
+
+// Rows a tile by the rows a sequence has on the mean; an item a wavefront where that fills the
+// device, else a workgroup, and where rows may be long (by the table's width: lengths are on the
+// device) their tokens shared out.
+inline int plan(Call* a, int dh, int size, Plan* p) {
   const i64 rows = ((i64)a->tokens * a->group + a->n - 1) / a->n;
-  const int most = dh == 256 ? (a->c.token_bytes == 1024 ? 1 : 2) : a->c.token_bytes == 512 ? 2 : 4;
-  p->mt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  if (p->mt > most) p->mt = most;
-  const int tile = 16 * p->mt;
-  const i64 tiles = a->offsets ? (i64)a->tokens * a->group / tile + a->n
-                               : a->n * (((i64)a->each * a->group + tile - 1) / tile);
-  const i64 units = tiles * a->c.kv_heads;
-  const i64 width = (i64)a->c.width << a->c.page_shift;
-  const int cus = current_units();
-  i64 splits = 1;
-  a->parts = units >= 16 * cus ? 1 : kWaves;
-  if (a->parts > 1) {
-    const i64 want = (4 * cus + units - 1) / units, longest = width / 512;
-    splits = want < longest ? want : longest;
-    if (splits < 1) splits = 1;
-    if (splits > 64) splits = 64;
-  }
-  const i64 items = units * splits;
+  const bool chunks = size == 2 && (dh == 64 || dh == 128) && rows > 64;
+  p->rows = chunks ? 128 : rows <= 16 || dh == 256 ? 16 : 32;
+  const i64 tiles = a->offsets ? (i64)a->tokens * a->group / p->rows + a->n
+                               : a->n * (((i64)a->each * a->group + p->rows - 1) / p->rows);
+  const i64 items = tiles * a->c.kv_heads;
   if (items >= (i64)1 << 24) return -1;
-  a->tiles = (int)tiles;
+  const i64 longest = (i64)a->c.width << a->c.page_shift;
+  const int cus = current_units();
   a->items = (int)items;
-  a->splits = (int)splits;
-  p->groups = a->parts > 1 ? items : (items + kWaves - 1) / kWaves;
+  p->groups = items;
+  if (items < 8 * cus && a->n <= kMostShared && longest > 512) {
+    p->mode = kShared;
+    const i64 most = items * ((longest + 63) / 64);
+    p->groups = (chunks ? 2 : 4) * cus;
+    if (p->groups > most) p->groups = most;
+  } else if (chunks || items < 8 * cus) {
+    p->mode = kGroup;
+  } else {
+    p->mode = kEach;
+    p->groups = (items + kWaves - 1) / kWaves;
+  }
   return 0;
 }
 
-inline i64 part_bytes(const Call& a, int dh) {
-  return a.splits > 1 ? (i64)a.splits * a.tokens * a.heads * (dh + 2) * (i64)sizeof(float) : 0;
+inline i64 part_floats(const Plan& p, int dh) { return p.groups * 2 * p.rows * dh; }
+inline i64 part_bytes(const Plan& p, int dh) {
+  return p.mode != kShared ? 0
+                           : (part_floats(p, dh) + p.groups * 2 * p.rows * 2) * (i64)sizeof(float) +
+                                 p.groups * kNote * (i64)sizeof(int);
+}
+
+// A launch with more than 64 KiB of LDS has to say so once a device and kernel.
+template <class K>
+int allow_lds(K* kernel, size_t bytes) {
+  if (bytes <= 64 * 1024) return 0;
+  return (int)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+
+template <class K>
+int launch(K* kernel, const Call& a, i64 groups, size_t lds, hipStream_t stream) {
+  if (const int bad = allow_lds(kernel, lds)) return bad;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(64 * kWaves), lds, stream, a);
+  return (int)hipGetLastError();
 }
 
 template <class T, int DH, int MT>
-int launch(const Call& a, i64 groups, hipStream_t stream) {
-  using Sh = Shape<T, DH>;
-  constexpr size_t kMerge = (size_t)kWaves * MT * 64 * (Sh::NJ * 4 + 2) * sizeof(float);
-  const size_t lds = a.parts > 1 ? kMerge : 0;
-  if constexpr (kMerge > 64 * 1024) {
-    if (lds > 0) {
-      const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(tree_kernel<T, DH, MT>),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)kMerge);
-      if (e != hipSuccess) return (int)e;
-    }
-  }
-  hipLaunchKernelGGL((tree_kernel<T, DH, MT>), dim3((unsigned)groups), dim3(64 * kWaves), lds, stream, a);
-  if (a.splits > 1) {
-    constexpr int kEach = 256 / (DH / 4);
-    const i64 rows = (i64)a.tokens * a.heads;
-    hipLaunchKernelGGL((join_kernel<T, DH>), dim3((unsigned)((rows + kEach - 1) / kEach)), dim3(256),
-                       0, stream, a);
-  }
-  return (int)hipGetLastError();
+int by_mode(const Call& a, const Plan& p, hipStream_t stream) {
+  constexpr size_t kMerge = merge_bytes<T, DH, MT>();
+  if (p.mode == kEach) return launch(tree_kernel<T, DH, MT, kEach>, a, p.groups, 0, stream);
+  if (p.mode == kGroup) return launch(tree_kernel<T, DH, MT, kGroup>, a, p.groups, kMerge, stream);
+  return launch(tree_kernel<T, DH, MT, kShared>, a, p.groups, kMerge + kShareBytes, stream);
 }
 
 template <class T, int DH>
 int by_rows(const Call& a, const Plan& p, hipStream_t stream) {
-  constexpr int kBytes = DH * (int)sizeof(typename T::storage);
-  if (p.mt == 1) return launch<T, DH, 1>(a, p.groups, stream);
-  if constexpr (kBytes < 1024) {
-    if (p.mt == 2) return launch<T, DH, 2>(a, p.groups, stream);
+  constexpr int kSize = sizeof(typename T::storage);
+  int rc = -1;
+  if (p.rows == 16) rc = by_mode<T, DH, 1>(a, p, stream);
+  if constexpr (DH < 256) {
+    if (p.rows == 32) rc = by_mode<T, DH, 2>(a, p, stream);
   }
-  if constexpr (kBytes < 512) {
-    if (p.mt == 4) return launch<T, DH, 4>(a, p.groups, stream);
+  if constexpr (kSize == 2 && (DH == 64 || DH == 128)) {
+    constexpr size_t kTiles = 2 * Chunk<T, DH>::kBytes;
+    if (p.rows == 128)
+      rc = p.mode == kGroup ? launch(chunk_kernel<T, DH, kGroup>, a, p.groups, kTiles, stream)
+                            : launch(chunk_kernel<T, DH, kShared>, a, p.groups, kTiles + kShareBytes, stream);
   }
-  return -1;
+  if (rc || p.mode != kShared) return rc;
+  constexpr int kEachRow = 256 / (DH / 4);
+  const int spread = (p.rows + kEachRow - 1) / kEachRow;
+  hipLaunchKernelGGL((join_kernel<T, DH>), dim3((unsigned)p.groups, (unsigned)spread), dim3(256), 0,
+                     stream, a, p.rows);
+  return (int)hipGetLastError();
 }
 
 template <class T>
@@ -829,6 +1215,7 @@ inline int view(const CugoTreeAttention* p, Call* a) {
   a->scale_log2 = scale * 1.4426950408889634f;  // softmax in base 2
   a->out = static_cast<char*>(p->out);
   a->part_o = a->part_ml = nullptr;
+  a->notes = nullptr;
   return 0;
 }
 
@@ -841,8 +1228,9 @@ int64_t cugo_tree_attention_workspace(const CugoTreeAttention* call) {
   using namespace cugo_amd::paged;
   Call a;
   Plan p;
-  if (view(call, &a) || a.tokens == 0 || plan(&a, (int)call->cache->dh, &p)) return 0;
-  return part_bytes(a, (int)call->cache->dh);
+  if (view(call, &a) || a.tokens == 0) return 0;
+  const int dh = (int)call->cache->dh;
+  return plan(&a, dh, element_size(call->cache->dtype), &p) ? 0 : part_bytes(p, dh);
 }
 
 int cugo_tree_attention(const CugoTreeAttention* call, void* workspace, int64_t workspace_bytes,
@@ -853,13 +1241,14 @@ int cugo_tree_attention(const CugoTreeAttention* call, void* workspace, int64_t 
   if (const int bad = view(call, &a)) return bad;
   if (a.tokens == 0) return 0;
   const int dh = (int)call->cache->dh;
-  if (const int bad = plan(&a, dh, &p)) return bad;
-  if (const int64_t need = part_bytes(a, dh)) {
+  if (const int bad = plan(&a, dh, element_size(call->cache->dtype), &p)) return bad;
+  if (const int64_t need = part_bytes(p, dh)) {
     if (!workspace) return -1;
     if (!aligned16(workspace)) return -4;
     if (workspace_bytes < need) return -5;
     a.part_o = static_cast<float*>(workspace);
-    a.part_ml = a.part_o + (int64_t)a.splits * a.tokens * a.heads * dh;
+    a.part_ml = a.part_o + part_floats(p, dh);
+    a.notes = reinterpret_cast<int*>(a.part_ml + p.groups * 2 * p.rows * 2);
   }
   switch (call->cache->dtype) {
     case CUGO_DTYPE_BF16:
