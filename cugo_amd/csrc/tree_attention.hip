@@ -26,6 +26,8 @@
 // Tiles in which some query may not see some token (the drafts, a row's end) take their scores
 // from the masks, and values that are infinite or NaN there go through products of their own
 // (indicators of +inf and -inf), since 0 x inf would show in queries that do not attend them.
+#include <type_traits>
+
 #include "paged.h"
 
 namespace cugo_amd {
@@ -82,10 +84,10 @@ constexpr float kNegInf = -__builtin_inff();
 constexpr float kSlack = 8.f;
 constexpr int kWaves = 4;
 
-__device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // The largest over the four lanes that hold one query (lane & 15).
-__device__ inline float query_max(float x) {
+__device__ __forceinline__ float query_max(float x) {
   const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
   const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -94,7 +96,7 @@ __device__ inline float query_max(float x) {
 
 // W bytes / 4 words at p.
 template <int N>
-__device__ inline void load_words(const char* p, uint32_t (&w)[N]) {
+__device__ __forceinline__ void load_words(const char* p, uint32_t (&w)[N]) {
   if constexpr (N == 1) {
     w[0] = *reinterpret_cast<const uint32_t*>(p);
   } else if constexpr (N == 2) {
@@ -129,7 +131,7 @@ struct Shape {
 
 // The parts of a tile's keys and values that a lane holds; at0 and at1: its first and second 16 tokens.
 template <class T, int DH>
-__device__ inline void load_keys(const char* at0, const char* at1,
+__device__ __forceinline__ void load_keys(const char* at0, const char* at1,
                                  u32x4 (&k)[Shape<T, DH>::KL][Shape<T, DH>::KC]) {
   using Sh = Shape<T, DH>;
   const unsigned lane = threadIdx.x & 63, mine = (lane & 15) * (DH * Sh::E) + (lane >> 4) * 16;
@@ -140,7 +142,7 @@ __device__ inline void load_keys(const char* at0, const char* at1,
       k[a][p] = *reinterpret_cast<const u32x4*>((a ? at1 : at0) + mine + p * 64);
 }
 template <class T, int DH>
-__device__ inline void load_values(const char* at0, const char* at1,
+__device__ __forceinline__ void load_values(const char* at0, const char* at1,
                                    uint32_t (&v)[Shape<T, DH>::N][Shape<T, DH>::H][Shape<T, DH>::RW]) {
   using Sh = Shape<T, DH>;
   const unsigned lane = threadIdx.x & 63;
@@ -166,12 +168,52 @@ struct Wave {
   struct Keys {
     u32x4 k[KL][KC];
   };
-  struct Values {
-    uint32_t v[N][Sh::H][Sh::RW];
-  };
   // A product operand of N numbers, rounded to the type.
   struct Weights {
     uint32_t w[4];
+  };
+  // A tile's values in registers.
+  struct Values {
+    static constexpr bool kInPlace = true;
+    uint32_t v[N][Sh::H][Sh::RW];
+    // Elements j of the lane's N tokens.
+    __device__ Weights column(int, int j) const {
+      Weights y;
+      const int h = j / Sh::W, e = j % Sh::W;
+      if constexpr (Sh::kWide) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) y.w[t] = v[t][h][e];
+      } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          y.w[t] = __builtin_amdgcn_perm(v[2 * t + 1][h][e / 2], v[2 * t][h][e / 2],
+                                         e & 1 ? 0x07060302u : 0x05040100u);
+      }
+      return y;
+    }
+    // Zeros for the tokens from `until` on; whether an infinity or NaN is left.
+    __device__ bool clear(int, int until) {
+      bool odd = false;
+#pragma unroll
+      for (int t = 0; t < N; ++t)
+#pragma unroll
+        for (int h = 0; h < Sh::H; ++h)
+#pragma unroll
+          for (int e = 0; e < Sh::RW; ++e) {
+            v[t][h][e] = Sh::place(t) < until ? v[t][h][e] : 0u;
+            odd |= finite(v[t][h][e]) != v[t][h][e];
+          }
+      return odd;
+    }
+    __device__ Weights cleared(int s, int j) const { return column(s, j); }
+    __device__ void only_finite(int) {
+#pragma unroll
+      for (int t = 0; t < N; ++t)
+#pragma unroll
+        for (int h = 0; h < Sh::H; ++h)
+#pragma unroll
+          for (int e = 0; e < Sh::RW; ++e) v[t][h][e] = finite(v[t][h][e]);
+    }
   };
 
   __device__ void clear() {
@@ -232,51 +274,31 @@ struct Wave {
       return T::mfma(u32x4{a.w[0], a.w[1], a.w[2], a.w[3]}, u32x4{p.w[0], p.w[1], p.w[2], p.w[3]}, c);
     }
   }
-  // Element j of the lane's N tokens.
-  __device__ static Weights column(const Values& x, int j) {
-    Weights y;
-    const int h = j / Sh::W, e = j % Sh::W;
-    if constexpr (Sh::kWide) {
-#pragma unroll
-      for (int t = 0; t < 4; ++t) y.w[t] = x.v[t][h][e];
-    } else {
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-        y.w[t] = __builtin_amdgcn_perm(x.v[2 * t + 1][h][e / 2], x.v[2 * t][h][e / 2],
-                                       e & 1 ? 0x07060302u : 0x05040100u);
-    }
-    return y;
-  }
-
-  // SUB tiles' share of every query.  keys(s) and values(s): the lane's parts of tile s.  all: every
-  // query attends every token; otherwise seen(s, m) has the bits of the lane's tokens that query m
-  // attends, and positions from inside(s) on after the tile's 4 g are past the row's end.  bad(s, half):
-  // the tokens of that half have no page.
-  template <int SUB, class KeysOf, class ValuesOf, class Seen, class Inside, class Bad>
-  __device__ void fold(float scale, bool all, KeysOf keys, ValuesOf values, Seen seen,
-                       Inside inside, Bad bad) {
+  // SUB tiles' share of every query.  kAll: every query attends every token, and each has a page.  keys(s): the lane's parts of tile s's keys; values.column(s, j):
+  // its operand for elements j of the values.  Otherwise seen(s, m) has the bits of the lane's tokens
+  // that query m attends, positions from inside(s) on after the tile's 4 g are past the row's end, and
+  // the tokens of half h of a tile with bad(s, h) have no page.
+  template <int SUB, bool kAll, class KeysOf, class V, class Seen, class Inside, class Bad>
+  __device__ __forceinline__ void fold(float scale, KeysOf keys, V& values, Seen seen, Inside inside, Bad bad) {
     float d[SUB][MT][N], most[MT];
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
       const Keys& x = keys(s);
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        scores(x, q[m], d[s][m]);
-#pragma unroll
-        for (int a = 0; a < KL; ++a)
-          if (bad(s, a))
-#pragma unroll
-            for (int e = 0; e < 4; ++e) d[s][m][4 * a + e] = __builtin_nanf("");
-      }
+      for (int m = 0; m < MT; ++m) scores(x, q[m], d[s][m]);
+      if constexpr (SUB > 1) __builtin_amdgcn_sched_barrier(0);  // one tile's keys in registers
     }
-    if (!all)
+    if constexpr (!kAll)
 #pragma unroll
       for (int s = 0; s < SUB; ++s)
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           const uint32_t bits = seen(s, m);
 #pragma unroll
-          for (int e = 0; e < N; ++e) d[s][m][e] = bits >> e & 1 ? d[s][m][e] : kNegInf;
+          for (int e = 0; e < N; ++e) {
+            const float x = bad(s, e / 4) ? __builtin_nanf("") : d[s][m][e];
+            d[s][m][e] = bits >> e & 1 ? x : kNegInf;
+          }
         }
     bool more = false;
 #pragma unroll
@@ -318,37 +340,28 @@ struct Wave {
     }
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
-      Values x = values(s);
-      if (!all) {
+      if constexpr (!kAll) {
         // tokens past the row's end hold anything; among the others infinities and NaN are rare
-        const int until = inside(s);
-        bool odd = false;
+        if (__ballot(values.clear(s, inside(s)))) {
+          fold_odd(values, s, [&](int m) { return seen(s, m); });
+          values.only_finite(s);
+        }
+        if constexpr (!V::kInPlace) {
 #pragma unroll
-        for (int t = 0; t < N; ++t)
+          for (int j = 0; j < NJ; ++j) {
+            __builtin_amdgcn_sched_barrier(0);
+            const Weights x = values.cleared(s, j);
 #pragma unroll
-          for (int h = 0; h < Sh::H; ++h)
-#pragma unroll
-            for (int e = 0; e < Sh::RW; ++e) {
-              const uint32_t y = Sh::place(t) < until ? x.v[t][h][e] : 0u;
-              x.v[t][h][e] = y;
-              if constexpr (Sh::kWide) odd = odd || (y & inf_bits()) == inf_bits();
-              else odd = odd || (y & inf_bits()) == inf_bits() || (y >> 16 & inf_bits()) == inf_bits();
-            }
-        if (__ballot(odd)) {
-          fold_odd(x, [&](int m) { return seen(s, m); });
-#pragma unroll
-          for (int t = 0; t < N; ++t)
-#pragma unroll
-            for (int h = 0; h < Sh::H; ++h)
-#pragma unroll
-              for (int e = 0; e < Sh::RW; ++e) x.v[t][h][e] = only_finite(x.v[t][h][e]);
+            for (int m = 0; m < MT; ++m) acc[m][j] = product(x, w[s][m], acc[m][j]);
+          }
+          continue;
         }
       }
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        const Weights a = column(x, j);
+        const Weights x = values.column(s, j);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) acc[m][j] = product(a, w[s][m], acc[m][j]);
+        for (int m = 0; m < MT; ++m) acc[m][j] = product(x, w[s][m], acc[m][j]);
       }
     }
   }
@@ -358,7 +371,7 @@ struct Wave {
     else return T::kInf;
   }
   // The word with its infinite numbers and NaN as zeros.
-  __device__ static uint32_t only_finite(uint32_t w) {
+  __device__ static uint32_t finite(uint32_t w) {
     if constexpr (Sh::kWide) return (w & inf_bits()) == inf_bits() ? 0u : w;
     if ((w & inf_bits()) == inf_bits()) w &= 0xffff0000u;
     if ((w >> 16 & inf_bits()) == inf_bits()) w &= 0x0000ffffu;
@@ -384,8 +397,8 @@ struct Wave {
     return pack(y);
   }
   // What infinite values and NaN bring to the queries that attend them.
-  template <class Seen>
-  __device__ void fold_odd(const Values& x, Seen seen) {
+  template <class V, class Seen>
+  __device__ void fold_odd(V& values, int s, Seen seen) {
     Weights who[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
@@ -399,7 +412,7 @@ struct Wave {
     for (int j = 0; j < NJ; ++j) {
       // one after another: interleaved, this rare path would decide the kernel's registers
       __builtin_amdgcn_sched_barrier(0);
-      const Weights a = column(x, j), positive = infinite(a, false), negative = infinite(a, true);
+      const Weights a = values.cleared(s, j), positive = infinite(a, false), negative = infinite(a, true);
       const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
@@ -417,7 +430,7 @@ struct Wave {
 // Bits of the N positions from `at` on that a query may attend: before `limit` and (with a mask)
 // before its prefix or set in its mask.
 template <int N>
-__device__ inline uint32_t seen_bits(int at, int limit, int prefix, const u64* mask, int words) {
+__device__ __forceinline__ uint32_t seen_bits(int at, int limit, int prefix, const u64* mask, int words) {
   uint32_t bits = (1u << N) - 1;
   if (mask != nullptr) {
     const int b = at - prefix;
@@ -441,7 +454,7 @@ struct Sequence {
   int length, prefix;
   int end;  // positions that some query may attend lie before it
 };
-__device__ inline Sequence sequence_at(const Call& a, int i) {
+__device__ __forceinline__ Sequence sequence_at(const Call& a, int i) {
   Sequence s;
   s.first = i * a.each;
   s.queries = a.each;
@@ -460,9 +473,21 @@ __device__ inline Sequence sequence_at(const Call& a, int i) {
   return s;
 }
 
+// What is the same in every lane, in scalar registers.
+__device__ __forceinline__ int same(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ u64 same(u64 x) {
+  return (u64)(unsigned)same((int)(x >> 32)) << 32 | (unsigned)same((int)x);
+}
+__device__ __forceinline__ Sequence same(Sequence s) {
+  s.first = same(s.first), s.queries = same(s.queries), s.row = (i64)same((u64)s.row);
+  s.length = same(s.length), s.prefix = same(s.prefix), s.end = same(s.end);
+  s.exists = same((int)s.exists);
+  return s;
+}
+
 // The sequence of tile x and the tile's place in it.  With offsets, sequence i's tiles begin at
 // floor((offsets[i] - offsets[0]) group / rows a tile) + i, which leaves room for what each needs.
-__device__ inline int find_tile(const Call& a, int x, int rows, int& tile) {
+__device__ __forceinline__ int find_tile(const Call& a, int x, int rows, int& tile) {
   if (a.offsets == nullptr) {
     const int each = (int)(((i64)a.each * a.group + rows - 1) / rows);
     const int i = (unsigned)x / (unsigned)each;
@@ -485,8 +510,8 @@ __device__ inline int find_tile(const Call& a, int x, int rows, int& tile) {
     span = min(step, span - last * step);
     low += last * step;
   }
-  low = __builtin_amdgcn_readfirstlane(low);
-  tile = x - start(low);
+  low = same(low);
+  tile = same(x - start(low));
   return low;
 }
 
@@ -498,7 +523,7 @@ constexpr int kMostShared = 1024;
 constexpr int kNote = 8;
 
 // before[i]: the work of the sequences before i; before[n]: all of it.  `scratch`: kWaves numbers.
-__device__ inline void sum_work(const Call& a, int rows, int tokens, u64* before, u64* scratch) {
+__device__ __forceinline__ void sum_work(const Call& a, int rows, int tokens, u64* before, u64* scratch) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   u64 carry = 0;
   for (int base = 0; base < a.n; base += 64 * kWaves) {
@@ -545,7 +570,7 @@ struct Share {
   const u64* before;
   u64 at, end;
   int n;
-  __device__ bool next(const Call& a, int rows, int tokens, Job& job) {
+  __device__ __forceinline__ bool next(const Call& a, int rows, int tokens, Job& job) {
     if (at >= end) return false;
     int low = 0, high = n;  // before[low] <= at < before[high]
     while (high - low > 1) {
@@ -553,16 +578,16 @@ struct Share {
       if (before[mid] <= at) low = mid;
       else high = mid;
     }
-    low = __builtin_amdgcn_readfirstlane(low);
-    job.s = sequence_at(a, low);
+    low = same(low);
+    job.s = same(sequence_at(a, low));
     const int tiles = (int)(((i64)job.s.queries * a.group + rows - 1) / rows);
     const int each = max(1, (job.s.end + tokens - 1) / tokens);
-    const u64 offset = at - before[low];
+    const u64 offset = at - same(before[low]);
     const u64 item = offset / (unsigned)each;
-    job.from = (int)(offset - item * each);
-    job.to = (int)min((u64)each, job.from + (end - at));
-    job.head = (int)(item / (unsigned)tiles);
-    job.tile = (int)(item - (u64)job.head * tiles);
+    job.from = same((int)(offset - item * each));
+    job.to = same((int)min((u64)each, job.from + (end - at)));
+    job.head = same((int)(item / (unsigned)tiles));
+    job.tile = same((int)(item - (u64)job.head * tiles));
     job.ends = job.to == each;
     job.slot = job.from > 0 ? 0 : job.ends ? -1 : 1;
     at += job.to - job.from;
@@ -572,15 +597,15 @@ struct Share {
 
 // Workgroups in an order that gives consecutive ones to one XCD (they go round the 8 of them): tiles
 // of one sequence read the same keys.
-__device__ inline unsigned in_order() {
+__device__ __forceinline__ unsigned in_order() {
   const unsigned groups = gridDim.x, whole = groups & ~7u;
   return blockIdx.x < whole ? (blockIdx.x & 7) * (whole >> 3) + (blockIdx.x >> 3) : blockIdx.x;
 }
 
-__device__ inline Share share_of(const Call& a, unsigned group, int rows, int tokens, int least,
+__device__ __forceinline__ Share share_of(const Call& a, unsigned group, int rows, int tokens, int least,
                                  u64* before, u64* scratch) {
   sum_work(a, rows, tokens, before, scratch);
-  const u64 all = before[a.n];
+  const u64 all = same(before[a.n]);
   // no less than `least` tiles of tokens each, unless there are more items; one at least
   u64 groups = max(all / (unsigned)least, (u64)a.items);
   groups = max(min(min(groups, (u64)gridDim.x), all), (u64)1);
@@ -588,14 +613,14 @@ __device__ inline Share share_of(const Call& a, unsigned group, int rows, int to
   s.before = before;
   s.n = a.n;
   s.at = s.end = 0;
-  if (group < groups) s.at = all * group / groups, s.end = all * (group + 1) / groups;
+  if (group < groups) s.at = same(all * group / groups), s.end = same(all * (group + 1) / groups);
   return s;
 }
 
 // What a workgroup tells the launch that joins: [0] it began an item that others went on with, of
 // which [1] first query, [2] first row, [3] rows, [4] key head; [5] it ended an item that others
 // began.
-__device__ inline void note(const Call& a, unsigned group, const Job& job, int row0, int M) {
+__device__ __forceinline__ void note(const Call& a, unsigned group, const Job& job, int row0, int M) {
   int* at = a.notes + group * kNote;
   if (job.slot == 1) {
     at[0] = 1, at[1] = job.s.first, at[2] = row0, at[3] = M, at[4] = job.head;
@@ -603,13 +628,13 @@ __device__ inline void note(const Call& a, unsigned group, const Job& job, int r
     at[5] = job.ends;
   }
 }
-__device__ inline void nothing_noted(const Call& a, unsigned group) {
+__device__ __forceinline__ void nothing_noted(const Call& a, unsigned group) {
   a.notes[group * kNote] = a.notes[group * kNote + 5] = 0;
 }
 
 // Stores W consecutive elements.
 template <class S, int W>
-__device__ inline void store_run(S* p, const float (&x)[W]) {
+__device__ __forceinline__ void store_run(S* p, const float (&x)[W]) {
   struct alignas(sizeof(S) * W) Run {
     S v[W];
   } y;
@@ -618,7 +643,7 @@ __device__ inline void store_run(S* p, const float (&x)[W]) {
   *reinterpret_cast<Run*>(p) = y;
 }
 template <int W>
-__device__ inline void store_floats(float* p, const float (&x)[W]) {
+__device__ __forceinline__ void store_floats(float* p, const float (&x)[W]) {
 #pragma unroll
   for (int e = 0; e < W; e += W < 4 ? 2 : 4) {
     if constexpr (W < 4) *reinterpret_cast<float2*>(p + e) = make_float2(x[e], x[e + 1]);
@@ -670,7 +695,7 @@ struct Queries {
 // The lane's row 4 g + i of O^T (element(j, 4 g + i) of query m) to its place: out, or a part.
 // `part_row`: the query's row in the part's slot, or -1.
 template <class T, int DH, int MT>
-__device__ inline void finish(const Call& a, const Queries<MT>& q, int m, int i, i64 part_row,
+__device__ __forceinline__ void finish(const Call& a, const Queries<MT>& q, int m, int i, i64 part_row,
                               bool exists, const f32x4 (&o)[DH / 16], int from, float total, float top) {
   using Sh = Shape<T, DH>;
   using S = typename T::storage;
@@ -729,17 +754,19 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(Call a) {
     if (threadIdx.x == 0) nothing_noted(a, group);
     // a tile of tokens each wavefront
     share = share_of(a, group, kRows, KT, kWaves, before, before + kMostShared + 1);
-    if (!share.next(a, kRows, KT, job)) return;
   } else {
     const unsigned item = MODE == kEach ? group * kWaves + wave : group;
     if (item >= (unsigned)a.items) return;
     const int x = item / (unsigned)c.kv_heads;
     job.head = item - x * (unsigned)c.kv_heads;
-    job.s = sequence_at(a, find_tile(a, x, kRows, job.tile));
+    job.s = same(sequence_at(a, find_tile(a, x, kRows, job.tile)));
     job.from = 0, job.to = 1 << 30, job.slot = -1;
     if ((i64)job.tile * kRows >= (i64)job.s.queries * a.group) return;
   }
   while (true) {
+    if constexpr (MODE == kShared) {
+      if (!share.next(a, kRows, KT, job)) return;
+    }
     const Sequence& s = job.s;
     const int M = s.queries * a.group, row0 = job.tile * kRows;
     Queries<MT> q;
@@ -784,27 +811,32 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(Call a) {
         id0 = __builtin_amdgcn_readlane(ids0, 0), id1 = __builtin_amdgcn_readlane(ids1, 0);
         load_keys<T, DH>(k_head + offset(id0, begin * KT), k_head + offset(id1, begin * KT + 16), now.k);
       }
-      for (int tile = begin; tile < to; tile += step) {
-        load_values<T, DH>(v_head + offset(id0, tile * KT), v_head + offset(id1, tile * KT + 16), values.v);
-        if (++at == 64) {
-          at = 0;
-          pages_from(tile + step);
+      int tile = begin;
+      // first the tiles that all of it attends, in a loop without what the others need
+      const auto run = [&](auto all) {
+        for (; tile < to && (!all || (tile < full_tiles && min(id0, id1) >= 0)); tile += step) {
+          load_values<T, DH>(v_head + offset(id0, tile * KT), v_head + offset(id1, tile * KT + 16), values.v);
+          if (++at == 64) {
+            at = 0;
+            pages_from(tile + step);
+          }
+          if (tile + step < to) {
+            next0 = __builtin_amdgcn_readlane(ids0, at), next1 = __builtin_amdgcn_readlane(ids1, at);
+            load_keys<T, DH>(k_head + offset(next0, (tile + step) * KT),
+                             k_head + offset(next1, (tile + step) * KT + 16), next.k);
+          }
+          const int mine = tile * KT + 4 * g;
+          w.template fold<1, decltype(all)::value>(
+              a.scale_log2, [&](int) -> const typename Wv::Keys& { return now; }, values,
+              [&](int, int m) { return q.template seen<N>(a, s, m, mine); },
+              [&](int) { return end - mine; },
+              [&](int, int half) { return (half ? id1 : id0) < 0; });
+          now = next;
+          id0 = next0, id1 = next1;
         }
-        if (tile + step < to) {
-          next0 = __builtin_amdgcn_readlane(ids0, at), next1 = __builtin_amdgcn_readlane(ids1, at);
-          load_keys<T, DH>(k_head + offset(next0, (tile + step) * KT),
-                           k_head + offset(next1, (tile + step) * KT + 16), next.k);
-        }
-        const int mine = tile * KT + 4 * g;
-        w.template fold<1>(
-            a.scale_log2, tile < full_tiles, [&](int) -> const typename Wv::Keys& { return now; },
-            [&](int) -> const typename Wv::Values& { return values; },
-            [&](int, int m) { return q.template seen<N>(a, s, m, mine); },
-            [&](int) { return end - mine; },
-            [&](int, int half) { return (half ? id1 : id0) < 0; });
-        now = next;
-        id0 = next0, id1 = next1;
-      }
+      };
+      run(std::true_type());
+      run(std::false_type());
     }
     const i64 slot = MODE == kShared && job.slot >= 0 ? ((i64)group * 2 + job.slot) * kRows : -1;
     if constexpr (MODE == kEach) {
@@ -855,24 +887,121 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(Call a) {
     }
     if constexpr (MODE != kShared) return;
     if (threadIdx.x == 0) note(a, group, job, row0, M);
-    if (!share.next(a, kRows, KT, job)) return;
     __syncthreads();  // the merge's last readers
   }
 }
 
-// Many rows: a workgroup's 4 wavefronts have 32 rows each and share tiles of 64 tokens, which go
-// through LDS (two buffers; a thread holds the next tile's 16-byte parts in registers meanwhile).
-// A key's row there is 16 bytes longer than it has to be, so that the 16 rows of an operand come from
-// different banks.
+// Many rows: a workgroup's 4 wavefronts have 32 rows each and share tiles of 64 tokens in LDS, two
+// buffers of them, which global_load_lds_dwordx4 fills without going through registers (1,024
+// consecutive bytes of LDS an instruction; a wavefront brings 16 tokens).  A token's 16-byte parts are
+// exchanged there, so that what is read at once comes from different banks: the same part of 16 keys,
+// or 32 bytes of four values, which ds_read_b64_tr_b16 turns as it reads (four lanes a token's 16
+// elements in, one element's four tokens a lane out; no v_perm_b32).  Elements j of the values are
+// 16 j ... 16 j + 15 here.
 template <class T, int DH>
 struct Chunk {
   static constexpr int kTokens = 64, kRows = 128, MT = 2;
-  static constexpr int kParts = DH / 8;                 // 16-byte parts a token
-  static constexpr int kMine = kTokens * kParts / 256;  // of them a thread moves
-  static constexpr int kStep = 256 / kParts;            // tokens between them
-  static constexpr int kKey = DH * 2 + 16, kValue = DH * 2;  // bytes from token to token
-  static constexpr int kValues = kTokens * kKey;        // where a buffer's values begin
-  static constexpr int kBytes = kValues + kTokens * kValue;
+  static constexpr int kToken = DH * 2;             // bytes
+  static constexpr int kTile = kTokens * kToken;    // of keys, and of values
+  static constexpr int kParts = DH / 8;             // 16-byte parts a token
+  static constexpr int kLoads = 16 * kToken / 1024;  // a wavefront's, of keys and of values
+  static_assert(4 * kTile <= 1 << 16, "global_load_lds_dwordx4's place in LDS has 16 bits");
+  // Where part `part` of a key or value lies among its token's.
+  __device__ static int key_part(int token, int part) {
+    return part ^ (kParts == 16 ? token & 15 : token >> 1 & 7);
+  }
+  __device__ static int value_part(int token, int part) {
+    return part ^ (kParts == 16 ? token & 3 : token >> 1 & 1) * 2;
+  }
+  static constexpr int kTurns = kParts == 16 ? 4 : 2;  // places of elements j that differ by more than j
+};
+
+// 16 bytes a lane from base + offset to LDS at `to` + 16 lane; waited for by wait_loads().  In
+// assembly, since the compiler takes every later read of LDS for one of what such a load brings and
+// waits for it first; here a barrier stands between them.
+__device__ __forceinline__ void load_to_lds(const char* base, unsigned offset, unsigned to) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Four 16-bit numbers a lane: of each 16 lanes, number l of those that lanes 4 k ... 4 k + 3 name
+// together, k = 0 ... 3.
+__device__ __forceinline__ uint2 read_turned(const char* p) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s16x4 Lds;
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)p));
+}
+
+// The lane's elements 16 j + 4 g ... + 3 of query m to their place: out, or a part (finish).
+template <class T, int DH, int MT>
+__device__ __forceinline__ void finish_turned(const Call& a, const Queries<MT>& q, int m, i64 part_row,
+                                     bool exists, const f32x4 (&o)[DH / 16], float total, float top) {
+  using S = typename T::storage;
+  if (!q.real[m]) return;
+  const int g = threadIdx.x >> 4 & 3;
+  if (part_row >= 0) {
+#pragma unroll
+    for (int j = 0; j < DH / 16; ++j)
+      *reinterpret_cast<f32x4*>(a.part_o + part_row * DH + 16 * j + 4 * g) = o[j];
+    if (g == 0) *reinterpret_cast<float2*>(a.part_ml + part_row * 2) = make_float2(top, total);
+    return;
+  }
+  const float scale = !exists ? __builtin_nanf("") : total == 0.f ? 0.f : 1.f / total;
+  S* out = reinterpret_cast<S*>(a.out) + ((i64)q.token[m] * a.heads + q.head[m]) * DH;
+#pragma unroll
+  for (int j = 0; j < DH / 16; ++j) {
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = o[j][e] * scale;
+    store_run<S, 4>(out + 16 * j + 4 * g, y);
+  }
+}
+
+// A tile's values in LDS; `at`: where the lane reads its elements j, j below kTurns, of the first.
+template <class T, int DH>
+struct TurnedValues {
+  using Wv = Wave<T, DH, Chunk<T, DH>::MT>;
+  using Weights = typename Wv::Weights;
+  static constexpr bool kInPlace = false;
+  static constexpr int kToken = Chunk<T, DH>::kToken, kTurns = Chunk<T, DH>::kTurns;
+  const char* at[kTurns];
+  uint32_t held[4];
+  bool all_finite;
+  __device__ Weights column(int s, int j) const {
+    const char* x = at[j % kTurns] + 32 * s * kToken + j / kTurns * kTurns * 32;
+    const uint2 low = read_turned(x), high = read_turned(x + 16 * kToken);
+    return Weights{{low.x, low.y, high.x, high.y}};
+  }
+  __device__ Weights cleared(int s, int j) const {
+    Weights x = column(s, j);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      x.w[t] &= held[t];
+      if (all_finite) x.w[t] = Wv::finite(x.w[t]);
+    }
+    return x;
+  }
+  __device__ bool clear(int s, int until) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      held[t] = (Wv::Sh::place(2 * t) < until ? 0xffffu : 0u) |
+                (Wv::Sh::place(2 * t + 1) < until ? 0xffff0000u : 0u);
+    all_finite = false;
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < Wv::NJ; ++j) {
+      const Weights x = cleared(s, j);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) odd |= Wv::finite(x.w[t]) != x.w[t];
+    }
+    asm volatile("" ::: "memory");  // read again afterwards, not kept
+    return odd;
+  }
+  __device__ void only_finite(int) {
+    all_finite = true;
+    asm volatile("" ::: "memory");
+  }
 };
 
 template <class T, int DH, int MODE>
@@ -890,20 +1019,39 @@ __global__ __launch_bounds__(64 * kWaves, 2) void chunk_kernel(Call a) {
   Job job;
   Share share;
   if constexpr (MODE == kShared) {
-    u64* before = reinterpret_cast<u64*>(lds + 2 * Ch::kBytes);
+    u64* before = reinterpret_cast<u64*>(lds + 4 * Ch::kTile);
     if (threadIdx.x == 0) nothing_noted(a, group);
     share = share_of(a, group, Ch::kRows, Ch::kTokens, 4, before, before + kMostShared + 1);
-    if (!share.next(a, Ch::kRows, Ch::kTokens, job)) return;
   } else {
     if (group >= (unsigned)a.items) return;
     const int x = group / (unsigned)c.kv_heads;
     job.head = group - x * (unsigned)c.kv_heads;
-    job.s = sequence_at(a, find_tile(a, x, Ch::kRows, job.tile));
+    job.s = same(sequence_at(a, find_tile(a, x, Ch::kRows, job.tile)));
     job.from = 0, job.to = 1 << 30, job.slot = -1;
     if ((i64)job.tile * Ch::kRows >= (i64)job.s.queries * a.group) return;
   }
-  const int token_of = threadIdx.x / Ch::kParts, part_of = threadIdx.x % Ch::kParts;
+  const unsigned lds_at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+  // the parts that the lane brings of its wavefront's 16 tokens
+  unsigned bring_k[Ch::kLoads], bring_v[Ch::kLoads];
+#pragma unroll
+  for (int i = 0; i < Ch::kLoads; ++i) {
+    const int token = (i * 64 + lane) / Ch::kParts, part = lane % Ch::kParts;
+    bring_k[i] = token * Ch::kToken + Ch::key_part(token, part) * 16;
+    bring_v[i] = token * Ch::kToken + Ch::value_part(token, part) * 16;
+  }
+  // what it reads: key r's parts 4 p + g, and elements j of value 4 g + r / 4
+  unsigned key_at[Sh::KC], value_at[Ch::kTurns];
+#pragma unroll
+  for (int p = 0; p < Sh::KC; ++p) key_at[p] = r * Ch::kToken + Ch::key_part(r, 4 * p + g) * 16;
+#pragma unroll
+  for (int j = 0; j < Ch::kTurns; ++j) {
+    const int token = 4 * g + (r >> 2), part = 2 * j + (r >> 1 & 1);
+    value_at[j] = token * Ch::kToken + Ch::value_part(token, part) * 16 + (r & 1) * 8;
+  }
   while (true) {
+    if constexpr (MODE == kShared) {
+      if (!share.next(a, Ch::kRows, Ch::kTokens, job)) return;
+    }
     const Sequence& s = job.s;
     const int M = s.queries * a.group, row0 = job.tile * Ch::kRows, mine0 = row0 + wave * 32;
     Queries<MT> q;
@@ -911,9 +1059,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void chunk_kernel(Call a) {
     Wv w;
     w.clear();
     if (s.exists) {
-      // positions that some query of the workgroup attends end at `end`, those that all of the
-      // wavefront's do at `full`
-      const int q_first = (unsigned)min(mine0, M - 1) / (unsigned)a.group;
+      // positions that some query of the workgroup attends end at `end`, those that all do at `full`
+      const int q_first = (unsigned)row0 / (unsigned)a.group;
       const int q_last = (unsigned)min(row0 + Ch::kRows - 1, M - 1) / (unsigned)a.group;
       const int end = a.mask ? s.end : min(s.end, s.prefix + q_last + 1);
       const int full = min(end, a.mask ? s.prefix : s.prefix + q_first + 1);
@@ -929,92 +1076,79 @@ __global__ __launch_bounds__(64 * kWaves, 2) void chunk_kernel(Call a) {
         const int first = min(tile * Ch::kTokens + lane * 16, end - 1);
         ids = page_of(c, table[first >> c.page_shift]);
       };
-      u32x4 kept_k[Ch::kMine], kept_v[Ch::kMine];
       int id[4];
-      const auto fetch = [&](int tile, int block) {  // block: the tile's first among the lanes' 64
+      const auto fetch = [&](int tile, int block, int buffer) {  // block: the tile's first of the lanes' 64
 #pragma unroll
         for (int b = 0; b < 4; ++b) id[b] = __builtin_amdgcn_readlane(ids, block + b);
-        const int in_page = (1 << c.page_shift) - 1;
+        const int page = max(__builtin_amdgcn_readlane(ids, block + wave), 0);
+        const i64 from = (i64)page * c.page_bytes +
+                         ((tile * Ch::kTokens + wave * 16) & ((1 << c.page_shift) - 1)) * Ch::kToken;
+        const unsigned here = lds_at + buffer * 2 * Ch::kTile + wave * 16 * Ch::kToken;
 #pragma unroll
-        for (int i = 0; i < Ch::kMine; ++i) {
-          const int token = token_of + i * Ch::kStep;
-          const int b = (wave * 64 / Ch::kParts + i * Ch::kStep) >> 4;  // the same for the wavefront
-          const int page = max(__builtin_amdgcn_readlane(ids, block + b), 0);
-          const i64 at = (i64)page * c.page_bytes +
-                         ((tile * Ch::kTokens + token) & in_page) * (DH * 2) + part_of * 16;
-          kept_k[i] = *reinterpret_cast<const u32x4*>(k_head + at);
-          kept_v[i] = *reinterpret_cast<const u32x4*>(v_head + at);
-        }
-      };
-      const auto put = [&](int buffer) {
-        char* at = lds + buffer * Ch::kBytes + part_of * 16;
-#pragma unroll
-        for (int i = 0; i < Ch::kMine; ++i) {
-          const int token = token_of + i * Ch::kStep;
-          *reinterpret_cast<u32x4*>(at + token * Ch::kKey) = kept_k[i];
-          *reinterpret_cast<u32x4*>(at + Ch::kValues + token * Ch::kValue) = kept_v[i];
+        for (int i = 0; i < Ch::kLoads; ++i) {
+          load_to_lds(k_head + from, bring_k[i], here + i * 1024);
+          load_to_lds(v_head + from, bring_v[i], here + Ch::kTile + i * 1024);
         }
       };
       int block = 0;
       if (job.from < to) {
         pages_from(job.from);
-        fetch(job.from, 0);
-        put(0);
+        fetch(job.from, 0, 0);
+        wait_loads();
         __syncthreads();
       }
-      int buffer = 0;
-      for (int tile = job.from; tile < to; ++tile) {
-        int now[4];
+      int buffer = 0, tile = job.from;
+      // first the tiles that all of it attends, in a loop without what the others need
+      const auto run = [&](auto all) {
+        for (; tile < to && (!all || ((tile + 1) * Ch::kTokens <= full &&
+                                      min(min(id[0], id[1]), min(id[2], id[3])) >= 0)); ++tile) {
+          int now[4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) now[b] = id[b];
-        if (tile + 1 < to) {
-          block += 4;
-          if (block == 64) {
-            block = 0;
-            pages_from(tile + 1);
+          for (int b = 0; b < 4; ++b) now[b] = id[b];
+          if (tile + 1 < to) {
+            block += 4;
+            if (block == 64) {
+              block = 0;
+              pages_from(tile + 1);
+            }
+            fetch(tile + 1, block, buffer ^ 1);
           }
-          fetch(tile + 1, block);
+          const char* keys = lds + buffer * 2 * Ch::kTile;
+          TurnedValues<T, DH> values;
+#pragma unroll
+          for (int j = 0; j < Ch::kTurns; ++j) values.at[j] = keys + Ch::kTile + value_at[j];
+          const int first = tile * Ch::kTokens + 4 * g;
+          if (mine0 < M)
+            w.template fold<2, decltype(all)::value>(
+                a.scale_log2,
+                [&](int t) {
+                  typename Wv::Keys x;
+#pragma unroll
+                  for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int p = 0; p < Sh::KC; ++p)
+                      x.k[h][p] = *reinterpret_cast<const u32x4*>(keys + key_at[p] +
+                                                                  (32 * t + 16 * h) * Ch::kToken);
+                  return x;
+                },
+                values, [&](int t, int m) { return q.template seen<N>(a, s, m, first + 32 * t); },
+                [&](int t) { return end - first - 32 * t; },
+                [&](int t, int half) { return now[2 * t + half] < 0; });
+          buffer ^= 1;
+          wait_loads();
+          __syncthreads();
         }
-        const char* keys = lds + buffer * Ch::kBytes + r * Ch::kKey + g * 16;
-        const char* values = lds + buffer * Ch::kBytes + Ch::kValues + 4 * g * Ch::kValue + r * (Sh::W * 2);
-        const int first = tile * Ch::kTokens + 4 * g;
-        if (mine0 < M)
-          w.template fold<2>(
-              a.scale_log2, (tile + 1) * Ch::kTokens <= full,
-              [&](int t) {
-                typename Wv::Keys x;
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                  for (int p = 0; p < Sh::KC; ++p)
-                    x.k[h][p] = *reinterpret_cast<const u32x4*>(keys + (32 * t + 16 * h) * Ch::kKey + p * 64);
-                return x;
-              },
-              [&](int t) {
-                typename Wv::Values x;
-#pragma unroll
-                for (int e = 0; e < N; ++e)
-                  load_words<Sh::RW>(values + (32 * t + Sh::place(e)) * Ch::kValue, x.v[e][0]);
-                return x;
-              },
-              [&](int t, int m) { return q.template seen<N>(a, s, m, first + 32 * t); },
-              [&](int t) { return end - first - 32 * t; },
-              [&](int t, int half) { return now[2 * t + half] < 0; });
-        buffer ^= 1;
-        if (tile + 1 < to) put(buffer);
-        __syncthreads();
-      }
+      };
+      run(std::true_type());
+      run(std::false_type());
     }
     const i64 slot = MODE == kShared && job.slot >= 0 ? ((i64)group * 2 + job.slot) * Ch::kRows : -1;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        finish<T, DH, MT>(a, q, m, i, slot < 0 ? -1 : slot + wave * 32 + 16 * m + r, s.exists, w.acc[m],
-                          i, w.sum[m][0], w.top[m]);
+      finish_turned<T, DH, MT>(a, q, m, slot < 0 ? -1 : slot + wave * 32 + 16 * m + r, s.exists, w.acc[m],
+                               w.sum[m][0], w.top[m]);
     if constexpr (MODE != kShared) return;
     if (threadIdx.x == 0) note(a, group, job, row0, M);
-    if (!share.next(a, Ch::kRows, Ch::kTokens, job)) return;
   }
 }
 
@@ -1152,7 +1286,7 @@ int by_rows(const Call& a, const Plan& p, hipStream_t stream) {
     if (p.rows == 32) rc = by_mode<T, DH, 2>(a, p, stream);
   }
   if constexpr (kSize == 2 && (DH == 64 || DH == 128)) {
-    constexpr size_t kTiles = 2 * Chunk<T, DH>::kBytes;
+    constexpr size_t kTiles = 4 * Chunk<T, DH>::kTile;
     if (p.rows == 128)
       rc = p.mode == kGroup ? launch(chunk_kernel<T, DH, kGroup>, a, p.groups, kTiles, stream)
                             : launch(chunk_kernel<T, DH, kShared>, a, p.groups, kTiles + kShareBytes, stream);
