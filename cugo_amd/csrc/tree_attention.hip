@@ -72,7 +72,8 @@ struct Call {
   char* out;
   float* part_o;   // shared-out items' parts: [workgroups, 2, rows, dh]
   float* part_ml;  // [workgroups, 2, rows, 2]: maximum (base 2) and sum
-  int* notes;      // [workgroups, kNote]
+  int* begun;      // [items]: 1 + the workgroup that began an item others went on with, or 0
+  int* ended;      // [workgroups]: whether it ended an item that others began
   int tokens, n, each;  // each: queries a sequence without offsets
   int heads, group, words;
   int items;       // (tile of rows, key head), at most so many
@@ -485,33 +486,35 @@ __device__ __forceinline__ Sequence same(Sequence s) {
   return s;
 }
 
-// The sequence of tile x and the tile's place in it.  With offsets, sequence i's tiles begin at
-// floor((offsets[i] - offsets[0]) group / rows a tile) + i, which leaves room for what each needs.
+// Tiles of rows over all sequences.  With offsets, sequence i's begin at floor((offsets[i] -
+// offsets[0]) group / rows a tile) + i, which leaves room for what each needs.
+__device__ __forceinline__ int tiles_before(const Call& a, int i, int rows, i64 origin) {
+  if (a.offsets == nullptr) return i * (int)(((i64)a.each * a.group + rows - 1) / rows);
+  const i64 o = a.offsets[i] - origin;
+  const i64 held = o < 0 ? 0 : o > a.tokens ? a.tokens : o;
+  return (int)((unsigned)(held * a.group) / (unsigned)rows) + i;
+}
+// The sequence of tile x and the tile's place in it.
 __device__ __forceinline__ int find_tile(const Call& a, int x, int rows, int& tile) {
   if (a.offsets == nullptr) {
-    const int each = (int)(((i64)a.each * a.group + rows - 1) / rows);
+    const int each = tiles_before(a, 1, rows, 0);
     const int i = (unsigned)x / (unsigned)each;
     tile = x - i * each;
     return i;
   }
   const int lane = threadIdx.x & 63;
   const i64 origin = a.offsets[0];
-  const auto start = [&](int i) {
-    const i64 o = a.offsets[i] - origin;
-    const i64 held = o < 0 ? 0 : o > a.tokens ? a.tokens : o;
-    return (int)((unsigned)(held * a.group) / (unsigned)rows) + i;
-  };
   // 64 probes a turn; the last that starts at or before x
   int low = 0, span = a.n;
   while (span > 1) {
     const int step = (span + 63) >> 6;
-    const bool before = lane * step < span && start(low + lane * step) <= x;
+    const bool before = lane * step < span && tiles_before(a, low + lane * step, rows, origin) <= x;
     const int last = 63 - __clzll((long long)(__ballot(before) | 1));
     span = min(step, span - last * step);
     low += last * step;
   }
   low = same(low);
-  tile = same(x - start(low));
+  tile = same(x - tiles_before(a, low, rows, origin));
   return low;
 }
 
@@ -520,7 +523,6 @@ __device__ __forceinline__ int find_tile(const Call& a, int x, int rows, int& ti
 // An item that a border cuts has parts, joined by a second launch.  Every workgroup sums up the
 // sequences' work for itself (kMostShared of them at most).
 constexpr int kMostShared = 1024;
-constexpr int kNote = 8;
 
 // before[i]: the work of the sequences before i; before[n]: all of it.  `scratch`: kWaves numbers.
 __device__ __forceinline__ void sum_work(const Call& a, int rows, int tokens, u64* before, u64* scratch) {
@@ -559,6 +561,7 @@ __device__ __forceinline__ void sum_work(const Call& a, int rows, int tokens, u6
 // One workgroup's (or wavefront's) work on an item.
 struct Job {
   Sequence s;
+  int sequence;
   int head, tile;  // the key head; the tile of rows
   int from, to;    // tiles of tokens
   int slot;        // -1: the whole item; 0: its end or middle, 1: its beginning
@@ -579,6 +582,7 @@ struct Share {
       else high = mid;
     }
     low = same(low);
+    job.sequence = low;
     job.s = same(sequence_at(a, low));
     const int tiles = (int)(((i64)job.s.queries * a.group + rows - 1) / rows);
     const int each = max(1, (job.s.end + tokens - 1) / tokens);
@@ -617,19 +621,14 @@ __device__ __forceinline__ Share share_of(const Call& a, unsigned group, int row
   return s;
 }
 
-// What a workgroup tells the launch that joins: [0] it began an item that others went on with, of
-// which [1] first query, [2] first row, [3] rows, [4] key head; [5] it ended an item that others
-// began.
-__device__ __forceinline__ void note(const Call& a, unsigned group, const Job& job, int row0, int M) {
-  int* at = a.notes + group * kNote;
-  if (job.slot == 1) {
-    at[0] = 1, at[1] = job.s.first, at[2] = row0, at[3] = M, at[4] = job.head;
-  } else if (job.slot == 0) {
-    at[5] = job.ends;
+// What a workgroup tells the launch that joins of a job.
+__device__ __forceinline__ void note(const Call& a, unsigned group, const Job& job, int rows) {
+  if (job.slot == 0) {
+    a.ended[group] = job.ends;
+  } else {
+    const int x = tiles_before(a, job.sequence, rows, a.offsets ? a.offsets[0] : 0) + job.tile;
+    a.begun[x * a.c.kv_heads + job.head] = job.slot == 1 ? (int)group + 1 : 0;
   }
-}
-__device__ __forceinline__ void nothing_noted(const Call& a, unsigned group) {
-  a.notes[group * kNote] = a.notes[group * kNote + 5] = 0;
 }
 
 // Stores W consecutive elements.
@@ -751,7 +750,7 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(Call a) {
   Share share;
   if constexpr (MODE == kShared) {
     u64* before = reinterpret_cast<u64*>(lds + merge_bytes<T, DH, MT>());
-    if (threadIdx.x == 0) nothing_noted(a, group);
+    if (threadIdx.x == 0) a.ended[group] = 0;
     // a tile of tokens each wavefront
     share = share_of(a, group, kRows, KT, kWaves, before, before + kMostShared + 1);
   } else {
@@ -886,7 +885,7 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(Call a) {
       }
     }
     if constexpr (MODE != kShared) return;
-    if (threadIdx.x == 0) note(a, group, job, row0, M);
+    if (threadIdx.x == 0) note(a, group, job, kRows);
     __syncthreads();  // the merge's last readers
   }
 }
@@ -1020,7 +1019,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void chunk_kernel(Call a) {
   Share share;
   if constexpr (MODE == kShared) {
     u64* before = reinterpret_cast<u64*>(lds + 4 * Ch::kTile);
-    if (threadIdx.x == 0) nothing_noted(a, group);
+    if (threadIdx.x == 0) a.ended[group] = 0;
     share = share_of(a, group, Ch::kRows, Ch::kTokens, 4, before, before + kMostShared + 1);
   } else {
     if (group >= (unsigned)a.items) return;
@@ -1148,51 +1147,75 @@ __global__ __launch_bounds__(64 * kWaves, 2) void chunk_kernel(Call a) {
       finish_turned<T, DH, MT>(a, q, m, slot < 0 ? -1 : slot + wave * 32 + 16 * m + r, s.exists, w.acc[m],
                                w.sum[m][0], w.top[m]);
     if constexpr (MODE != kShared) return;
-    if (threadIdx.x == 0) note(a, group, job, row0, M);
+    if (threadIdx.x == 0) note(a, group, job, Ch::kRows);
   }
 }
 
-// Joins the parts of the item that a workgroup began: four elements a lane, DH / 4 lanes a row.
+// Joins the parts of items: a row a wavefront, whose lanes have a part's maximum and sum each, then
+// four elements of every 64 / (DH / 4)-th part.
 template <class T, int DH>
-__global__ __launch_bounds__(256) void join_kernel(Call a, int rows) {
+__global__ __launch_bounds__(64 * kWaves) void join_kernel(Call a, int rows, int groups) {
   using S = typename T::storage;
-  constexpr int kLanes = DH / 4;
-  const unsigned group = blockIdx.x;
-  const int* said = a.notes + group * kNote;
-  if (!said[0]) return;
+  constexpr int kLanes = DH / 4, kSides = 64 / kLanes;
   const int lane = threadIdx.x & 63;
-  int parts = 2;  // with the one that ends it
-  for (unsigned base = group + 1; base < gridDim.x; base += 64) {
-    const bool ends = base + lane < gridDim.x && a.notes[(base + lane) * kNote + 5];
-    const unsigned long long ballot = __ballot(ends);
-    if (ballot) {
-      parts += (int)(base - group - 1) + __builtin_ctzll(ballot);
+  const int x = blockIdx.x / (unsigned)a.c.kv_heads, key_head = blockIdx.x - x * a.c.kv_heads;
+  int tile;
+  const Sequence s = sequence_at(a, find_tile(a, x, rows, tile));
+  const int M = s.queries * a.group, row0 = tile * rows;
+  if (row0 >= M) return;
+  const int begun = a.begun[blockIdx.x];
+  if (begun == 0) return;
+  const int group = begun - 1;
+  int parts = 1;
+  for (int base = group + 1; base < groups; base += 64) {
+    const u64 ends = __ballot(base + lane < groups && a.ended[min(base + lane, groups - 1)]);
+    if (ends) {
+      parts = base - group + __builtin_ctzll(ends) + 1;
       break;
     }
   }
-  const int first = said[1], row0 = said[2], M = said[3], key_head = said[4];
-  const int at = threadIdx.x % kLanes * 4;
-  for (int row = blockIdx.y * (256 / kLanes) + threadIdx.x / kLanes; row < rows && row0 + row < M;
-       row += gridDim.y * (256 / kLanes)) {
-    const auto slot = [&](int k) { return ((i64)(group + k) * 2 + (k == 0)) * rows + row; };
+  const auto slot = [&](int k, int row) { return ((i64)(group + k) * 2 + (k == 0)) * rows + row; };
+  for (int row = blockIdx.y * kWaves + (threadIdx.x >> 6); row < rows && row0 + row < M;
+       row += gridDim.y * kWaves) {
     float top = kNegInf;
-    for (int k = 0; k < parts; ++k) top = fmaxf(top, a.part_ml[slot(k) * 2]);
+    for (int k = lane; k < parts; k += 64) top = fmaxf(top, a.part_ml[slot(k, row) * 2]);
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
     float total = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < parts; ++k) {
-      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + slot(k) * 2);
-      const f32x4 y = *reinterpret_cast<const f32x4*>(a.part_o + slot(k) * DH + at);
-      const float less = ml.x == kNegInf ? 0.f : exp2_fast(ml.x - top);
-      total += ml.y * less;
-      o += y * less;
+    const int side = lane / kLanes, at = lane % kLanes * 4;
+    for (int base = 0; base < parts; base += 64) {
+      float less = 0.f;
+      if (base + lane < parts) {
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + slot(base + lane, row) * 2);
+        less = ml.x == kNegInf ? 0.f : exp2_fast(ml.x - top);
+        total += ml.y * less;
+      }
+      const int here = min(64, parts - base);
+#pragma unroll 4
+      for (int k = 0; k < here; k += kSides) {
+        const int mine = k + side;
+        const float weight = __shfl(less, mine & 63);
+        if (mine < here) {
+          const f32x4 y = *reinterpret_cast<const f32x4*>(a.part_o + slot(base + mine, row) * DH + at);
+          o += y * weight;
+        }
+      }
     }
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) total += __shfl_xor(total, off);
+#pragma unroll
+    for (int off = kLanes; off < 64; off <<= 1)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], off);
+    if (side != 0) continue;
     const float scale = total == 0.f ? 0.f : 1.f / total;
     float y[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = o[e] * scale;
     const int query = (unsigned)(row0 + row) / (unsigned)a.group;
     const int head = key_head * a.group + (row0 + row - query * a.group);
-    store_run<S, 4>(reinterpret_cast<S*>(a.out) + ((i64)(first + query) * a.heads + head) * DH + at, y);
+    store_run<S, 4>(reinterpret_cast<S*>(a.out) + ((i64)(s.first + query) * a.heads + head) * DH + at, y);
   }
 }
 
@@ -1248,10 +1271,10 @@ inline int plan(Call* a, int dh, int size, Plan* p) {
 }
 
 inline i64 part_floats(const Plan& p, int dh) { return p.groups * 2 * p.rows * dh; }
-inline i64 part_bytes(const Plan& p, int dh) {
+inline i64 part_bytes(const Plan& p, int dh, i64 items) {
   return p.mode != kShared ? 0
                            : (part_floats(p, dh) + p.groups * 2 * p.rows * 2) * (i64)sizeof(float) +
-                                 p.groups * kNote * (i64)sizeof(int);
+                                 (items + p.groups) * (i64)sizeof(int);
 }
 
 // A launch with more than 64 KiB of LDS has to say so once a device and kernel.
@@ -1292,10 +1315,10 @@ int by_rows(const Call& a, const Plan& p, hipStream_t stream) {
                             : launch(chunk_kernel<T, DH, kShared>, a, p.groups, kTiles + kShareBytes, stream);
   }
   if (rc || p.mode != kShared) return rc;
-  constexpr int kEachRow = 256 / (DH / 4);
-  const int spread = (p.rows + kEachRow - 1) / kEachRow;
-  hipLaunchKernelGGL((join_kernel<T, DH>), dim3((unsigned)p.groups, (unsigned)spread), dim3(256), 0,
-                     stream, a, p.rows);
+  // four rows a workgroup, or as many as make 2,048 workgroups
+  const int most = (p.rows + kWaves - 1) / kWaves, want = 2048 / a.items + 1;
+  hipLaunchKernelGGL((join_kernel<T, DH>), dim3((unsigned)a.items, (unsigned)(want < most ? want : most)),
+                     dim3(64 * kWaves), 0, stream, a, p.rows, (int)p.groups);
   return (int)hipGetLastError();
 }
 
@@ -1349,7 +1372,7 @@ inline int view(const CugoTreeAttention* p, Call* a) {
   a->scale_log2 = scale * 1.4426950408889634f;  // softmax in base 2
   a->out = static_cast<char*>(p->out);
   a->part_o = a->part_ml = nullptr;
-  a->notes = nullptr;
+  a->begun = a->ended = nullptr;
   return 0;
 }
 
@@ -1364,7 +1387,7 @@ int64_t cugo_tree_attention_workspace(const CugoTreeAttention* call) {
   Plan p;
   if (view(call, &a) || a.tokens == 0) return 0;
   const int dh = (int)call->cache->dh;
-  return plan(&a, dh, element_size(call->cache->dtype), &p) ? 0 : part_bytes(p, dh);
+  return plan(&a, dh, element_size(call->cache->dtype), &p) ? 0 : part_bytes(p, dh, a.items);
 }
 
 int cugo_tree_attention(const CugoTreeAttention* call, void* workspace, int64_t workspace_bytes,
@@ -1376,13 +1399,14 @@ int cugo_tree_attention(const CugoTreeAttention* call, void* workspace, int64_t 
   if (a.tokens == 0) return 0;
   const int dh = (int)call->cache->dh;
   if (const int bad = plan(&a, dh, element_size(call->cache->dtype), &p)) return bad;
-  if (const int64_t need = part_bytes(p, dh)) {
+  if (const int64_t need = part_bytes(p, dh, a.items)) {
     if (!workspace) return -1;
     if (!aligned16(workspace)) return -4;
     if (workspace_bytes < need) return -5;
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + part_floats(p, dh);
-    a.notes = reinterpret_cast<int*>(a.part_ml + p.groups * 2 * p.rows * 2);
+    a.begun = reinterpret_cast<int*>(a.part_ml + p.groups * 2 * p.rows * 2);
+    a.ended = a.begun + a.items;
   }
   switch (call->cache->dtype) {
     case CUGO_DTYPE_BF16:
