@@ -41,7 +41,7 @@ struct BF16 {
   using storage = __bf16;
   typedef __bf16 vec __attribute__((ext_vector_type(8)));
   static constexpr uint32_t kInf = 0x7f80u;
-  __device__ static f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+  __device__ __forceinline__ static f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vec, a),
                                                    __builtin_bit_cast(vec, b), c, 0, 0, 0);
   }
@@ -50,7 +50,7 @@ struct F16 {
   using storage = _Float16;
   typedef _Float16 vec __attribute__((ext_vector_type(8)));
   static constexpr uint32_t kInf = 0x7c00u;
-  __device__ static f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+  __device__ __forceinline__ static f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vec, a),
                                                   __builtin_bit_cast(vec, b), c, 0, 0, 0);
   }
@@ -125,9 +125,9 @@ struct Shape {
   static constexpr int RW = W * E / 4;             // words a run
   static constexpr int NJ = DH / 16;               // 16 x 16 tiles of O^T
   // The place of a lane's token e in the tile, after 4 g.
-  __device__ static constexpr int place(int e) { return e + (e >= 4 ? 12 : 0); }
+  __device__ __forceinline__ static constexpr int place(int e) { return e + (e >= 4 ? 12 : 0); }
   // The element that row 4 g + i of tile j of O^T is.
-  __device__ static int element(int j, int row) { return j / W * 16 * W + W * row + j % W; }
+  __device__ __forceinline__ static int element(int j, int row) { return j / W * 16 * W + W * row + j % W; }
 };
 
 // The parts of a tile's keys and values that a lane holds; at0 and at1: its first and second 16 tokens.
@@ -178,7 +178,7 @@ struct Wave {
     static constexpr bool kInPlace = true;
     uint32_t v[N][Sh::H][Sh::RW];
     // Elements j of the lane's N tokens.
-    __device__ Weights column(int, int j) const {
+    __device__ __forceinline__ Weights column(int, int j) const {
       Weights y;
       const int h = j / Sh::W, e = j % Sh::W;
       if constexpr (Sh::kWide) {
@@ -192,9 +192,9 @@ struct Wave {
       }
       return y;
     }
-    // Zeros for the tokens from `until` on; whether an infinity or NaN is left.
-    __device__ bool clear(int, int until) {
-      bool odd = false;
+    // Zeros for the tokens from `until` on after the lane's first; whether an infinity or NaN is left.
+    __device__ __forceinline__ bool clear(int until) {
+      uint32_t odd = 0;
 #pragma unroll
       for (int t = 0; t < N; ++t)
 #pragma unroll
@@ -202,12 +202,12 @@ struct Wave {
 #pragma unroll
           for (int e = 0; e < Sh::RW; ++e) {
             v[t][h][e] = Sh::place(t) < until ? v[t][h][e] : 0u;
-            odd |= finite(v[t][h][e]) != v[t][h][e];
+            odd |= odd_bits(v[t][h][e]);
           }
-      return odd;
+      return odd & kSigns;
     }
-    __device__ Weights cleared(int s, int j) const { return column(s, j); }
-    __device__ void only_finite(int) {
+    __device__ __forceinline__ Weights cleared(int j) const { return column(0, j); }
+    __device__ __forceinline__ void only_finite() {
 #pragma unroll
       for (int t = 0; t < N; ++t)
 #pragma unroll
@@ -217,7 +217,7 @@ struct Wave {
     }
   };
 
-  __device__ void clear() {
+  __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       top[m] = kNegInf;
@@ -228,7 +228,7 @@ struct Wave {
   }
 
   // d[e]: the product of query lane & 15 with the lane's token e.
-  __device__ static void scores(const Keys& x, const u32x4 (&qm)[KC], float (&d)[N]) {
+  __device__ __forceinline__ static void scores(const Keys& x, const u32x4 (&qm)[KC], float (&d)[N]) {
 #pragma unroll
     for (int a = 0; a < KL; ++a) {
       f32x4 s = {0.f, 0.f, 0.f, 0.f};
@@ -248,7 +248,7 @@ struct Wave {
     }
   }
 
-  __device__ static Weights pack(const float (&p)[N]) {
+  __device__ __forceinline__ static Weights pack(const float (&p)[N]) {
     Weights x;
     if constexpr (Sh::kWide) {
 #pragma unroll
@@ -264,7 +264,7 @@ struct Wave {
     return x;
   }
   // c += A P^T for the A operand `a` of N tokens.
-  __device__ static f32x4 product(const Weights& a, const Weights& p, f32x4 c) {
+  __device__ __forceinline__ static f32x4 product(const Weights& a, const Weights& p, f32x4 c) {
     if constexpr (Sh::kWide) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -276,11 +276,15 @@ struct Wave {
     }
   }
   // SUB tiles' share of every query.  kAll: every query attends every token, and each has a page.  keys(s): the lane's parts of tile s's keys; values.column(s, j):
-  // its operand for elements j of the values.  Otherwise seen(s, m) has the bits of the lane's tokens
-  // that query m attends, positions from inside(s) on after the tile's 4 g are past the row's end, and
-  // the tokens of half h of a tile with bad(s, h) have no page.
-  template <int SUB, bool kAll, class KeysOf, class V, class Seen, class Inside, class Bad>
-  __device__ __forceinline__ void fold(float scale, KeysOf keys, V& values, Seen seen, Inside inside, Bad bad) {
+  // its operand for elements j of the values.  Otherwise window(m) has a bit for each position of
+  // the tile (one then) that query m attends, positions from `inside` on are past the row's end, and
+  // bit h of `bad` says that the tile's half h has no page.
+  template <int SUB, bool kAll, class KeysOf, class V, class Window>
+  __device__ __forceinline__ void fold(float scale, KeysOf keys, V& values, Window window, int inside,
+                                       unsigned bad) {
+    static_assert(kAll || SUB == 1, "tiles with masks come alone");
+    const int g = threadIdx.x >> 4 & 3;
+    uint32_t seen[MT];
     float d[SUB][MT][N], most[MT];
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
@@ -289,18 +293,25 @@ struct Wave {
       for (int m = 0; m < MT; ++m) scores(x, q[m], d[s][m]);
       if constexpr (SUB > 1) __builtin_amdgcn_sched_barrier(0);  // one tile's keys in registers
     }
-    if constexpr (!kAll)
+    if constexpr (!kAll) {
+      // The scores read here, in the products' block: where the masks' branches came between, ROCm 7.2's
+      // compiler left two wait states of the eight (float32: ten) that a matrix instruction's result
+      // needs, and the last score read was an older one.
 #pragma unroll
-      for (int s = 0; s < SUB; ++s)
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          const uint32_t bits = seen(s, m);
+        for (int e = 0; e < N; ++e) asm volatile("" : "+v"(d[0][m][e]));
 #pragma unroll
-          for (int e = 0; e < N; ++e) {
-            const float x = bad(s, e / 4) ? __builtin_nanf("") : d[s][m][e];
-            d[s][m][e] = bits >> e & 1 ? x : kNegInf;
-          }
+      for (int m = 0; m < MT; ++m) {
+        const uint32_t w = (uint32_t)window(m) >> 4 * g;
+        seen[m] = (w & 0xfu) | (N == 8 ? w >> 12 & 0xf0u : 0u);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float x = bad >> e / 4 & 1 ? __builtin_nanf("") : d[0][m][e];
+          d[0][m][e] = seen[m] >> e & 1 ? x : kNegInf;
         }
+      }
+    }
     bool more = false;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
@@ -343,15 +354,15 @@ struct Wave {
     for (int s = 0; s < SUB; ++s) {
       if constexpr (!kAll) {
         // tokens past the row's end hold anything; among the others infinities and NaN are rare
-        if (__ballot(values.clear(s, inside(s)))) {
-          fold_odd(values, s, [&](int m) { return seen(s, m); });
-          values.only_finite(s);
+        if (__ballot(values.clear(inside - 4 * g))) {
+          fold_odd(values, seen);
+          values.only_finite();
         }
         if constexpr (!V::kInPlace) {
 #pragma unroll
           for (int j = 0; j < NJ; ++j) {
             __builtin_amdgcn_sched_barrier(0);
-            const Weights x = values.cleared(s, j);
+            const Weights x = values.cleared(j);
 #pragma unroll
             for (int m = 0; m < MT; ++m) acc[m][j] = product(x, w[s][m], acc[m][j]);
           }
@@ -367,19 +378,25 @@ struct Wave {
     }
   }
 
-  __device__ static constexpr uint32_t inf_bits() {
+  __device__ __forceinline__ static constexpr uint32_t inf_bits() {
     if constexpr (Sh::kWide) return 0x7f800000u;
     else return T::kInf;
   }
+  // A sign bit of this is set where the word holds an infinite number or NaN.
+  static constexpr uint32_t kSigns = Sh::kWide ? 0x80000000u : 0x80008000u;
+  __device__ __forceinline__ static uint32_t odd_bits(uint32_t w) {
+    constexpr uint32_t both = Sh::kWide ? 1u : 0x10001u, exponent = inf_bits() * both;
+    return (w & exponent) + (0x8000u * (Sh::kWide ? 0x10000u : both) - exponent);
+  }
   // The word with its infinite numbers and NaN as zeros.
-  __device__ static uint32_t finite(uint32_t w) {
+  __device__ __forceinline__ static uint32_t finite(uint32_t w) {
     if constexpr (Sh::kWide) return (w & inf_bits()) == inf_bits() ? 0u : w;
     if ((w & inf_bits()) == inf_bits()) w &= 0xffff0000u;
     if ((w >> 16 & inf_bits()) == inf_bits()) w &= 0x0000ffffu;
     return w;
   }
   // 1 where a value is an infinity of the sign `negative`, or NaN (which is both), else 0.
-  __device__ static Weights infinite(const Weights& a, bool negative) {
+  __device__ __forceinline__ static Weights infinite(const Weights& a, bool negative) {
     float y[N];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -398,22 +415,21 @@ struct Wave {
     return pack(y);
   }
   // What infinite values and NaN bring to the queries that attend them.
-  template <class V, class Seen>
-  __device__ void fold_odd(V& values, int s, Seen seen) {
+  template <class V>
+  __device__ __forceinline__ void fold_odd(V& values, const uint32_t (&seen)[MT]) {
     Weights who[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      const uint32_t bits = seen(m);
       float yes[N];
 #pragma unroll
-      for (int e = 0; e < N; ++e) yes[e] = bits >> e & 1 ? 1.f : 0.f;
+      for (int e = 0; e < N; ++e) yes[e] = seen[m] >> e & 1 ? 1.f : 0.f;
       who[m] = pack(yes);
     }
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       // one after another: interleaved, this rare path would decide the kernel's registers
       __builtin_amdgcn_sched_barrier(0);
-      const Weights a = values.cleared(s, j), positive = infinite(a, false), negative = infinite(a, true);
+      const Weights a = values.cleared(j), positive = infinite(a, false), negative = infinite(a, true);
       const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
@@ -428,23 +444,27 @@ struct Wave {
   }
 };
 
-// Bits of the N positions from `at` on that a query may attend: before `limit` and (with a mask)
-// before its prefix or set in its mask.
-template <int N>
-__device__ __forceinline__ uint32_t seen_bits(int at, int limit, int prefix, const u64* mask, int words) {
-  uint32_t bits = (1u << N) - 1;
+// The low `n` bits set (n <= 0: none, n >= 64: all).
+__device__ __forceinline__ u64 low_bits(int n) {
+  return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
+}
+
+// Which of the 64 positions from `at` on a query may attend: those before `limit`, with a mask those
+// before its prefix or set in it.  (`at`, `limit` and `prefix` are the same for a tile, or nearly.)
+__device__ __forceinline__ u64 window_of(int at, int limit, int prefix, const u64* mask, int words) {
+  u64 bits = low_bits(limit - at);
   if (mask != nullptr) {
     const int b = at - prefix;
-    if (b > -N) {
-      const int first = b < 0 ? 0 : b, word = first >> 6, shift = first & 63;
+    if (b >= 0) {
+      const int word = b >> 6, shift = b & 63;
       u64 x = word < words ? mask[word] >> shift : 0;
-      if (shift > 64 - N && word + 1 < words) x |= mask[word + 1] << (64 - shift);
-      if (b < 0) x = x << -b | ((1ull << -b) - 1);
-      bits &= (uint32_t)x;
+      if (shift != 0 && word + 1 < words) x |= mask[word + 1] << (64 - shift);
+      bits &= x;
+    } else if (b > -64) {
+      bits &= (words > 0 ? mask[0] << -b : 0) | low_bits(-b);
     }
   }
-  const int left = limit - at;
-  return left >= N ? bits : left <= 0 ? 0u : bits & ((1u << left) - 1);
+  return bits;
 }
 
 // A sequence as its wavefronts see it.
@@ -476,11 +496,11 @@ __device__ __forceinline__ Sequence sequence_at(const Call& a, int i) {
 
 // What is the same in every lane, in scalar registers.
 __device__ __forceinline__ int same(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ u64 same(u64 x) {
-  return (u64)(unsigned)same((int)(x >> 32)) << 32 | (unsigned)same((int)x);
+__device__ __forceinline__ i64 same(i64 x) {
+  return (i64)((u64)(unsigned)same((int)(x >> 32)) << 32 | (unsigned)same((int)x));
 }
 __device__ __forceinline__ Sequence same(Sequence s) {
-  s.first = same(s.first), s.queries = same(s.queries), s.row = (i64)same((u64)s.row);
+  s.first = same(s.first), s.queries = same(s.queries), s.row = same(s.row);
   s.length = same(s.length), s.prefix = same(s.prefix), s.end = same(s.end);
   s.exists = same((int)s.exists);
   return s;
@@ -519,32 +539,33 @@ __device__ __forceinline__ int find_tile(const Call& a, int x, int rows, int& ti
 }
 
 // Sharing out: the work of all items (a tile of rows over one key head) in a row, an item's being its
-// sequence's tiles of tokens; workgroup b of B does what lies between W b / B and W (b + 1) / B.
+// sequence's tiles of tokens; each of the workgroups does as much of it, in order.
 // An item that a border cuts has parts, joined by a second launch.  Every workgroup sums up the
 // sequences' work for itself (kMostShared of them at most).
 constexpr int kMostShared = 1024;
 
 // before[i]: the work of the sequences before i; before[n]: all of it.  `scratch`: kWaves numbers.
-__device__ __forceinline__ void sum_work(const Call& a, int rows, int tokens, u64* before, u64* scratch) {
+__device__ __forceinline__ void sum_work(const Call& a, int rows, int tokens, unsigned* before,
+                                         unsigned* scratch) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  u64 carry = 0;
+  unsigned carry = 0;
   for (int base = 0; base < a.n; base += 64 * kWaves) {
     const int i = base + threadIdx.x;
-    u64 x = 0;
+    unsigned x = 0;
     if (i < a.n) {
       const Sequence s = sequence_at(a, i);
       const int tiles = (int)(((i64)s.queries * a.group + rows - 1) / rows);
-      x = (u64)tiles * a.c.kv_heads * max(1, (s.end + tokens - 1) / tokens);
+      x = (unsigned)tiles * a.c.kv_heads * max(1, (s.end + tokens - 1) / tokens);
     }
-    const u64 mine = x;
+    const unsigned mine = x;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-      const u64 y = __shfl_up(x, off);
+      const unsigned y = __shfl_up(x, off);
       if (lane >= off) x += y;
     }
     if (lane == 63) scratch[wave] = x;
     __syncthreads();
-    u64 total = 0;
+    unsigned total = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
       if (w < wave) x += scratch[w];
@@ -570,8 +591,8 @@ struct Job {
 
 // The jobs of a workgroup in order.
 struct Share {
-  const u64* before;
-  u64 at, end;
+  const unsigned* before;
+  unsigned at, end;
   int n;
   __device__ __forceinline__ bool next(const Call& a, int rows, int tokens, Job& job) {
     if (at >= end) return false;
@@ -586,12 +607,12 @@ struct Share {
     job.s = same(sequence_at(a, low));
     const int tiles = (int)(((i64)job.s.queries * a.group + rows - 1) / rows);
     const int each = max(1, (job.s.end + tokens - 1) / tokens);
-    const u64 offset = at - same(before[low]);
-    const u64 item = offset / (unsigned)each;
+    const unsigned offset = at - (unsigned)same((int)before[low]);
+    const unsigned item = offset / (unsigned)each;
     job.from = same((int)(offset - item * each));
-    job.to = same((int)min((u64)each, job.from + (end - at)));
+    job.to = same((int)min((unsigned)each, job.from + (end - at)));
     job.head = same((int)(item / (unsigned)tiles));
-    job.tile = same((int)(item - (u64)job.head * tiles));
+    job.tile = same((int)(item - (unsigned)job.head * tiles));
     job.ends = job.to == each;
     job.slot = job.from > 0 ? 0 : job.ends ? -1 : 1;
     at += job.to - job.from;
@@ -607,17 +628,18 @@ __device__ __forceinline__ unsigned in_order() {
 }
 
 __device__ __forceinline__ Share share_of(const Call& a, unsigned group, int rows, int tokens, int least,
-                                 u64* before, u64* scratch) {
+                                          unsigned* before, unsigned* scratch) {
   sum_work(a, rows, tokens, before, scratch);
-  const u64 all = same(before[a.n]);
+  const unsigned all = (unsigned)same((int)before[a.n]);
   // no less than `least` tiles of tokens each, unless there are more items; one at least
-  u64 groups = max(all / (unsigned)least, (u64)a.items);
-  groups = max(min(min(groups, (u64)gridDim.x), all), (u64)1);
+  unsigned groups = max(all / (unsigned)least, (unsigned)a.items);
+  groups = max(min(min(groups, gridDim.x), all), 1u);
+  const unsigned each = all / groups, more = all - each * groups;  // the first `more` do one more
   Share s;
   s.before = before;
   s.n = a.n;
-  s.at = s.end = 0;
-  if (group < groups) s.at = same(all * group / groups), s.end = same(all * (group + 1) / groups);
+  s.at = (unsigned)same((int)(group < groups ? each * group + min(group, more) : all));
+  s.end = (unsigned)same((int)(group < groups ? s.at + each + (group < more) : all));
   return s;
 }
 
@@ -656,7 +678,7 @@ struct Queries {
   bool real[MT];
   int index[MT];  // in the sequence
   int token[MT], head[MT];
-  __device__ void find(const Call& a, const Sequence& s, int key_head, int row0, int M) {
+  __device__ __forceinline__ void find(const Call& a, const Sequence& s, int key_head, int row0, int M) {
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       const int row = row0 + 16 * m + (threadIdx.x & 15), held = min(row, M - 1);
@@ -667,7 +689,7 @@ struct Queries {
     }
   }
   template <class Wv>
-  __device__ void load(const Call& a, Wv& w) const {
+  __device__ __forceinline__ void load(const Call& a, Wv& w) const {
     using Sh = typename Wv::Sh;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
@@ -680,14 +702,11 @@ struct Queries {
       }
     }
   }
-  // Bits of a lane's N tokens that its query m attends, `at` being the first one's position.
-  template <int N>
-  __device__ uint32_t seen(const Call& a, const Sequence& s, int m, int at) const {
+  // Of the 64 positions from `at` on, those that the lane's query m attends.
+  __device__ __forceinline__ u64 window(const Call& a, const Sequence& s, int m, int at) const {
     const u64* mask = a.mask ? a.mask + (a.mask_rows == a.tokens ? token[m] : index[m]) * (i64)a.words : nullptr;
     const int limit = a.mask ? s.end : min(s.end, s.prefix + index[m] + 1);
-    uint32_t bits = seen_bits<4>(at, limit, s.prefix, mask, a.words);
-    if constexpr (N == 8) bits |= seen_bits<4>(at + 16, limit, s.prefix, mask, a.words) << 4;
-    return bits;
+    return window_of(at, limit, s.prefix, mask, a.words);
   }
 };
 
@@ -733,7 +752,7 @@ template <class T, int DH, int MT>
 constexpr size_t merge_bytes() {
   return (size_t)kWaves * MT * 64 * (DH / 4 + 2) * sizeof(float);
 }
-constexpr size_t kShareBytes = (kMostShared + 1 + kWaves) * sizeof(u64);
+constexpr size_t kShareBytes = (kMostShared + 1 + kWaves) * sizeof(unsigned);
 
 template <class T, int DH, int MT, int MODE>
 __global__ __launch_bounds__(64 * kWaves) void tree_kernel(Call a) {
@@ -749,7 +768,7 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(Call a) {
   Job job;
   Share share;
   if constexpr (MODE == kShared) {
-    u64* before = reinterpret_cast<u64*>(lds + merge_bytes<T, DH, MT>());
+    unsigned* before = reinterpret_cast<unsigned*>(lds + merge_bytes<T, DH, MT>());
     if (threadIdx.x == 0) a.ended[group] = 0;
     // a tile of tokens each wavefront
     share = share_of(a, group, kRows, KT, kWaves, before, before + kMostShared + 1);
@@ -812,7 +831,7 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(Call a) {
       }
       int tile = begin;
       // first the tiles that all of it attends, in a loop without what the others need
-      const auto run = [&](auto all) {
+      const auto run = [&](auto all) __attribute__((always_inline)) {
         for (; tile < to && (!all || (tile < full_tiles && min(id0, id1) >= 0)); tile += step) {
           load_values<T, DH>(v_head + offset(id0, tile * KT), v_head + offset(id1, tile * KT + 16), values.v);
           if (++at == 64) {
@@ -824,12 +843,10 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(Call a) {
             load_keys<T, DH>(k_head + offset(next0, (tile + step) * KT),
                              k_head + offset(next1, (tile + step) * KT + 16), next.k);
           }
-          const int mine = tile * KT + 4 * g;
           w.template fold<1, decltype(all)::value>(
               a.scale_log2, [&](int) -> const typename Wv::Keys& { return now; }, values,
-              [&](int, int m) { return q.template seen<N>(a, s, m, mine); },
-              [&](int) { return end - mine; },
-              [&](int, int half) { return (half ? id1 : id0) < 0; });
+              [&](int m) { return q.window(a, s, m, tile * KT); }, end - tile * KT,
+              (unsigned)(id0 < 0) | (unsigned)(id1 < 0) << 1);
           now = next;
           id0 = next0, id1 = next1;
         }
@@ -890,9 +907,9 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(Call a) {
   }
 }
 
-// Many rows: a workgroup's 4 wavefronts have 32 rows each and share tiles of 64 tokens in LDS, two
-// buffers of them, which global_load_lds_dwordx4 fills without going through registers (1,024
-// consecutive bytes of LDS an instruction; a wavefront brings 16 tokens).  A token's 16-byte parts are
+// Many rows: a workgroup's 4 wavefronts have 32 rows each and share tiles of 64 tokens in LDS, in 64
+// KiB of buffers, which global_load_lds_dwordx4 fills without going through registers (1,024
+// consecutive bytes of LDS an instruction; a wavefront brings a quarter of a tile).  A token's 16-byte parts are
 // exchanged there, so that what is read at once comes from different banks: the same part of 16 keys,
 // or 32 bytes of four values, which ds_read_b64_tr_b16 turns as it reads (four lanes a token's 16
 // elements in, one element's four tokens a lane out; no v_perm_b32).  Elements j of the values are
@@ -902,14 +919,19 @@ struct Chunk {
   static constexpr int kTokens = 64, kRows = 128, MT = 2;
   static constexpr int kToken = DH * 2;             // bytes
   static constexpr int kTile = kTokens * kToken;    // of keys, and of values
+  static constexpr int kBuffers = 2, kLds = kBuffers * 2 * kTile;
+  static_assert(kLds <= 65536, "the loads' place in LDS has 16 bits");
+  static constexpr int kResident = DH == 64 ? 3 : 2;  // workgroups a compute unit
+  static constexpr int kBlocks = kTokens / 16;      // of 16 tokens, which share a page
+  static constexpr int kSub = kTokens / 32;
   static constexpr int kParts = DH / 8;             // 16-byte parts a token
-  static constexpr int kLoads = 16 * kToken / 1024;  // a wavefront's, of keys and of values
-  static_assert(4 * kTile <= 1 << 16, "global_load_lds_dwordx4's place in LDS has 16 bits");
+  static constexpr int kBring = kTokens / kWaves;   // tokens a wavefront brings
+  static constexpr int kLoads = kBring * kToken / 1024;  // of keys, and as many of values
   // Where part `part` of a key or value lies among its token's.
-  __device__ static int key_part(int token, int part) {
+  __device__ __forceinline__ static int key_part(int token, int part) {
     return part ^ (kParts == 16 ? token & 15 : token >> 1 & 7);
   }
-  __device__ static int value_part(int token, int part) {
+  __device__ __forceinline__ static int value_part(int token, int part) {
     return part ^ (kParts == 16 ? token & 3 : token >> 1 & 1) * 2;
   }
   static constexpr int kTurns = kParts == 16 ? 4 : 2;  // places of elements j that differ by more than j
@@ -922,7 +944,11 @@ __device__ __forceinline__ void load_to_lds(const char* base, unsigned offset, u
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base)
                : "memory", "m0");
 }
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// Until at most kLeft of them are on their way.
+template <int kLeft>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLeft) : "memory");
+}
 
 // Four 16-bit numbers a lane: of each 16 lanes, number l of those that lanes 4 k ... 4 k + 3 name
 // together, k = 0 ... 3.
@@ -967,13 +993,13 @@ struct TurnedValues {
   const char* at[kTurns];
   uint32_t held[4];
   bool all_finite;
-  __device__ Weights column(int s, int j) const {
+  __device__ __forceinline__ Weights column(int s, int j) const {
     const char* x = at[j % kTurns] + 32 * s * kToken + j / kTurns * kTurns * 32;
     const uint2 low = read_turned(x), high = read_turned(x + 16 * kToken);
     return Weights{{low.x, low.y, high.x, high.y}};
   }
-  __device__ Weights cleared(int s, int j) const {
-    Weights x = column(s, j);
+  __device__ __forceinline__ Weights cleared(int j) const {
+    Weights x = column(0, j);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       x.w[t] &= held[t];
@@ -981,30 +1007,30 @@ struct TurnedValues {
     }
     return x;
   }
-  __device__ bool clear(int s, int until) {
+  __device__ __forceinline__ bool clear(int until) {
 #pragma unroll
     for (int t = 0; t < 4; ++t)
       held[t] = (Wv::Sh::place(2 * t) < until ? 0xffffu : 0u) |
                 (Wv::Sh::place(2 * t + 1) < until ? 0xffff0000u : 0u);
     all_finite = false;
-    bool odd = false;
+    uint32_t odd = 0;
 #pragma unroll
     for (int j = 0; j < Wv::NJ; ++j) {
-      const Weights x = cleared(s, j);
+      const Weights x = cleared(j);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) odd |= Wv::finite(x.w[t]) != x.w[t];
+      for (int t = 0; t < 4; ++t) odd |= Wv::odd_bits(x.w[t]);
     }
     asm volatile("" ::: "memory");  // read again afterwards, not kept
-    return odd;
+    return odd & Wv::kSigns;
   }
-  __device__ void only_finite(int) {
+  __device__ __forceinline__ void only_finite() {
     all_finite = true;
     asm volatile("" ::: "memory");
   }
 };
 
 template <class T, int DH, int MODE>
-__global__ __launch_bounds__(64 * kWaves, 2) void chunk_kernel(Call a) {
+__global__ __launch_bounds__(64 * kWaves, (Chunk<T, DH>::kResident)) void chunk_kernel(Call a) {
   using Ch = Chunk<T, DH>;
   constexpr int MT = Ch::MT;
   using Sh = Shape<T, DH>;
@@ -1018,7 +1044,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void chunk_kernel(Call a) {
   Job job;
   Share share;
   if constexpr (MODE == kShared) {
-    u64* before = reinterpret_cast<u64*>(lds + 4 * Ch::kTile);
+    unsigned* before = reinterpret_cast<unsigned*>(lds + Ch::kLds);
     if (threadIdx.x == 0) a.ended[group] = 0;
     share = share_of(a, group, Ch::kRows, Ch::kTokens, 4, before, before + kMostShared + 1);
   } else {
@@ -1034,7 +1060,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void chunk_kernel(Call a) {
   unsigned bring_k[Ch::kLoads], bring_v[Ch::kLoads];
 #pragma unroll
   for (int i = 0; i < Ch::kLoads; ++i) {
-    const int token = (i * 64 + lane) / Ch::kParts, part = lane % Ch::kParts;
+    const int token = wave * Ch::kBring % 16 + (i * 64 + lane) / Ch::kParts, part = lane % Ch::kParts;
     bring_k[i] = token * Ch::kToken + Ch::key_part(token, part) * 16;
     bring_v[i] = token * Ch::kToken + Ch::value_part(token, part) * 16;
   }
@@ -1075,66 +1101,82 @@ __global__ __launch_bounds__(64 * kWaves, 2) void chunk_kernel(Call a) {
         const int first = min(tile * Ch::kTokens + lane * 16, end - 1);
         ids = page_of(c, table[first >> c.page_shift]);
       };
-      int id[4];
-      const auto fetch = [&](int tile, int block, int buffer) {  // block: the tile's first of the lanes' 64
+      // Brings a tile to a buffer; kBlocks bits of `bad` a buffer: blocks without a page.
+      unsigned bad = 0;
+      int block = 0;  // the next tile's first among the lanes' 64
+      const auto fetch = [&](int tile, int buffer) {
+        if (block == 64) {
+          block = 0;
+          pages_from(tile);
+        }
+        unsigned none = 0;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) id[b] = __builtin_amdgcn_readlane(ids, block + b);
-        const int page = max(__builtin_amdgcn_readlane(ids, block + wave), 0);
-        const i64 from = (i64)page * c.page_bytes +
-                         ((tile * Ch::kTokens + wave * 16) & ((1 << c.page_shift) - 1)) * Ch::kToken;
-        const unsigned here = lds_at + buffer * 2 * Ch::kTile + wave * 16 * Ch::kToken;
+        for (int b = 0; b < Ch::kBlocks; ++b)
+          none |= (unsigned)(__builtin_amdgcn_readlane(ids, block + b) < 0) << b;
+        const int shift = buffer * Ch::kBlocks;
+        bad = (bad & ~(((1u << Ch::kBlocks) - 1) << shift)) | none << shift;
+        const int page = max(__builtin_amdgcn_readlane(ids, block + wave * Ch::kBring / 16), 0);
+        block += Ch::kBlocks;
+        const int first = tile * Ch::kTokens + wave * Ch::kBring / 16 * 16;
+        const i64 from = (i64)page * c.page_bytes + (first & ((1 << c.page_shift) - 1)) * Ch::kToken;
+        const unsigned here = lds_at + buffer * 2 * Ch::kTile + wave * Ch::kLoads * 1024;
 #pragma unroll
         for (int i = 0; i < Ch::kLoads; ++i) {
           load_to_lds(k_head + from, bring_k[i], here + i * 1024);
           load_to_lds(v_head + from, bring_v[i], here + Ch::kTile + i * 1024);
         }
       };
-      int block = 0;
-      if (job.from < to) {
-        pages_from(job.from);
-        fetch(job.from, 0, 0);
-        wait_loads();
+      constexpr int kAhead = Ch::kBuffers - 1;  // tiles on their way while one is worked on
+      int buffer = 0, tile = job.from;
+      if (tile < to) {
+        pages_from(tile);
+#pragma unroll
+        for (int t = 0; t < kAhead; ++t)
+          if (tile + t < to) fetch(tile + t, t);
+        if (tile + kAhead <= to) wait_loads<(kAhead - 1) * 2 * Ch::kLoads>();
+        else wait_loads<0>();
         __syncthreads();
       }
-      int buffer = 0, tile = job.from;
       // first the tiles that all of it attends, in a loop without what the others need
-      const auto run = [&](auto all) {
-        for (; tile < to && (!all || ((tile + 1) * Ch::kTokens <= full &&
-                                      min(min(id[0], id[1]), min(id[2], id[3])) >= 0)); ++tile) {
-          int now[4];
-#pragma unroll
-          for (int b = 0; b < 4; ++b) now[b] = id[b];
-          if (tile + 1 < to) {
-            block += 4;
-            if (block == 64) {
-              block = 0;
-              pages_from(tile + 1);
-            }
-            fetch(tile + 1, block, buffer ^ 1);
-          }
+      const auto run = [&](auto all) __attribute__((always_inline)) {
+        for (; tile < to; ++tile) {
+          const unsigned now = bad >> buffer * Ch::kBlocks & ((1u << Ch::kBlocks) - 1);
+          if (all && ((tile + 1) * Ch::kTokens > full || now)) break;
+          const bool more = tile + kAhead < to;
+          if (more) fetch(tile + kAhead, buffer == 0 ? kAhead : buffer - 1);
           const char* keys = lds + buffer * 2 * Ch::kTile;
           TurnedValues<T, DH> values;
 #pragma unroll
           for (int j = 0; j < Ch::kTurns; ++j) values.at[j] = keys + Ch::kTile + value_at[j];
-          const int first = tile * Ch::kTokens + 4 * g;
-          if (mine0 < M)
-            w.template fold<2, decltype(all)::value>(
-                a.scale_log2,
-                [&](int t) {
-                  typename Wv::Keys x;
+          const auto part = [&](int t) {
+            typename Wv::Keys x;
 #pragma unroll
-                  for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int p = 0; p < Sh::KC; ++p)
-                      x.k[h][p] = *reinterpret_cast<const u32x4*>(keys + key_at[p] +
-                                                                  (32 * t + 16 * h) * Ch::kToken);
-                  return x;
-                },
-                values, [&](int t, int m) { return q.template seen<N>(a, s, m, first + 32 * t); },
-                [&](int t) { return end - first - 32 * t; },
-                [&](int t, int half) { return now[2 * t + half] < 0; });
-          buffer ^= 1;
-          wait_loads();
+              for (int p = 0; p < Sh::KC; ++p)
+                x.k[h][p] = *reinterpret_cast<const u32x4*>(keys + key_at[p] + (32 * t + 16 * h) * Ch::kToken);
+            return x;
+          };
+          if (mine0 >= M) {
+          } else if constexpr (decltype(all)::value) {
+            w.template fold<Ch::kSub, true>(a.scale_log2, part, values, [](int) { return u64(0); }, 0, 0u);
+          } else {
+            u64 seen[MT];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) seen[m] = q.window(a, s, m, tile * Ch::kTokens);
+#pragma unroll 1
+            for (int t = 0; t < Ch::kSub; ++t) {
+              w.template fold<1, false>(
+                  a.scale_log2, [&](int) { return part(t); }, values, [&](int m) { return seen[m] >> 32 * t; },
+                  end - tile * Ch::kTokens - 32 * t, now >> 2 * t);
+#pragma unroll
+              for (int j = 0; j < Ch::kTurns; ++j) values.at[j] += 32 * Ch::kToken;
+            }
+          }
+          buffer = buffer == kAhead ? 0 : buffer + 1;
+          // the next tile is there; nobody reads this one any more
+          if (more) wait_loads<(kAhead - 1) * 2 * Ch::kLoads>();
+          else wait_loads<0>();
           __syncthreads();
         }
       };
@@ -1256,10 +1298,10 @@ inline int plan(Call* a, int dh, int size, Plan* p) {
   const int cus = current_units();
   a->items = (int)items;
   p->groups = items;
-  if (items < 8 * cus && a->n <= kMostShared && longest > 512) {
+  const i64 most = items * ((longest + 15) / 16);  // tiles of tokens, which are counted in 32 bits
+  if (items < 8 * cus && a->n <= kMostShared && longest > 512 && most < (i64)1 << 31) {
     p->mode = kShared;
-    const i64 most = items * ((longest + 63) / 64);
-    p->groups = (chunks ? 2 : 4) * cus;
+    p->groups = (chunks ? dh == 64 ? 3 : 2 : 4) * cus;
     if (p->groups > most) p->groups = most;
   } else if (chunks || items < 8 * cus) {
     p->mode = kGroup;
@@ -1309,7 +1351,7 @@ int by_rows(const Call& a, const Plan& p, hipStream_t stream) {
     if (p.rows == 32) rc = by_mode<T, DH, 2>(a, p, stream);
   }
   if constexpr (kSize == 2 && (DH == 64 || DH == 128)) {
-    constexpr size_t kTiles = 4 * Chunk<T, DH>::kTile;
+    constexpr size_t kTiles = Chunk<T, DH>::kLds;
     if (p.rows == 128)
       rc = p.mode == kGroup ? launch(chunk_kernel<T, DH, kGroup>, a, p.groups, kTiles, stream)
                             : launch(chunk_kernel<T, DH, kShared>, a, p.groups, kTiles + kShareBytes, stream);
