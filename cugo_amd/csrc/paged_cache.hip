@@ -57,36 +57,51 @@ struct alignas(16) Plan {
   int tokens;   // branch: the row's length afterwards; accept: kept tokens
   int page;     // branch: the page in which the kept tokens end, if more follow, or -1
   int part;     // branch: its kept tokens; accept: start
-  int first;    // branch: the first of its new pages, counted over all entries
   int had;      // accept: pages the row had
+  int unused;
 };
-constexpr int kFine = 1, kSame = 2, kCopy = 4, kLacking = 8;
+constexpr int kFine = 1, kSame = 2;
 
 // bad[i] = 1 for every entry whose dst is another entry's dst or (other than that entry's own) src.
-// mark[row] need not be set before: it names an entry of the row if that entry says so too.
-__global__ __launch_bounds__(kOneGroup) void claim_kernel(const i64* __restrict__ dst,
-                                                          const i64* __restrict__ src, i64 n,
-                                                          i64 rows, int* __restrict__ mark,
-                                                          int* __restrict__ bad) {
-  for (i64 i = threadIdx.x; i < n; i += kOneGroup) {
+// mark[row] need not be set before: it names an entry of the row if that entry says so too.  Two
+// steps, with all of the first before any of the second.
+struct Claim {
+  const i64 *dst, *src;  // src may be NULL: none
+  i64 n, rows;
+  int *mark, *bad;
+  __device__ void set(i64 i) const {
     bad[i] = 0;
     const i64 d = dst[i];
-    if (d >= 0 && d < rows) __hip_atomic_store(mark + d, (int)i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    if (d >= 0 && d < rows) mark[d] = (int)i;
   }
-  __syncthreads();
-  for (i64 i = threadIdx.x; i < n; i += kOneGroup) {
+  __device__ void check(i64 i) const {
     const i64 d = dst[i];
     if (d >= 0 && d < rows) {
-      const int w = __hip_atomic_load(mark + d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      const int w = mark[d];
       if (w != (int)i) bad[i] = 1, bad[w] = 1;
     }
-    if (src == nullptr) continue;
+    if (src == nullptr) return;
     const i64 s = src[i];
     if (s != d && s >= 0 && s < rows) {
-      const int w = __hip_atomic_load(mark + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      const int w = mark[s];
       if (w >= 0 && w < n && dst[w] == s) bad[w] = 1;
     }
   }
+  // Both by one workgroup.
+  __device__ void all() const {
+    for (i64 i = threadIdx.x; i < n; i += blockDim.x) set(i);
+    __syncthreads();
+    for (i64 i = threadIdx.x; i < n; i += blockDim.x) check(i);
+    __syncthreads();
+  }
+};
+__global__ __launch_bounds__(kThreads) void set_kernel(Claim c) {
+  const i64 i = (i64)blockIdx.x * kThreads + threadIdx.x;
+  if (i < c.n) c.set(i);
+}
+__global__ __launch_bounds__(kThreads) void check_kernel(Claim c) {
+  const i64 i = (i64)blockIdx.x * kThreads + threadIdx.x;
+  if (i < c.n) c.check(i);
 }
 
 // One row less holds `page`; the last one sets its bit in `free`.
@@ -104,33 +119,52 @@ __device__ inline void give_back_row(const Cache& c, const int32_t* row, int fir
 
 // ------------------------------------------------------------------------------ branch
 
-__global__ __launch_bounds__(kThreads) void release_kernel(
-    Cache c, const i64* __restrict__ dst, const i64* __restrict__ src,
-    const i64* __restrict__ length, i64 n, const int* __restrict__ bad, Plan* __restrict__ plan) {
-  const i64 i = (i64)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
-  if (i >= n) return;
-  const i64 d = dst[i], s = src[i], want = length[i];
-  Plan p{};
-  p.page = -1;
-  const i64 most = (i64)c.width << c.page_shift;
-  if (d >= 0 && d < c.rows && s >= 0 && s < c.rows && want >= 0 && want <= most && !bad[i]) {
-    const bool same = d == s;
-    // a row that is another entry's src is no entry's dst: its length and table stand still
-    const int have = row_length(c, c.length[s]);
-    const int kept = have < (int)want ? have : (int)want;
-    p.flags = kFine | (same ? kSame : 0);
-    p.whole = kept >> c.page_shift;
-    p.part = kept & ((1 << c.page_shift) - 1);
-    p.held = pages_of(c, (int)want);
-    p.tokens = (int)want;
-    if (p.part > 0 && (int)want > kept)
-      p.page = page_of(c, c.table[s * c.width + p.whole]);
-    else if (p.part > 0)
-      ++p.whole;  // nothing will be written behind the kept tokens
-    const int old = pages_of(c, same ? have : row_length(c, c.length[d]));
-    give_back_row(c, c.table + d * c.width, same ? p.held : 0, old);
+struct Branch {
+  Cache c;
+  const i64 *dst, *src, *length;
+  i64 n;
+  const int* bad;
+  Plan* plan;
+  int2* asked;   // new pages an entry needs at most; the page that it keeps if no other row holds it, or -1
+  int* given;    // twice the first of its new pages (counted over all entries), 1 more if it keeps that
+                 // page; -1: none
+  int* fresh;    // the new pages
+  uint8_t* ok;
+
+  // By a wavefront: what becomes of entry i; its old pages given back.
+  __device__ void release(i64 i) const {
+    const i64 d = dst[i], s = src[i], want = length[i];
+    Plan p{};
+    int2 ask = make_int2(0, -1);
+    p.page = -1;
+    const i64 most = (i64)c.width << c.page_shift;
+    if (d >= 0 && d < c.rows && s >= 0 && s < c.rows && want >= 0 && want <= most && !bad[i]) {
+      const bool same = d == s;
+      // a row that is another entry's src is no entry's dst: its length and table stand still
+      const int have = row_length(c, c.length[s]);
+      const int kept = have < (int)want ? have : (int)want;
+      p.flags = kFine | (same ? kSame : 0);
+      p.whole = kept >> c.page_shift;
+      p.part = kept & ((1 << c.page_shift) - 1);
+      p.held = pages_of(c, (int)want);
+      p.tokens = (int)want;
+      if (p.part > 0) {
+        if ((int)want > kept) p.page = page_of(c, c.table[s * c.width + p.whole]);
+        // kept as it is where nothing will be written behind the kept tokens, or is none in place
+        if ((int)want == kept || (same && p.page < 0)) ++p.whole;
+      }
+      ask.x = p.held > p.whole ? p.held - p.whole : 0;
+      if (same) ask.y = p.page;
+      const int old = pages_of(c, same ? have : row_length(c, c.length[d]));
+      give_back_row(c, c.table + d * c.width, same ? p.held : 0, old);
+    }
+    if ((threadIdx.x & 63) == 0) plan[i] = p, asked[i] = ask;
   }
-  if ((threadIdx.x & 63) == 0) plan[i] = p;
+};
+
+__global__ __launch_bounds__(kThreads) void release_kernel(Branch b) {
+  const i64 i = (i64)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+  if (i < b.n) b.release(i);
 }
 
 // Inclusive sum over the workgroup's threads; `total` of all.  The buffer holds one a wavefront.
@@ -155,75 +189,122 @@ __device__ inline i64 group_scan(i64 x, i64* buffer, i64& total) {
   return x + before;
 }
 
-// New pages' numbers: each entry's first among all of them, then the lowest free pages in order
-// (`fresh`), as many as the entries that fit use.
-__global__ __launch_bounds__(kOneGroup) void place_kernel(Cache c, i64 n, Plan* __restrict__ plan,
-                                                          int* __restrict__ fresh,
-                                                          uint8_t* __restrict__ ok) {
-  __shared__ i64 buffer[kOneGroup / 64];
-  __shared__ int last_used;
+// What other wavefronts' atomics wrote, past the caches that they do not reach.
+template <class T>
+__device__ inline T fresh_load(const T* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+constexpr int kAtOnce = 8;        // entries a thread takes at once
+constexpr int kWordsAtOnce = 4096;  // words of free bits that the workgroup holds
+
+struct PlaceShared {
+  i64 buffer[kOneGroup / 64];
+  unsigned long long word[kWordsAtOnce];
+  int before[kWordsAtOnce];
+  int used;
+};
+
+// New pages' numbers, by one workgroup: each entry's first among all of them, then the lowest free
+// pages in order (`fresh`), as many as the entries that fit use.
+__device__ inline void place(const Branch& b, PlaceShared& sh) {
+  const Cache& c = b.c;
+  constexpr int kWordsEach = kWordsAtOnce / kOneGroup;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  constexpr int kWaves = kOneGroup / 64;
-  if (threadIdx.x == 0) last_used = 0;
-  // the free pages, a run of words a wavefront
   const int words = (c.pages + 63) >> 6;
-  const int run = (words + kWaves - 1) / kWaves;
-  const int from = min(wave * run, words), to = min(from + run, words);
-  i64 count = 0, available;
-  for (int w = from + lane; w < to; w += 64) count += __popcll(c.free[w]);
-  const i64 upto = group_scan(count, buffer, available);
-  // the free pages before this wavefront's run: its last lane's sum less its lanes' counts
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) count += __shfl_xor(count, off);
-  int rank = (int)(__shfl(upto, 63) - count);
+  if (threadIdx.x == 0) sh.used = 0;
+  i64 available = 0;
+  {
+    i64 count = 0;
+    for (int w = threadIdx.x; w < words; w += kOneGroup) count += __popcll(fresh_load(c.free + w));
+    group_scan(count, sh.buffer, available);
+  }
   i64 before = 0;
-  for (i64 base = 0; base < n; base += kOneGroup) {
-    const i64 i = base + threadIdx.x;
-    Plan p{};
-    int need = 0;
-    if (i < n) {
-      p = plan[i];
-      if (p.flags & kFine) {
-        // the part-filled page is copied unless it is the row's own already
-        const bool ends = p.part > 0 && p.whole < p.held && p.page != -1;
-        const bool gap = p.part > 0 && p.whole < p.held && p.page == -1;  // a table entry that is none
-        if (ends && (p.flags & kSame) && c.refs[p.page] <= 1) ++p.whole;
-        else if (ends) p.flags |= kCopy;
-        else if (gap && (p.flags & kSame)) ++p.whole;
-        need = p.held > p.whole ? p.held - p.whole : 0;
-      }
+  for (i64 base = 0; base < b.n; base += kOneGroup * kAtOnce) {
+    const i64 first = base + (i64)threadIdx.x * kAtOnce;
+    int2 ask[kAtOnce];
+    bool own[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) ask[k] = first + k < b.n ? b.asked[first + k] : make_int2(0, -1);
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) own[k] = ask[k].y >= 0 && fresh_load(c.refs + ask[k].y) <= 1;
+    i64 mine = 0, total;
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) mine += ask[k].x -= own[k];
+    i64 at = before + group_scan(mine, sh.buffer, total) - mine;
+    int used = 0;
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      if (first + k >= b.n) break;
+      const i64 end = at + ask[k].x;
+      const bool fits = ask[k].x == 0 || end <= available;
+      if (fits && ask[k].x > 0) used = (int)end;
+      b.given[first + k] = fits ? (ask[k].x ? (int)at << 1 : 0) | own[k] : -1;
+      b.ok[first + k] = fits && (b.plan[first + k].flags & kFine);
+      at = end;
     }
-    i64 total;
-    const i64 sum = group_scan(need, buffer, total);
-    if (i < n) {
-      const i64 end = before + sum;
-      const bool fine = (p.flags & kFine) && (need == 0 || end <= available);
-      if (fine && need > 0) atomicMax(&last_used, (int)end);
-      p.first = fine ? (int)(end - need) : 0;
-      if (!fine && (p.flags & kFine)) p.flags = (p.flags & kSame) | kLacking;
-      plan[i] = p;
-      ok[i] = fine;
-    }
+    if (used > 0) atomicMax(&sh.used, used);
     before += total;
   }
   __syncthreads();
-  const int used = last_used;
-  for (int w = from; w < to && rank < used; w += 64) {
-    const unsigned long long mine = w + lane < to ? c.free[w + lane] : 0;
-    for (int k = 0; k < 64 && w + k < to && rank < used; ++k) {
-      const unsigned long long bits = __shfl(mine, k);
-      const int at = rank + __popcll(bits & ((1ull << lane) - 1));
-      const bool take = (bits >> lane & 1) && at < used;
-      if (take) {
-        const int page = ((w + k) << 6) + lane;
-        fresh[at] = page;
+  const int used = sh.used;
+  int rank = 0;  // of the free pages before this segment
+  for (int segment = 0; segment < words && rank < used; segment += kWordsAtOnce) {
+    const int here = min(kWordsAtOnce, words - segment);
+    unsigned long long mine[kWordsEach];
+    i64 count = 0, total;
+#pragma unroll
+    for (int k = 0; k < kWordsEach; ++k) {
+      const int w = threadIdx.x * kWordsEach + k;
+      mine[k] = w < here ? fresh_load(c.free + segment + w) : 0;
+      count += __popcll(mine[k]);
+    }
+    int at = rank + (int)(group_scan(count, sh.buffer, total) - count);
+#pragma unroll
+    for (int k = 0; k < kWordsEach; ++k) {
+      const int w = threadIdx.x * kWordsEach + k, pages = __popcll(mine[k]);
+      sh.word[w] = mine[k];
+      sh.before[w] = at;
+      if (w < here && at < used && pages > 0) {  // the lowest of them are taken
+        unsigned long long left = 0;
+        if (at + pages > used) {
+          left = mine[k];
+          for (int t = at; t < used; ++t) left &= left - 1;
+        }
+        c.free[segment + w] = left;
+      }
+      at += pages;
+    }
+    __syncthreads();
+    // a word a wavefront at a time, a page a lane
+#pragma unroll 4
+    for (int w = wave; w < here; w += kOneGroup / 64) {
+      const unsigned long long bits = sh.word[w];
+      const int to = sh.before[w] + __popcll(bits & ((1ull << lane) - 1));
+      if ((bits >> lane & 1) && to < used) {
+        const int page = ((segment + w) << 6) + lane;
+        b.fresh[to] = page;
         c.refs[page] = 1;
       }
-      const unsigned long long gone = __ballot(take);
-      if (lane == 0 && gone) c.free[w + k] = bits & ~gone;
-      rank += __popcll(bits);
     }
+    rank += (int)total;
+    __syncthreads();  // the segment's last readers
   }
+}
+
+__global__ __launch_bounds__(kOneGroup) void place_kernel(Branch b) {
+  __shared__ PlaceShared sh;
+  place(b, sh);
+}
+
+// Few entries: everything before apply by one workgroup.
+__global__ __launch_bounds__(kOneGroup) void few_kernel(Branch b, Claim claim) {
+  __shared__ PlaceShared sh;
+  claim.all();
+  for (i64 i = threadIdx.x >> 6; i < b.n; i += kOneGroup / 64) b.release(i);
+  __threadfence();
+  __syncthreads();
+  place(b, sh);
 }
 
 // Copies `units` 16-byte units of every segment from page `a` to page `b`, segments first, first +
@@ -241,31 +322,30 @@ __device__ inline void copy_page(const Cache& c, int a, int b, int units, int fi
   }
 }
 
-__global__ __launch_bounds__(kThreads) void apply_kernel(Cache c, const i64* __restrict__ dst,
-                                                         const i64* __restrict__ src, i64 n,
-                                                         const Plan* __restrict__ plan,
-                                                         const int* __restrict__ fresh) {
+__global__ __launch_bounds__(kThreads) void apply_kernel(Branch b) {
+  const Cache& c = b.c;
   const i64 i = blockIdx.x;
-  const Plan p = plan[i];
-  if (!(p.flags & (kFine | kLacking))) return;  // refused from the start
-  const i64 d = dst[i], s = src[i];
-  if (p.flags & kLacking) {
-    if (!(p.flags & kSame) && blockIdx.y == 0 && threadIdx.x == 0) c.length[d] = 0;
+  const Plan p = b.plan[i];
+  const int given = b.given[i];
+  if (!(p.flags & kFine)) return;
+  const i64 d = b.dst[i], s = b.src[i];
+  const bool same = p.flags & kSame;
+  if (given < 0) {  // no pages left
+    if (!same && blockIdx.y == 0 && threadIdx.x == 0) c.length[d] = 0;
     return;
   }
-  const int wave = threadIdx.x >> 6;
-  if (p.flags & kCopy) {
-    const int units = p.part * c.token_bytes / 16;
-    copy_page(c, p.page, fresh[p.first], units, blockIdx.y * (kThreads / 64) + wave,
-              gridDim.y * (kThreads / 64));
-  }
+  const bool copy = p.page >= 0 && !(given & 1);
+  const int whole = p.whole + (given & 1);
+  const int* fresh = b.fresh + (given >> 1);
+  if (copy)
+    copy_page(c, p.page, fresh[0], p.part * c.token_bytes / 16,
+              blockIdx.y * (kThreads / 64) + (threadIdx.x >> 6), gridDim.y * (kThreads / 64));
   if (blockIdx.y != 0) return;
   int32_t* row = c.table + d * c.width;
   const int32_t* from = c.table + s * c.width;
-  const bool same = p.flags & kSame;
   for (int j = threadIdx.x; j < p.held; j += kThreads) {
-    if (j >= p.whole) {
-      row[j] = fresh[p.first + j - p.whole];
+    if (j >= whole) {
+      row[j] = fresh[j - whole];
     } else if (!same) {
       const int32_t entry = from[j];
       const int page = page_of(c, entry);
@@ -274,22 +354,27 @@ __global__ __launch_bounds__(kThreads) void apply_kernel(Cache c, const i64* __r
     }
   }
   if (threadIdx.x == 0) {
-    if (same && (p.flags & kCopy)) give_back(c, p.page);
+    if (same && copy) give_back(c, p.page);
     c.length[d] = p.tokens;
   }
 }
 
 // ------------------------------------------------------------------------------ accept
 
-// A wavefront an entry: which tokens are kept, and whether they may be.
-__global__ __launch_bounds__(kThreads) void decide_kernel(
-    Cache c, const i64* __restrict__ rows, const i64* __restrict__ start_in,
-    const i64* __restrict__ keep, i64 keep_stride, i64 most, i64 n, const int* __restrict__ bad,
-    Plan* __restrict__ plan, uint8_t* __restrict__ ok) {
-  const i64 i = (i64)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
-  if (i >= n) return;
+struct Accept {
+  Cache c;
+  const i64 *rows, *start, *keep;
+  i64 keep_stride, most, n;
+  const int* bad;
+  Plan* plan;
+  uint8_t* ok;
+  __device__ void decide(i64 i) const;
+};
+
+// By a wavefront: which tokens of entry i are kept, and whether they may be.
+__device__ inline void Accept::decide(i64 i) const {
   const int lane = threadIdx.x & 63;
-  const i64 row = rows[i], start = start_in[i];
+  const i64 row = rows[i], start = this->start[i];
   Plan p{};
   bool fine = row >= 0 && row < c.rows && !bad[i];
   const int length = fine ? row_length(c, c.length[row]) : 0;
@@ -338,6 +423,17 @@ __global__ __launch_bounds__(kThreads) void decide_kernel(
     plan[i] = p;
     ok[i] = fine;
   }
+}
+
+__global__ __launch_bounds__(kThreads) void decide_kernel(Accept a) {
+  const i64 i = (i64)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+  if (i < a.n) a.decide(i);
+}
+
+// Few entries: with the claims, by one workgroup.
+__global__ __launch_bounds__(kOneGroup) void few_decide_kernel(Accept a, Claim claim) {
+  claim.all();
+  for (i64 i = threadIdx.x >> 6; i < a.n; i += kOneGroup / 64) a.decide(i);
 }
 
 constexpr int kPathChunk = 256;  // kept tokens whose places a workgroup holds at once
@@ -397,20 +493,32 @@ __global__ __launch_bounds__(kThreads) void move_kernel(Cache c, const i64* __re
 // ------------------------------------------------------------------------------ the host's part
 
 // Of a call's workspace: entries' plans, then words.
-inline i64 workspace_bytes(const Cache& c, i64 n, bool fresh) {
+inline i64 workspace_bytes(const Cache& c, i64 n, bool branch) {
   return n * (i64)(sizeof(Plan) + sizeof(int)) + c.rows * (i64)sizeof(int) +
-         (fresh ? c.pages * (i64)sizeof(int) : 0);
+         (branch ? n * (i64)(sizeof(int2) + sizeof(int)) + c.pages * (i64)sizeof(int) : 0);
 }
 
 struct Workspace {
   Plan* plan;
-  int *bad, *mark, *fresh;
-  Workspace(void* at, const Cache& c, i64 n)
-      : plan(static_cast<Plan*>(at)), bad(reinterpret_cast<int*>(plan + n)), mark(bad + n),
-        fresh(mark + c.rows) {}
+  int2* asked;
+  int *bad, *mark, *given, *fresh;
+  Workspace(void* at, const Cache& c, i64 n, bool branch)
+      : plan(static_cast<Plan*>(at)), asked(reinterpret_cast<int2*>(plan + n)),
+        bad(reinterpret_cast<int*>(asked + (branch ? n : 0))), mark(bad + n), given(mark + c.rows),
+        fresh(given + n) {}
 };
 
 constexpr i64 kMostEntries = (i64)1 << 23;  // a launch has fewer than 2^32 threads in x
+// Up to so many entries one workgroup does what would otherwise be launches of its own.
+constexpr i64 kFew = 256;
+
+inline unsigned groups_of(i64 n, int each) { return (unsigned)((n + each - 1) / each); }
+
+// The claims of many entries.
+inline void claim(const Claim& c, hipStream_t stream) {
+  hipLaunchKernelGGL(set_kernel, dim3(groups_of(c.n, kThreads)), dim3(kThreads), 0, stream, c);
+  hipLaunchKernelGGL(check_kernel, dim3(groups_of(c.n, kThreads)), dim3(kThreads), 0, stream, c);
+}
 
 // Workgroups over an entry's segments: enough for 2,048 in all, at most one for each four
 // wavefronts' worth.
@@ -467,15 +575,17 @@ int cugo_paged_branch(const CugoPagedCache* cache, const int64_t* dst, const int
   if (n == 0) return 0;
   if (!aligned16(workspace)) return -4;
   if (workspace_size < workspace_bytes(c, n, true)) return -5;
-  const Workspace w(workspace, c, n);
-  const unsigned waves = (unsigned)((n + kThreads / 64 - 1) / (kThreads / 64));
-  hipLaunchKernelGGL(claim_kernel, dim3(1), dim3(kOneGroup), 0, stream, dst, src, n, c.rows, w.mark,
-                     w.bad);
-  hipLaunchKernelGGL(release_kernel, dim3(waves), dim3(kThreads), 0, stream, c, dst, src, length, n,
-                     w.bad, w.plan);
-  hipLaunchKernelGGL(place_kernel, dim3(1), dim3(kOneGroup), 0, stream, c, n, w.plan, w.fresh, ok);
-  hipLaunchKernelGGL(apply_kernel, dim3((unsigned)n, slices(c, n, 1)), dim3(kThreads), 0, stream, c,
-                     dst, src, n, w.plan, w.fresh);
+  const Workspace w(workspace, c, n, true);
+  const Claim named{dst, src, n, c.rows, w.mark, w.bad};
+  const Branch b{c, dst, src, length, n, w.bad, w.plan, w.asked, w.given, w.fresh, ok};
+  if (n <= kFew) {
+    hipLaunchKernelGGL(few_kernel, dim3(1), dim3(kOneGroup), 0, stream, b, named);
+  } else {
+    claim(named, stream);
+    hipLaunchKernelGGL(release_kernel, dim3(groups_of(n, kThreads / 64)), dim3(kThreads), 0, stream, b);
+    hipLaunchKernelGGL(place_kernel, dim3(1), dim3(kOneGroup), 0, stream, b);
+  }
+  hipLaunchKernelGGL(apply_kernel, dim3((unsigned)n, slices(c, n, 1)), dim3(kThreads), 0, stream, b);
   return (int)hipGetLastError();
 }
 
@@ -497,12 +607,15 @@ int cugo_paged_accept(const CugoPagedCache* cache, const int64_t* rows, const in
   if (n == 0) return 0;
   if (!aligned16(workspace)) return -4;
   if (workspace_size < workspace_bytes(c, n, false)) return -5;
-  const Workspace w(workspace, c, n);
-  const unsigned waves = (unsigned)((n + kThreads / 64 - 1) / (kThreads / 64));
-  hipLaunchKernelGGL(claim_kernel, dim3(1), dim3(kOneGroup), 0, stream, rows,
-                     static_cast<const int64_t*>(nullptr), n, c.rows, w.mark, w.bad);
-  hipLaunchKernelGGL(decide_kernel, dim3(waves), dim3(kThreads), 0, stream, c, rows, start, keep,
-                     keep_stride, most, n, w.bad, w.plan, ok);
+  const Workspace w(workspace, c, n, false);
+  const Claim named{rows, nullptr, n, c.rows, w.mark, w.bad};
+  const Accept a{c, rows, start, keep, keep_stride, most, n, w.bad, w.plan, ok};
+  if (n <= kFew) {
+    hipLaunchKernelGGL(few_decide_kernel, dim3(1), dim3(kOneGroup), 0, stream, a, named);
+  } else {
+    claim(named, stream);
+    hipLaunchKernelGGL(decide_kernel, dim3(groups_of(n, kThreads / 64)), dim3(kThreads), 0, stream, a);
+  }
   hipLaunchKernelGGL(move_kernel, dim3((unsigned)n, slices(c, n, 1024 / c.token_bytes)),
                      dim3(kThreads), 0, stream, c, rows, keep, keep_stride, w.plan);
   return (int)hipGetLastError();

@@ -78,7 +78,7 @@ Tensor blocks(const Tensor& t) {
   const bool near = t.size(0) <= 1 || (t.stride(0) >= t.size(1) * t.size(2) &&
                                        t.stride(0) * t.element_size() % 16 == 0);
   const bool aligned = (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0;
-  return dense && near && aligned ? t : t.clone(at::MemoryFormat::Contiguous);
+  return dense && near && aligned ? t : t.detach().clone(at::MemoryFormat::Contiguous);
 }
 int64_t block_stride(const Tensor& t) {
   return t.size(0) <= 1 ? t.size(1) * t.size(2) : t.stride(0);
@@ -208,7 +208,7 @@ Tensor tree_attention(const Tensor& k, const Tensor& v, const Tensor& table, con
   a.prefix = prefix.data_ptr<int64_t>();
   a.out = out.data_ptr();
   const int64_t bytes = cugo_tree_attention_workspace(&a);
-  const auto scratch = torch::empty({bytes}, on(k, at::kByte));
+  const auto scratch = bytes ? torch::empty({bytes}, on(k, at::kByte)) : Tensor();
   check_call(cugo_tree_attention(&a, bytes ? scratch.data_ptr() : nullptr, bytes, stream()),
              "tree_attention");
   return out;

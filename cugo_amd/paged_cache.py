@@ -57,7 +57,6 @@ def _state(cache) -> tuple:
     return cache.k, cache.v, cache.table, cache.length, cache.refs, cache.free
 
 
-@torch.no_grad()
 def branch(ext, cache, dst: torch.Tensor, src: torch.Tensor, length: torch.Tensor) -> torch.Tensor:
     """Row dst[i] becomes the first min(cache.length[src[i]], length[i]) tokens of row src[i], with
     pages for length[i] (int64 [n] each); bool [n]: which entries were done.
@@ -71,7 +70,6 @@ def branch(ext, cache, dst: torch.Tensor, src: torch.Tensor, length: torch.Tenso
     return ext.paged_branch(*_state(cache), dst, src, length)
 
 
-@torch.no_grad()
 def append(ext, cache, layer: int, k_new: torch.Tensor, v_new: torch.Tensor, pos: torch.Tensor,
            rows: torch.Tensor | None = None) -> None:
     """Token i's key and value (k_new and v_new [n, kv_heads, dh], any distance between tokens) to
@@ -80,7 +78,6 @@ def append(ext, cache, layer: int, k_new: torch.Tensor, v_new: torch.Tensor, pos
     ext.paged_append(*_state(cache), layer, k_new, v_new, pos, rows)
 
 
-@torch.no_grad()
 def accept(ext, cache, rows: torch.Tensor, start: torch.Tensor, keep: torch.Tensor) -> torch.Tensor:
     """Of the tokens of row rows[i] from position start[i] on, those at start[i] + keep[i, j] move to
     start[i] + j, in every layer, and the row ends behind them; bool [n]: which entries were done.
@@ -92,7 +89,6 @@ def accept(ext, cache, rows: torch.Tensor, start: torch.Tensor, keep: torch.Tens
     return ext.paged_accept(*_state(cache), rows, start, keep)
 
 
-@torch.no_grad()
 def tree_attention(ext, cache, layer: int, q: torch.Tensor, prefix: torch.Tensor, *,
                    mask: torch.Tensor | None = None, rows: torch.Tensor | None = None,
                    offsets: torch.Tensor | None = None, scale: float | None = None,
