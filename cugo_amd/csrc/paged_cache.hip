@@ -99,6 +99,7 @@ __global__ __launch_bounds__(kThreads) void set_kernel(Claim c) {
   const i64 i = (i64)blockIdx.x * kThreads + threadIdx.x;
   if (i < c.n) c.set(i);
 }
+__global__ __launch_bounds__(kOneGroup) void claim_kernel(Claim c) { c.all(); }
 __global__ __launch_bounds__(kThreads) void check_kernel(Claim c) {
   const i64 i = (i64)blockIdx.x * kThreads + threadIdx.x;
   if (i < c.n) c.check(i);
@@ -125,7 +126,8 @@ struct Branch {
   i64 n;
   const int* bad;
   Plan* plan;
-  int2* asked;   // new pages an entry needs at most; the page that it keeps if no other row holds it, or -1
+  int2* asked;   // new pages an entry needs at most (-1: refused); the page that it keeps if no other row
+                 // holds it, or -1
   int* given;    // twice the first of its new pages (counted over all entries), 1 more if it keeps that
                  // page; -1: none
   int* fresh;    // the new pages
@@ -135,7 +137,7 @@ struct Branch {
   __device__ void release(i64 i) const {
     const i64 d = dst[i], s = src[i], want = length[i];
     Plan p{};
-    int2 ask = make_int2(0, -1);
+    int2 ask = make_int2(-1, -1);
     p.page = -1;
     const i64 most = (i64)c.width << c.page_shift;
     if (d >= 0 && d < c.rows && s >= 0 && s < c.rows && want >= 0 && want <= most && !bad[i]) {
@@ -167,26 +169,33 @@ __global__ __launch_bounds__(kThreads) void release_kernel(Branch b) {
   if (i < b.n) b.release(i);
 }
 
-// Inclusive sum over the workgroup's threads; `total` of all.  The buffer holds one a wavefront.
-__device__ inline i64 group_scan(i64 x, i64* buffer, i64& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// Sums that stop at 2^32 - 1, which is more than there are pages.
+__device__ inline unsigned plus(unsigned a, unsigned b) { return __builtin_elementwise_add_sat(a, b); }
+
+// Inclusive sum over the wavefront's lanes.
+__device__ inline unsigned wave_scan(unsigned x) {
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
-    const i64 y = __shfl_up(x, off);
-    if (lane >= off) x += y;
+    const unsigned y = __shfl_up(x, off);
+    if ((int)(threadIdx.x & 63) >= off) x = plus(x, y);
   }
+  return x;
+}
+// The sum of the wavefronts' x before this one; `total` of all.  The buffer holds one a wavefront.
+__device__ inline unsigned before_wave(unsigned x, unsigned* buffer, unsigned& total) {
+  const int wave = threadIdx.x >> 6;
   __syncthreads();  // the buffer's last readers
-  if (lane == 63) buffer[wave] = x;
+  if ((threadIdx.x & 63) == 0) buffer[wave] = x;
   __syncthreads();
-  i64 before = 0;
+  unsigned before = 0;
   total = 0;
 #pragma unroll
   for (int w = 0; w < kOneGroup / 64; ++w) {
-    const i64 y = buffer[w];
-    before += w < wave ? y : 0;
-    total += y;
+    const unsigned y = buffer[w];
+    if (w < wave) before = plus(before, y);
+    total = plus(total, y);
   }
-  return x + before;
+  return before;
 }
 
 // What other wavefronts' atomics wrote, past the caches that they do not reach.
@@ -195,106 +204,109 @@ __device__ inline T fresh_load(const T* p) {
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-constexpr int kAtOnce = 8;        // entries a thread takes at once
-constexpr int kWordsAtOnce = 4096;  // words of free bits that the workgroup holds
+constexpr int kWaves = kOneGroup / 64;
+constexpr int kWordsAtOnce = kOneGroup;  // words of free bits that the workgroup holds: 65,536 pages
 
 struct PlaceShared {
-  i64 buffer[kOneGroup / 64];
+  unsigned buffer[kWaves];
   unsigned long long word[kWordsAtOnce];
-  int before[kWordsAtOnce];
-  int used;
+  unsigned before[kWordsAtOnce];
+  unsigned used;
 };
 
+// A segment of free words, one a thread, to LDS with the free pages before each; their number.
+__device__ inline unsigned load_words(const Cache& c, int segment, int words, unsigned before,
+                                      PlaceShared& sh) {
+  const int w = threadIdx.x;
+  const unsigned long long word = segment + w < words ? fresh_load(c.free + segment + w) : 0;
+  const unsigned pages = __popcll(word), sum = wave_scan(pages);
+  unsigned total;
+  before += before_wave(__shfl(sum, 63), sh.buffer, total);
+  sh.word[w] = word;
+  sh.before[w] = before + sum - pages;
+  __syncthreads();
+  return total;
+}
+
 // New pages' numbers, by one workgroup: each entry's first among all of them, then the lowest free
-// pages in order (`fresh`), as many as the entries that fit use.
+// pages in order (`fresh`), as many as the entries that fit use.  A lane takes kAtOnce entries, 64
+// apart, at once.  Short code counts here: one workgroup fetches each instruction from memory anew.
+template <int kAtOnce>
 __device__ inline void place(const Branch& b, PlaceShared& sh) {
   const Cache& c = b.c;
-  constexpr int kWordsEach = kWordsAtOnce / kOneGroup;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int words = (c.pages + 63) >> 6;
   if (threadIdx.x == 0) sh.used = 0;
-  i64 available = 0;
-  {
-    i64 count = 0;
-    for (int w = threadIdx.x; w < words; w += kOneGroup) count += __popcll(fresh_load(c.free + w));
-    group_scan(count, sh.buffer, available);
-  }
-  i64 before = 0;
+  unsigned available = 0;
+  for (int segment = 0; segment < words; segment += kWordsAtOnce)
+    available += load_words(c, segment, words, available, sh);
+  unsigned carry = 0;  // what the entries before need
   for (i64 base = 0; base < b.n; base += kOneGroup * kAtOnce) {
-    const i64 first = base + (i64)threadIdx.x * kAtOnce;
+    const i64 first = base + wave * (kAtOnce * 64) + lane;
     int2 ask[kAtOnce];
-    bool own[kAtOnce];
+    unsigned own = 0, end[kAtOnce], mine = 0, total, used = 0;
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) ask[k] = first + k < b.n ? b.asked[first + k] : make_int2(0, -1);
+    for (int k = 0; k < kAtOnce; ++k)
+      ask[k] = first + k * 64 < b.n ? b.asked[first + k * 64] : make_int2(-1, -1);
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) own[k] = ask[k].y >= 0 && fresh_load(c.refs + ask[k].y) <= 1;
-    i64 mine = 0, total;
-#pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) mine += ask[k].x -= own[k];
-    i64 at = before + group_scan(mine, sh.buffer, total) - mine;
-    int used = 0;
+    for (int k = 0; k < kAtOnce; ++k)
+      if (ask[k].y >= 0 && fresh_load(c.refs + ask[k].y) <= 1) own |= 1u << k, --ask[k].x;
 #pragma unroll
     for (int k = 0; k < kAtOnce; ++k) {
-      if (first + k >= b.n) break;
-      const i64 end = at + ask[k].x;
-      const bool fits = ask[k].x == 0 || end <= available;
-      if (fits && ask[k].x > 0) used = (int)end;
-      b.given[first + k] = fits ? (ask[k].x ? (int)at << 1 : 0) | own[k] : -1;
-      b.ok[first + k] = fits && (b.plan[first + k].flags & kFine);
-      at = end;
+      const unsigned sum = wave_scan(max(ask[k].x, 0));
+      end[k] = plus(mine, sum);
+      mine = plus(mine, __shfl(sum, 63));
+    }
+    const unsigned before = plus(carry, before_wave(mine, sh.buffer, total));
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      if (first + k * 64 >= b.n) continue;
+      const unsigned to = plus(before, end[k]);
+      const bool fits = ask[k].x == 0 || (ask[k].x > 0 && to <= available);
+      if (fits && ask[k].x > 0) used = to;
+      b.given[first + k * 64] = fits ? (ask[k].x ? (int)(to - ask[k].x) << 1 : 0) | (int)(own >> k & 1) : -1;
+      b.ok[first + k * 64] = fits;
     }
     if (used > 0) atomicMax(&sh.used, used);
-    before += total;
+    carry = plus(carry, total);
   }
   __syncthreads();
-  const int used = sh.used;
-  int rank = 0;  // of the free pages before this segment
+  const unsigned used = sh.used;
+  unsigned rank = 0;  // of the free pages before this segment
   for (int segment = 0; segment < words && rank < used; segment += kWordsAtOnce) {
+    // a pool of one segment is still there
+    const unsigned total = words > kWordsAtOnce ? load_words(c, segment, words, rank, sh) : available;
     const int here = min(kWordsAtOnce, words - segment);
-    unsigned long long mine[kWordsEach];
-    i64 count = 0, total;
-#pragma unroll
-    for (int k = 0; k < kWordsEach; ++k) {
-      const int w = threadIdx.x * kWordsEach + k;
-      mine[k] = w < here ? fresh_load(c.free + segment + w) : 0;
-      count += __popcll(mine[k]);
-    }
-    int at = rank + (int)(group_scan(count, sh.buffer, total) - count);
-#pragma unroll
-    for (int k = 0; k < kWordsEach; ++k) {
-      const int w = threadIdx.x * kWordsEach + k, pages = __popcll(mine[k]);
-      sh.word[w] = mine[k];
-      sh.before[w] = at;
-      if (w < here && at < used && pages > 0) {  // the lowest of them are taken
-        unsigned long long left = 0;
-        if (at + pages > used) {
-          left = mine[k];
-          for (int t = at; t < used; ++t) left &= left - 1;
-        }
+    for (int w = threadIdx.x; w < here; w += kOneGroup) {
+      unsigned long long left = sh.word[w];
+      const unsigned at = sh.before[w], pages = __popcll(left);
+      if (at < used && pages > 0) {  // the lowest of them are taken
+        if (at + pages <= used) left = 0;
+        else
+          for (unsigned t = at; t < used; ++t) left &= left - 1;
         c.free[segment + w] = left;
       }
-      at += pages;
     }
-    __syncthreads();
     // a word a wavefront at a time, a page a lane
-#pragma unroll 4
-    for (int w = wave; w < here; w += kOneGroup / 64) {
+    for (int w = wave; w < here; w += kWaves) {
+      if (sh.before[w] >= used) break;
       const unsigned long long bits = sh.word[w];
-      const int to = sh.before[w] + __popcll(bits & ((1ull << lane) - 1));
+      const unsigned to = sh.before[w] + __popcll(bits & ((1ull << lane) - 1));
       if ((bits >> lane & 1) && to < used) {
         const int page = ((segment + w) << 6) + lane;
         b.fresh[to] = page;
         c.refs[page] = 1;
       }
     }
-    rank += (int)total;
+    rank += total;
     __syncthreads();  // the segment's last readers
   }
 }
 
+template <int kAtOnce>
 __global__ __launch_bounds__(kOneGroup) void place_kernel(Branch b) {
   __shared__ PlaceShared sh;
-  place(b, sh);
+  place<kAtOnce>(b, sh);
 }
 
 // Few entries: everything before apply by one workgroup.
@@ -304,7 +316,7 @@ __global__ __launch_bounds__(kOneGroup) void few_kernel(Branch b, Claim claim) {
   for (i64 i = threadIdx.x >> 6; i < b.n; i += kOneGroup / 64) b.release(i);
   __threadfence();
   __syncthreads();
-  place(b, sh);
+  place<1>(b, sh);
 }
 
 // Copies `units` 16-byte units of every segment from page `a` to page `b`, segments first, first +
@@ -436,7 +448,7 @@ __global__ __launch_bounds__(kOneGroup) void few_decide_kernel(Accept a, Claim c
   for (i64 i = threadIdx.x >> 6; i < a.n; i += kOneGroup / 64) a.decide(i);
 }
 
-constexpr int kPathChunk = 256;  // kept tokens whose places a workgroup holds at once
+constexpr int kPathChunk = kThreads;  // kept tokens whose places a workgroup holds at once
 constexpr int kInFlight = 8;     // tokens a lane reads before it writes
 
 // Moves the kept tokens of one entry's segments.  Kept ones rise, so a token's new place is never
@@ -444,13 +456,15 @@ constexpr int kInFlight = 8;     // tokens a lane reads before it writes
 // of different segments or parts never meet.
 __global__ __launch_bounds__(kThreads) void move_kernel(Cache c, const i64* __restrict__ rows,
                                                         const i64* __restrict__ keep,
-                                                        i64 keep_stride,
+                                                        i64 keep_stride, i64 most,
                                                         const Plan* __restrict__ plan) {
   __shared__ i64 from[kPathChunk], to[kPathChunk];
   const i64 i = blockIdx.x;
   const Plan p = plan[i];
-  if (!(p.flags & kFine)) return;
   const i64 row = rows[i];
+  // the first kept tokens are asked for before it is known which move
+  const i64 early = threadIdx.x < most ? keep[i * keep_stride + threadIdx.x] : -1;
+  if (!(p.flags & kFine)) return;
   const int32_t* table = c.table + row * c.width;
   const int units = c.token_bytes / 16;  // a power of two, at most 64
   const int log = 31 - __builtin_clz(units);
@@ -461,18 +475,21 @@ __global__ __launch_bounds__(kThreads) void move_kernel(Cache c, const i64* __re
     const int page = page_of(c, table[at >> c.page_shift]);
     return page < 0 ? (i64)-1 : slot_offset(c, page, 0, at & ((1 << c.page_shift) - 1));
   };
-  for (int base = p.whole; base < p.tokens; base += kPathChunk) {
+  for (int base = 0; base < p.tokens; base += kPathChunk) {
+    const int skip = max(p.whole - base, 0);  // tokens that stay where they are
     const int here = min(kPathChunk, p.tokens - base);
+    if (skip >= here) continue;
     __syncthreads();
-    for (int j = threadIdx.x; j < here; j += kThreads) {
-      from[j] = place(p.part + (int)keep[i * keep_stride + base + j]);
+    const int j = threadIdx.x;
+    if (j >= skip && j < here) {
+      from[j] = place(p.part + (int)(base == 0 ? early : keep[i * keep_stride + base + j]));
       to[j] = place(p.part + base + j);
     }
     __syncthreads();
     for (int s = (blockIdx.y * (kThreads / 64) + wave) * at_once + sub; s < segments;
          s += gridDim.y * (kThreads / 64) * at_once) {
       char* at = segment(c, s, 0) + unit * 16;
-      for (int j = 0; j < here; j += kInFlight) {
+      for (int j = skip; j < here; j += kInFlight) {
         uint4 x[kInFlight];
 #pragma unroll
         for (int q = 0; q < kInFlight; ++q)
@@ -514,8 +531,13 @@ constexpr i64 kFew = 256;
 
 inline unsigned groups_of(i64 n, int each) { return (unsigned)((n + each - 1) / each); }
 
-// The claims of many entries.
+// The claims of many entries: by one workgroup, or two launches (257 entries 2.2 us against 3.8, 8,192
+// 25 against 8.5).
 inline void claim(const Claim& c, hipStream_t stream) {
+  if (c.n <= 2048) {
+    hipLaunchKernelGGL(claim_kernel, dim3(1), dim3(kOneGroup), 0, stream, c);
+    return;
+  }
   hipLaunchKernelGGL(set_kernel, dim3(groups_of(c.n, kThreads)), dim3(kThreads), 0, stream, c);
   hipLaunchKernelGGL(check_kernel, dim3(groups_of(c.n, kThreads)), dim3(kThreads), 0, stream, c);
 }
@@ -583,7 +605,10 @@ int cugo_paged_branch(const CugoPagedCache* cache, const int64_t* dst, const int
   } else {
     claim(named, stream);
     hipLaunchKernelGGL(release_kernel, dim3(groups_of(n, kThreads / 64)), dim3(kThreads), 0, stream, b);
-    hipLaunchKernelGGL(place_kernel, dim3(1), dim3(kOneGroup), 0, stream, b);
+    if (n <= kOneGroup)
+      hipLaunchKernelGGL(place_kernel<1>, dim3(1), dim3(kOneGroup), 0, stream, b);
+    else
+      hipLaunchKernelGGL(place_kernel<8>, dim3(1), dim3(kOneGroup), 0, stream, b);
   }
   hipLaunchKernelGGL(apply_kernel, dim3((unsigned)n, slices(c, n, 1)), dim3(kThreads), 0, stream, b);
   return (int)hipGetLastError();
@@ -617,7 +642,7 @@ int cugo_paged_accept(const CugoPagedCache* cache, const int64_t* rows, const in
     hipLaunchKernelGGL(decide_kernel, dim3(groups_of(n, kThreads / 64)), dim3(kThreads), 0, stream, a);
   }
   hipLaunchKernelGGL(move_kernel, dim3((unsigned)n, slices(c, n, 1024 / c.token_bytes)),
-                     dim3(kThreads), 0, stream, c, rows, keep, keep_stride, w.plan);
+                     dim3(kThreads), 0, stream, c, rows, keep, keep_stride, most, w.plan);
   return (int)hipGetLastError();
 }
 
