@@ -1285,7 +1285,9 @@ struct Plan {
 
 // Rows a tile by the rows a sequence has on the mean; an item a wavefront where that fills the
 // device, else a workgroup, and where rows may be long (by the table's width: lengths are on the
-// device) their tokens shared out.
+// device) their tokens shared out.  Sharing out costs a second launch and 5 us: at 64 queries x 4
+// heads of one row (dh 64), us of a workgroup an item / shared, 540 tokens 17 / 22, 1,100 tokens 25 /
+// 23, 2,200 tokens 42 / 27; at 4 queries 1,100 tokens 10.3 / 14.4, 2,200 tokens 15.8 / 17.
 inline int plan(Call* a, int dh, int size, Plan* p) {
   const i64 rows = ((i64)a->tokens * a->group + a->n - 1) / a->n;
   const bool chunks = size == 2 && (dh == 64 || dh == 128) && rows > 64;
@@ -1299,7 +1301,8 @@ inline int plan(Call* a, int dh, int size, Plan* p) {
   a->items = (int)items;
   p->groups = items;
   const i64 most = items * ((longest + 15) / 16);  // tiles of tokens, which are counted in 32 bits
-  if (items < 8 * cus && a->n <= kMostShared && longest > 512 && most < (i64)1 << 31) {
+  if (items < 8 * cus && a->n <= kMostShared && longest > (chunks ? 1024 : 4096) &&
+      most < (i64)1 << 31) {
     p->mode = kShared;
     p->groups = (chunks ? dh == 64 ? 3 : 2 : 4) * cus;
     if (p->groups > most) p->groups = most;
