@@ -20,8 +20,11 @@
 //
 // The running maximum moves only when a score exceeds it by more than 2^8 in the weight (kSlack):
 // until then weights are at most 2^8, which neither type nor the sums mind, and a tile needs no
-// exchange between lanes.  Weights are rounded to the cache's type for the product with V; their sum
-// is taken from the rounded ones (a matrix instruction with ones), so they add up to one.
+// exchange between lanes.  16-bit weights meet V as the sum of two numbers of the type, which costs
+// nothing beside the memory (4,096 trees over 320 tokens: the same 181 us) and leaves the output's
+// rounding alone; where many rows make the products the bound (chunk_kernel), rounded once, half a
+// step each, as much again as the output's rounding.  Their sum is taken from what meets V (a matrix
+// instruction with ones), so they add up to one.
 //
 // Tiles in which some query may not see some token (the drafts, a row's end) take their scores
 // from the masks, and values that are infinite or NaN there go through products of their own
@@ -275,11 +278,21 @@ struct Wave {
       return T::mfma(u32x4{a.w[0], a.w[1], a.w[2], a.w[3]}, u32x4{p.w[0], p.w[1], p.w[2], p.w[3]}, c);
     }
   }
-  // SUB tiles' share of every query.  kAll: every query attends every token, and each has a page.  keys(s): the lane's parts of tile s's keys; values.column(s, j):
+  // What rounding to the type left of N numbers, rounded to it too.
+  __device__ __forceinline__ static Weights rest(const float (&p)[N], const Weights& x) {
+    float y[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      y[e] = p[e] - (float)__builtin_bit_cast(typename T::storage, (uint16_t)(x.w[e / 2] >> 16 * (e % 2)));
+    return pack(y);
+  }
+
+  // SUB tiles' share of every query.  kTwice: 16-bit weights as the sum of two numbers.  kAll: every query
+  // attends every token, and each has a page.  keys(s): the lane's parts of tile s's keys; values.column(s, j):
   // its operand for elements j of the values.  Otherwise window(m) has a bit for each position of
   // the tile (one then) that query m attends, positions from `inside` on are past the row's end, and
   // bit h of `bad` says that the tile's half h has no page.
-  template <int SUB, bool kAll, class KeysOf, class V, class Window>
+  template <int SUB, bool kAll, bool kTwice, class KeysOf, class V, class Window>
   __device__ __forceinline__ void fold(float scale, KeysOf keys, V& values, Window window, int inside,
                                        unsigned bad) {
     static_assert(kAll || SUB == 1, "tiles with masks come alone");
@@ -338,7 +351,8 @@ struct Wave {
 #pragma unroll
     for (int e = 0; e < N; ++e) one[e] = 1.f;
     const Weights ones = pack(one);
-    Weights w[SUB][MT];
+    Weights w[SUB][MT], low[kTwice ? MT : 1];
+    static_assert(!kTwice || SUB == 1, "two weights for one tile");
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       const float base = top[m] == kNegInf ? 0.f : top[m];
@@ -348,6 +362,10 @@ struct Wave {
         for (int e = 0; e < N; ++e) d[s][m][e] = exp2_fast(__builtin_fmaf(d[s][m][e], scale, -base));
         w[s][m] = pack(d[s][m]);
         sum[m] = product(ones, w[s][m], sum[m]);
+        if constexpr (kTwice) {
+          low[m] = rest(d[s][m], w[s][m]);
+          sum[m] = product(ones, low[m], sum[m]);
+        }
       }
     }
 #pragma unroll
@@ -364,7 +382,7 @@ struct Wave {
             __builtin_amdgcn_sched_barrier(0);
             const Weights x = values.cleared(j);
 #pragma unroll
-            for (int m = 0; m < MT; ++m) acc[m][j] = product(x, w[s][m], acc[m][j]);
+            for (int m = 0; m < MT; ++m) acc[m][j] = product(x, w[s][m], acc[m][j]);  // (never twice)
           }
           continue;
         }
@@ -374,6 +392,9 @@ struct Wave {
         const Weights x = values.column(s, j);
 #pragma unroll
         for (int m = 0; m < MT; ++m) acc[m][j] = product(x, w[s][m], acc[m][j]);
+        if constexpr (kTwice)
+#pragma unroll
+          for (int m = 0; m < MT; ++m) acc[m][j] = product(x, low[m], acc[m][j]);
       }
     }
   }
@@ -843,7 +864,7 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(Call a) {
             load_keys<T, DH>(k_head + offset(next0, (tile + step) * KT),
                              k_head + offset(next1, (tile + step) * KT + 16), next.k);
           }
-          w.template fold<1, decltype(all)::value>(
+          w.template fold<1, decltype(all)::value, !Sh::kWide>(
               a.scale_log2, [&](int) -> const typename Wv::Keys& { return now; }, values,
               [&](int m) { return q.window(a, s, m, tile * KT); }, end - tile * KT,
               (unsigned)(id0 < 0) | (unsigned)(id1 < 0) << 1);
@@ -1159,14 +1180,14 @@ __global__ __launch_bounds__(64 * kWaves, (Chunk<T, DH>::kResident)) void chunk_
           };
           if (mine0 >= M) {
           } else if constexpr (decltype(all)::value) {
-            w.template fold<Ch::kSub, true>(a.scale_log2, part, values, [](int) { return u64(0); }, 0, 0u);
+            w.template fold<Ch::kSub, true, false>(a.scale_log2, part, values, [](int) { return u64(0); }, 0, 0u);
           } else {
             u64 seen[MT];
 #pragma unroll
             for (int m = 0; m < MT; ++m) seen[m] = q.window(a, s, m, tile * Ch::kTokens);
 #pragma unroll 1
             for (int t = 0; t < Ch::kSub; ++t) {
-              w.template fold<1, false>(
+              w.template fold<1, false, false>(
                   a.scale_log2, [&](int) { return part(t); }, values, [&](int m) { return seen[m] >> 32 * t; },
                   end - tile * Ch::kTokens - 32 * t, now >> 2 * t);
 #pragma unroll
