@@ -218,7 +218,8 @@ struct PlaceShared {
 __device__ inline unsigned load_words(const Cache& c, int segment, int words, unsigned before,
                                       PlaceShared& sh) {
   const int w = threadIdx.x;
-  const unsigned long long word = segment + w < words ? fresh_load(c.free + segment + w) : 0;
+  unsigned long long word = segment + w < words ? fresh_load(c.free + segment + w) : 0;
+  if (segment + w == words - 1 && (c.pages & 63)) word &= (1ull << (c.pages & 63)) - 1;  // no page beyond
   const unsigned pages = __popcll(word), sum = wave_scan(pages);
   unsigned total;
   before += before_wave(__shfl(sum, 63), sh.buffer, total);

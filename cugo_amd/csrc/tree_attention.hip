@@ -527,8 +527,13 @@ __device__ __forceinline__ Sequence same(Sequence s) {
   return s;
 }
 
-// Tiles of rows over all sequences.  With offsets, sequence i's begin at floor((offsets[i] -
-// offsets[0]) group / rows a tile) + i, which leaves room for what each needs.
+// Tiles of rows over all sequences.  With offsets, sequence i's begin at floor((offsets[i] - origin)
+// group / rows a tile) + i, origin = offsets[0], which leaves room for what each needs: for any
+// offsets, those of a sequence that is one (0 <= offsets[i] < offsets[i + 1] <= tokens) end before
+// floor(tokens group / rows) + n, since the origin is not negative.
+__device__ __forceinline__ i64 origin_of(const Call& a) {
+  return a.offsets == nullptr || a.offsets[0] < 0 ? 0 : a.offsets[0];
+}
 __device__ __forceinline__ int tiles_before(const Call& a, int i, int rows, i64 origin) {
   if (a.offsets == nullptr) return i * (int)(((i64)a.each * a.group + rows - 1) / rows);
   const i64 o = a.offsets[i] - origin;
@@ -544,7 +549,7 @@ __device__ __forceinline__ int find_tile(const Call& a, int x, int rows, int& ti
     return i;
   }
   const int lane = threadIdx.x & 63;
-  const i64 origin = a.offsets[0];
+  const i64 origin = origin_of(a);
   // 64 probes a turn; the last that starts at or before x
   int low = 0, span = a.n;
   while (span > 1) {
@@ -629,11 +634,13 @@ struct Share {
     const int tiles = (int)(((i64)job.s.queries * a.group + rows - 1) / rows);
     const int each = max(1, (job.s.end + tokens - 1) / tokens);
     const unsigned offset = at - (unsigned)same((int)before[low]);
-    const unsigned item = offset / (unsigned)each;
+    const unsigned item = offset / (unsigned)each;  // (each >= 1)
     job.from = same((int)(offset - item * each));
     job.to = same((int)min((unsigned)each, job.from + (end - at)));
-    job.head = same((int)(item / (unsigned)tiles));
+    job.head = same((int)(item / (unsigned)max(tiles, 1)));
     job.tile = same((int)(item - (unsigned)job.head * tiles));
+    // (offsets of sequences that overlap can hold more work than 32 bits count)
+    if (tiles <= 0 || job.head >= a.c.kv_heads) return false;
     job.ends = job.to == each;
     job.slot = job.from > 0 ? 0 : job.ends ? -1 : 1;
     at += job.to - job.from;
@@ -669,7 +676,7 @@ __device__ __forceinline__ void note(const Call& a, unsigned group, const Job& j
   if (job.slot == 0) {
     a.ended[group] = job.ends;
   } else {
-    const int x = tiles_before(a, job.sequence, rows, a.offsets ? a.offsets[0] : 0) + job.tile;
+    const int x = tiles_before(a, job.sequence, rows, origin_of(a)) + job.tile;
     a.begun[x * a.c.kv_heads + job.head] = job.slot == 1 ? (int)group + 1 : 0;
   }
 }
@@ -1316,7 +1323,7 @@ inline int plan(Call* a, int dh, int size, Plan* p) {
   const i64 tiles = a->offsets ? (i64)a->tokens * a->group / p->rows + a->n
                                : a->n * (((i64)a->each * a->group + p->rows - 1) / p->rows);
   const i64 items = tiles * a->c.kv_heads;
-  if (items >= (i64)1 << 24) return -1;
+  if (items >= (i64)1 << 26) return -1;
   const i64 longest = (i64)a->c.width << a->c.page_shift;
   const int cus = current_units();
   a->items = (int)items;
@@ -1333,7 +1340,7 @@ inline int plan(Call* a, int dh, int size, Plan* p) {
     p->mode = kEach;
     p->groups = (items + kWaves - 1) / kWaves;
   }
-  return 0;
+  return p->groups < (i64)1 << 24 ? 0 : -1;  // a launch has fewer than 2^32 threads in x
 }
 
 inline i64 part_floats(const Plan& p, int dh) { return p.groups * 2 * p.rows * dh; }

@@ -98,8 +98,8 @@ def tree_attention(ext, cache, layer: int, q: torch.Tensor, prefix: torch.Tensor
 
     q [tokens, heads, dh] (any distance between tokens; heads a multiple of the cache's kv_heads,
     head h reads kv_head h // (heads // kv_heads)) holds the queries of n sequences one after
-    another: sequence i's are offsets[i] ... offsets[i + 1] - 1 (int64 [n + 1]; None: as many for
-    each), its row rows[i] (int64 [n]; None: row i).  Query j of sequence i attends the positions
+    another: sequence i's are offsets[i] ... offsets[i + 1] - 1 (int64 [n + 1], not falling; None: as
+    many for each), its row rows[i] (int64 [n]; None: row i).  Query j of sequence i attends the positions
     below prefix[i] (int64 [n], taken into [0, length]) and from there on those whose bit is set in
     its mask, bit b for position prefix[i] + b, never past the row's length.  mask int64
     [tokens, words], bit b being bit b % 64 of word b // 64, or without offsets [tokens / n, words]

@@ -853,8 +853,9 @@ int cugo_paged_accept(const CugoPagedCache* cache, const int64_t* rows, const in
 
 /* cugo_tree_attention: n sequences' queries over the rows they belong to, in one layer.  q [tokens,
  * heads, dh] (tokens q_stride elements apart), heads a multiple of kv_heads; sequence i has the
- * queries offsets[i] ... offsets[i + 1] - 1 (NULL: tokens / n each; tokens outside every sequence
- * are left as they were) and row rows[i] (NULL: i).  With prefix[i] in [0, length] (taken into it),
+ * queries offsets[i] ... offsets[i + 1] - 1 (not falling, or which are served is not said; none
+ * where they are not among the tokens; NULL: tokens / n each; tokens outside every sequence are left
+ * as they were) and row rows[i] (NULL: i).  With prefix[i] in [0, length] (taken into it),
  * query number j of sequence i attends the row's positions t < length with
  *   t < prefix[i], or bit (t - prefix[i]) of its mask set              (mask given)
  *   t <= prefix[i] + j                                                 (mask NULL)

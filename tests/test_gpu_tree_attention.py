@@ -176,6 +176,46 @@ def test_what_is_not_there(ext):
           q[:4], i64([0, 7]), mask=nothing, rows=i64([1, 1]))
 
 
+@pytest.mark.parametrize("queries_each,width", [(3, 4), (40, 300), (3, 300)])
+def test_offsets_outside_the_tokens(ext, queries_each, width):
+    """Sequences that begin before the tokens or end past them have no queries, and the others are
+    served, however the rows are dealt out; offsets that fall, which no caller may give, leave every
+    token's place as it was or with some sequence's result."""
+    announce(f"tree attention with offsets outside, {queries_each} queries, width {width}")
+    rng = np.random.default_rng(16)
+    cache = on_gpu(random_cache(rng, [60, 50, 64, 7], kv_heads=2, dh=64, width=width))
+    each = queries_each
+    tokens = 4 * each
+    q = queries(rng, tokens, 8, 64, torch.bfloat16)
+    prefix, rows = i64([40, 50, 10, 7]), i64([0, 1, 2, 3])
+    for offsets, there in (([-50, 0, each, 2 * each, 9 * each], {1: 0, 2: each}),
+                           ([-9, -8, -7, 1 << 40, 1 << 41], {}),
+                           ([each, 2 * each, 2 * each, 4 * each, 4 * each], {0: each, 2: 2 * each})):
+        out = torch.full_like(q, 7.0)
+        pc.tree_attention(ext, cache, 0, q, prefix, rows=rows, offsets=i64(offsets), out=out)
+        for i, first in there.items():
+            last = offsets[i + 1]
+            part = slice(first, last)
+            close(out[part], cache, q[part], prefix[i:i + 1], rows=rows[i:i + 1])
+            out[part] = 7.0
+        assert (out == 7).all()
+    for offsets in ([2 * each, 3 * each, 4 * each, each, each], [0, tokens, 0, tokens, 0],
+                    [0, each, 0, 2 * each, 9 * each], [-50, 0, tokens, 0, tokens]):
+        out = pc.tree_attention(ext, cache, 0, q, prefix, rows=rows, offsets=i64(offsets),
+                                out=torch.full_like(q, 7.0))
+        assert out.shape == q.shape
+
+
+def test_negative_scale(ext):
+    announce("tree attention with a negative scale")
+    rng = np.random.default_rng(17)
+    for dtype in TYPES.values():
+        cache = on_gpu(random_cache(rng, [60, 50], kv_heads=2, dh=32, dtype=dtype))
+        q = queries(rng, 6, 4, 32, dtype)
+        got = pc.tree_attention(ext, cache, 0, q, i64([57, 47]), scale=-0.3)
+        assert torch.equal(got, pc.tree_attention(ext, cache, 0, -q, i64([57, 47]), scale=0.3))
+
+
 def test_strided_queries(ext):
     announce("tree attention of a packed projection's columns")
     rng = np.random.default_rng(12)
@@ -257,7 +297,8 @@ def test_refusals(ext):
                       ((0, q, p), dict(mask=ok[:, 0])), ((0, q, p), dict(mask=ok[:3], offsets=i64([0, 3, 6]))),
                       ((0, q, p), dict(mask=ok.cpu())), ((0, q, p), dict(rows=i64([0]))),
                       ((0, q, p), dict(offsets=i64([0, 6]))), ((0, q, p), dict(rows=p.int())),
-                      ((0, q, p), dict(out=q[:5])), ((0, q, p), dict(out=q.float())), ((0, q, i64([])), {})):
+                      ((0, q, p), dict(scale=0.0)), ((0, q, p), dict(scale=float("inf"))),
+                      ((0, q, p), dict(scale=float("nan"))), ((0, q, p), dict(out=q[:5])), ((0, q, p), dict(out=q.float())), ((0, q, i64([])), {})):
         with pytest.raises(RuntimeError):
             pc.tree_attention(ext, cache, *args, **how)
 
