@@ -944,12 +944,13 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(Call a) {
 // 16 j ... 16 j + 15 here.
 template <class T, int DH>
 struct Chunk {
-  static constexpr int kTokens = 64, kRows = 128, MT = 2;
+  static constexpr int kTokens = DH == 256 ? 32 : 64;
+  static constexpr int MT = 2, kRows = 16 * MT * kWaves;
   static constexpr int kToken = DH * 2;             // bytes
   static constexpr int kTile = kTokens * kToken;    // of keys, and of values
   static constexpr int kBuffers = 2, kLds = kBuffers * 2 * kTile;
   static_assert(kLds <= 65536, "the loads' place in LDS has 16 bits");
-  static constexpr int kResident = DH == 64 ? 3 : 2;  // workgroups a compute unit
+  static constexpr int kResident = DH == 64 ? 3 : DH == 128 ? 2 : 1;  // workgroups a compute unit
   static constexpr int kBlocks = kTokens / 16;      // of 16 tokens, which share a page
   static constexpr int kSub = kTokens / 32;
   static constexpr int kParts = DH / 8;             // 16-byte parts a token
@@ -957,12 +958,13 @@ struct Chunk {
   static constexpr int kLoads = kBring * kToken / 1024;  // of keys, and as many of values
   // Where part `part` of a key or value lies among its token's.
   __device__ __forceinline__ static int key_part(int token, int part) {
-    return part ^ (kParts == 16 ? token & 15 : token >> 1 & 7);
+    return part ^ (kParts >= 16 ? token & 15 : token >> 1 & 7);
   }
   __device__ __forceinline__ static int value_part(int token, int part) {
-    return part ^ (kParts == 16 ? token & 3 : token >> 1 & 1) * 2;
+    return part ^ (kParts >= 16 ? token & 3 : token >> 1 & 1) * 2;
   }
-  static constexpr int kTurns = kParts == 16 ? 4 : 2;  // places of elements j that differ by more than j
+  static constexpr int kTurns = kParts >= 16 ? 4 : 2;  // places of elements j that differ by more than j
+  static constexpr int kKeyTurns = kParts >= 16 ? 4 : 2;  // and of a key's parts 4 p + g
 };
 
 // 16 bytes a lane from base + offset to LDS at `to` + 16 lane; waited for by wait_loads().  In
@@ -1093,9 +1095,9 @@ __global__ __launch_bounds__(64 * kWaves, (Chunk<T, DH>::kResident)) void chunk_
     bring_v[i] = token * Ch::kToken + Ch::value_part(token, part) * 16;
   }
   // what it reads: key r's parts 4 p + g, and elements j of value 4 g + r / 4
-  unsigned key_at[Sh::KC], value_at[Ch::kTurns];
+  unsigned key_at[Ch::kKeyTurns], value_at[Ch::kTurns];
 #pragma unroll
-  for (int p = 0; p < Sh::KC; ++p) key_at[p] = r * Ch::kToken + Ch::key_part(r, 4 * p + g) * 16;
+  for (int p = 0; p < Ch::kKeyTurns; ++p) key_at[p] = r * Ch::kToken + Ch::key_part(r, 4 * p + g) * 16;
 #pragma unroll
   for (int j = 0; j < Ch::kTurns; ++j) {
     const int token = 4 * g + (r >> 2), part = 2 * j + (r >> 1 & 1);
@@ -1106,7 +1108,7 @@ __global__ __launch_bounds__(64 * kWaves, (Chunk<T, DH>::kResident)) void chunk_
       if (!share.next(a, Ch::kRows, Ch::kTokens, job)) return;
     }
     const Sequence& s = job.s;
-    const int M = s.queries * a.group, row0 = job.tile * Ch::kRows, mine0 = row0 + wave * 32;
+    const int M = s.queries * a.group, row0 = job.tile * Ch::kRows, mine0 = row0 + wave * 16 * MT;
     Queries<MT> q;
     q.find(a, s, job.head, mine0, M);
     Wv w;
@@ -1182,7 +1184,9 @@ __global__ __launch_bounds__(64 * kWaves, (Chunk<T, DH>::kResident)) void chunk_
             for (int h = 0; h < 2; ++h)
 #pragma unroll
               for (int p = 0; p < Sh::KC; ++p)
-                x.k[h][p] = *reinterpret_cast<const u32x4*>(keys + key_at[p] + (32 * t + 16 * h) * Ch::kToken);
+                x.k[h][p] = *reinterpret_cast<const u32x4*>(keys + key_at[p % Ch::kKeyTurns] +
+                                                            p / Ch::kKeyTurns * Ch::kKeyTurns * 64 +
+                                                            (32 * t + 16 * h) * Ch::kToken);
             return x;
           };
           if (mine0 >= M) {
@@ -1214,7 +1218,7 @@ __global__ __launch_bounds__(64 * kWaves, (Chunk<T, DH>::kResident)) void chunk_
     const i64 slot = MODE == kShared && job.slot >= 0 ? ((i64)group * 2 + job.slot) * Ch::kRows : -1;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
-      finish_turned<T, DH, MT>(a, q, m, slot < 0 ? -1 : slot + wave * 32 + 16 * m + r, s.exists, w.acc[m],
+      finish_turned<T, DH, MT>(a, q, m, slot < 0 ? -1 : slot + (wave * MT + m) * 16 + r, s.exists, w.acc[m],
                                w.sum[m][0], w.top[m]);
     if constexpr (MODE != kShared) return;
     if (threadIdx.x == 0) note(a, group, job, Ch::kRows);
@@ -1262,7 +1266,7 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(Call a, int rows, int
         total += ml.y * less;
       }
       const int here = min(64, parts - base);
-#pragma unroll 4
+#pragma unroll 8
       for (int k = 0; k < here; k += kSides) {
         const int mine = k + side;
         const float weight = __shfl(less, mine & 63);
@@ -1318,21 +1322,25 @@ struct Plan {
 // 23, 2,200 tokens 42 / 27; at 4 queries 1,100 tokens 10.3 / 14.4, 2,200 tokens 15.8 / 17.
 inline int plan(Call* a, int dh, int size, Plan* p) {
   const i64 rows = ((i64)a->tokens * a->group + a->n - 1) / a->n;
-  const bool chunks = size == 2 && (dh == 64 || dh == 128) && rows > 64;
+  const int cus = current_units();
+  // chunk_kernel for many rows: more than 64, or than 32 where few items leave the memory to be kept
+  // busy (24 rows of up to 32,768 tokens, dh 128: 42 rows 327 us against 484, 16 rows 316 against 312;
+  // 4,096 rows of up to 320 tokens, 6 rows 832 against 610)
+  const bool many = ((i64)a->tokens * a->group / 32 + a->n) * a->c.kv_heads >= 8 * cus;
+  const bool chunks = size == 2 && dh >= 64 && rows > (many ? 64 : 32);
   p->rows = chunks ? 128 : rows <= 16 || dh == 256 ? 16 : 32;
   const i64 tiles = a->offsets ? (i64)a->tokens * a->group / p->rows + a->n
                                : a->n * (((i64)a->each * a->group + p->rows - 1) / p->rows);
   const i64 items = tiles * a->c.kv_heads;
   if (items >= (i64)1 << 26) return -1;
   const i64 longest = (i64)a->c.width << a->c.page_shift;
-  const int cus = current_units();
   a->items = (int)items;
   p->groups = items;
   const i64 most = items * ((longest + 15) / 16);  // tiles of tokens, which are counted in 32 bits
   if (items < 8 * cus && a->n <= kMostShared && longest > (chunks ? 1024 : 4096) &&
       most < (i64)1 << 31) {
     p->mode = kShared;
-    p->groups = (chunks ? dh == 64 ? 3 : 2 : 4) * cus;
+    p->groups = (!chunks ? 4 : dh == 64 ? 3 : dh == 128 ? 2 : 1) * cus;
     if (p->groups > most) p->groups = most;
   } else if (chunks || items < 8 * cus) {
     p->mode = kGroup;
@@ -1381,7 +1389,7 @@ int by_rows(const Call& a, const Plan& p, hipStream_t stream) {
   if constexpr (DH < 256) {
     if (p.rows == 32) rc = by_mode<T, DH, 2>(a, p, stream);
   }
-  if constexpr (kSize == 2 && (DH == 64 || DH == 128)) {
+  if constexpr (kSize == 2 && DH >= 64) {
     constexpr size_t kTiles = Chunk<T, DH>::kLds;
     if (p.rows == 128)
       rc = p.mode == kGroup ? launch(chunk_kernel<T, DH, kGroup>, a, p.groups, kTiles, stream)
