@@ -5,7 +5,7 @@
 //
 // over the positions t of the query's row that lie before its sequence's prefix or whose bit is
 // set in its mask.  A sequence's queries and the heads that share a key head make the M = queries x
-// group rows of one product with that head's keys, 16 MT of them (MT = 1, 2, 4) a wavefront, so
+// group rows of one product with that head's keys, 16 MT of them (MT = 1, 2) a wavefront, so
 // each key and value is read once for all of them.  A wavefront goes through tiles of 32 tokens (16
 // in float32) with one running maximum and sum; nothing but the partial results of split rows leaves
 // it.
@@ -29,7 +29,7 @@
 // Bound: memory where a key head has few rows (4,096 trees of 16 tokens over rows of up to 320, dh 32
 // bf16: 181 us, 4.7 TB/s; 24 trees over rows of up to 32,768, dh 128 float16: 345 us, 5.3 TB/s), the
 // matrix and vector pipes in turn where it has many (4 x 512 queries over 14,336 tokens, dh 128 bf16:
-// 147 us, 730 TFLOP/s), latency in the smallest calls (one query: 4.7 us).
+// 137 us, 777 TFLOP/s), latency in the smallest calls (one query: 4.7 us).
 //
 // Tiles in which some query may not see some token (the drafts, a row's end) take their scores
 // from the masks, and values that are infinite or NaN there go through products of their own
@@ -387,7 +387,7 @@ struct Wave {
             __builtin_amdgcn_sched_barrier(0);
             const Weights x = values.cleared(j);
 #pragma unroll
-            for (int m = 0; m < MT; ++m) acc[m][j] = product(x, w[s][m], acc[m][j]);  // (never twice)
+            for (int m = 0; m < MT; ++m) acc[m][j] = product(x, w[s][m], acc[m][j]);
           }
           continue;
         }
@@ -940,13 +940,13 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(Call a) {
   }
 }
 
-// Many rows: a workgroup's 4 wavefronts have 32 rows each and share tiles of 64 tokens in LDS, in 64
-// KiB of buffers, which global_load_lds_dwordx4 fills without going through registers (1,024
-// consecutive bytes of LDS an instruction; a wavefront brings a quarter of a tile).  A token's 16-byte parts are
-// exchanged there, so that what is read at once comes from different banks: the same part of 16 keys,
-// or 32 bytes of four values, which ds_read_b64_tr_b16 turns as it reads (four lanes a token's 16
-// elements in, one element's four tokens a lane out; no v_perm_b32).  Elements j of the values are
-// 16 j ... 16 j + 15 here.
+// Many rows: a workgroup's 4 wavefronts have 32 rows each and share tiles of 64 tokens (32 at dh 256)
+// in LDS, in two buffers (32 KiB at dh 64, else 64), which global_load_lds_dwordx4 fills without going
+// through registers (1,024 consecutive bytes of LDS an instruction; a wavefront brings a quarter of a
+// tile).  A token's 16-byte parts are exchanged there, so that what is read at once comes from
+// different banks: the same part of 16 keys, or 32 bytes of four values, which ds_read_b64_tr_b16 turns
+// as it reads (four lanes a token's 16 elements in, one element's four tokens a lane out; no
+// v_perm_b32).  Elements j of the values are 16 j ... 16 j + 15 here.
 template <class T, int DH>
 struct Chunk {
   static constexpr int kTokens = DH == 256 ? 32 : 64;
