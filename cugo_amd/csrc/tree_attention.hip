@@ -29,7 +29,7 @@
 // Bound: memory where a key head has few rows (4,096 trees of 16 tokens over rows of up to 320, dh 32
 // bf16: 181 us, 4.7 TB/s; 24 trees over rows of up to 32,768, dh 128 float16: 345 us, 5.3 TB/s), the
 // matrix and vector pipes in turn where it has many (4 x 512 queries over 14,336 tokens, dh 128 bf16:
-// 137 us, 777 TFLOP/s), latency in the smallest calls (one query: 4.7 us).
+// 137 to 145 us, 730 to 777 TFLOP/s), latency in the smallest calls (one query: 4.7 us).
 //
 // Tiles in which some query may not see some token (the drafts, a row's end) take their scores
 // from the masks, and values that are infinite or NaN there go through products of their own
