@@ -974,9 +974,10 @@ struct Chunk {
 
 // 16 bytes a lane from base + offset to LDS at `to` + 16 lane; waited for by wait_loads().  In
 // assembly, since the compiler takes every later read of LDS for one of what such a load brings and
-// waits for it first; here a barrier stands between them.
+// waits for it first; here a barrier stands between them.  A load to LDS must not come directly behind
+// the scalar instruction that writes m0 (one wait state), which the compiler does not see to in here.
 __device__ __forceinline__ void load_to_lds(const char* base, unsigned offset, unsigned to) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base)
                : "memory", "m0");
 }
 // Until at most kLeft of them are on their way.
