@@ -125,7 +125,7 @@ SOURCES = ("kernels.hip", "decode.hip", "selfplay.hip", "mlp.hip", "linear.hip",
            "policy_loss.hip", "advantages.hip", "adamw.hip", "paged_cache.hip",
            "tree_attention.hip")
 HEADERS = (CSRC / "engine.h", CSRC / "learner.h", CSRC / "paged.h",
-           REPO / "include" / "cugo_hip.h")
+           CSRC / "tree_share.h", REPO / "include" / "cugo_hip.h")
 EXT_SOURCES = ("torch_ext.cpp", "learner_ext.cpp", "paged_ext.cpp")
 
 

@@ -31,6 +31,9 @@ struct Cache {
   int token_bytes;  // of one head's token: dh elements
 };
 
+// A sum that stops at 2^32 - 1.
+__host__ __device__ inline unsigned plus(unsigned a, unsigned b) { return __builtin_elementwise_add_sat(a, b); }
+
 // The tokens of a row, whatever its length says.
 __host__ __device__ inline int row_length(const Cache& c, i64 length) {
   const i64 most = (i64)c.width << c.page_shift;

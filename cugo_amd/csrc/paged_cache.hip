@@ -172,10 +172,7 @@ __global__ __launch_bounds__(kThreads) void release_kernel(Branch b) {
   if (i < b.n) b.release(i);
 }
 
-// Sums that stop at 2^32 - 1, which is more than there are pages.
-__device__ inline unsigned plus(unsigned a, unsigned b) { return __builtin_elementwise_add_sat(a, b); }
-
-// Inclusive sum over the wavefront's lanes.
+// Inclusive sum over the wavefront's lanes (2^32 - 1 is more than there are pages).
 __device__ inline unsigned wave_scan(unsigned x) {
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {

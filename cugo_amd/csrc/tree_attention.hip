@@ -36,14 +36,13 @@
 // (indicators of +inf and -inf), since 0 x inf would show in queries that do not attend them.
 #include <type_traits>
 
-#include "paged.h"
+#include "tree_share.h"
 
 namespace cugo_amd {
 namespace paged {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned long long u64;
 
 struct BF16 {
   using storage = __bf16;
@@ -65,28 +64,6 @@ struct F16 {
 };
 struct F32 {
   using storage = float;
-};
-
-struct Call {
-  Cache c;
-  i64 layer_offset;
-  const char* q;
-  i64 q_stride;  // bytes
-  i64 mask_rows;
-  const i64* prefix;
-  const i64* rows;
-  const i64* offsets;
-  const u64* mask;
-  char* out;
-  float* part_o;   // shared-out items' parts: [workgroups, 2, rows, dh]
-  float* part_ml;  // [workgroups, 2, rows, 2]: maximum (base 2) and sum
-  int* begun;      // [items]: 1 + the workgroup that began an item others went on with, or 0
-  int* ended;      // [workgroups]: whether it ended an item that others began
-  int tokens, n, each;  // each: queries a sequence without offsets
-  int heads, group, words;
-  int items;       // (tile of rows, key head), at most so many
-  float scale_log2;  // > 0: a negative scale turns q's signs
-  uint32_t flip;
 };
 
 constexpr float kNegInf = -__builtin_inff();
@@ -493,58 +470,6 @@ __device__ __forceinline__ u64 window_of(int at, int limit, int prefix, const u6
   return bits;
 }
 
-// A sequence as its wavefronts see it.
-struct Sequence {
-  int first, queries;  // its queries
-  i64 row;
-  bool exists;  // the row
-  int length, prefix;
-  int end;  // positions that some query may attend lie before it
-};
-__device__ __forceinline__ Sequence sequence_at(const Call& a, int i) {
-  Sequence s;
-  s.first = i * a.each;
-  s.queries = a.each;
-  if (a.offsets != nullptr) {
-    const i64 first = a.offsets[i], end = a.offsets[i + 1];
-    const bool fine = first >= 0 && end <= a.tokens && first < end;
-    s.first = fine ? (int)first : 0;
-    s.queries = fine ? (int)(end - first) : 0;
-  }
-  s.row = a.rows ? a.rows[i] : i;
-  s.exists = s.row >= 0 && s.row < a.c.rows;
-  s.length = s.exists ? row_length(a.c, a.c.length[s.row]) : 0;
-  const i64 given = a.prefix[i];
-  s.prefix = (int)(given < 0 ? 0 : given > s.length ? s.length : given);
-  s.end = (int)min((i64)s.length, (i64)s.prefix + (a.mask ? (i64)64 * a.words : (i64)s.queries));
-  return s;
-}
-
-// What is the same in every lane, in scalar registers.
-__device__ __forceinline__ int same(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ i64 same(i64 x) {
-  return (i64)((u64)(unsigned)same((int)(x >> 32)) << 32 | (unsigned)same((int)x));
-}
-__device__ __forceinline__ Sequence same(Sequence s) {
-  s.first = same(s.first), s.queries = same(s.queries), s.row = same(s.row);
-  s.length = same(s.length), s.prefix = same(s.prefix), s.end = same(s.end);
-  s.exists = same((int)s.exists);
-  return s;
-}
-
-// Tiles of rows over all sequences.  With offsets, sequence i's begin at floor((offsets[i] - origin)
-// group / rows a tile) + i, origin = offsets[0], which leaves room for what each needs: for any
-// offsets, those of a sequence that is one (0 <= offsets[i] < offsets[i + 1] <= tokens) end before
-// floor(tokens group / rows) + n, since the origin is not negative.
-__device__ __forceinline__ i64 origin_of(const Call& a) {
-  return a.offsets == nullptr || a.offsets[0] < 0 ? 0 : a.offsets[0];
-}
-__device__ __forceinline__ int tiles_before(const Call& a, int i, int rows, i64 origin) {
-  if (a.offsets == nullptr) return i * (int)(((i64)a.each * a.group + rows - 1) / rows);
-  const i64 o = a.offsets[i] - origin;
-  const i64 held = o < 0 ? 0 : o > a.tokens ? a.tokens : o;
-  return (int)((unsigned)(held * a.group) / (unsigned)rows) + i;
-}
 // The sequence of tile x and the tile's place in it.
 __device__ __forceinline__ int find_tile(const Call& a, int x, int rows, int& tile) {
   if (a.offsets == nullptr) {
@@ -569,12 +494,6 @@ __device__ __forceinline__ int find_tile(const Call& a, int x, int rows, int& ti
   return low;
 }
 
-// Sharing out: the work of all items (a tile of rows over one key head) in a row, an item's being its
-// sequence's tiles of tokens; each of the workgroups does as much of it, in order.
-// An item that a border cuts has parts, joined by a second launch.  Every workgroup sums up the
-// sequences' work for itself (kMostShared of them at most).
-constexpr int kMostShared = 1024;
-
 // before[i]: the work of the sequences before i; before[n]: all of it.  `scratch`: kWaves numbers.
 __device__ __forceinline__ void sum_work(const Call& a, int rows, int tokens, unsigned* before,
                                          unsigned* scratch) {
@@ -582,108 +501,34 @@ __device__ __forceinline__ void sum_work(const Call& a, int rows, int tokens, un
   unsigned carry = 0;
   for (int base = 0; base < a.n; base += 64 * kWaves) {
     const int i = base + threadIdx.x;
-    unsigned x = 0;
-    if (i < a.n) {
-      const Sequence s = sequence_at(a, i);
-      const int tiles = (int)(((i64)s.queries * a.group + rows - 1) / rows);
-      x = (unsigned)tiles * a.c.kv_heads * max(1, (s.end + tokens - 1) / tokens);
-    }
+    unsigned x = i < a.n ? work_of(a, i, rows, tokens) : 0;
     const unsigned mine = x;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
       const unsigned y = __shfl_up(x, off);
-      if (lane >= off) x += y;
+      if (lane >= off) x = plus(x, y);
     }
     if (lane == 63) scratch[wave] = x;
     __syncthreads();
     unsigned total = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      if (w < wave) x += scratch[w];
-      total += scratch[w];
+      if (w < wave) x = plus(x, scratch[w]);
+      total = plus(total, scratch[w]);
     }
-    if (i < a.n) before[i] = carry + x - mine;
-    carry += total;
+    if (i < a.n) before[i] = plus(carry, x) - mine;
+    carry = plus(carry, total);
     __syncthreads();
   }
   if (threadIdx.x == 0) before[a.n] = carry;
   __syncthreads();
 }
 
-// One workgroup's (or wavefront's) work on an item.
-struct Job {
-  Sequence s;
-  int sequence;
-  int head, tile;  // the key head; the tile of rows
-  int from, to;    // tiles of tokens
-  int slot;        // -1: the whole item; 0: its end or middle, 1: its beginning
-  bool ends;       // to is the item's end
-};
-
-// The jobs of a workgroup in order.
-struct Share {
-  const unsigned* before;
-  unsigned at, end;
-  int n;
-  __device__ __forceinline__ bool next(const Call& a, int rows, int tokens, Job& job) {
-    if (at >= end) return false;
-    int low = 0, high = n;  // before[low] <= at < before[high]
-    while (high - low > 1) {
-      const int mid = (low + high) >> 1;
-      if (before[mid] <= at) low = mid;
-      else high = mid;
-    }
-    low = same(low);
-    job.sequence = low;
-    job.s = same(sequence_at(a, low));
-    const int tiles = (int)(((i64)job.s.queries * a.group + rows - 1) / rows);
-    const int each = max(1, (job.s.end + tokens - 1) / tokens);
-    const unsigned offset = at - (unsigned)same((int)before[low]);
-    const unsigned item = offset / (unsigned)each;  // (each >= 1)
-    job.from = same((int)(offset - item * each));
-    job.to = same((int)min((unsigned)each, job.from + (end - at)));
-    job.head = same((int)(item / (unsigned)max(tiles, 1)));
-    job.tile = same((int)(item - (unsigned)job.head * tiles));
-    // (offsets of sequences that overlap can hold more work than 32 bits count)
-    if (tiles <= 0 || job.head >= a.c.kv_heads) return false;
-    job.ends = job.to == each;
-    job.slot = job.from > 0 ? 0 : job.ends ? -1 : 1;
-    at += job.to - job.from;
-    return true;
-  }
-};
-
 // Workgroups in an order that gives consecutive ones to one XCD (they go round the 8 of them): tiles
 // of one sequence read the same keys.
 __device__ __forceinline__ unsigned in_order() {
   const unsigned groups = gridDim.x, whole = groups & ~7u;
   return blockIdx.x < whole ? (blockIdx.x & 7) * (whole >> 3) + (blockIdx.x >> 3) : blockIdx.x;
-}
-
-__device__ __forceinline__ Share share_of(const Call& a, unsigned group, int rows, int tokens, int least,
-                                          unsigned* before, unsigned* scratch) {
-  sum_work(a, rows, tokens, before, scratch);
-  const unsigned all = (unsigned)same((int)before[a.n]);
-  // no less than `least` tiles of tokens each, unless there are more items; one at least
-  unsigned groups = max(all / (unsigned)least, (unsigned)a.items);
-  groups = max(min(min(groups, gridDim.x), all), 1u);
-  const unsigned each = all / groups, more = all - each * groups;  // the first `more` do one more
-  Share s;
-  s.before = before;
-  s.n = a.n;
-  s.at = (unsigned)same((int)(group < groups ? each * group + min(group, more) : all));
-  s.end = (unsigned)same((int)(group < groups ? s.at + each + (group < more) : all));
-  return s;
-}
-
-// What a workgroup tells the launch that joins of a job.
-__device__ __forceinline__ void note(const Call& a, unsigned group, const Job& job, int rows) {
-  if (job.slot == 0) {
-    a.ended[group] = job.ends;
-  } else {
-    const int x = tiles_before(a, job.sequence, rows, origin_of(a)) + job.tile;
-    a.begun[x * a.c.kv_heads + job.head] = job.slot == 1 ? (int)group + 1 : 0;
-  }
 }
 
 // Stores W consecutive elements.
@@ -802,9 +647,9 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(Call a) {
   Share share;
   if constexpr (MODE == kShared) {
     unsigned* before = reinterpret_cast<unsigned*>(lds + merge_bytes<T, DH, MT>());
-    if (threadIdx.x == 0) a.ended[group] = 0;
-    // a tile of tokens each wavefront
-    share = share_of(a, group, kRows, KT, kWaves, before, before + kMostShared + 1);
+    if (threadIdx.x == 0) note_none(a, group);
+    sum_work(a, kRows, KT, before, before + kMostShared + 1);
+    share = share_of(a, before, group, gridDim.x, kWaves);  // a tile of tokens each wavefront
   } else {
     const unsigned item = MODE == kEach ? group * kWaves + wave : group;
     if (item >= (unsigned)a.items) return;
@@ -1081,8 +926,9 @@ __global__ __launch_bounds__(64 * kWaves, (Chunk<T, DH>::kResident)) void chunk_
   Share share;
   if constexpr (MODE == kShared) {
     unsigned* before = reinterpret_cast<unsigned*>(lds + Ch::kLds);
-    if (threadIdx.x == 0) a.ended[group] = 0;
-    share = share_of(a, group, Ch::kRows, Ch::kTokens, 4, before, before + kMostShared + 1);
+    if (threadIdx.x == 0) note_none(a, group);
+    sum_work(a, Ch::kRows, Ch::kTokens, before, before + kMostShared + 1);
+    share = share_of(a, before, group, gridDim.x, 4);
   } else {
     if (group >= (unsigned)a.items) return;
     const int x = group / (unsigned)c.kv_heads;
@@ -1240,12 +1086,13 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(Call a, int rows, int
   const int lane = threadIdx.x & 63;
   const int x = blockIdx.x / (unsigned)a.c.kv_heads, key_head = blockIdx.x - x * a.c.kv_heads;
   int tile;
-  const Sequence s = sequence_at(a, find_tile(a, x, rows, tile));
+  const int sequence = find_tile(a, x, rows, tile);
+  const Sequence s = sequence_at(a, sequence);
   const int M = s.queries * a.group, row0 = tile * rows;
   if (row0 >= M) return;
-  const int begun = a.begun[blockIdx.x];
-  if (begun == 0) return;
-  const int group = begun - 1;
+  const int group = begun_by(a, blockIdx.x, groups);
+  if (group < 0) return;
+  const bool did = did_begin(a, group, blockIdx.x, sequence);
   int parts = 1;
   for (int base = group + 1; base < groups; base += 64) {
     const u64 ends = __ballot(base + lane < groups && a.ended[min(base + lane, groups - 1)]);
@@ -1254,6 +1101,7 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(Call a, int rows, int
       break;
     }
   }
+  if (!did) return;
   // many parts of a row: the workgroup's wavefronts take 64 of them in turn and merge through LDS
   __shared__ float merged[kWaves][64][6];
   const int wave = threadIdx.x >> 6;
@@ -1390,7 +1238,7 @@ inline i64 part_floats(const Plan& p, int dh) { return p.groups * 2 * p.rows * d
 inline i64 part_bytes(const Plan& p, int dh, i64 items) {
   return p.mode != kShared ? 0
                            : (part_floats(p, dh) + p.groups * 2 * p.rows * 2) * (i64)sizeof(float) +
-                                 (items + p.groups) * (i64)sizeof(int);
+                                 p.groups * (i64)sizeof(int2) + (items + p.groups) * (i64)sizeof(int);
 }
 
 // A launch with more than 64 KiB of LDS has to say so once a device and kernel.
@@ -1488,6 +1336,7 @@ inline int view(const CugoTreeAttention* p, Call* a) {
   a->scale_log2 = scale * 1.4426950408889634f;  // softmax in base 2
   a->out = static_cast<char*>(p->out);
   a->part_o = a->part_ml = nullptr;
+  a->left = nullptr;
   a->begun = a->ended = nullptr;
   return 0;
 }
@@ -1521,7 +1370,8 @@ int cugo_tree_attention(const CugoTreeAttention* call, void* workspace, int64_t 
     if (workspace_bytes < need) return -5;
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + part_floats(p, dh);
-    a.begun = reinterpret_cast<int*>(a.part_ml + p.groups * 2 * p.rows * 2);
+    a.left = reinterpret_cast<int2*>(a.part_ml + p.groups * 2 * p.rows * 2);
+    a.begun = reinterpret_cast<int*>(a.left + p.groups);
     a.ended = a.begun + a.items;
   }
   switch (call->cache->dtype) {
