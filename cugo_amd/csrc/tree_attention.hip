@@ -21,10 +21,11 @@
 // The running maximum moves only when a score exceeds it by more than 2^8 in the weight (kSlack):
 // until then weights are at most 2^8, which neither type nor the sums mind, and a tile needs no
 // exchange between lanes.  16-bit weights meet V as the sum of two numbers of the type, which costs
-// nothing beside the memory (4,096 trees over 320 tokens: the same 181 us) and leaves the output's
-// rounding alone; where many rows make the products the bound (chunk_kernel), rounded once, half a
-// step each, as much again as the output's rounding.  Their sum is taken from what meets V (a matrix
-// instruction with ones), so they add up to one.
+// nothing beside the memory (4,096 trees over 320 tokens: the same 181 us) and leaves little but the
+// output's rounding (2^-16 of a weight in bfloat16; 2^-22 in float16, or 2^-32 of the largest weight,
+// half its smallest step, where that is more); where many rows make the products the bound
+// (chunk_kernel), rounded once, half a step each, as much again as the output's rounding.  Their sum
+// is taken from what meets V (a matrix instruction with ones), so they add up to one.
 //
 // Bound: memory where a key head has few rows (4,096 trees of 16 tokens over rows of up to 320, dh 32
 // bf16: 181 us, 4.7 TB/s; 24 trees over rows of up to 32,768, dh 128 float16: 345 us, 5.3 TB/s), the
@@ -44,7 +45,11 @@ namespace paged {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
+// kLift: weights are 2^kLift times what they are against the running maximum (with kSlack at most 2^15,
+// which float16 holds; its smallest step is then 2^-31 of the largest weight, not 2^-24).  Sums and
+// outputs carry the factor alike.  The other types' steps are far below any that matters.
 struct BF16 {
+  static constexpr float kLift = 0.f;
   using storage = __bf16;
   typedef __bf16 vec __attribute__((ext_vector_type(8)));
   static constexpr uint32_t kInf = 0x7f80u;
@@ -54,6 +59,7 @@ struct BF16 {
   }
 };
 struct F16 {
+  static constexpr float kLift = 7.f;
   using storage = _Float16;
   typedef _Float16 vec __attribute__((ext_vector_type(8)));
   static constexpr uint32_t kInf = 0x7c00u;
@@ -63,6 +69,7 @@ struct F16 {
   }
 };
 struct F32 {
+  static constexpr float kLift = 0.f;
   using storage = float;
 };
 
@@ -337,7 +344,7 @@ struct Wave {
     static_assert(!kTwice || SUB == 1, "two weights for one tile");
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      const float base = top[m] == kNegInf ? 0.f : top[m];
+      const float base = top[m] == kNegInf ? 0.f : top[m] - T::kLift;
 #pragma unroll
       for (int s = 0; s < SUB; ++s) {
 #pragma unroll

@@ -865,7 +865,7 @@ int cugo_paged_accept(const CugoPagedCache* cache, const int64_t* rows, const in
  * nothing gets zeros; one whose row is none, or that attends a position whose page is none, NaN.
  * What masked places hold is never used.  Sums and softmax in float32; 16-bit types' weights meet v
  * rounded to the type (dh >= 64 and more than 64 queries x group, or 32 in few sequences) or
- * as the sum of two numbers of it.  workspace: at least
+ * as the sum of two numbers of it; float16's to 2^-32 of the largest.  workspace: at least
  * cugo_tree_attention_workspace(...) bytes (asked on the device of the call; may be 0). */
 typedef struct CugoTreeAttention {
   const CugoPagedCache* cache;
