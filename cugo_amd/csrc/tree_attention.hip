@@ -33,8 +33,10 @@
 // 137 to 145 us, 730 to 777 TFLOP/s), latency in the smallest calls (one query: 4.7 us).
 //
 // Tiles in which some query may not see some token (the drafts, a row's end) take their scores
-// from the masks, and values that are infinite or NaN there go through products of their own
-// (indicators of +inf and -inf), since 0 x inf would show in queries that do not attend them.
+// from the masks.  Values that are infinite or NaN go through products of their own (indicators of
+// +inf and -inf), since 0 x inf would show in queries that do not attend them, and be NaN in those
+// whose weight, or its second number, is 0: found among a tile's values (4,096 trees: the same time), or by
+// chunk_kernel, whose full tiles do not pass through registers first, in its outputs.
 #include <type_traits>
 
 #include "tree_share.h"
@@ -53,6 +55,11 @@ struct BF16 {
   using storage = __bf16;
   typedef __bf16 vec __attribute__((ext_vector_type(8)));
   static constexpr uint32_t kInf = 0x7f80u;
+  // x, or NaN where one of the word's numbers is infinite or NaN.
+  __device__ __forceinline__ static float unless_odd(uint32_t w, float x) {
+    typedef __bf16 pair __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pair, w), __builtin_bit_cast(pair, 0), x, false);
+  }
   __device__ __forceinline__ static f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vec, a),
                                                    __builtin_bit_cast(vec, b), c, 0, 0, 0);
@@ -63,6 +70,10 @@ struct F16 {
   using storage = _Float16;
   typedef _Float16 vec __attribute__((ext_vector_type(8)));
   static constexpr uint32_t kInf = 0x7c00u;
+  __device__ __forceinline__ static float unless_odd(uint32_t w, float x) {
+    typedef _Float16 pair __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(pair, w), __builtin_bit_cast(pair, 0), x, false);
+  }
   __device__ __forceinline__ static f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vec, a),
                                                   __builtin_bit_cast(vec, b), c, 0, 0, 0);
@@ -71,6 +82,9 @@ struct F16 {
 struct F32 {
   static constexpr float kLift = 0.f;
   using storage = float;
+  __device__ __forceinline__ static float unless_odd(uint32_t w, float x) {
+    return __builtin_fmaf(__uint_as_float(w), 0.f, x);
+  }
 };
 
 constexpr float kNegInf = -__builtin_inff();
@@ -78,6 +92,11 @@ constexpr float kSlack = 8.f;
 constexpr int kWaves = 4;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// x times a weight, of which infinities and NaN are left where it is so small that it is 0.
+__device__ __forceinline__ float scaled(float x, float weight) {
+  return weight == 0.f && x - x != 0.f ? x : x * weight;
+}
 
 // The largest over the four lanes that hold one query (lane & 15).
 __device__ __forceinline__ float query_max(float x) {
@@ -183,6 +202,17 @@ struct Wave {
                                          e & 1 ? 0x07060302u : 0x05040100u);
       }
       return y;
+    }
+    // Whether an infinity or NaN is among them.
+    __device__ __forceinline__ bool odd() const {
+      float x = 0.f;  // one instruction a word
+#pragma unroll
+      for (int t = 0; t < N; ++t)
+#pragma unroll
+        for (int h = 0; h < Sh::H; ++h)
+#pragma unroll
+          for (int e = 0; e < Sh::RW; ++e) x = T::unless_odd(v[t][h][e], x);
+      return x != x;
     }
     // Zeros for the tokens from `until` on after the lane's first; whether an infinity or NaN is left.
     __device__ __forceinline__ bool clear(int until) {
@@ -333,7 +363,14 @@ struct Wave {
         top[m] = now;
         sum[m] *= less;
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[m][j] *= less;
+        for (int j = 0; j < NJ; ++j) {
+          if constexpr (kAll && !V::kInPlace) {
+            acc[m][j] *= less;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[m][j][e] = scaled(acc[m][j][e], less);
+          }
+        }
       }
     }
     float one[N];
@@ -375,6 +412,14 @@ struct Wave {
           }
           continue;
         }
+      } else if constexpr (V::kInPlace) {
+        // (an infinity times a weight's second number, or one that is 0, is none)
+        if (__ballot(values.odd())) {
+#pragma unroll
+          for (int m = 0; m < MT; ++m) seen[m] = ~0u;
+          fold_odd(values, seen);
+          values.only_finite();
+        }
       }
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
@@ -386,6 +431,18 @@ struct Wave {
           for (int m = 0; m < MT; ++m) acc[m][j] = product(x, low[m], acc[m][j]);
       }
     }
+  }
+
+  // Whether an output of the wavefront is infinite or NaN.
+  __device__ __forceinline__ bool odd() const {
+    float x = 0.f;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x = __builtin_fmaf(acc[m][j][e], 0.f, x);
+    return __ballot(x != x) != 0;
   }
 
   __device__ __forceinline__ static constexpr uint32_t inf_bits() {
@@ -690,27 +747,25 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(Call a) {
       const char* k_head = c.k + head_offset;
       const char* v_head = c.v + head_offset;
       const int32_t* table = c.table + s.row * c.width;
-      // the pages of the next 64 tiles, one a lane; -1 for none
+      // the pages of the next 64 tiles, one a lane; -1 for none (past the last: the last's).  Without a branch
+      // by lanes: at its end, in the largest of these kernels, the compiler (ROCm 7.2) saved a register that
+      // all lanes need while only those of the branch were on
       int ids0 = -1, ids1 = -1;
       const auto pages_from = [&](int tile) {
-        const int mine = tile + lane * step;
-        ids0 = ids1 = -1;
-        if (mine < to) {
-          const int first = mine * KT, last = min(first + KT, end) - 1;
-          ids0 = page_of(c, table[first >> c.page_shift]);
-          ids1 = page_of(c, table[last >> c.page_shift]);
-        }
+        const int first = min(tile + lane * step, to - 1) * KT, last = min(first + KT, end) - 1;
+        ids0 = page_of(c, table[first >> c.page_shift]);
+        ids1 = page_of(c, table[last >> c.page_shift]);
       };
       typename Wv::Keys now, next;
       typename Wv::Values values;
       int at = 0;  // the current tile among the 64
       int id0 = 0, id1 = 0, next0 = 0, next1 = 0;
-      pages_from(begin);
       const int in_page = (1 << c.page_shift) - 1;
       const auto offset = [&](int id, int position) {  // of 16 tokens from a position on
         return (i64)max(id, 0) * c.page_bytes + (position & in_page) * (DH * Sh::E);
       };
       if (begin < to) {
+        pages_from(begin);
         id0 = __builtin_amdgcn_readlane(ids0, 0), id1 = __builtin_amdgcn_readlane(ids1, 0);
         load_keys<T, DH>(k_head + offset(id0, begin * KT), k_head + offset(id1, begin * KT + 16), now.k);
       }
@@ -781,7 +836,7 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(Call a) {
           o[j][0] = 0.f;
 #pragma unroll
           for (int v = 0; v < kWaves; ++v)
-            o[j][0] += merged[v * kPart + ((m * NJ + j) * 4 + i) * 64 + lane] * less[v];
+            o[j][0] += scaled(merged[v * kPart + ((m * NJ + j) * 4 + i) * 64 + lane], less[v]);
         }
         finish<T, DH, MT>(a, q, m, i, slot < 0 ? -1 : slot + 16 * m + r, s.exists, o, 0, total, top);
       }
@@ -992,7 +1047,7 @@ __global__ __launch_bounds__(64 * kWaves, (Chunk<T, DH>::kResident)) void chunk_
       };
       // Brings a tile to a buffer; kBlocks bits of `bad` a buffer: blocks without a page.
       unsigned bad = 0;
-      int block = 0;  // the next tile's first among the lanes' 64
+      int block;  // the next tile's first among the lanes' 64
       const auto fetch = [&](int tile, int buffer) {
         if (block == 64) {
           block = 0;
@@ -1016,16 +1071,19 @@ __global__ __launch_bounds__(64 * kWaves, (Chunk<T, DH>::kResident)) void chunk_
         }
       };
       constexpr int kAhead = Ch::kBuffers - 1;  // tiles on their way while one is worked on
-      int buffer = 0, tile = job.from;
-      if (tile < to) {
-        pages_from(tile);
+      int buffer, tile;
+      const auto start = [&]() __attribute__((always_inline)) {
+        buffer = block = 0, tile = job.from;
+        if (tile < to) {
+          pages_from(tile);
 #pragma unroll
-        for (int t = 0; t < kAhead; ++t)
-          if (tile + t < to) fetch(tile + t, t);
-        if (tile + kAhead <= to) wait_loads<(kAhead - 1) * 2 * Ch::kLoads>();
-        else wait_loads<0>();
-        __syncthreads();
-      }
+          for (int t = 0; t < kAhead; ++t)
+            if (tile + t < to) fetch(tile + t, t);
+          if (tile + kAhead <= to) wait_loads<(kAhead - 1) * 2 * Ch::kLoads>();
+          else wait_loads<0>();
+          __syncthreads();
+        }
+      };
       // first the tiles that all of it attends, in a loop without what the others need
       const auto run = [&](auto all) __attribute__((always_inline)) {
         for (; tile < to; ++tile) {
@@ -1071,8 +1129,23 @@ __global__ __launch_bounds__(64 * kWaves, (Chunk<T, DH>::kResident)) void chunk_
           __syncthreads();
         }
       };
+      // Outputs that are not finite: everything once more, by all wavefronts, as tiles with masks, which
+      // take infinite values apart (an infinity times a weight that is 0 is NaN).
+      start();
       run(std::true_type());
       run(std::false_type());
+      int* again = reinterpret_cast<int*>(lds);  // nobody reads or brings a tile now
+      if (threadIdx.x == 0) *again = 0;
+      __syncthreads();
+      if (w.odd() && lane == 0) *again = 1;
+      __syncthreads();
+      const int odd = same(*again);
+      __syncthreads();  // its readers
+      if (odd) {
+        w.clear();
+        start();
+        run(std::false_type());
+      }
     }
     const i64 slot = MODE == kShared && job.slot >= 0 ? ((i64)group * 2 + job.slot) * Ch::kRows : -1;
 #pragma unroll
@@ -1123,27 +1196,39 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(Call a, int rows, int
     for (int k = first + lane; k < parts; k += step) top = fmaxf(top, a.part_ml[slot(k, row) * 2]);
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
-    float total = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    float total;
+    f32x4 o;
     const int side = lane / kLanes, at = lane % kLanes * 4;
-    for (int base = first; base < parts; base += step) {
-      float less = 0.f;
-      if (base + lane < parts) {
-        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + slot(base + lane, row) * 2);
-        less = ml.x == kNegInf ? 0.f : exp2_fast(ml.x - top);
-        total += ml.y * less;
-      }
-      const int here = min(64, parts - base);
+    const auto sum_up = [&](auto small) __attribute__((always_inline)) {
+      total = 0.f;
+      o = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int base = first; base < parts; base += step) {
+        float less = 0.f;
+        if (base + lane < parts) {
+          const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + slot(base + lane, row) * 2);
+          less = ml.x == kNegInf ? 0.f : exp2_fast(ml.x - top);
+          total += ml.y * less;
+        }
+        const int here = min(64, parts - base);
 #pragma unroll 16
-      for (int k = 0; k < here; k += kSides) {
-        const int mine = k + side;
-        const float weight = __shfl(less, mine & 63);
-        if (mine < here) {
-          const f32x4 y = *reinterpret_cast<const f32x4*>(a.part_o + slot(base + mine, row) * DH + at);
-          o += y * weight;
+        for (int k = 0; k < here; k += kSides) {
+          const int mine = k + side;
+          const float weight = __shfl(less, mine & 63);
+          if (mine < here) {
+            const f32x4 y = *reinterpret_cast<const f32x4*>(a.part_o + slot(base + mine, row) * DH + at);
+            if constexpr (decltype(small)::value) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[e] += scaled(y[e], weight);
+            } else {
+              o += y * weight;
+            }
+          }
         }
       }
-    }
+    };
+    sum_up(std::false_type());
+    const float sum = o[0] + o[1] + o[2] + o[3];
+    if (__ballot(sum - sum != 0.f)) sum_up(std::true_type());  // infinities of parts whose weight is 0
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) total += __shfl_xor(total, off);
 #pragma unroll
@@ -1167,7 +1252,7 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(Call a, int rows, int
         const float less = x[0] == kNegInf ? 0.f : exp2_fast(x[0] - least);
         total += x[1] * less;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] += x[2 + e] * less;
+        for (int e = 0; e < 4; ++e) o[e] += scaled(x[2 + e], less);
       }
       __syncthreads();  // its readers
       if (wave != 0) continue;
