@@ -23,21 +23,24 @@ constexpr int kOneGroup = 1024;  // of the launches of one workgroup
 // ------------------------------------------------------------------------------ append
 
 // One 16-byte part of a token's key and value a thread: `parts` of them a token, whose head is
-// part >> head_shift.
+// part >> head_shift.  ok (NULL: not asked): whether the token had a place.
 __global__ __launch_bounds__(kThreads) void append_kernel(
     Cache c, i64 layer, const char* __restrict__ k_new, i64 k_stride,
     const char* __restrict__ v_new, i64 v_stride, const i64* __restrict__ pos_in,
-    const i64* __restrict__ rows, i64 n, int parts, int head_shift, int each) {
+    const i64* __restrict__ rows, i64 n, int parts, int head_shift, int each, uint8_t* __restrict__ ok) {
   // `each` tokens a workgroup, or one whose parts the workgroup goes through
   const int in_group = each > 1 ? threadIdx.x / parts : 0;
   const i64 i = (i64)blockIdx.x * each + in_group;
   if (in_group >= each || i >= n) return;
   const i64 row = rows ? rows[i] : i;
-  if (row < 0 || row >= c.rows) return;
   const i64 pos = pos_in[i];
-  if (pos < 0 || pos >= row_length(c, c.length[row])) return;
-  const int page = page_of(c, c.table[row * c.width + (pos >> c.page_shift)]);
-  if (page < 0 || c.refs[page] != 1) return;
+  int page = -1;
+  if (row >= 0 && row < c.rows && pos >= 0 && pos < row_length(c, c.length[row])) {
+    page = page_of(c, c.table[row * c.width + (pos >> c.page_shift)]);
+    if (page >= 0 && c.refs[page] != 1) page = -1;
+  }
+  if (ok != nullptr && (int)threadIdx.x == in_group * parts) ok[i] = page >= 0;
+  if (page < 0) return;
   const int slot = (int)(pos & ((1 << c.page_shift) - 1));
   const i64 base = layer * c.layer_bytes;
   for (int u = threadIdx.x - in_group * parts; u < parts; u += kThreads) {
@@ -559,6 +562,12 @@ extern "C" {
 int cugo_paged_append(const CugoPagedCache* cache, int64_t layer, const void* k_new,
                       int64_t k_stride, const void* v_new, int64_t v_stride, const int64_t* pos,
                       const int64_t* rows, int64_t n, hipStream_t stream) {
+  return cugo_paged_append_ok(cache, layer, k_new, k_stride, v_new, v_stride, pos, rows, n, nullptr, stream);
+}
+
+int cugo_paged_append_ok(const CugoPagedCache* cache, int64_t layer, const void* k_new,
+                         int64_t k_stride, const void* v_new, int64_t v_stride, const int64_t* pos,
+                         const int64_t* rows, int64_t n, uint8_t* ok, hipStream_t stream) {
   using namespace cugo_amd::paged;
   Cache c;
   if (const int bad = view(cache, &c)) return bad;
@@ -576,7 +585,7 @@ int cugo_paged_append(const CugoPagedCache* cache, int64_t layer, const void* k_
   hipLaunchKernelGGL(append_kernel, dim3((unsigned)groups), dim3(kThreads), 0, stream, c, layer,
                      static_cast<const char*>(k_new), k_stride * size,
                      static_cast<const char*>(v_new), v_stride * size, pos, rows, n, parts,
-                     31 - __builtin_clz(c.token_bytes / 16), each);
+                     31 - __builtin_clz(c.token_bytes / 16), each, ok);
   return (int)hipGetLastError();
 }
 

@@ -84,9 +84,9 @@ int64_t block_stride(const Tensor& t) {
   return t.size(0) <= 1 ? t.size(1) * t.size(2) : t.stride(0);
 }
 
-void paged_append(const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& length,
-                  const Tensor& refs, const Tensor& free, int64_t layer, const Tensor& k_new,
-                  const Tensor& v_new, const Tensor& pos, const Optional& rows) {
+Tensor paged_append(const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& length,
+                    const Tensor& refs, const Tensor& free, int64_t layer, const Tensor& k_new,
+                    const Tensor& v_new, const Tensor& pos, const Optional& rows, const Optional& out) {
   const Paged p(k, v, table, length, refs, free);
   p.check_layer(layer);
   TORCH_CHECK(k_new.dim() == 3 && k_new.size(1) == p.c.kv_heads && k_new.size(2) == p.c.dh &&
@@ -105,10 +105,13 @@ void paged_append(const Tensor& k, const Tensor& v, const Tensor& table, const T
   }
   const DeviceGuard guard(k.device());
   const Tensor kn = blocks(k_new), vn = blocks(v_new);
-  check_call(cugo_paged_append(&p.c, layer, kn.data_ptr(), block_stride(kn), vn.data_ptr(),
-                               block_stride(vn), pos.data_ptr<int64_t>(),
-                               rows.has_value() ? rows->data_ptr<int64_t>() : nullptr, n, stream()),
+  const auto ok = out_or_new(out, {n}, at::kBool, k, "out");
+  check_call(cugo_paged_append_ok(&p.c, layer, kn.data_ptr(), block_stride(kn), vn.data_ptr(),
+                                  block_stride(vn), pos.data_ptr<int64_t>(),
+                                  rows.has_value() ? rows->data_ptr<int64_t>() : nullptr, n, u8p(ok),
+                                  stream()),
              "paged_append");
+  return ok;
 }
 
 Tensor paged_branch(const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& length,
@@ -221,10 +224,10 @@ Tensor tree_attention(const Tensor& k, const Tensor& v, const Tensor& table, con
 void bind_paged(pybind11::module_& m) {
   namespace py = pybind11;
   const auto none = py::none();
-  m.def("paged_append", &paged_append, "New keys and values into their rows' pages, in place",
+  m.def("paged_append", &paged_append, "New keys and values into their rows' pages, in place; ok [n]",
         py::arg("k"), py::arg("v"), py::arg("table"), py::arg("length"), py::arg("refs"),
         py::arg("free"), py::arg("layer"), py::arg("k_new"), py::arg("v_new"), py::arg("pos"),
-        py::arg("rows") = none);
+        py::arg("rows") = none, py::arg("out") = none);
   m.def("paged_branch", &paged_branch, "Rows become copies of others, sharing their pages; ok [n]",
         py::arg("k"), py::arg("v"), py::arg("table"), py::arg("length"), py::arg("refs"),
         py::arg("free"), py::arg("dst"), py::arg("src"), py::arg("want"));

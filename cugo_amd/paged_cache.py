@@ -66,16 +66,18 @@ def branch(ext, cache, dst: torch.Tensor, src: torch.Tensor, length: torch.Tenso
     pages are the lowest free ones, entry after entry; one that would need more than there are, with
     those before it, gets none (its dst is empty then; a row that is its own src stays).  After a
     call the positions from the kept tokens up to length[i] are the row's alone, to `append`
-    into."""
+    into, until a row branched from it keeps tokens that end in one of their pages: cut a row to its
+    tokens before (`accept`, or `branch` to itself), and grow it afterwards."""
     return ext.paged_branch(*_state(cache), dst, src, length)
 
 
 def append(ext, cache, layer: int, k_new: torch.Tensor, v_new: torch.Tensor, pos: torch.Tensor,
-           rows: torch.Tensor | None = None) -> None:
+           rows: torch.Tensor | None = None, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """Token i's key and value (k_new and v_new [n, kv_heads, dh], any distance between tokens) to
-    position pos[i] of row rows[i] (None: row i), int64 [n], in place.  Nothing is written outside
-    a row's length or into a page that several rows hold.  No two tokens may have one place."""
-    ext.paged_append(*_state(cache), layer, k_new, v_new, pos, rows)
+    position pos[i] of row rows[i] (None: row i), int64 [n], in place; bool [n] (`out`, if given):
+    which tokens were written.  Nothing is written outside a row's length or into a page that
+    several rows hold (see `branch`).  No two tokens may have one place."""
+    return ext.paged_append(*_state(cache), layer, k_new, v_new, pos, rows, out)
 
 
 def accept(ext, cache, rows: torch.Tensor, start: torch.Tensor, keep: torch.Tensor) -> torch.Tensor:
@@ -127,21 +129,25 @@ def tree_mask(parents: Sequence[int], device=None) -> torch.Tensor:
 def tree_step(model: nn.Module, ext, cache, x: torch.Tensor, prefix: torch.Tensor,
               pos: torch.Tensor, token_rows: torch.Tensor, *, mask: torch.Tensor | None = None,
               rows: torch.Tensor | None = None, offsets: torch.Tensor | None = None,
-              final_norm: nn.Module | None = None):
+              final_norm: nn.Module | None = None, placed: torch.Tensor | None = None):
     """A policy's encoder layers over drafted tokens x [tokens, d] of n sequences: token t's key and
     value go to position pos[t] of row token_rows[t] at every layer, then the tokens attend
     (`tree_attention`'s prefix, mask, rows and offsets).  For modules laid out as
-    `seq_decode.cached_step` takes them; the cache's rows need pages for the drafts (`branch`).
-    Returns the final hidden states, and with final_norm (that, its norm)."""
+    `seq_decode.cached_step` takes them; the cache's rows need pages for the drafts (`branch`):
+    `placed`, if given, bool [tokens], takes which tokens had a place (`append`); where one had none,
+    those that attend it attend what is there.  Returns the final hidden states, and with
+    final_norm (that, its norm)."""
     tokens, d = x.shape
     heads = cache.k.shape[2]
     layers = model.encoder.layers
     x, h = add_norm(x, None, layers[0].norm1)
+    if placed is None:
+        placed = torch.empty(tokens, dtype=torch.bool, device=x.device)
     for i, layer in enumerate(layers):
         sa = layer.self_attn
         q, k, v = (t.reshape(tokens, heads, d // heads)
                    for t in linear(h, sa.in_proj_weight, sa.in_proj_bias).chunk(3, -1))
-        append(ext, cache, i, k, v, pos, token_rows)
+        append(ext, cache, i, k, v, pos, token_rows, out=placed)
         a = tree_attention(ext, cache, i, q, prefix, mask=mask, rows=rows, offsets=offsets)
         last = i + 1 == len(layers)
         norm = final_norm if last else layers[i + 1].norm1

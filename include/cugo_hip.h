@@ -816,10 +816,18 @@ typedef struct CugoPagedCache {
 /* cugo_paged_append: new token i's key and value (k_new and v_new [n, kv_heads, dh] of the cache's
  * type, tokens k_stride and v_stride elements apart) to position pos[i] of row rows[i] (NULL: i)
  * in one layer.  Nothing is written where the row or the position (outside [0, length)) is none,
- * nor into a page that several rows hold.  Two tokens must not have the same place. */
+ * nor into a page that several rows hold.  Two tokens must not have the same place.
+ * cugo_paged_append_ok: the same, and ok (bool [n], NULL: not asked) whether token i was written.
+ *
+ * A row that others were branched from shares the page in which they end, with its own room behind
+ * them if it has any there: cut it to its tokens before (accept, or branch to itself).  Where it
+ * was not, a cut and growing again (branch to itself, twice) give it a page of its own. */
 int cugo_paged_append(const CugoPagedCache* cache, int64_t layer, const void* k_new,
                       int64_t k_stride, const void* v_new, int64_t v_stride, const int64_t* pos,
                       const int64_t* rows, int64_t n, hipStream_t stream);
+int cugo_paged_append_ok(const CugoPagedCache* cache, int64_t layer, const void* k_new,
+                         int64_t k_stride, const void* v_new, int64_t v_stride, const int64_t* pos,
+                         const int64_t* rows, int64_t n, uint8_t* ok, hipStream_t stream);
 
 /* cugo_paged_branch: row dst[i] becomes the first min(length of src[i], length[i]) tokens of row
  * src[i] with pages for length[i], for n entries at once, as the rows are before the call.  In

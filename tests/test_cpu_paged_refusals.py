@@ -170,3 +170,15 @@ def test_operations_refuse_cpu_tensors():
         pc.accept(m, c, i, i, i[:, None])
     with pytest.raises(RuntimeError, match="CUDA"):
         pc.tree_attention(m, c, 0, x, i)
+
+
+def test_append_with_answers(lib):
+    f = lib.cugo_paged_append_ok
+    f.argtypes = [P, I64, P, I64, P, I64, P, P, I64, P, P]
+    c = ctypes.byref(_cache())
+    for ok in (AT, None):
+        assert f(c, 0, AT, 64, AT, 64, AT, None, 0, ok, None) == 0
+        assert f(c, 2, AT, 64, AT, 64, AT, None, 1, ok, None) == -1
+        assert f(c, 0, AT, 64, AT, 64, AT, None, -1, ok, None) == -1
+        assert f(c, 0, AT + 8, 64, AT, 64, AT, None, 1, ok, None) == -4
+        assert f(ctypes.byref(_cache(dh=48)), 0, AT, 64, AT, 64, AT, None, 1, ok, None) == -3
