@@ -222,10 +222,11 @@ def random_cache(rng, lengths, *, layers=1, kv_heads=2, page=16, dh=32, width=No
     return cache
 
 
-def dense_attention(cache, layer, q, prefix, mask=None, rows=None, offsets=None, scale=None):
+def dense_attention(cache, layer, q, prefix, mask=None, rows=None, offsets=None, scale=None, twice=False):
     """PagedRef.attention with torch in float64 on the tensors' device, for larger cases.  Returns the
     outputs, and for each how far one in `dtype` may be off when scores, softmax and sums are
-    float32 and weights and outputs are rounded to the type (all bounds worked out below)."""
+    float32 and weights and outputs are rounded to the type (all bounds worked out below); `twice`:
+    weights as the sum of two numbers of the type."""
     import torch
 
     tokens, heads, dh = q.shape
@@ -275,8 +276,11 @@ def dense_attention(cache, layer, q, prefix, mask=None, rows=None, offsets=None,
         off = 2 * (dh + 8) * single * size + 4 * single
         # the weights' sum and the outputs' over `have` tokens, rescaled now and then; a weight
         # rounded to the type
-        off = off + 2 * (have + 64) * single + (half if q.dtype != torch.float32 else 0.0)
+        weight = 0.0 if q.dtype == torch.float32 else half * half if twice else half
+        off = off + 2 * (have + 64) * single + weight
         far = half * y.abs() + 2 * off * spread + torch.finfo(q.dtype).smallest_normal
+        if twice and q.dtype == torch.float16:  # half its smallest step, of weights of 2^7 at the top
+            far = far + have * 2.0**-32 * safe_v.abs().amax(1)[:, None, None]
         out[first:end] = y.permute(2, 0, 1, 3).reshape(t, heads, dh)
         bound[first:end] = far.permute(2, 0, 1, 3).reshape(t, heads, dh)
     return out, bound
