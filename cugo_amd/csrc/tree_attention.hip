@@ -647,7 +647,7 @@ struct Queries {
   // Of the 64 positions from `at` on, those that the lane's query m attends.
   __device__ __forceinline__ u64 window(const Call& a, const Sequence& s, int m, int at) const {
     const u64* mask = a.mask ? a.mask + (a.mask_rows == a.tokens ? token[m] : index[m]) * (i64)a.words : nullptr;
-    const int limit = a.mask ? s.end : min(s.end, s.prefix + index[m] + 1);
+    const int limit = a.mask ? s.end : end_of(s, index[m]);
     return window_of(at, limit, s.prefix, mask, a.words);
   }
 };
@@ -737,8 +737,8 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(Call a) {
       // positions that some query of the tile attends end at `end`, those that all do at `full`
       const int q_first = (unsigned)row0 / (unsigned)a.group;
       const int q_last = (unsigned)min(row0 + kRows - 1, M - 1) / (unsigned)a.group;
-      const int end = a.mask ? s.end : min(s.end, s.prefix + q_last + 1);
-      const int full_tiles = min(end, a.mask ? s.prefix : s.prefix + q_first + 1) / KT;
+      const int end = a.mask ? s.end : end_of(s, q_last);
+      const int full_tiles = (a.mask ? s.prefix : end_of(s, q_first)) / KT;
       const int to = min(job.to, (end + KT - 1) / KT);
       const int step = MODE == kEach ? 1 : kWaves;
       const int begin = job.from + (MODE == kEach ? 0 : wave);
@@ -1031,8 +1031,8 @@ __global__ __launch_bounds__(64 * kWaves, (Chunk<T, DH>::kResident)) void chunk_
       // positions that some query of the workgroup attends end at `end`, those that all do at `full`
       const int q_first = (unsigned)row0 / (unsigned)a.group;
       const int q_last = (unsigned)min(row0 + Ch::kRows - 1, M - 1) / (unsigned)a.group;
-      const int end = a.mask ? s.end : min(s.end, s.prefix + q_last + 1);
-      const int full = min(end, a.mask ? s.prefix : s.prefix + q_first + 1);
+      const int end = a.mask ? s.end : end_of(s, q_last);
+      const int full = a.mask ? s.prefix : end_of(s, q_first);
       const int to = min(job.to, (end + Ch::kTokens - 1) / Ch::kTokens);
       q.load(a, w);
       const i64 head_offset = a.layer_offset + slot_offset(c, 0, job.head, 0);

@@ -73,6 +73,10 @@ __host__ __device__ __forceinline__ Sequence sequence_at(const Call& a, int i) {
   s.end = (int)(s.prefix + behind < s.length ? s.prefix + behind : s.length);
   return s;
 }
+// Without a mask: where what query `index` may attend ends (a sum of two of these numbers may not fit).
+__host__ __device__ __forceinline__ int end_of(const Sequence& s, int index) {
+  return s.end - s.prefix > index ? s.prefix + index + 1 : s.end;
+}
 __host__ __device__ __forceinline__ Sequence same(Sequence s) {
   s.first = same(s.first), s.queries = same(s.queries), s.row = same(s.row);
   s.length = same(s.length), s.prefix = same(s.prefix), s.end = same(s.end);

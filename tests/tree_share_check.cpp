@@ -21,7 +21,25 @@ struct Part {
   int sequence, item, from, to;
 };
 
+// Where queries' positions end, near the longest row too.
+int ends_fit() {
+  std::mt19937_64 rng(12);
+  for (int i = 0; i < 200000; ++i) {
+    Sequence s{};
+    s.length = (int)(kMostTokens - 1) >> (rng() % 2 ? 0 : rng() % 31);
+    s.prefix = rng() % 2 ? s.length - (int)(rng() % (1 + (s.length >> rng() % 31))) : s.length;
+    s.queries = 1 + (int)(rng() % (1 << 24) >> rng() % 24);
+    const i64 whole = (i64)s.prefix + s.queries;
+    s.end = (int)(whole < s.length ? whole : s.length);
+    const int index = (int)(rng() % s.queries);
+    const i64 want = (i64)s.prefix + index + 1;
+    CHECK(end_of(s, index) == (want < s.end ? want : s.end));
+  }
+  return 0;
+}
+
 int main() {
+  if (ends_fit()) return 1;
   std::mt19937_64 rng(11);
   int too_much = 0, cut = 0, served = 0;
   for (int round = 0; round < 3000; ++round) {
