@@ -201,8 +201,9 @@ Tensor tree_attention(const Tensor& k, const Tensor& v, const Tensor& table, con
     a.mask = reinterpret_cast<const uint64_t*>(a.words && a.mask_rows ? mask->data_ptr<int64_t>()
                                                                       : prefix.data_ptr<int64_t>());
   }
-  TORCH_CHECK(!scale.has_value() || (std::isfinite(static_cast<float>(*scale)) && static_cast<float>(*scale) != 0.f),
-              "scale must be finite and not 0");
+  TORCH_CHECK(!scale.has_value() || (std::isfinite(static_cast<float>(*scale) * 1.4426950408889634f) &&
+                                     static_cast<float>(*scale) != 0.f),
+              "scale must be finite (times log2(e) too) and not 0");
   a.scale = static_cast<float>(scale.value_or(1.0 / std::sqrt(static_cast<double>(p.c.dh))));
   const DeviceGuard guard(k.device());
   const Tensor q = blocks(q_in);

@@ -1426,6 +1426,7 @@ inline int view(const CugoTreeAttention* p, Call* a) {
   const float scale = p->scale < 0.f ? -p->scale : p->scale;
   a->flip = p->scale < 0.f ? (size == 4 ? 0x80000000u : 0x80008000u) : 0u;
   a->scale_log2 = scale * 1.4426950408889634f;  // softmax in base 2
+  if (a->scale_log2 - a->scale_log2 != 0.f) return -1;
   a->out = static_cast<char*>(p->out);
   a->part_o = a->part_ml = nullptr;
   a->left = nullptr;

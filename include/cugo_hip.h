@@ -868,6 +868,7 @@ int cugo_paged_accept(const CugoPagedCache* cache, const int64_t* rows, const in
  *   t < prefix[i], or bit (t - prefix[i]) of its mask set              (mask given)
  *   t <= prefix[i] + j                                                 (mask NULL)
  *   out = sum_t softmax_t(q . k_t scale) v_t                           (out [tokens, heads, dh])
+ * (scale finite, times log2(e) too, and not 0.)
  * mask: uint64 [tokens, words], or [tokens / n, words] with mask_rows = tokens / n and offsets
  * NULL, the same for every sequence; bit b is bit b % 64 of word b / 64.  A query that attends
  * nothing gets zeros; one whose row is none, or that attends a position whose page is none, NaN.

@@ -172,6 +172,15 @@ def test_operations_refuse_cpu_tensors():
         pc.tree_attention(m, c, 0, x, i)
 
 
+@pytest.mark.parametrize("scale", [2.5e38, -3.4e38])
+def test_scales_that_are_infinite_in_base_2(lib, scale):
+    cache = _cache()
+    a = Attention(cache=ctypes.addressof(cache), layer=1, q=AT, q_stride=128, tokens=6, heads=4, n=2,
+                  prefix=AT, scale=scale, out=AT)
+    assert lib.cugo_tree_attention(ctypes.byref(a), AT, 1 << 30, None) == -1
+    assert lib.cugo_tree_attention_workspace(ctypes.byref(a)) == 0
+
+
 def test_append_with_answers(lib):
     f = lib.cugo_paged_append_ok
     f.argtypes = [P, I64, P, I64, P, I64, P, P, I64, P, P]
