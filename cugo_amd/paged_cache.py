@@ -107,8 +107,9 @@ def tree_attention(ext, cache, layer: int, q: torch.Tensor, prefix: torch.Tensor
     [tokens, words], bit b being bit b % 64 of word b // 64, or without offsets [tokens / n, words]
     for every sequence alike (`tree_mask`); None: the positions up to prefix[i] + j.
 
-    A query that attends nothing gets zeros, one whose row does not exist NaN; tokens outside every
-    sequence are left as they were in `out`.  scale None: dh ** -0.5.  No gradients."""
+    A query that attends nothing, or only scores of -inf, gets zeros, one whose row does not exist
+    NaN; tokens outside every sequence are left as they were in `out`.  scale None: dh ** -0.5.  No
+    gradients."""
     return ext.tree_attention(*_state(cache), layer, q, prefix, mask, rows, offsets, scale, out)
 
 

@@ -871,8 +871,9 @@ int cugo_paged_accept(const CugoPagedCache* cache, const int64_t* rows, const in
  * (scale finite, times log2(e) too, and not 0.)
  * mask: uint64 [tokens, words], or [tokens / n, words] with mask_rows = tokens / n and offsets
  * NULL, the same for every sequence; bit b is bit b % 64 of word b / 64.  A query that attends
- * nothing gets zeros; one whose row is none, or that attends a position whose page is none, NaN.
- * What masked places hold is never used.  Sums and softmax in float32; 16-bit types' weights meet v
+ * nothing, or only scores of -inf, gets zeros; one whose row is none, or that attends a position whose
+ * page is none, NaN.  What masked places hold is never used.  An infinite value that a query attends
+ * is its result however small the weight (two of different signs: NaN).  Sums and softmax in float32; 16-bit types' weights meet v
  * rounded to the type (dh >= 64 and more than 64 queries x group, or 32 in few sequences) or
  * as the sum of two numbers of it; float16's to 2^-32 of the largest.  workspace: at least
  * cugo_tree_attention_workspace(...) bytes (asked on the device of the call; may be 0). */

@@ -177,6 +177,9 @@ class PagedRef:
                     v = self.v[layer, pages, h // group, slots]
                     with np.errstate(invalid="ignore"):
                         s = k @ q[t, h] * scale
+                        if s.max() == -np.inf:  # zeros
+                            out[t, h] = 0.0
+                            continue
                         e = np.exp(s - s.max())
                         out[t, h] = (e / e.sum()) @ v
         return out
@@ -264,15 +267,15 @@ def dense_attention(cache, layer, q, prefix, mask=None, rows=None, offsets=None,
         # masked places hold anything, NaN too: their keys are left out one way or the other
         s = (x @ k.mT).view(kv_heads, group, t, have) * scale
         s = s.masked_fill(~seen, -torch.inf)
-        some = seen.any(1)
-        w = s.masked_fill(~some[:, None], 0.0).softmax(3).masked_fill(~seen, 0.0)
+        none = s.amax(3, keepdim=True) == -torch.inf  # nothing is attended, or only scores of -inf
+        w = s.masked_fill(none, 0.0).softmax(3).masked_fill(~seen | none, 0.0)
         safe_v = torch.where(seen.any(0)[:, None], v, 0.0)
         y = (w.reshape(kv_heads, group * t, have) @ safe_v).view(kv_heads, group, t, dh)
         spread = (w.reshape(kv_heads, group * t, have) @ safe_v.abs()).view(kv_heads, group, t, dh)
         # a score's error: dh products and sums and the scaling, each half a step of the sum of
         # magnitudes; exp2 of a number of that size, a step of it and two of the result
         size = (x.abs() @ k.abs().mT).view(kv_heads, group, t, have) * scale
-        size = size.masked_fill(~seen, 0.0).amax(3, keepdim=True)
+        size = size.masked_fill(~seen | (s == -torch.inf), 0.0).amax(3, keepdim=True)
         off = 2 * (dh + 8) * single * size + 4 * single
         # the weights' sum and the outputs' over `have` tokens, rescaled now and then; a weight
         # rounded to the type

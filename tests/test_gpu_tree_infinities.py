@@ -98,6 +98,34 @@ def test_infinite_values(ext, dtype, dh, dealt):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("dh", [32, 64, 128, 256])
 @pytest.mark.parametrize("dealt", DEALT)
+def test_scores_of_minus_infinity(ext, dtype, dh, dealt):
+    """Keys that some queries cannot score: of weight 0 for those, and zeros where all are."""
+    announce(f"tree attention of scores of -inf {dtype} dh {dh}, {dealt}")
+    lengths, n, t, group, width = DEALT[dealt]
+    rng = np.random.default_rng(dh + n)
+    cache = on_gpu(random_cache(rng, lengths, kv_heads=2, dh=dh, width=width, dtype=TYPES[dtype]))
+    cache.k[0, :, :, :, 0] = -torch.inf
+    cache.k[0, :, :, 1::3, 0] = 0.0
+    few = len(lengths)
+    q = torch.from_numpy(rng.standard_normal((few, t, 2 * group, dh))).to("cuda", TYPES[dtype])
+    q[..., 0] = 1.0
+    rows = np.arange(n) % few
+    prefix = i64(np.array(lengths)[rows] - t)
+    tree = pc.tree_mask(drafts_tree(rng, t), "cuda")
+    for turn in range(2):
+        got = pc.tree_attention(ext, cache, 0, q[rows].flatten(0, 1), prefix, mask=tree, rows=i64(rows))
+        want, bound = dense_attention(cache, 0, q.flatten(0, 1), i64(np.array(lengths) - t), tree)
+        far = (got.view(n, t, 2 * group, dh).double() - want.view(few, t, 2 * group, dh)[rows]).abs()
+        assert (far <= bound.view(few, t, 2 * group, dh)[rows]).all()
+        if turn == 0:
+            assert want.abs().amax() > 0
+            cache.k[0, :, :, :, 0] = -torch.inf
+    assert not got.any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dh", [32, 64, 128, 256])
+@pytest.mark.parametrize("dealt", DEALT)
 @pytest.mark.parametrize("gap", [5.0, 30.0, 100.0])
 def test_small_weights_of_infinities(ext, dtype, dh, dealt, gap):
     """An infinite value whose weight is e^-gap of another token's: an infinity all the same, before and
