@@ -9,9 +9,9 @@
 //            numbers) -> apply (table, references, copies of part-filled pages)
 //   accept:  decide (a wavefront an entry) -> move (tokens, pages given back)
 // Bound: the copies by memory (8,192 children of rows of up to 48 tokens in four layers, 540 MB: apply
-// 104 us, 5.2 TB/s; append of 49,000 tokens, 100 MB: 20.2 us), moves by half lines where a token of a head
+// 104 us, 5.2 TB/s; append of 49,000 tokens, 100 MB: 21.2 us), moves by half lines where a token of a head
 // is 64 bytes (4,096 paths: 33 us), the rest by the launches' latency (place 14 us for 8,192 entries,
-// few_kernel 12.4 for 16).
+// few_kernel 12.5 for 16).
 #include "paged.h"
 
 namespace cugo_amd {

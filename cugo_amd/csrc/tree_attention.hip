@@ -21,21 +21,23 @@
 // The running maximum moves only when a score exceeds it by more than 2^8 in the weight (kSlack):
 // until then weights are at most 2^8, which neither type nor the sums mind, and a tile needs no
 // exchange between lanes.  16-bit weights meet V as the sum of two numbers of the type, which costs
-// nothing beside the memory (4,096 trees over 320 tokens: the same 181 us) and leaves little but the
+// nothing beside the memory (4,096 trees over 320 tokens: the same time) and leaves little but the
 // output's rounding (2^-16 of a weight in bfloat16; 2^-22 in float16, or 2^-32 of the largest weight,
 // half its smallest step, where that is more); where many rows make the products the bound
 // (chunk_kernel), rounded once, half a step each, as much again as the output's rounding.  Their sum
 // is taken from what meets V (a matrix instruction with ones), so they add up to one.
 //
-// Bound: memory where a key head has few rows (4,096 trees of 16 tokens over rows of up to 320, dh 32
-// bf16: 181 us, 4.7 TB/s; 24 trees over rows of up to 32,768, dh 128 float16: 345 us, 5.3 TB/s), the
-// matrix and vector pipes in turn where it has many (4 x 512 queries over 14,336 tokens, dh 128 bf16:
-// 137 to 145 us, 730 to 777 TFLOP/s), latency in the smallest calls (one query: 4.7 us).
+// Bound (us a call among others, joining included): memory where a key head has few rows (4,096 trees of
+// 16 tokens over rows of up to 320, dh 32 bf16: 183 us, 4.7 TB/s; 24 trees over rows of up to 32,768,
+// dh 128 float16: 377 us, 4.8 TB/s), the matrix and vector pipes in turn where it has many (4 x 512
+// queries over 14,336 tokens, dh 128 bf16: 142 to 155 us, 690 to 751 TFLOP/s), latency in the smallest
+// calls (one query: 9.3 us, its kernel 4.9).
 //
 // Tiles in which some query may not see some token (the drafts, a row's end) take their scores
 // from the masks.  Values that are infinite or NaN go through products of their own (indicators of
 // +inf and -inf), since 0 x inf would show in queries that do not attend them, and be NaN in those
-// whose weight, or its second number, is 0: found among a tile's values (4,096 trees: the same time), or by
+// whose weight, or its second number, is 0: found among a tile's values (4,096 trees: the same time; where
+// products are the bound, 2,048 queries of dh 32 131 -> 139 us, of float32 1,125 -> 1,154), or by
 // chunk_kernel, whose full tiles do not pass through registers first, in its outputs.
 #include <type_traits>
 
